@@ -227,6 +227,28 @@ int mi_linear(const void *x, const void *weight, const void *bias, void *out, in
               int in_features, int out_features, void *stream);
 int mi_linear_f32(const void *x, const void *weight, float *out, int accumulate, int rows,
                   int in_features, int out_features, void *stream);
+/* Beyond the reference (whose weights are fp16): projections through 4-bit
+ * weights. A weight (out, in) is codes, (out, in / 2) bytes, two codes a byte,
+ * the first in the low bits, and scales and zeros, (out, in / group) fp16
+ * each: the weight at input i of an output stands for code * scale + zero of
+ * its group i / group. group is 32, 64 or 128 and divides in; codes, x and
+ * the fp16 weight are 16-byte aligned.
+ * mi_quantise_int4 makes them from fp16 weights (finite) by the page
+ * quantiser's rule: the zero a group's least value, the scale the least fp16
+ * whose 15 steps reach the group's range, codes rounded half to even.
+ * mi_linear_int4: out (rows, out) fp16 = x (rows, in) W^T + bias (out fp16, or
+ * null), fp32 sums rounded once. mi_linear_int4_accumulate: out (rows, out)
+ * fp32 += x W^T. The sums' order depends on the sizes alone. For a decode
+ * row or the rows of some sequences' steps; many rows (a prompt's) are better
+ * multiplied by mi_linear against fp16 weights. */
+int mi_quantise_int4(const void *weight, void *codes, void *scales, void *zeros, int group,
+                     int in_features, int out_features, void *stream);
+int mi_linear_int4(const void *x, const void *codes, const void *scales, const void *zeros,
+                   int group, const void *bias, void *out, int rows, int in_features,
+                   int out_features, void *stream);
+int mi_linear_int4_accumulate(const void *x, const void *codes, const void *scales,
+                              const void *zeros, int group, float *out, int rows, int in_features,
+                              int out_features, void *stream);
 /* reference: embed.cu:60-76, bindings_device.cpp:321-334 (embed_f32) and
  * :383-396 (embed): out (count, hidden) = table rows ids[i], fp16 or widened
  * to fp32 (out_is_f32); an id outside [0, vocab) gives a zero row. */

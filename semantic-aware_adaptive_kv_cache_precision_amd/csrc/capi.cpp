@@ -846,6 +846,35 @@ int mi_linear_f32(const void *x, const void *weight, float *out, int accumulate,
   });
 }
 
+int mi_quantise_int4(const void *weight, void *codes, void *scales, void *zeros, int group,
+                     int in_features, int out_features, void *stream)
+{
+  return guarded([&] {
+    mi::launch_quantise_int4(weight, codes, scales, zeros, group, in_features, out_features,
+                             as_stream(stream));
+  });
+}
+
+int mi_linear_int4(const void *x, const void *codes, const void *scales, const void *zeros,
+                   int group, const void *bias, void *out, int rows, int in_features,
+                   int out_features, void *stream)
+{
+  return guarded([&] {
+    mi::launch_linear_int4(x, codes, scales, zeros, group, bias, out, rows, in_features,
+                           out_features, as_stream(stream));
+  });
+}
+
+int mi_linear_int4_accumulate(const void *x, const void *codes, const void *scales,
+                              const void *zeros, int group, float *out, int rows, int in_features,
+                              int out_features, void *stream)
+{
+  return guarded([&] {
+    mi::launch_linear_int4_accumulate(x, codes, scales, zeros, group, out, rows, in_features,
+                                      out_features, as_stream(stream));
+  });
+}
+
 int mi_embed(const int32_t *ids, int count, const void *table, void *out, int out_is_f32,
              int hidden, int vocab, void *stream)
 {

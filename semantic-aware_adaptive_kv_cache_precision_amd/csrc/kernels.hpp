@@ -596,4 +596,19 @@ namespace mi
   };
   void launch_qkv_step(const QkvStep &s, hipStream_t stream);
 
+  // ---- 4-bit weights (int4.hip) -----------------------------------------------------
+  // A weight (out, in) as codes (out, in / 2) bytes, two a byte, the first in
+  // the low bits, and fp16 scales and zeros (out, in / group): group 32, 64
+  // or 128, codes and weight 16-byte aligned. Weights are finite.
+  void launch_quantise_int4(const void *weight, void *codes, void *scales, void *zeros, int group,
+                            int in_features, int out_features, hipStream_t stream);
+  // out (rows, out) fp16 = x (rows, in) W^T + bias (may be null), rounded
+  // once; or out (rows, out) fp32 += x W^T. x 16-byte aligned.
+  void launch_linear_int4(const void *x, const void *codes, const void *scales, const void *zeros,
+                          int group, const void *bias, void *out, int rows, int in_features,
+                          int out_features, hipStream_t stream);
+  void launch_linear_int4_accumulate(const void *x, const void *codes, const void *scales,
+                                     const void *zeros, int group, float *out, int rows,
+                                     int in_features, int out_features, hipStream_t stream);
+
 } // namespace mi

@@ -133,6 +133,9 @@ SIGNATURES = {
     "mi_add": ((_vp, _vp, _vp, _sz, _vp), C.c_int),
     "mi_driver_version": ((_ip,), C.c_int),
     "mi_linear": ((_vp, _vp, _vp, _vp, _i, _i, _i, _vp), C.c_int),
+    "mi_quantise_int4": ((_vp, _vp, _vp, _vp, _i, _i, _i, _vp), C.c_int),
+    "mi_linear_int4": ((_vp, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _vp), C.c_int),
+    "mi_linear_int4_accumulate": ((_vp, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _vp), C.c_int),
     "mi_linear_f32": ((_vp, _vp, _vp, _i, _i, _i, _i, _vp), C.c_int),
     "mi_embed": ((_vp, _i, _vp, _vp, _i, _i, _i, _vp), C.c_int),
     "mi_argmax_rows": ((_vp, _i, _i, _vp, _vp), C.c_int),
@@ -660,6 +663,15 @@ def _at(x, count: int, what: str) -> int:
     held = x.count if isinstance(x, Span) else x.numel
     if held < count:
         raise ValueError(f"{what} holds {held}, and the operation needs {count}")
+    return x.address
+
+
+def _bytes_at(x, nbytes: int, what: str) -> int:
+    """The address of a tensor (its `nbytes`) or of a view (fp16 elements)
+    that must hold `nbytes` bytes."""
+    held = 2 * x.count if isinstance(x, Span) else x.nbytes
+    if held < nbytes:
+        raise ValueError(f"{what} holds {held} bytes, and the operation needs {nbytes}")
     return x.address
 
 
@@ -1418,6 +1430,55 @@ def _device_linear_accumulate(x, weight, out: FloatTensor, rows, in_features, ou
     _check(lib.mi_linear_f32(xa, wa, oa, 1, rows, in_features, out_features, None))
 
 
+def _int4_at(codes, scales, zeros, group, in_features, out_features):
+    """The addresses of an int4 weight's parts (mi_quantise_int4's layout)."""
+    if group not in (32, 64, 128):
+        raise ValueError(f"int4 weights have groups of 32, 64 or 128 inputs, not {group}")
+    if in_features < 0 or out_features < 0 or in_features % group:
+        raise ValueError(f"in_features {in_features} and out_features {out_features} must not be "
+                         f"negative, and in_features whole groups of {group}")
+    groups = out_features * (in_features // group)
+    return (_bytes_at(codes, out_features * in_features // 2, "codes"),
+            _bytes_at(scales, 2 * groups, "scales"), _bytes_at(zeros, 2 * groups, "zeros"))
+
+
+def _device_quantise_int4(weight, codes, scales, zeros, group, in_features, out_features):
+    """Beyond the reference: an fp16 weight (out, in) as 4-bit codes, two a
+    byte, the first in the low bits, with an fp16 scale and zero for every
+    `group` (32, 64 or 128) inputs of a row; the weight at input i stands for
+    code * scale + zero."""
+    ca, sa, za = _int4_at(codes, scales, zeros, group, in_features, out_features)
+    wa = _at(weight, out_features * in_features, "weight")
+    _check(lib.mi_quantise_int4(wa, ca, sa, za, group, in_features, out_features, None))
+
+
+def _device_linear_int4(x, codes, scales, zeros, group, bias, out, rows, in_features,
+                        out_features):
+    """linear through an int4 weight (beyond the reference): fp32 sums of x
+    and code * scale + zero, the bias added, rounded once. For a row or the
+    rows of a batch of sequences' steps."""
+    _non_negative(rows, "rows")
+    ca, sa, za = _int4_at(codes, scales, zeros, group, in_features, out_features)
+    xa = _at(x, rows * in_features, "x")
+    ba = _at(bias, out_features, "bias") if bias is not None else None
+    oa = _at(out, rows * out_features, "out")
+    if oa == xa:
+        raise ValueError("an int4 projection cannot write over its input")
+    _check(lib.mi_linear_int4(xa, ca, sa, za, group, ba, oa, rows, in_features, out_features,
+                              None))
+
+
+def _device_linear_int4_accumulate(x, codes, scales, zeros, group, out: FloatTensor, rows,
+                                   in_features, out_features):
+    """linear_accumulate through an int4 weight: out += x @ W.T in fp32."""
+    _non_negative(rows, "rows")
+    ca, sa, za = _int4_at(codes, scales, zeros, group, in_features, out_features)
+    xa = _at(x, rows * in_features, "x")
+    oa = _floats(out, rows * out_features, "out")
+    _check(lib.mi_linear_int4_accumulate(xa, ca, sa, za, group, oa, rows, in_features,
+                                         out_features, None))
+
+
 def _device_embed(ids: DeviceIndex, table, out, hidden, vocab):
     ta = _at(table, vocab * hidden, "table")
     oa = _at(out, ids.count * hidden, "out")
@@ -1576,6 +1637,9 @@ device = SimpleNamespace(
     embed_f32=_device_embed_f32,
     linear=_device_linear,
     linear_accumulate=_device_linear_accumulate,
+    quantise_int4=_device_quantise_int4,
+    linear_int4=_device_linear_int4,
+    linear_int4_accumulate=_device_linear_int4_accumulate,
     rmsnorm=_device_rmsnorm,
     rmsnorm_f32=_device_rmsnorm_f32,
     rope=_device_rope,
