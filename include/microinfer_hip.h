@@ -388,6 +388,42 @@ int mi_kv_attention_kept(mi_kv_pages *kv, int layer, const void *q, const void *
                          int head_dim, const void *keys, const void *values);
 int mi_kv_fold_kept(mi_kv_pages *kv, float *mass, long long mass_stride, float *scores,
                     long long scores_stride, float alpha);
+/* Beyond the reference (whose decode takes one sequence): one token of every
+ * sequence of a batch. Sequence b's query (q, (batch, heads, head_dim) fp16)
+ * reads its tokens before lengths[b], the query's own among them, through its
+ * row of a page table: `pages` (batch, max_pages) addresses of 32-token pages
+ * (mi_quantised_page_layout, or FP16 rows) and `tiers`, both on the device as
+ * `lengths` is, read when the kernels run, so that a captured graph serves
+ * every step. A length over max_pages pages is cut to them. A page whose tier
+ * is not 0..3, or whose address is 0, is not read. With window > 0 a query
+ * sees its last `window` tokens (its own counted) and the first `sinks`.
+ * out (batch, heads, head_dim) fp16; a sequence with nothing to see (length 0)
+ * gives zeros. mass (batch, heads, max_pages) fp32 or NULL: each page's share
+ * of each head's softmax, 0 for pages not read. partials:
+ * mi_attention_batch_partials floats (for sequences of up to max_pages pages;
+ * 0 where one launch does), the caller's until the launch is done, or NULL:
+ * then a sequence's pages are walked by one workgroup a few KV heads, and no
+ * mass can be asked for. Calls that may overlap need partials of their own.
+ * head_dim 64 or 128; at most 16 query heads a KV head; q, out and partials
+ * 16-byte aligned, pages as an allocator's. Keys hold their bias, if any.
+ * mi_kv_attention_batch: the same for `count` caches of one shape, the query
+ * of cache i at position seq_k[i] - 1 of `layer` (seq_k in host memory; 0: no
+ * token), its row stored before, as mi_kv_attention takes it: a cache that
+ * seals reads the row from keys, values (count, kv_width) fp16. A cache may be
+ * named twice. mass (count, heads, mass_pages). partials: for max_pages =
+ * mass_pages, or without mass the longest sequence's pages. On the runtime's
+ * current stream; the caches' pages must not move while a captured one is
+ * replayed. */
+int mi_attention_batch_partials(int batch, int max_pages, int heads, int kv_heads, int head_dim,
+                                int window, int sinks, int with_mass, size_t *floats);
+int mi_attention_batch(const void *q, const unsigned long long *pages, const uint8_t *tiers,
+                       const int *lengths, int batch, int max_pages, int page_tokens, void *out,
+                       int heads, int kv_heads, int head_dim, int window, int sinks, float *mass,
+                       float *partials, size_t partials_floats, void *stream);
+int mi_kv_attention_batch(mi_kv_pages *const *kv, const int *seq_k, int count, int layer,
+                          const void *q, void *out, int heads, int kv_heads, int head_dim,
+                          const void *keys, const void *values, int window, int sinks, float *mass,
+                          int mass_pages, float *partials, size_t partials_floats);
 /* Beyond the reference: the store and the decode of a step whose position
  * lives in device memory, what mi_decode_step's graph launches, for callers
  * that capture graphs of their own (the reference's KVPages.store and

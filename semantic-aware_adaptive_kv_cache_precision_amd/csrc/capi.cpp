@@ -13,6 +13,7 @@
 #include <mutex>
 #include <new>
 #include <string>
+#include <vector>
 
 // A KVPages keeps its allocator alive (the reference's binding does the
 // same, bindings_device.cpp:701-718): the allocator goes when its own handle
@@ -224,6 +225,27 @@ namespace
       throw mi::InvalidArgument("seq_q " + std::to_string(seq_q) + " exceeds seq_k " +
                                 std::to_string(seq_k));
     }
+  }
+
+  mi::BatchAttention batch_of(const void *q, int batch, int max_pages, int page_tokens, void *out,
+                              int heads, int kv_heads, int head_dim, int window, int sinks,
+                              float *mass, float *partials, std::size_t partials_floats)
+  {
+    mi::BatchAttention t{};
+    t.q = q;
+    t.out = out;
+    t.batch = batch;
+    t.max_pages = max_pages;
+    t.page_tokens = page_tokens;
+    t.heads = heads;
+    t.kv_heads = kv_heads;
+    t.head_dim = head_dim;
+    t.window = window;
+    t.sinks = sinks;
+    t.mass = mass;
+    t.partials = partials;
+    t.partials_floats = partials_floats;
+    return t;
   }
 } // namespace
 
@@ -1274,6 +1296,79 @@ int mi_kv_attention_layers(mi_kv_pages *kv, int first_layer, int layers, const v
     kv->impl.attention_layers(first_layer, layers, q, q_stride, out, out_stride, seq_k, heads,
                               kv_heads, head_dim, keys, values, kv_stride, mass, mass_stride,
                               scores, scores_stride, alpha);
+  });
+}
+
+int mi_attention_batch_partials(int batch, int max_pages, int heads, int kv_heads, int head_dim,
+                                int window, int sinks, int with_mass, size_t *floats)
+{
+  return guarded([&] {
+    need(floats, "floats");
+    mi::BatchAttention t = batch_of(nullptr, batch, max_pages, mi::kBatchPageTokens, nullptr, heads,
+                                    kv_heads, head_dim, window, sinks, nullptr, nullptr, 0);
+    *floats = mi::batch_attention_floats(t, with_mass != 0);
+  });
+}
+
+int mi_attention_batch(const void *q, const unsigned long long *pages, const uint8_t *tiers,
+                       const int *lengths, int batch, int max_pages, int page_tokens, void *out,
+                       int heads, int kv_heads, int head_dim, int window, int sinks, float *mass,
+                       float *partials, size_t partials_floats, void *stream)
+{
+  return guarded([&] {
+    mi::BatchAttention t = batch_of(q, batch, max_pages, page_tokens, out, heads, kv_heads,
+                                    head_dim, window, sinks, mass, partials, partials_floats);
+    t.pages = pages;
+    t.tiers = tiers;
+    t.lengths = lengths;
+    mi::launch_batch_attention(t, as_stream(stream));
+  });
+}
+
+int mi_kv_attention_batch(mi_kv_pages *const *kv, const int *seq_k, int count, int layer,
+                          const void *q, void *out, int heads, int kv_heads, int head_dim,
+                          const void *keys, const void *values, int window, int sinks, float *mass,
+                          int mass_pages, float *partials, size_t partials_floats)
+{
+  return guarded([&] {
+    if (count < 0)
+    {
+      throw mi::InvalidArgument("a batch of " + std::to_string(count) + " sequences");
+    }
+    if (count == 0)
+    {
+      return;
+    }
+    need(kv, "the caches");
+    need(seq_k, "seq_k");
+    const auto *k = static_cast<const std::uint16_t *>(keys);
+    const auto *v = static_cast<const std::uint16_t *>(values);
+    const std::size_t width = static_cast<std::size_t>(std::max(kv_heads, 0)) * std::max(head_dim, 0);
+    std::vector<mi::BatchSequence> held(static_cast<std::size_t>(count));
+    int most = 0, page_tokens = mi::kBatchPageTokens;
+    for (int i = 0; i < count; ++i)
+    {
+      need(kv[i], "a cache");
+      held[i] = kv[i]->impl.batch_sequence(layer, seq_k[i], kv_heads, head_dim,
+                                           k != nullptr ? k + i * width : nullptr,
+                                           v != nullptr ? v + i * width : nullptr);
+      if (kv[i]->impl.page_tokens() != page_tokens)
+      {
+        page_tokens = kv[i]->impl.page_tokens(); // refused below, by its size
+        break;
+      }
+      most = std::max(most, (seq_k[i] + page_tokens - 1) / page_tokens);
+    }
+    if (mass != nullptr && mass_pages < most)
+    {
+      throw mi::InvalidArgument("the masses hold " + std::to_string(mass_pages) +
+                                " pages a head; the longest sequence has " + std::to_string(most));
+    }
+    mi::BatchAttention t =
+        batch_of(q, count, mass != nullptr ? mass_pages : most, page_tokens, out, heads, kv_heads,
+                 head_dim, window, sinks, mass, partials, partials_floats);
+    t.held = held.data();
+    mi::launch_batch_attention(t, mi::runtime_stream());
   });
 }
 

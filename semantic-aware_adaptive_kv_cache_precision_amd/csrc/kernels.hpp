@@ -611,4 +611,46 @@ namespace mi
                                      const void *zeros, int group, float *out, int rows,
                                      int in_features, int out_features, hipStream_t stream);
 
+  // ---- one token of every sequence of a batch (batch.hip) --------------------------
+  // A sequence whose cache the host holds: its page table's row, and where a
+  // cache that seals keeps the token's own page (`open` null: in the table).
+  struct BatchSequence
+  {
+    const unsigned long long *pages;
+    const std::uint8_t *tiers;
+    const std::uint16_t *open; // the page being filled: 32 key rows, 32 value rows
+    const std::uint16_t *own_k;
+    const std::uint16_t *own_v;
+    int length;
+  };
+  constexpr int kBatchHeld = 32; // sequences that go in one launch's arguments
+
+  struct BatchAttention
+  {
+    const void *q; // (batch, heads, head_dim) fp16
+    void *out;
+    // The tables on the device, (batch, max_pages) and (batch); or `held`,
+    // `batch` sequences in host memory.
+    const unsigned long long *pages;
+    const std::uint8_t *tiers;
+    const int *lengths;
+    const BatchSequence *held;
+    int batch;
+    int max_pages;
+    int page_tokens;
+    int heads;
+    int kv_heads;
+    int head_dim;
+    int window; // the last tokens visible; 0: every one
+    int sinks;  // the first tokens visible beside a window's
+    float *mass; // (batch, heads, max_pages), or null
+    // Null: a workgroup a sequence and KV heads, no masses; else at least
+    // batch_attention_floats, used until the launch is done.
+    float *partials;
+    std::size_t partials_floats;
+  };
+  constexpr int kBatchPageTokens = 32;
+  std::size_t batch_attention_floats(const BatchAttention &t, bool with_mass);
+  void launch_batch_attention(const BatchAttention &t, hipStream_t stream);
+
 } // namespace mi

@@ -1229,6 +1229,52 @@ namespace mi
     launch_attention(kv, a, stream);
   }
 
+  BatchSequence KVPages::batch_sequence(int layer, int seq_k, int kv_heads, int head_dim,
+                                        const std::uint16_t *key, const std::uint16_t *value)
+  {
+    require_layer(layer);
+    if (kv_heads != kv_heads_ || head_dim != head_dim_)
+    {
+      throw InvalidArgument("the batch's sequences have " + std::to_string(kv_heads) +
+                            " KV heads of " + std::to_string(head_dim) + "; this cache holds " +
+                            std::to_string(kv_heads_) + " of " + std::to_string(head_dim_));
+    }
+    if (seq_k < 0 || seq_k > capacity_tokens())
+    {
+      throw OutOfRange("seq_k " + std::to_string(seq_k) + " exceeds the " +
+                       std::to_string(capacity_tokens()) + " positions on pages");
+    }
+    BatchSequence s{};
+    if (seq_k == 0)
+    {
+      return s;
+    }
+    if (seals_ && (key == nullptr || value == nullptr))
+    {
+      throw InvalidArgument("attention at a quantised tier reads each query's own page from the "
+                            "rows the queries stored; pass them");
+    }
+    if (seals_ && !open_pages_)
+    {
+      throw LogicError("attention before any position was reserved");
+    }
+    sync_tables(runtime_stream());
+    const std::size_t row = static_cast<std::size_t>(layer) * table_.stride();
+    s.length = seq_k;
+    if (pages_ > 0)
+    {
+      s.pages = table_.addresses() + row;
+      s.tiers = table_.tiers() + row;
+    }
+    if (seals_)
+    {
+      s.open = open_page(layer, attend_open_[layer]);
+      s.own_k = key;
+      s.own_v = value;
+    }
+    return s;
+  }
+
   void KVPages::attention_kept(int layer, const void *q, const void *k_bias,
                                const RopeTable *rope, void *out, int seq_k, int heads,
                                int kv_heads, int head_dim, const void *keys, const void *values)

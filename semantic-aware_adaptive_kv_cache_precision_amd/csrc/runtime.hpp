@@ -588,6 +588,12 @@ namespace mi
                         const void *keys, const void *values);
     void fold_kept(float *mass, long long mass_stride, float *scores, long long scores_stride,
                    float alpha);
+    // Beyond the reference: this cache as one sequence of a batch's decode
+    // (launch_batch_attention), its token at position seq_k - 1 (seq_k 0: no
+    // token). A cache that seals reads the token's row from key and value
+    // (kv_width fp16 each). Good until the cache's next call.
+    BatchSequence batch_sequence(int layer, int seq_k, int kv_heads, int head_dim,
+                                 const std::uint16_t *key, const std::uint16_t *value);
     // Beyond the reference: the pieces of a decode step whose position lives
     // on the device, so that one captured graph serves every step of a run.
     // store_step stores one row at *position (sealing the page it

@@ -76,6 +76,11 @@ SIGNATURES = {
     "mi_device_count": ((_ip,), C.c_int), "mi_device_name": ((C.c_char_p, _sz), C.c_int),
     "mi_runtime_version": ((_ip,), C.c_int),
     "mi_host_alloc": ((C.POINTER(_vp), C.POINTER(_vp), _sz), C.c_int),
+    "mi_attention_batch_partials": ((_i, _i, _i, _i, _i, _i, _i, _i, _szp), C.c_int),
+    "mi_attention_batch": ((_vp, _vp, _vp, _vp, _i, _i, _i, _vp, _i, _i, _i, _i, _i, _vp, _vp, _sz,
+                            _vp), C.c_int),
+    "mi_kv_attention_batch": ((C.POINTER(_vp), _ip, _i, _i, _vp, _vp, _i, _i, _i, _vp, _vp, _i, _i,
+                               _vp, _i, _vp, _sz), C.c_int),
     "mi_kv_store_at": ((_vp, _i, _vp, _vp, _vp), C.c_int),
     "mi_kv_attention_at": ((_vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp), C.c_int),
     "mi_kv_stored_on_device": ((_vp, _i), C.c_int),
@@ -1351,6 +1356,85 @@ def _device_attention(q, k, v, k_bias, rope_table, out, seq_q, seq_k, heads, kv_
                             head_dim, pa, None))
 
 
+@functools.lru_cache(maxsize=256, typed=True)
+def _attention_batch_partials(batch: int, max_pages: int, heads: int, kv_heads: int, head_dim: int,
+                              window: int = 0, sinks: int = 0, mass: bool = False) -> int:
+    """Floats of partials attention_batch needs for these sizes."""
+    out = C.c_size_t()
+    _check(lib.mi_attention_batch_partials(batch, max_pages, heads, kv_heads, head_dim, window,
+                                           sinks, int(bool(mass)), C.byref(out)))
+    return out.value
+
+
+def _entries(x) -> int:
+    """The elements of a device array of any type."""
+    return x.numel if hasattr(x, "numel") else x.count
+
+
+def _held(x, count: int, what: str) -> int:
+    if _entries(x) < count:
+        raise ValueError(f"{what} holds {_entries(x)}, and the operation needs {count}")
+    return x.address
+
+
+def _batch_sizes(batch, max_pages, heads, head_dim, q, out, mass):
+    """The addresses of a batch's queries, outputs and masses."""
+    _non_negative(batch, "batch")
+    _non_negative(max_pages, "max_pages")
+    per = batch * heads
+    qa = _at(q, per * head_dim, "q")
+    oa = _at(out, per * head_dim, "out")
+    ma = _floats(mass, per * max_pages, "mass") if mass is not None else None
+    return qa, oa, ma
+
+
+def _device_attention_batch(q, pages, tiers, lengths, out, batch, max_pages, heads, kv_heads,
+                            head_dim, window=0, sinks=0, mass=None, partials=None):
+    """Beyond the reference: one token of every sequence of a batch over paged,
+    mixed-precision caches. q and out hold (batch, heads, head_dim) fp16;
+    `pages` (batch, max_pages) 64-bit device addresses of 32-token pages,
+    `tiers` their tiers (bytes; 255: not read) and `lengths` (batch) int32 each
+    sequence's tokens, the query's own counted, all device arrays read when
+    the kernels run. With `window`, a query sees its last `window` tokens and
+    the first `sinks`. `mass` (batch, heads, max_pages) floats takes each
+    page's share of the softmax. `partials` holds attention_batch_partials
+    floats and lets a sequence be read by several workgroups; masses need it."""
+    qa, oa, ma = _batch_sizes(batch, max_pages, heads, head_dim, q, out, mass)
+    pa = _held(pages, batch * max_pages, "pages")
+    ta = _held(tiers, batch * max_pages, "tiers")
+    la = _held(lengths, batch, "lengths")
+    wa, floats = (partials.address, partials.numel) if partials is not None else (None, 0)
+    _check(lib.mi_attention_batch(qa, pa, ta, la, batch, max_pages, P_DEFAULT, oa, heads, kv_heads,
+                                  head_dim, window, sinks, ma, wa, floats, None))
+
+
+def _device_attention_caches(caches, seq_k, layer, q, out, heads, kv_heads, head_dim, keys=None,
+                             values=None, window=0, sinks=0, mass=None, mass_pages=None,
+                             partials=None):
+    """attention_batch over KVPages: the query of caches[i] is at position
+    seq_k[i] - 1 of `layer` (0: no token), stored before; caches that seal
+    read its row from keys and values (len(caches), kv_width). `mass` holds
+    (len(caches), heads, mass_pages) floats, mass_pages the longest sequence's
+    pages where it is not given."""
+    n = len(caches)
+    if len(seq_k) != n:
+        raise ValueError(f"{n} caches and {len(seq_k)} positions")
+    if n == 0:
+        return
+    width = kv_heads * head_dim
+    if mass is None:
+        mass_pages = 0
+    elif mass_pages is None:
+        mass_pages = max(-(-k // P_DEFAULT) for k in seq_k)
+    qa, oa, ma = _batch_sizes(n, mass_pages, heads, head_dim, q, out, mass)
+    ka = _at(keys, n * width, "keys") if keys is not None else None
+    va = _at(values, n * width, "values") if values is not None else None
+    wa, floats = (partials.address, partials.numel) if partials is not None else (None, 0)
+    _check(lib.mi_kv_attention_batch((_vp * n)(*(c._h for c in caches)), (C.c_int * n)(*seq_k), n,
+                                     layer, qa, oa, heads, kv_heads, head_dim, ka, va, window, sinks,
+                                     ma, mass_pages, wa, floats))
+
+
 def _device_rmsnorm(x, weight, out, rows, hidden, eps):
     xa = _at(x, rows * hidden, "x")
     wa = _at(weight, hidden, "weight")
@@ -1648,6 +1732,9 @@ device = SimpleNamespace(
     attention_partials=_attention_partials,
     attention_split=lambda seq_q, seq_k, heads, kv_heads, page_tokens=0: _split(
         seq_q, seq_k, heads, kv_heads, page_tokens),
+    attention_batch=_device_attention_batch,
+    attention_batch_partials=_attention_batch_partials,
+    attention_caches=_device_attention_caches,
     RopeTable=RopeTable,
     add=_device_add,
     swiglu=_device_swiglu,
