@@ -194,6 +194,24 @@ int mi_attention_paged_causal_noalloc(const void *q, const unsigned long long *s
                                       void *out, int seq_k, int heads, int kv_heads, int head_dim,
                                       float *mass, float *scores, float alpha, void *stream);
 
+/* Beyond the reference (whose attention sees every position): a prompt's
+ * queries over contiguous keys and values through a sliding window. q (seq_q,
+ * heads, head_dim) are the last of the seq_k positions of k and v (seq_k,
+ * kv_heads, head_dim), fp16; token strides in elements (0: contiguous), so
+ * that the three may lie in one projection's rows. The query at position p
+ * sees key j <= p where window is 0, or j > p - window, or j < sinks. out
+ * (seq_q, heads, head_dim) contiguous. head_dim 64 or 128, any whole number of
+ * query heads a KV head; rows 16-byte aligned (strides multiples of 8).
+ * partials: mi_attention_window_partials floats, the caller's until the launch
+ * is done, which let few rows' keys be split over the device; or NULL. Calls
+ * that may overlap need partials of their own. */
+int mi_attention_window_partials(int seq_q, int seq_k, int heads, int kv_heads, int head_dim,
+                                 int window, int sinks, size_t *floats);
+int mi_attention_window(const void *q, const void *k, const void *v, void *out, long long q_stride,
+                        long long k_stride, long long v_stride, int seq_q, int seq_k, int heads,
+                        int kv_heads, int head_dim, int window, int sinks, float *partials,
+                        size_t partials_floats, void *stream);
+
 /* ---- pages, rows and scores ----------------------------------------------
  * reference: page_copy.cu:41-70, kv_pages.cu:47-60, importance_scores.cu:18-50. */
 int mi_copy_pages(const void *const *from, void *const *to, size_t bytes, int count, void *stream);

@@ -21,16 +21,23 @@ def visible(position: int, keys: int, window: int, sinks: int) -> np.ndarray:
 
 def window_attention(q, k, v, window: int, sinks: int):
     """q (seq_q, heads, hd), the last of k, v (seq_k, kv, hd)'s positions.
-    Returns (out, bound), bound as attention_bound's."""
-    seq_q, seq_k = len(q), len(k)
-    out, bound = np.zeros(np.shape(q)), np.zeros(np.shape(q))
-    for i in range(seq_q):
-        at = seq_k - seq_q + i
-        seen = visible(at, seq_k, window, sinks)
-        ki, vi = np.asarray(k, np.float64)[seen], np.asarray(v, np.float64)[seen]
-        out[i:i + 1], w = att.attention64(q[i:i + 1], ki, vi)
-        bound[i:i + 1] = att.attention_bound(q[i:i + 1], ki, vi, w)
-    return out, bound
+    Returns (out, bound, terms): bound as attention_bound's, terms the sums of
+    p |v|, which a relative error of every weight weighs."""
+    q, k, v = (np.asarray(x, np.float64) for x in (q, k, v))
+    seq_q, heads, hd = q.shape
+    seq_k, group = len(k), heads // k.shape[1]
+    seen = np.stack([visible(seq_k - seq_q + i, seq_k, window, sinks) for i in range(seq_q)])
+    out, bound, terms = np.zeros(q.shape), np.zeros(q.shape), np.zeros(q.shape)
+    for h in range(heads):
+        kh, vh = k[:, h // group], v[:, h // group]
+        s = np.where(seen, q[:, h] @ kh.T / np.sqrt(hd), -np.inf)
+        p = np.exp(s - s.max(1, keepdims=True))
+        p /= p.sum(1, keepdims=True)
+        out[:, h], terms[:, h] = p @ vh, p @ np.abs(vh)
+        size = np.where(seen, np.abs(q[:, h]) @ np.abs(kh).T / np.sqrt(hd), 0.0).max(1)
+        bound[:, h] = ((np.sqrt(seen.sum(1)) + np.sqrt(hd) * size)[:, None] *
+                       att.FP32_REL_ULP * terms[:, h])
+    return out, bound, terms
 
 
 def paged_token(q, k, v, length: int, unread, window: int, sinks: int, page_tokens: int):

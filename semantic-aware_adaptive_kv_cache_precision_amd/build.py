@@ -22,9 +22,8 @@ ARCH = os.environ.get("MI_OFFLOAD_ARCH", "gfx950")
 
 SOURCES = ["quant.hip", "page_jobs.hip", "pages.hip", "pointwise.hip", "attention.hip",
            "decode.hip", "prefill.hip", "chunk.hip", "dense.hip", "step.hip", "int4.hip", "batch.hip",
-           "linear.cpp",
-           "page_allocator.cpp", "shadow_store.cpp", "scores_rope.cpp", "kv_cache.cpp",
-           "decode_step.cpp", "capi.cpp"]
+           "window.hip", "linear.cpp", "page_allocator.cpp", "shadow_store.cpp",
+           "scores_rope.cpp", "kv_cache.cpp", "decode_step.cpp", "capi.cpp"]
 ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 # The dense projections call hipBLASLt.
 LIBS = [f"-L{ROCM / 'lib'}", f"-Wl,-rpath,{ROCM / 'lib'}", "-lhipblaslt"]

@@ -1299,6 +1299,36 @@ int mi_kv_attention_layers(mi_kv_pages *kv, int first_layer, int layers, const v
   });
 }
 
+int mi_attention_window_partials(int seq_q, int seq_k, int heads, int kv_heads, int head_dim,
+                                 int window, int sinks, size_t *floats)
+{
+  return guarded([&] {
+    need(floats, "floats");
+    mi::WindowAttention t{};
+    t.seq_q = seq_q;
+    t.seq_k = seq_k;
+    t.heads = heads;
+    t.kv_heads = kv_heads;
+    t.head_dim = head_dim;
+    t.window = window;
+    t.sinks = sinks;
+    *floats = mi::window_attention_floats(t);
+  });
+}
+
+int mi_attention_window(const void *q, const void *k, const void *v, void *out, long long q_stride,
+                        long long k_stride, long long v_stride, int seq_q, int seq_k, int heads,
+                        int kv_heads, int head_dim, int window, int sinks, float *partials,
+                        size_t partials_floats, void *stream)
+{
+  return guarded([&] {
+    const mi::WindowAttention t{q,        k,     v,        out,      q_stride, k_stride,
+                                v_stride, seq_q, seq_k,    heads,    kv_heads, head_dim,
+                                window,   sinks, partials, partials_floats};
+    mi::launch_window_attention(t, as_stream(stream));
+  });
+}
+
 int mi_attention_batch_partials(int batch, int max_pages, int heads, int kv_heads, int head_dim,
                                 int window, int sinks, int with_mass, size_t *floats)
 {

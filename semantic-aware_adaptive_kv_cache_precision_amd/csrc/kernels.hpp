@@ -653,4 +653,29 @@ namespace mi
   std::size_t batch_attention_floats(const BatchAttention &t, bool with_mass);
   void launch_batch_attention(const BatchAttention &t, hipStream_t stream);
 
+  // ---- a prompt through a sliding window (window.hip) --------------------------------
+  struct WindowAttention
+  {
+    const void *q; // (seq_q, heads, head_dim) fp16, the last of k's positions
+    const void *k; // (seq_k, kv_heads, head_dim)
+    const void *v;
+    void *out; // (seq_q, heads, head_dim), contiguous
+    long long q_stride; // elements between tokens; 0: contiguous
+    long long k_stride;
+    long long v_stride;
+    int seq_q;
+    int seq_k;
+    int heads;
+    int kv_heads;
+    int head_dim;
+    int window; // the last tokens visible, the query's own counted; 0: every one
+    int sinks;  // the first tokens visible beside a window's
+    // Null: no row's keys are split over workgroups; else at least
+    // window_attention_floats, used until the launch is done.
+    float *partials;
+    std::size_t partials_floats;
+  };
+  std::size_t window_attention_floats(const WindowAttention &t);
+  void launch_window_attention(const WindowAttention &t, hipStream_t stream);
+
 } // namespace mi

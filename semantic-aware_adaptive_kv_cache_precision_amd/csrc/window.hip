@@ -1,0 +1,731 @@
+// Attention of a prompt's queries over contiguous keys and values, causal,
+// through a sliding window with the first `sinks` tokens kept visible.
+//
+// Query i of seq_q is at position p = seq_k - seq_q + i and sees key j <= p if
+// there is no window, or j > p - window, or j < sinks. out = softmax(q . k /
+// sqrt(hd)) v over those; every query sees itself at least.
+//
+// A workgroup takes one KV head and consecutive (query, head) rows of its
+// group, query by query, so that its rows' windows nearly coincide; 32 * RT
+// rows a wave. Steps of kKeys keys, of which only those some row of the
+// workgroup sees are taken (the sink steps, then the window's), pass through
+// LDS, double buffered, copied there directly from memory. In the matrix
+// cores' terms, with keys as M and rows as N:
+//   S^T (32 keys x 32 rows) = K . Q^T      lane l holds row l % 32
+//   O^T (32 channels x 32 rows) += V^T . P^T  P from the lane's own scores,
+//                                             V^T by transposing LDS reads
+// so that the softmax stays in a lane but for one exchange with lane ^ 32.
+//
+// A key or value in LDS lies in 16-byte pieces, piece c of row t at place
+// c ^ swizzle(t) of its row: the 16 lanes that read one piece of 16 rows, and
+// the 32 lanes that a transposing read serves at a time (four rows, four
+// pieces), meet no bank twice.
+//
+// P is rounded to fp16 once (half a step is 2^-11 of a weight, as much as the
+// output's own rounding; the sums are of the unrounded weights), held against
+// a reference that is moved up only when a score passes it by 2^kRise: P is at
+// most 2^(kRise + kProb) = 2^14, and a weight keeps its 11 bits down to 2^-22
+// of the reference.
+//
+// With few rows the range of keys is split over workgroups, whose parts a
+// second launch joins.
+
+#include "common.hpp"
+#include "kernels.hpp"
+#include "lane_ops.hpp"
+
+#include <algorithm>
+#include <cmath>
+#include <string>
+
+namespace mi
+{
+  namespace
+  {
+    typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+    typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+    typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+    typedef float f32x16 __attribute__((ext_vector_type(16)));
+    typedef float f32x4 __attribute__((ext_vector_type(4)));
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+    typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+    typedef short i16x4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) i16x4 *lds_i16x4;
+    typedef __attribute__((address_space(3))) void *lds_void;
+    typedef const __attribute__((address_space(1))) void *global_void;
+
+    constexpr float kRise = 6.0f;
+    constexpr float kProb = 8.0f; // P x 2^8
+    constexpr float kProbUnscale = 1.0f / 256.0f;
+    constexpr int kMaxSplits = 256;
+
+    struct WindowArgs
+    {
+      const std::uint16_t *q;
+      const std::uint16_t *k;
+      const std::uint16_t *v;
+      std::uint16_t *out;
+      long long q_stride; // elements between tokens
+      long long k_stride;
+      long long v_stride;
+      int seq_q;
+      int seq_k;
+      int heads;
+      int kv_heads;
+      int group;
+      int window; // 0: none
+      int sinks;
+      int splits;
+      float scale;    // log2 e / sqrt(hd)
+      float *part_ml; // splits > 1: [split][row] maximum and sum (row = query * heads + head),
+      float *part_o;  // and hd outputs
+    };
+
+    __device__ inline half8 as_half8(u32x4 v) { return __builtin_bit_cast(half8, v); }
+
+    __device__ inline f32x16 mfma32(half8 a, half8 b, f32x16 c)
+    {
+      return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    }
+
+    // The place of piece c of row t (see above): for rows of 8 pieces two rows
+    // span the banks, so rows differ by t / 2; bits reversed, so that rows 0-3
+    // of a transposing read differ in the bits its four pieces do not use.
+    template <int HD>
+    __device__ inline int swizzle(int t)
+    {
+      if constexpr (HD == 64)
+      {
+        const int u = t >> 1;
+        return ((u & 1) << 2) | (u & 2) | ((u >> 2) & 1);
+      }
+      else
+      {
+        return ((t & 1) << 3) | ((t & 2) << 1) | ((t >> 1) & 2) | ((t >> 3) & 1);
+      }
+    }
+
+    // Four keys of the lane's channel: the 16 lanes of a row group address
+    // four rows' 16 channels (lane s: row s / 4, channels 4 (s % 4) ..) and
+    // lane s receives channel s of the four.
+    __device__ inline half4 transposed(const std::uint16_t *p)
+    {
+      return __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)(p)));
+    }
+
+    __device__ inline bool is_finite(std::uint16_t v) { return (v & 0x7c00u) != 0x7c00u; }
+
+    // Zeros where a value is not finite.
+    __device__ inline half8 finite_only(half8 v)
+    {
+      u32x4 bits = __builtin_bit_cast(u32x4, v);
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+      {
+        const unsigned word = bits[w];
+        bits[w] = (is_finite(static_cast<std::uint16_t>(word)) ? word & 0xFFFFu : 0u) |
+                  (is_finite(static_cast<std::uint16_t>(word >> 16)) ? word & 0xFFFF0000u : 0u);
+      }
+      return as_half8(bits);
+    }
+
+    // Whether every value of a step is finite.
+    template <int HD, int kKeys>
+    __device__ inline bool finite_values(const std::uint16_t *values, int lane)
+    {
+      bool fine = true;
+#pragma unroll 4
+      for (int i = 0; i < kKeys * HD / 512; ++i)
+      {
+        const u32x4 x = *reinterpret_cast<const u32x4 *>(values + 512 * i + 8 * lane);
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+        {
+          const unsigned word = x[w];
+          fine = fine && is_finite(static_cast<std::uint16_t>(word)) &&
+                 is_finite(static_cast<std::uint16_t>(word >> 16));
+        }
+      }
+      return __all(fine);
+    }
+
+    // A wave's 32 rows: weights are 2^(score - m), l is their sum, o x 2^kProb.
+    template <int HD>
+    struct Rows
+    {
+      float m;
+      float l;
+      f32x16 o[HD / 32];
+    };
+
+    // The keys of steps: [0, sink_steps) and from `first` on.
+    struct Steps
+    {
+      int sink_steps;
+      int first; // the window's first step
+      int count;
+      __device__ int key(int i, int keys) const
+      {
+        return (i < sink_steps ? i : first + i - sink_steps) * keys;
+      }
+    };
+
+    template <int HD, int RT, int NW, int kKeys>
+    __global__ void __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) window_kernel(WindowArgs a)
+    {
+      constexpr int kPieces = HD / 8;          // 16-byte pieces a row
+      constexpr int kTile = kKeys * HD;        // halves of a step's keys
+      constexpr int kStage = 2 * kTile;        // keys, then values
+      constexpr int kRows = 32 * RT * NW;      // rows a workgroup
+      constexpr int N = kKeys / 32;
+      extern __shared__ __align__(16) std::uint16_t stages[]; // two of kStage
+
+      const int lane = threadIdx.x & 63;
+      const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+      const int n = lane & 31;
+      const int half = lane >> 5;
+      const int kvh = blockIdx.y;
+      const int split = blockIdx.z;
+      const int G = a.group;
+      const int past = a.seq_k - a.seq_q;
+      const long long all_rows = static_cast<long long>(a.seq_q) * G;
+      const long long row0 = static_cast<long long>(blockIdx.x) * kRows;
+
+      // The workgroup's positions, and the steps they see.
+      const int lo_pos = past + static_cast<int>(row0 / G);
+      const int hi_pos = past + static_cast<int>((min(row0 + kRows, all_rows) - 1) / G);
+      Steps steps{0, 0, 0};
+      if (a.window > 0 && a.window <= lo_pos)
+      {
+        steps.first = (lo_pos - a.window + 1) / kKeys;
+        steps.sink_steps = min(a.sinks / kKeys + (a.sinks % kKeys > 0 ? 1 : 0), steps.first);
+      }
+      steps.count = steps.sink_steps + hi_pos / kKeys + 1 - steps.first;
+      const int per = (steps.count + a.splits - 1) / a.splits;
+      const int begin = min(split * per, steps.count);
+      const int end = min(begin + per, steps.count);
+
+      bool valid[RT];
+      int pos[RT];
+      std::size_t row_at[RT]; // query * heads + head
+      half8 q[RT][HD / 16];
+      Rows<HD> run[RT];
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+      {
+        const long long row = row0 + 32 * (RT * wave + t) + n;
+        valid[t] = row < all_rows;
+        const int query = valid[t] ? static_cast<int>(row / G) : 0;
+        const int head = kvh * G + (valid[t] ? static_cast<int>(row % G) : 0);
+        pos[t] = past + query;
+        row_at[t] = static_cast<std::size_t>(query) * a.heads + head;
+        const std::uint16_t *from = a.q + query * a.q_stride + head * HD + 8 * half;
+#pragma unroll
+        for (int c = 0; c < HD / 16; ++c)
+        {
+          q[t][c] = as_half8(*reinterpret_cast<const u32x4 *>(from + 16 * c));
+        }
+        run[t].m = -INFINITY;
+        run[t].l = 0.0f;
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d)
+        {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+          {
+            run[t].o[d][i] = 0.0f;
+          }
+        }
+      }
+      // The wave's positions (a wave past the rows computes nothing).
+      const long long wave_row = row0 + 32 * RT * wave;
+      const bool computes = wave_row < all_rows;
+      const int wave_lo = past + static_cast<int>(min(wave_row, all_rows - 1) / G);
+      const int wave_hi = past + static_cast<int>((min(wave_row + 32 * RT, all_rows) - 1) / G);
+
+      // A step's rows to LDS, 16 bytes a lane; rows past the last repeat it.
+      const auto copy = [&](int step, int buf) {
+        const int key0 = steps.key(step, kKeys);
+        std::uint16_t *stage = stages + buf * kStage;
+#pragma unroll
+        for (int i = 0; i < kTile / 8 / (64 * NW); ++i)
+        {
+          const int place = (i * NW + wave) * 64 + lane;
+          const int t = place / kPieces;
+          const int c = (place % kPieces) ^ swizzle<HD>(t);
+          const long long row = min(key0 + t, a.seq_k - 1);
+          std::uint16_t *to = stage + (i * NW + wave) * 512;
+          __builtin_amdgcn_global_load_lds(
+              (global_void)(a.k + row * a.k_stride + kvh * HD + 8 * c), (lds_void)(to), 16, 0, 0);
+          __builtin_amdgcn_global_load_lds(
+              (global_void)(a.v + row * a.v_stride + kvh * HD + 8 * c), (lds_void)(to + kTile), 16,
+              0, 0);
+        }
+      };
+      if (begin < end)
+      {
+        copy(begin, 0);
+      }
+      for (int step = begin; step < end; ++step)
+      {
+        const int buf = (step - begin) & 1;
+        // This step's copies have landed (a wave waits for its own before the
+        // barrier), and every wave is done with the other buffer.
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_s_waitcnt(0x0F70); // vmcnt(0)
+        __syncthreads();
+        if (step + 1 < end)
+        {
+          copy(step + 1, buf ^ 1);
+        }
+        const int key0 = steps.key(step, kKeys);
+        const bool sees = key0 <= wave_hi &&
+                          (a.window == 0 || key0 + kKeys - 1 > wave_lo - a.window ||
+                           key0 < a.sinks);
+        if (!computes || !sees)
+        {
+          continue;
+        }
+        const std::uint16_t *keys = stages + buf * kStage;
+        const std::uint16_t *values = keys + kTile;
+        f32x16 s[RT][N];
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+        {
+#pragma unroll
+          for (int j = 0; j < N; ++j)
+          {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+            {
+              s[t][j][i] = 0.0f;
+            }
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < HD / 16; ++c)
+        {
+#pragma unroll
+          for (int j = 0; j < N; ++j)
+          {
+            const int t0 = 32 * j + n;
+            const half8 k = as_half8(*reinterpret_cast<const u32x4 *>(
+                keys + t0 * HD + 8 * ((2 * c + half) ^ swizzle<HD>(t0))));
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+            {
+              s[t][j] = mfma32(k, q[t][c], s[t][j]);
+            }
+          }
+        }
+        // Whether some row of the wave does not see some key of the step.
+        const bool edge = key0 + kKeys - 1 > wave_lo ||
+                          (a.window > 0 && key0 <= wave_hi - a.window &&
+                           key0 + kKeys > a.sinks);
+        if (edge)
+        {
+#pragma unroll
+          for (int t = 0; t < RT; ++t)
+          {
+            const int from = a.window > 0 ? pos[t] - a.window : -1; // keys after it are seen
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+            {
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+              {
+                const int key = key0 + 32 * j + 8 * (i / 4) + 4 * half + i % 4;
+                const bool seen = key <= pos[t] && (key > from || key < a.sinks);
+                s[t][j][i] = seen ? s[t][j][i] : -INFINITY;
+              }
+            }
+          }
+        }
+        half8 p[RT][N][2];
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+        {
+          float top = s[t][0][0];
+#pragma unroll
+          for (int j = 0; j < N; ++j)
+          {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+            {
+              top = fmaxf(top, s[t][j][i]);
+            }
+          }
+          top = lane_max32(top) * a.scale;
+          if (__any(top > run[t].m + kRise))
+          {
+            const float m = fmaxf(run[t].m, top);
+            const float keep = run[t].m == m ? 1.0f : __builtin_amdgcn_exp2f(run[t].m - m);
+            run[t].m = m;
+            run[t].l *= keep;
+#pragma unroll
+            for (int d = 0; d < HD / 32; ++d)
+            {
+              run[t].o[d] *= keep;
+            }
+          }
+          const float from = (run[t].m == -INFINITY ? 0.0f : run[t].m) - kProb;
+          float sum = 0.0f;
+#pragma unroll
+          for (int j = 0; j < N; ++j)
+          {
+#pragma unroll
+            for (int i = 0; i < 16; i += 2)
+            {
+              const f32x2 w = {
+                  __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][j][i], a.scale, -from)),
+                  __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][j][i + 1], a.scale, -from))};
+              sum += w[0] + w[1];
+              const half2v h = __builtin_convertvector(w, half2v);
+              p[t][j][i / 8][i % 8] = h[0];
+              p[t][j][i / 8][i % 8 + 1] = h[1];
+            }
+          }
+          run[t].l += sum;
+        }
+        // A value some row does not see may be anything: if one of an edge
+        // step's is not finite, the products take it as zero, and the rows
+        // that do see it add it after them.
+        const bool spoilt = edge && !finite_values<HD, kKeys>(values, lane);
+        // Lane l's P of a 16-key product: keys 8 e + 4 half + {0..3}, e = 0, 1.
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+        {
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+          {
+#pragma unroll
+            for (int d = 0; d < HD / 32; ++d)
+            {
+              half8 vt;
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+              {
+                const int t0 = 32 * j + 16 * u + 8 * e + 4 * half + (lane % 16) / 4;
+                const int ch = 32 * d + 16 * ((lane / 16) & 1) + 4 * (lane % 4);
+                const half4 x = transposed(values + t0 * HD +
+                                           8 * ((ch / 8) ^ swizzle<HD>(t0)) + ch % 8);
+                vt[4 * e] = x[0];
+                vt[4 * e + 1] = x[1];
+                vt[4 * e + 2] = x[2];
+                vt[4 * e + 3] = x[3];
+              }
+              if (spoilt)
+              {
+                vt = finite_only(vt);
+              }
+#pragma unroll
+              for (int t = 0; t < RT; ++t)
+              {
+                run[t].o[d] = mfma32(vt, p[t][j][u], run[t].o[d]);
+              }
+            }
+          }
+        }
+        if (spoilt)
+        {
+          for (int key = key0; key < min(key0 + kKeys, a.seq_k); ++key)
+          {
+            const std::uint16_t *row = values + (key - key0) * HD;
+            const int swap = swizzle<HD>(key - key0);
+#pragma unroll
+            for (int d = 0; d < HD / 32; ++d)
+            {
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+              {
+                const int ch = 32 * d + 8 * (i / 4) + 4 * half + i % 4;
+                const std::uint16_t v = row[8 * ((ch / 8) ^ swap) + ch % 8];
+#pragma unroll
+                for (int t = 0; t < RT; ++t)
+                {
+                  const bool seen = key <= pos[t] && (a.window == 0 || key > pos[t] - a.window ||
+                                                      key < a.sinks);
+                  run[t].o[d][i] += seen && !is_finite(v) ? h2f(v) : 0.0f;
+                }
+              }
+            }
+          }
+        }
+      }
+
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+      {
+        const float sum = lane_sum32(run[t].l) * kProbUnscale;
+        if (!valid[t])
+        {
+          continue;
+        }
+        if (a.splits == 1)
+        {
+          const float inv = kProbUnscale / sum;
+          std::uint16_t *out = a.out + row_at[t] * HD + 4 * half;
+#pragma unroll
+          for (int d = 0; d < HD / 32; ++d)
+          {
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+            {
+              const f32x16 &o = run[t].o[d];
+              const half2v x = {static_cast<_Float16>(o[4 * b] * inv),
+                                static_cast<_Float16>(o[4 * b + 1] * inv)};
+              const half2v y = {static_cast<_Float16>(o[4 * b + 2] * inv),
+                                static_cast<_Float16>(o[4 * b + 3] * inv)};
+              *reinterpret_cast<u32x2 *>(out + 32 * d + 8 * b) =
+                  u32x2{__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, y)};
+            }
+          }
+          continue;
+        }
+        const std::size_t at =
+            static_cast<std::size_t>(split) * a.seq_q * a.heads + row_at[t];
+        if (half == 0)
+        {
+          *reinterpret_cast<f32x2 *>(a.part_ml + 2 * at) = f32x2{run[t].m, sum};
+        }
+        float *out = a.part_o + at * HD + 4 * half;
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d)
+        {
+#pragma unroll
+          for (int b = 0; b < 4; ++b)
+          {
+            f32x4 x;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+            {
+              x[i] = run[t].o[d][4 * b + i] * kProbUnscale;
+            }
+            *reinterpret_cast<f32x4 *>(out + 32 * d + 8 * b) = x;
+          }
+        }
+      }
+    }
+
+    // The splits of a (query, head) row joined, four channels a thread.
+    template <int HD>
+    __global__ void __launch_bounds__(256) window_join_kernel(WindowArgs a, std::size_t rows)
+    {
+      constexpr int kLanes = HD / 4;
+      const std::size_t i = static_cast<std::size_t>(blockIdx.x) * 256 + threadIdx.x;
+      const std::size_t row = i / kLanes;
+      const int d = 4 * static_cast<int>(i % kLanes);
+      if (row >= rows)
+      {
+        return;
+      }
+      float top = -INFINITY;
+#pragma unroll 4
+      for (int s = 0; s < a.splits; ++s)
+      {
+        top = fmaxf(top, a.part_ml[2 * (s * rows + row)]);
+      }
+      const float from = top == -INFINITY ? 0.0f : top;
+      float sum = 0.0f;
+      f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+      for (int s = 0; s < a.splits; ++s)
+      {
+        const f32x2 ml = *reinterpret_cast<const f32x2 *>(a.part_ml + 2 * (s * rows + row));
+        const f32x4 o = *reinterpret_cast<const f32x4 *>(a.part_o + (s * rows + row) * HD + d);
+        const float w = __builtin_amdgcn_exp2f(ml[0] - from);
+        sum += ml[1] * w;
+        acc += o * w;
+      }
+      const half2v x = {static_cast<_Float16>(acc[0] / sum), static_cast<_Float16>(acc[1] / sum)};
+      const half2v y = {static_cast<_Float16>(acc[2] / sum), static_cast<_Float16>(acc[3] / sum)};
+      *reinterpret_cast<u32x2 *>(a.out + row * HD + d) =
+          u32x2{__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, y)};
+    }
+
+    // How a launch is cut: the rows and keys of a workgroup's tile, and the
+    // workgroups a row's keys are split over.
+    struct Cut
+    {
+      bool few; // a wave of 32 rows a workgroup, 32 keys a step
+      int rows;
+      int keys;
+      int blocks; // workgroups over the rows, a KV head
+      int splits;
+    };
+
+    constexpr int kFewRows = 32, kFewKeys = 32, kManyKeys = 64, kManyWaves = 4;
+    template <int HD>
+    constexpr int kRowTiles = HD == 64 ? 2 : 1;
+
+    Cut cut_of(const WindowAttention &t, bool may_split)
+    {
+      const int group = t.heads / t.kv_heads;
+      const long long rows = static_cast<long long>(t.seq_q) * group;
+      Cut c{};
+      const long long few = (rows + kFewRows - 1) / kFewRows;
+      c.few = few * t.kv_heads <= 512;
+      const int tiles = t.head_dim == 64 ? kRowTiles<64> : kRowTiles<128>;
+      c.rows = c.few ? kFewRows : 32 * tiles * kManyWaves;
+      c.keys = c.few ? kFewKeys : kManyKeys;
+      c.blocks = static_cast<int>((rows + c.rows - 1) / c.rows);
+      c.splits = 1;
+      if (may_split && c.blocks > 0)
+      {
+        // The most steps a workgroup takes.
+        long long steps = (t.seq_k + c.keys - 1) / c.keys;
+        if (t.window > 0)
+        {
+          const long long span = static_cast<long long>(t.window) + (c.rows - 1) / group + 1;
+          steps = std::min(steps, (span + c.keys - 1) / c.keys + 1 +
+                                      (static_cast<long long>(t.sinks) + c.keys - 1) / c.keys);
+        }
+        // Four workgroups of a wave, or one of four, a CU, each with four
+        // steps to take.
+        const long long fill = (c.few ? 1024 : 256) / (static_cast<long long>(c.blocks) * t.kv_heads);
+        c.splits = static_cast<int>(
+            std::max<long long>(1, std::min<long long>({fill, steps / 4, kMaxSplits})));
+      }
+      return c;
+    }
+
+    void check_window(const WindowAttention &t)
+    {
+      if (t.seq_q < 0 || t.seq_k < 0 || t.window < 0 || t.sinks < 0)
+      {
+        throw InvalidArgument("seq_q, seq_k, window and sinks must not be negative, got " +
+                              std::to_string(t.seq_q) + ", " + std::to_string(t.seq_k) + ", " +
+                              std::to_string(t.window) + ", " + std::to_string(t.sinks));
+      }
+      if (t.seq_q > t.seq_k)
+      {
+        throw InvalidArgument("seq_q " + std::to_string(t.seq_q) + " exceeds seq_k " +
+                              std::to_string(t.seq_k));
+      }
+      constexpr int kMostKeys = 0x7fffff00; // a step's last key stays a position
+      if (t.seq_k > kMostKeys)
+      {
+        throw InvalidArgument("seq_k " + std::to_string(t.seq_k) + " exceeds window attention's " +
+                              std::to_string(kMostKeys));
+      }
+      if (t.head_dim != 64 && t.head_dim != 128)
+      {
+        throw InvalidArgument("window attention takes head_dim 64 or 128, got " +
+                              std::to_string(t.head_dim));
+      }
+      if (t.kv_heads <= 0 || t.heads <= 0 || t.heads % t.kv_heads != 0 || t.kv_heads > 65535)
+      {
+        throw InvalidArgument("window attention takes a whole number of query heads a KV head, got " +
+                              std::to_string(t.heads) + " and " + std::to_string(t.kv_heads));
+      }
+    }
+
+    template <int HD, int RT, int NW, int kKeys>
+    void launch(const WindowArgs &a, const Cut &c, hipStream_t stream)
+    {
+      const std::size_t lds = sizeof(std::uint16_t) * 2 * 2 * kKeys * HD;
+      window_kernel<HD, RT, NW, kKeys>
+          <<<dim3(c.blocks, a.kv_heads, c.splits), 64 * NW, lds, stream>>>(a);
+      hip_check(hipGetLastError(), "window_kernel");
+    }
+
+    template <int HD>
+    void launch_any(const WindowArgs &a, const Cut &c, hipStream_t stream)
+    {
+      if (c.few)
+      {
+        launch<HD, 1, 1, kFewKeys>(a, c, stream);
+      }
+      else
+      {
+        launch<HD, kRowTiles<HD>, kManyWaves, kManyKeys>(a, c, stream);
+      }
+      if (c.splits > 1)
+      {
+        const std::size_t rows = static_cast<std::size_t>(a.seq_q) * a.heads;
+        const std::size_t blocks = (rows * (HD / 4) + 255) / 256;
+        window_join_kernel<HD><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(a, rows);
+        hip_check(hipGetLastError(), "window_join_kernel");
+      }
+    }
+  } // namespace
+
+  std::size_t window_attention_floats(const WindowAttention &t)
+  {
+    check_window(t);
+    const Cut c = cut_of(t, true);
+    return c.splits > 1 ? static_cast<std::size_t>(c.splits) * t.seq_q * t.heads * (t.head_dim + 2)
+                        : 0;
+  }
+
+  void launch_window_attention(const WindowAttention &t, hipStream_t stream)
+  {
+    check_window(t);
+    if (t.seq_q == 0)
+    {
+      return;
+    }
+    if (t.q == nullptr || t.k == nullptr || t.v == nullptr || t.out == nullptr)
+    {
+      throw InvalidArgument("window attention needs q, k, v and out");
+    }
+    const long long width = static_cast<long long>(t.kv_heads) * t.head_dim;
+    const long long q_width = static_cast<long long>(t.heads) * t.head_dim;
+    const long long q_stride = t.q_stride > 0 ? t.q_stride : q_width;
+    const long long k_stride = t.k_stride > 0 ? t.k_stride : width;
+    const long long v_stride = t.v_stride > 0 ? t.v_stride : width;
+    if (t.q_stride < 0 || t.k_stride < 0 || t.v_stride < 0 || q_stride < q_width ||
+        k_stride < width || v_stride < width)
+    {
+      throw InvalidArgument("window attention's strides are of a token's " +
+                            std::to_string(q_width) + " query and " + std::to_string(width) +
+                            " key and value elements at least (0: those); got " +
+                            std::to_string(t.q_stride) + ", " + std::to_string(t.k_stride) +
+                            " and " + std::to_string(t.v_stride));
+    }
+    if ((reinterpret_cast<std::uintptr_t>(t.q) | reinterpret_cast<std::uintptr_t>(t.k) |
+         reinterpret_cast<std::uintptr_t>(t.v) | reinterpret_cast<std::uintptr_t>(t.out) |
+         reinterpret_cast<std::uintptr_t>(t.partials)) % 16 != 0 ||
+        (q_stride | k_stride | v_stride) % 8 != 0)
+    {
+      throw InvalidArgument("window attention's rows and partials must be 16-byte aligned");
+    }
+    if (t.out == t.q)
+    {
+      throw InvalidArgument("window attention cannot write over its queries");
+    }
+    const Cut c = cut_of(t, t.partials != nullptr);
+    if (t.partials != nullptr && t.partials_floats < window_attention_floats(t))
+    {
+      throw InvalidArgument("window attention's partials need " +
+                            std::to_string(window_attention_floats(t)) + " floats; got " +
+                            std::to_string(t.partials_floats));
+    }
+    WindowArgs a{};
+    a.q = static_cast<const std::uint16_t *>(t.q);
+    a.k = static_cast<const std::uint16_t *>(t.k);
+    a.v = static_cast<const std::uint16_t *>(t.v);
+    a.out = static_cast<std::uint16_t *>(t.out);
+    a.q_stride = q_stride;
+    a.k_stride = k_stride;
+    a.v_stride = v_stride;
+    a.seq_q = t.seq_q;
+    a.seq_k = t.seq_k;
+    a.heads = t.heads;
+    a.kv_heads = t.kv_heads;
+    a.group = t.heads / t.kv_heads;
+    a.window = t.window;
+    a.sinks = t.sinks;
+    a.splits = c.splits;
+    a.scale = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(t.head_dim)));
+    if (c.splits > 1)
+    {
+      const std::size_t rows = static_cast<std::size_t>(t.seq_q) * t.heads;
+      a.part_o = t.partials;
+      a.part_ml = t.partials + rows * c.splits * t.head_dim;
+    }
+    t.head_dim == 64 ? launch_any<64>(a, c, stream) : launch_any<128>(a, c, stream);
+  }
+
+} // namespace mi

@@ -76,6 +76,9 @@ SIGNATURES = {
     "mi_device_count": ((_ip,), C.c_int), "mi_device_name": ((C.c_char_p, _sz), C.c_int),
     "mi_runtime_version": ((_ip,), C.c_int),
     "mi_host_alloc": ((C.POINTER(_vp), C.POINTER(_vp), _sz), C.c_int),
+    "mi_attention_window_partials": ((_i, _i, _i, _i, _i, _i, _i, _szp), C.c_int),
+    "mi_attention_window": ((_vp, _vp, _vp, _vp, _ll, _ll, _ll, _i, _i, _i, _i, _i, _i, _i, _vp, _sz,
+                             _vp), C.c_int),
     "mi_attention_batch_partials": ((_i, _i, _i, _i, _i, _i, _i, _i, _szp), C.c_int),
     "mi_attention_batch": ((_vp, _vp, _vp, _vp, _i, _i, _i, _vp, _i, _i, _i, _i, _i, _vp, _vp, _sz,
                             _vp), C.c_int),
@@ -1357,6 +1360,43 @@ def _device_attention(q, k, v, k_bias, rope_table, out, seq_q, seq_k, heads, kv_
 
 
 @functools.lru_cache(maxsize=256, typed=True)
+def _attention_window_partials(seq_q: int, seq_k: int, heads: int, kv_heads: int, head_dim: int,
+                               window: int = 0, sinks: int = 0) -> int:
+    """Floats of partials attention_window uses at these sizes."""
+    out = C.c_size_t()
+    _check(lib.mi_attention_window_partials(seq_q, seq_k, heads, kv_heads, head_dim, window, sinks,
+                                            C.byref(out)))
+    return out.value
+
+
+def _strided(tokens: int, stride: int, width: int) -> int:
+    """The elements `tokens` rows of `width` span, `stride` apart."""
+    return (tokens - 1) * (stride or width) + width if tokens > 0 else 0
+
+
+def _device_attention_window(q, k, v, out, seq_q, seq_k, heads, kv_heads, head_dim, window=0,
+                             sinks=0, q_stride=0, k_stride=0, v_stride=0, partials=None):
+    """Beyond the reference: attention whose query at position p sees the keys
+    (p - window, p] and the first `sinks` (every key up to its own where
+    `window` is 0). q holds the last seq_q of the seq_k positions of k and v;
+    strides are elements between tokens (0: contiguous). `partials`
+    (attention_window_partials floats) lets few rows' keys be split."""
+    for value, what in ((seq_q, "seq_q"), (q_stride, "q_stride"), (k_stride, "k_stride"),
+                        (v_stride, "v_stride")):
+        _non_negative(value, what)
+    if seq_q > seq_k:
+        raise ValueError(f"seq_q {seq_q} exceeds seq_k {seq_k}")
+    width, q_width = kv_heads * head_dim, heads * head_dim
+    qa = _at(q, _strided(seq_q, q_stride, q_width), "q")
+    ka = _at(k, _strided(seq_k, k_stride, width), "k")
+    va = _at(v, _strided(seq_k, v_stride, width), "v")
+    oa = _at(out, seq_q * q_width, "out")
+    wa, floats = (partials.address, partials.numel) if partials is not None else (None, 0)
+    _check(lib.mi_attention_window(qa, ka, va, oa, q_stride, k_stride, v_stride, seq_q, seq_k, heads,
+                                   kv_heads, head_dim, window, sinks, wa, floats, None))
+
+
+@functools.lru_cache(maxsize=256, typed=True)
 def _attention_batch_partials(batch: int, max_pages: int, heads: int, kv_heads: int, head_dim: int,
                               window: int = 0, sinks: int = 0, mass: bool = False) -> int:
     """Floats of partials attention_batch needs for these sizes."""
@@ -1732,6 +1772,8 @@ device = SimpleNamespace(
     attention_partials=_attention_partials,
     attention_split=lambda seq_q, seq_k, heads, kv_heads, page_tokens=0: _split(
         seq_q, seq_k, heads, kv_heads, page_tokens),
+    attention_window=_device_attention_window,
+    attention_window_partials=_attention_window_partials,
     attention_batch=_device_attention_batch,
     attention_batch_partials=_attention_batch_partials,
     attention_caches=_device_attention_caches,

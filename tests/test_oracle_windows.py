@@ -12,7 +12,8 @@ from oracle import windows
 def test_window_attention_is_the_loop(window, sinks):
     rng = np.random.default_rng(window + sinks)
     q, k, v = (rng.standard_normal(s) for s in ((7, 4, 8), (11, 2, 8), (11, 2, 8)))
-    out, _ = windows.window_attention(q, k, v, window, sinks)
+    out, bound, terms = windows.window_attention(q, k, v, window, sinks)
+    assert (terms >= np.abs(out)).all() and (bound > 0).all()
     for i in range(7):
         at = 4 + i
         for h in range(4):
@@ -29,7 +30,7 @@ def test_a_token_is_the_last_query_and_masses_sum_to_one():
     k, v = rng.standard_normal((2, 64, 2, 8))
     for length, window, sinks in ((64, 0, 0), (50, 20, 3), (1, 5, 0)):
         out, mass, _ = windows.paged_token(q[0], k, v, length, np.zeros(64, bool), window, sinks, 16)
-        want, _ = windows.window_attention(q, k[:length], v[:length], window, sinks)
+        want, _, _ = windows.window_attention(q, k[:length], v[:length], window, sinks)
         np.testing.assert_allclose(out, want[0], atol=1e-12)
         np.testing.assert_allclose(mass.sum(1), 1.0)
     out, mass, _ = windows.paged_token(q[0], k, v, 0, np.zeros(64, bool), 0, 0, 16)
