@@ -9,24 +9,32 @@
 // code * scale + zero, not rounded again, so that
 //   y = sum over groups of scale (x . codes) + zero sum(x).
 //
-// linear_int4_kernel. A wave takes tiles of 16 outputs: the matrix cores form
-// x . codes (A: 16 rows of x, B: the codes as fp16 integers, exact) and
-// sum(x) (B: ones) of a group in fp32, 32 inputs an instruction, and two fmas
-// an output scale them. Nothing is rounded before the one rounding of y. A
-// lane reads its row's codes straight from memory, 16 bytes at a time
-// where the group is 128 (8 at 64, 4 at 32: an instruction's four lane groups
-// must lie in one group of the weight); x goes through LDS, a phase of inputs
-// at a time. A code becomes fp16 by the mask that splices it under the
-// exponent of 1024 (or, four bits up, 1024 + 16 code), nine instructions for
-// eight; this leaves them in the order 0 4 1 5 2 6 3 7, in which x is laid in
-// LDS. A tile's inputs are split over up to eight waves, whose sums meet in
-// LDS in wave order: the bits do not depend on timing.
+// Few rows (int4_rows_kernel, up to four): bound by the weight's bytes. A lane
+// takes 32 codes, 16 bytes, of one output; sixteen lanes take 256 bytes of a
+// row and a wave 4 R rows at a time, so that every line is asked for once and
+// whole; v_dot2 multiplies pairs into fp32.
+//
+// More rows (int4_tiles_kernel): the matrix cores form x . codes (A: 16 rows of
+// x, B: 16 outputs' codes as fp16 integers, exact) and sum(x) (B: ones) of 32
+// inputs an instruction in fp32, and two fmas an output scale a group. A lane
+// loads 16 bytes of its output's codes, 32 inputs of the 128 its three
+// neighbours (lane ^ 16, 32, 48) complete; lane swaps transpose the four
+// words, so that an instruction's inputs are 32 in a row: of one group,
+// whatever its size, and a row of x is read 64 bytes at a time.
+//
+// A code becomes fp16 by the mask that splices it under the exponent of 1024
+// (or, four bits up, 1024 + 16 code): nine instructions for eight, which
+// leaves them in the order 0 4 1 5 2 6 3 7; x is turned to that order, once
+// for all the outputs a wave takes. Nothing is rounded before the one
+// rounding of y. An output's inputs are split over up to sixteen waves, whose
+// sums meet in LDS in wave order: the bits do not depend on timing.
 
 #include "kernels.hpp"
 #include "quant_core.hpp"
 
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 namespace mi
 {
@@ -36,7 +44,6 @@ namespace mi
     typedef _Float16 half2v __attribute__((ext_vector_type(2)));
     typedef float f32x4 __attribute__((ext_vector_type(4)));
     typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-    typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
     // ---- the quantiser ------------------------------------------------------
 
@@ -106,12 +113,6 @@ namespace mi
 
     // ---- the projection -----------------------------------------------------
 
-    constexpr int kWaves = 8;
-    constexpr int kThreads = 64 * kWaves;
-    constexpr int kChunk = 128;               // inputs a wave takes at a time
-    constexpr int kStageHalves = 24 * 1024;   // x in LDS: 48 KB, three workgroups a CU
-    constexpr int kRowPad = 8;                // halves: 16 rows a read, no bank twice
-
     enum class Int4Out : int
     {
       kHalf,       // fp16, with the bias if there is one
@@ -129,10 +130,9 @@ namespace mi
       int rows;
       int in;
       int features;
-      int groups;      // a row's
-      int splits;      // waves a tile's inputs are split over: 1, 2, 4 or 8
-      int phase;       // inputs of a phase, whole chunks
-      int row_stride;  // of x in LDS, halves
+      int groups;   // a row's
+      int splits;   // waves an output's inputs are split over, a power of two
+      int group_32; // log2 of a group's runs of 32
     };
 
     // Eight codes, the first in the lowest bits, as fp16 in the order
@@ -155,86 +155,257 @@ namespace mi
       return half8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
     }
 
-    // A wave's part of a chunk of 128 inputs: FT tiles' codes, and the scales
-    // and zeros of the lane's output (row), Words = group / 32.
-    template <int Words, int FT>
-    struct Fetched
+    // Eight inputs in the codes' order.
+    __device__ inline u32x4 turned(u32x4 v)
     {
-      static constexpr int kGroups = 4 / Words;
-      unsigned w[FT][4];
-      std::uint16_t s[FT][kGroups];
-      std::uint16_t z[FT][kGroups];
-    };
+      const unsigned a = v.x, b = v.y, c = v.z, d = v.w;
+      return u32x4{__builtin_amdgcn_perm(c, a, 0x05040100u), __builtin_amdgcn_perm(c, a, 0x07060302u),
+                   __builtin_amdgcn_perm(d, b, 0x05040100u), __builtin_amdgcn_perm(d, b, 0x07060302u)};
+    }
 
-    template <int Words, int FT>
-    __device__ inline void fetch(Fetched<Words, FT> &f, const Int4Args &a, const int (&row)[FT],
-                                 int chunk, int g)
+    // One output, stored. (Added to in memory by its one owner.)
+    template <Int4Out Out>
+    __device__ inline void store(const Int4Args &a, int row, int feature, float y)
     {
-      constexpr int kGroups = 4 / Words;
-#pragma unroll
-      for (int t = 0; t < FT; ++t)
+      const std::size_t to = static_cast<std::size_t>(row) * a.features + feature;
+      if constexpr (Out == Int4Out::kHalf)
       {
-        const std::uint8_t *codes = a.codes + static_cast<std::size_t>(row[t]) * (a.in / 2);
-        const std::size_t meta = static_cast<std::size_t>(row[t]) * a.groups;
-#pragma unroll
-        for (int h = 0; h < kGroups; ++h)
-        {
-          // (Past the row's last group: the first's, multiplied by zeros.)
-          const int group = chunk * kGroups + h;
-          const bool there = group < a.groups;
-          const int at = there ? group : 0;
-          const std::uint8_t *p = codes + (at * (32 * Words) + 8 * Words * g) / 2;
-          if constexpr (Words == 4)
-          {
-            const u32x4 v = *reinterpret_cast<const u32x4 *>(p);
-            f.w[t][0] = v.x;
-            f.w[t][1] = v.y;
-            f.w[t][2] = v.z;
-            f.w[t][3] = v.w;
-          }
-          else if constexpr (Words == 2)
-          {
-            const u32x2 v = *reinterpret_cast<const u32x2 *>(p);
-            f.w[t][2 * h] = v.x;
-            f.w[t][2 * h + 1] = v.y;
-          }
-          else
-          {
-            f.w[t][h] = *reinterpret_cast<const unsigned *>(p);
-          }
-          f.s[t][h] = there ? a.scales[meta + at] : std::uint16_t{0};
-          f.z[t][h] = there ? a.zeros[meta + at] : std::uint16_t{0};
-        }
+        const float bias = a.bias != nullptr ? h2f(a.bias[feature]) : 0.0f;
+        static_cast<std::uint16_t *>(a.out)[to] = __half_as_ushort(__float2half(y + bias));
+      }
+      else
+      {
+        static_cast<float *>(a.out)[to] += y;
       }
     }
 
-    template <int Words, int NT, int FT, Int4Out Out>
-    __global__ void __launch_bounds__(kThreads) linear_int4_kernel(Int4Args a)
+    // ---- up to four rows ----------------------------------------------------
+
+    constexpr int kRowWaves = 8;
+
+    // The sum over the 16 lanes of a row group, in every lane.
+    __device__ inline float row_sum(float v)
     {
-      constexpr int kGroups = 4 / Words;
-      extern __shared__ __align__(16) std::uint16_t x_lds[];
+      const auto turn = [](float x, auto ctrl) {
+        return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(ctrl)::value,
+                                                          0xf, 0xf, true));
+      };
+      v += turn(v, std::integral_constant<int, 0x128>{}); // row_ror:8
+      v += turn(v, std::integral_constant<int, 0x124>{});
+      v += turn(v, std::integral_constant<int, 0x122>{});
+      v += turn(v, std::integral_constant<int, 0x121>{});
+      return v;
+    }
+
+    template <int R>
+    struct RowFetch
+    {
+      u32x4 w[R];
+      std::uint16_t s[R];
+      std::uint16_t z[R];
+    };
+
+    template <int Rows, int R, Int4Out Out>
+    __global__ void __launch_bounds__(64 * kRowWaves) int4_rows_kernel(Int4Args a)
+    {
+      __shared__ float parts[kRowWaves][4 * R * Rows];
+      const int lane = threadIdx.x & 63;
+      const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+      const int f = lane >> 4; // the output of each four
+      const int c = lane & 15; // the run of 32 inputs of each sixteen
+      const int split = wave & (a.splits - 1);
+      const int tile = static_cast<int>(blockIdx.x) * (kRowWaves / a.splits) + wave / a.splits;
+      const int runs = a.in / 32;
+      const int steps = (runs + 15) / 16;
+      const std::uint8_t *codes[R];
+      std::size_t meta[R];
+#pragma unroll
+      for (int u = 0; u < R; ++u)
+      {
+        const int row = min(tile * 4 * R + 4 * u + f, a.features - 1);
+        codes[u] = a.codes + static_cast<std::size_t>(row) * (a.in / 2);
+        meta[u] = static_cast<std::size_t>(row) * a.groups;
+      }
+      const auto fetch = [&](RowFetch<R> &to, int step) {
+        const int run = min(16 * step + c, runs - 1);
+#pragma unroll
+        for (int u = 0; u < R; ++u)
+        {
+          to.w[u] = *reinterpret_cast<const u32x4 *>(codes[u] + 16 * static_cast<std::size_t>(run));
+        }
+#pragma unroll
+        for (int u = 0; u < R; ++u)
+        {
+          to.s[u] = a.scales[meta[u] + (run >> a.group_32)];
+          to.z[u] = a.zeros[meta[u] + (run >> a.group_32)];
+        }
+      };
+      float y[R][Rows] = {};
+      RowFetch<R> next;
+      if (split < steps)
+      {
+        fetch(next, split);
+      }
+#pragma unroll 2
+      for (int step = split; step < steps; step += a.splits)
+      {
+        const RowFetch<R> now = next;
+        fetch(next, min(step + a.splits, steps - 1));
+        const int run = 16 * step + c;
+        u32x4 x[Rows][4];
+        float sum[Rows];
+#pragma unroll
+        for (int r = 0; r < Rows; ++r)
+        {
+          const std::uint16_t *from =
+              a.x + static_cast<std::size_t>(min(r, a.rows - 1)) * a.in + 32 * min(run, runs - 1);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+          {
+            x[r][j] = *reinterpret_cast<const u32x4 *>(from + 8 * j);
+            x[r][j] = run < runs ? turned(x[r][j]) : u32x4{0u, 0u, 0u, 0u};
+          }
+        }
+        const _Float16 one = static_cast<_Float16>(1.0f);
+#pragma unroll
+        for (int r = 0; r < Rows; ++r)
+        {
+          sum[r] = 0.0f;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+          {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+            {
+              const unsigned word = x[r][j][i];
+              sum[r] = __builtin_amdgcn_fdot2(__builtin_bit_cast(half2v, word), half2v{one, one},
+                                              sum[r], false);
+            }
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < R; ++u)
+        {
+          float dot[Rows] = {};
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+          {
+            const unsigned code_word = now.w[u][j];
+            const u32x4 q = __builtin_bit_cast(u32x4, codes_as_half(code_word));
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+            {
+              const unsigned pair = q[i];
+#pragma unroll
+              for (int r = 0; r < Rows; ++r)
+              {
+                const unsigned word = x[r][j][i];
+                dot[r] = __builtin_amdgcn_fdot2(__builtin_bit_cast(half2v, word),
+                                                __builtin_bit_cast(half2v, pair), dot[r], false);
+              }
+            }
+          }
+          const float s = h2f(now.s[u]), z = h2f(now.z[u]);
+#pragma unroll
+          for (int r = 0; r < Rows; ++r)
+          {
+            y[u][r] = __builtin_fmaf(s, dot[r], __builtin_fmaf(z, sum[r], y[u][r]));
+          }
+        }
+      }
+      // Lane c keeps the sum of (output set c / Rows, row c % Rows).
+      float mine = 0.0f;
+#pragma unroll
+      for (int u = 0; u < R; ++u)
+      {
+#pragma unroll
+        for (int r = 0; r < Rows; ++r)
+        {
+          const float total = row_sum(y[u][r]);
+          mine = c == u * Rows + r ? total : mine;
+        }
+      }
+      if (a.splits > 1)
+      {
+        if (c < R * Rows)
+        {
+          parts[wave][4 * c + f] = mine;
+        }
+        __syncthreads();
+        if (split > 0)
+        {
+          return;
+        }
+        if (c < R * Rows)
+        {
+          for (int p = 1; p < a.splits; ++p)
+          {
+            mine += parts[wave + p][4 * c + f];
+          }
+        }
+      }
+      const int feature = tile * 4 * R + 4 * (c / Rows) + f;
+      if (c < R * Rows && c % Rows < a.rows && feature < a.features)
+      {
+        store<Out>(a, c % Rows, feature, mine);
+      }
+    }
+
+    // ---- more rows ----------------------------------------------------------
+
+    // Words j of lanes g = 0..3 (lane / 16) to word g of lanes j.
+    __device__ inline void transpose_words(u32x4 &w)
+    {
+      unsigned a = w.x, b = w.y, c = w.z, d = w.w;
+      // The upper lanes' a and the lower lanes' c change places, and b's and d's;
+      // then the odd row groups' a and the even ones' b.
+      asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(a), "+v"(c));
+      asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(b), "+v"(d));
+      asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b));
+      asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(c), "+v"(d));
+      w = u32x4{a, b, c, d};
+    }
+
+    constexpr int kChunk = 128; // inputs a wave takes at a time
+
+    // NT tiles of 16 rows, FT tiles of 16 outputs a wave; Groups: groups in a
+    // chunk.
+    template <int Groups, int FT>
+    struct TileFetch
+    {
+      u32x4 w[FT];
+      std::uint16_t s[FT][Groups];
+      std::uint16_t z[FT][Groups];
+    };
+
+    template <int Groups, int NT, int FT, int Waves, Int4Out Out>
+    __global__ void __launch_bounds__(64 * Waves) int4_tiles_kernel(Int4Args a)
+    {
+      constexpr int kPer = 4 / Groups; // instructions a group
+      extern __shared__ __align__(16) f32x4 parts[];
       const int lane = threadIdx.x & 63;
       const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
       const int n = lane & 15;
       const int g = lane >> 4;
-      const int split = wave % a.splits;
-      const int tiles = kWaves / a.splits * FT; // of 16 outputs a workgroup
-      const int tile0 = (static_cast<int>(blockIdx.x) * tiles + wave / a.splits * FT) * 16;
+      const int split = wave & (a.splits - 1);
+      const int tile0 =
+          (static_cast<int>(blockIdx.x) * (Waves / a.splits) + wave / a.splits) * FT * 16;
       const int row0 = static_cast<int>(blockIdx.y) * 16 * NT;
       const int rows = min(a.rows - row0, 16 * NT);
-      const std::uint16_t *x = a.x + static_cast<std::size_t>(row0) * a.in;
-
-      int row[FT];
+      const std::uint8_t *codes[FT];
+      std::size_t meta[FT];
 #pragma unroll
-      for (int t = 0; t < FT; ++t)
+      for (int u = 0; u < FT; ++u)
       {
-        row[t] = min(tile0 + 16 * t + n, a.features - 1);
+        const int row = min(tile0 + 16 * u + n, a.features - 1);
+        codes[u] = a.codes + static_cast<std::size_t>(row) * (a.in / 2);
+        meta[u] = static_cast<std::size_t>(row) * a.groups;
       }
-      int at[NT]; // the lane's row of x in LDS (a row past the last repeats it)
+      const std::uint16_t *x[NT]; // (a row past the last repeats it)
 #pragma unroll
       for (int t = 0; t < NT; ++t)
       {
-        at[t] = min(16 * t + n, rows - 1) * a.row_stride + 8 * Words * g;
+        x[t] = a.x + static_cast<std::size_t>(row0 + min(16 * t + n, rows - 1)) * a.in + 8 * g;
       }
       f32x4 y[NT][FT];
 #pragma unroll
@@ -249,83 +420,97 @@ namespace mi
       const _Float16 one = static_cast<_Float16>(1.0f);
       const half8 ones = {one, one, one, one, one, one, one, one};
       const f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f};
-
       const int chunks = (a.in + kChunk - 1) / kChunk;
-      int chunk = split;
-      Fetched<Words, FT> next;
-      fetch<Words, FT>(next, a, row, min(chunk, chunks - 1), g);
-      for (int from = 0; from < a.in; from += a.phase)
-      {
-        // The phase's inputs of every row, zeros past the last.
-        const int width = min(a.phase, (a.in - from + kChunk - 1) / kChunk * kChunk);
-        if (from > 0)
+      const auto fetch = [&](TileFetch<Groups, FT> &to, int chunk) {
+        // (Inputs past the last, and groups: the first's, which no product takes.)
+        const int k = chunk * kChunk + 32 * g;
+#pragma unroll
+        for (int u = 0; u < FT; ++u)
         {
-          __syncthreads();
+          to.w[u] = *reinterpret_cast<const u32x4 *>(codes[u] + (k < a.in ? k : 0) / 2);
         }
-        for (int i = threadIdx.x; i < rows * (width / 8); i += kThreads)
+#pragma unroll
+        for (int u = 0; u < FT; ++u)
         {
-          const int r = i / (width / 8);
-          const int k = i % (width / 8) * 8;
-          u32x4 v = {0u, 0u, 0u, 0u};
-          if (from + k < a.in)
+#pragma unroll
+          for (int h = 0; h < Groups; ++h)
           {
-            v = *reinterpret_cast<const u32x4 *>(x + static_cast<std::size_t>(r) * a.in + from + k);
+            const int group = chunk * Groups + h;
+            const std::size_t at = meta[u] + (group < a.groups ? group : 0);
+            to.s[u][h] = a.scales[at];
+            to.z[u][h] = a.zeros[at];
           }
-          const u32x4 turned = {__builtin_amdgcn_perm(v.z, v.x, 0x05040100u),
-                                __builtin_amdgcn_perm(v.z, v.x, 0x07060302u),
-                                __builtin_amdgcn_perm(v.w, v.y, 0x05040100u),
-                                __builtin_amdgcn_perm(v.w, v.y, 0x07060302u)};
-          *reinterpret_cast<u32x4 *>(x_lds + r * a.row_stride + k) = turned;
         }
-        __syncthreads();
-        const int phase_end = (from + width) / kChunk;
-#pragma unroll 2
-        for (; chunk < phase_end; chunk += a.splits)
+      };
+      TileFetch<Groups, FT> next;
+      if (split < chunks)
+      {
+        fetch(next, split);
+      }
+      for (int chunk = split; chunk < chunks; chunk += a.splits)
+      {
+        TileFetch<Groups, FT> now = next;
+        fetch(next, min(chunk + a.splits, chunks - 1));
+        const int k0 = chunk * kChunk;
+        u32x4 xa[NT][4];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
         {
-          const Fetched<Words, FT> now = next;
-          fetch<Words, FT>(next, a, row, min(chunk + a.splits, chunks - 1), g);
-          const int k0 = chunk * kChunk - from;
 #pragma unroll
-          for (int h = 0; h < kGroups; ++h)
+          for (int j = 0; j < 4; ++j)
           {
-            f32x4 dot[NT][FT], sum[NT];
+            xa[t][j] = *reinterpret_cast<const u32x4 *>(x[t] + (k0 + 32 * j < a.in ? k0 + 32 * j : 0));
+          }
+        }
 #pragma unroll
-            for (int j = 0; j < Words; ++j)
+        for (int u = 0; u < FT; ++u)
+        {
+          transpose_words(now.w[u]);
+        }
+#pragma unroll
+        for (int h = 0; h < Groups; ++h)
+        {
+          if (h > 0 && k0 + 32 * kPer * h >= a.in)
+          {
+            break;
+          }
+          f32x4 dot[NT][FT], sum[NT];
+#pragma unroll
+          for (int j = 0; j < kPer; ++j)
+          {
+            half8 xt[NT];
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
             {
-              half8 xa[NT];
-#pragma unroll
-              for (int t = 0; t < NT; ++t)
-              {
-                xa[t] = *reinterpret_cast<const half8 *>(x_lds + at[t] + k0 + 32 * Words * h +
-                                                         8 * j);
-                sum[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xa[t], ones, j ? sum[t] : none, 0,
-                                                                0, 0);
-              }
-#pragma unroll
-              for (int u = 0; u < FT; ++u)
-              {
-                const half8 c = codes_as_half(now.w[u][h * Words + j]);
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-                {
-                  dot[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xa[t], c, j ? dot[t][u] : none,
-                                                                     0, 0, 0);
-                }
-              }
+              xt[t] = __builtin_bit_cast(half8, turned(xa[t][h * kPer + j]));
+              sum[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xt[t], ones, j ? sum[t] : none, 0, 0,
+                                                              0);
             }
 #pragma unroll
             for (int u = 0; u < FT; ++u)
             {
-              const float s = h2f(now.s[u][h]), z = h2f(now.z[u][h]);
+              const unsigned word = now.w[u][h * kPer + j];
+              const half8 q = codes_as_half(word);
 #pragma unroll
               for (int t = 0; t < NT; ++t)
               {
+                dot[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xt[t], q, j ? dot[t][u] : none, 0,
+                                                                   0, 0);
+              }
+            }
+          }
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                {
-                  y[t][u][i] = __builtin_fmaf(s, dot[t][u][i],
-                                              __builtin_fmaf(z, sum[t][i], y[t][u][i]));
-                }
+          for (int u = 0; u < FT; ++u)
+          {
+            const float s = h2f(now.s[u][h]), z = h2f(now.z[u][h]);
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+            {
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+              {
+                y[t][u][i] = __builtin_fmaf(s, dot[t][u][i],
+                                            __builtin_fmaf(z, sum[t][i], y[t][u][i]));
               }
             }
           }
@@ -335,8 +520,6 @@ namespace mi
       // The splits' sums, added by the tile's first wave in wave order.
       if (a.splits > 1)
       {
-        f32x4 *parts = reinterpret_cast<f32x4 *>(x_lds);
-        __syncthreads();
         if (split > 0)
         {
 #pragma unroll
@@ -354,7 +537,7 @@ namespace mi
         {
           return;
         }
-        for (int s = 1; s < a.splits; ++s)
+        for (int p = 1; p < a.splits; ++p)
         {
 #pragma unroll
           for (int t = 0; t < NT; ++t)
@@ -362,7 +545,7 @@ namespace mi
 #pragma unroll
             for (int u = 0; u < FT; ++u)
             {
-              y[t][u] += parts[(((wave + s) * NT + t) * FT + u) * 64 + lane];
+              y[t][u] += parts[(((wave + p) * NT + t) * FT + u) * 64 + lane];
             }
           }
         }
@@ -371,11 +554,6 @@ namespace mi
       for (int u = 0; u < FT; ++u)
       {
         const int feature = tile0 + 16 * u + n;
-        if (feature >= a.features)
-        {
-          continue;
-        }
-        const float bias = Out == Int4Out::kHalf && a.bias != nullptr ? h2f(a.bias[feature]) : 0.0f;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
         {
@@ -383,20 +561,9 @@ namespace mi
           for (int i = 0; i < 4; ++i)
           {
             const int r = 16 * t + 4 * g + i;
-            if (r >= rows)
+            if (r < rows && feature < a.features)
             {
-              continue;
-            }
-            const std::size_t to =
-                static_cast<std::size_t>(row0 + r) * a.features + feature;
-            if constexpr (Out == Int4Out::kHalf)
-            {
-              static_cast<std::uint16_t *>(a.out)[to] =
-                  __half_as_ushort(__float2half(y[t][u][i] + bias));
-            }
-            else
-            {
-              static_cast<float *>(a.out)[to] += y[t][u][i];
+              store<Out>(a, row0 + r, feature, y[t][u][i]);
             }
           }
         }
@@ -428,49 +595,87 @@ namespace mi
       }
     }
 
-    template <int Words, int NT, int FT>
-    void project(const Int4Args &a, Int4Out out, hipStream_t stream)
+    // The waves an output's inputs are split over: a power of two up to
+    // `most`, while the waves would not fill the device twice over and each
+    // keeps two of its steps.
+    int splits_of(int tiles, int steps, int most)
     {
-      const int tiles = kWaves / a.splits * FT;
-      const dim3 grid((a.features + 16 * tiles - 1) / (16 * tiles),
-                      (a.rows + 16 * NT - 1) / (16 * NT));
-      const std::size_t stage =
-          static_cast<std::size_t>(std::min(a.rows, 16 * NT)) * a.row_stride * 2;
-      const std::size_t parts = a.splits > 1 ? sizeof(f32x4) * kWaves * NT * FT * 64 : 0;
-      const std::size_t lds = std::max(stage, parts);
+      int splits = 1;
+      while (splits < most && static_cast<long long>(tiles) * splits < 4096 && steps >= 4 * splits)
+      {
+        splits *= 2;
+      }
+      return splits;
+    }
+
+    template <int Rows, int R>
+    void project_rows(Int4Args a, Int4Out out, hipStream_t stream)
+    {
+      const int tiles = (a.features + 4 * R - 1) / (4 * R);
+      a.splits = splits_of(tiles, (a.in / 32 + 15) / 16, kRowWaves);
+      const int per = kRowWaves / a.splits;
+      const dim3 grid((tiles + per - 1) / per);
       if (out == Int4Out::kHalf)
       {
-        linear_int4_kernel<Words, NT, FT, Int4Out::kHalf><<<grid, kThreads, lds, stream>>>(a);
+        int4_rows_kernel<Rows, R, Int4Out::kHalf><<<grid, 64 * kRowWaves, 0, stream>>>(a);
       }
       else
       {
-        linear_int4_kernel<Words, NT, FT, Int4Out::kAccumulate><<<grid, kThreads, lds, stream>>>(a);
+        int4_rows_kernel<Rows, R, Int4Out::kAccumulate><<<grid, 64 * kRowWaves, 0, stream>>>(a);
       }
-      hip_check(hipGetLastError(), "linear_int4_kernel");
+      hip_check(hipGetLastError(), "int4_rows_kernel");
     }
 
-    template <int Words>
-    void project_rows(Int4Args a, Int4Out out, hipStream_t stream)
+    template <int Groups, int NT, int FT, int Waves>
+    void project_tiles(Int4Args a, Int4Out out, hipStream_t stream)
     {
-      const int tiles = (a.features + 15) / 16;
-      const int chunks = (a.in + kChunk - 1) / kChunk;
-      const int nt = a.rows <= 16 ? 1 : a.rows <= 32 ? 2 : 4;
-      const int ft = a.rows <= 16 ? 1 : 2;
-      // A tile's inputs are split while the waves would not fill the CUs and
-      // each keeps two chunks.
-      a.splits = 1;
-      while (a.splits < kWaves && (tiles / ft) * a.splits < 2048 && chunks >= 4 * a.splits)
+      const int tiles = (a.features + 16 * FT - 1) / (16 * FT);
+      const int row_tiles = (a.rows + 16 * NT - 1) / (16 * NT);
+      a.splits = splits_of(static_cast<int>(std::min<long long>(
+                               static_cast<long long>(tiles) * row_tiles, 1 << 20)),
+                           (a.in + kChunk - 1) / kChunk, Waves);
+      const int per = Waves / a.splits;
+      const dim3 grid((tiles + per - 1) / per, row_tiles);
+      const std::size_t lds = a.splits > 1 ? sizeof(f32x4) * Waves * NT * FT * 64 : 0;
+      if (out == Int4Out::kHalf)
       {
-        a.splits *= 2;
+        int4_tiles_kernel<Groups, NT, FT, Waves, Int4Out::kHalf>
+            <<<grid, 64 * Waves, lds, stream>>>(a);
       }
-      const int rows = std::min(a.rows, 16 * nt);
-      a.phase = std::min(chunks, std::max(1, (kStageHalves / rows - kRowPad) / kChunk)) * kChunk;
-      a.row_stride = a.phase + kRowPad;
-      switch (nt)
+      else
       {
-      case 1: project<Words, 1, 1>(a, out, stream); break;
-      case 2: project<Words, 2, 2>(a, out, stream); break;
-      default: project<Words, 4, 2>(a, out, stream); break;
+        int4_tiles_kernel<Groups, NT, FT, Waves, Int4Out::kAccumulate>
+            <<<grid, 64 * Waves, lds, stream>>>(a);
+      }
+      hip_check(hipGetLastError(), "int4_tiles_kernel");
+    }
+
+    template <int Groups>
+    void project(const Int4Args &a, Int4Out out, hipStream_t stream)
+    {
+      if (a.rows <= 4)
+      {
+        // Four sets of outputs a wave where there are plenty.
+        const bool many = a.features >= 16384;
+        switch (a.rows)
+        {
+        case 1: many ? project_rows<1, 4>(a, out, stream) : project_rows<1, 1>(a, out, stream); break;
+        case 2: many ? project_rows<2, 4>(a, out, stream) : project_rows<2, 1>(a, out, stream); break;
+        default: many ? project_rows<4, 4>(a, out, stream) : project_rows<4, 1>(a, out, stream); break;
+        }
+        return;
+      }
+      if (a.rows <= 16)
+      {
+        project_tiles<Groups, 1, 1, 16>(a, out, stream);
+      }
+      else if (a.rows <= 32)
+      {
+        project_tiles<Groups, 2, 1, 16>(a, out, stream);
+      }
+      else
+      {
+        project_tiles<Groups, 4, 2, 8>(a, out, stream);
       }
     }
 
@@ -516,11 +721,12 @@ namespace mi
       a.in = in;
       a.features = features;
       a.groups = in / group;
+      a.group_32 = group == 32 ? 0 : group == 64 ? 1 : 2;
       switch (group)
       {
-      case 32: project_rows<1>(a, kind, stream); break;
-      case 64: project_rows<2>(a, kind, stream); break;
-      default: project_rows<4>(a, kind, stream); break;
+      case 32: project<4>(a, kind, stream); break;
+      case 64: project<2>(a, kind, stream); break;
+      default: project<1>(a, kind, stream); break;
       }
     }
   } // namespace

@@ -85,7 +85,7 @@ def test_quantise_is_the_oracle_s(out, n_in, group):
     np.testing.assert_array_equal(zeros.read().view(np.float16).reshape(want[2].shape), want[2])
 
 
-@pytest.mark.parametrize("rows", [1, 2, 15, 16, 17, 32, 33, 64, 65, 130])
+@pytest.mark.parametrize("rows", [1, 2, 3, 4, 5, 15, 16, 17, 32, 33, 64, 65, 130])
 @pytest.mark.parametrize("out,n_in,group", [
     (1, 32, 32), (17, 96, 32), (128, 896, 32), (40, 64, 64), (65, 192, 64), (130, 896, 64),
     (16, 128, 128), (50, 640, 128), (300, 1536, 128)])
@@ -145,6 +145,21 @@ def test_a_row_that_is_not_finite_stays_in_its_row():
     assert np.isnan(got[1]).all() and not np.isfinite(got[3]).any()
     keep = [0, 2, 4]
     check_half(got[keep], clean[keep], w.bound(x[keep]))
+
+
+@pytest.mark.parametrize("rows", [1, 4, 16])
+def test_inputs_and_steps_below_fp16_s_normals(rows):
+    """x of 2^-16 and steps of 2^-20: no product is taken for zero."""
+    d = mi().device
+    rng = np.random.default_rng(rows)
+    w = Int4(fp16_exact(rng.standard_normal((20, 256)) * 2.0**-18), 64)
+    x = fp16_exact(rng.standard_normal((rows, 256)) * 2.0**-16)
+    acc = d.upload_f32(np.zeros(rows * 20, np.float32))
+    announce("small values", rows)
+    d.linear_int4_accumulate(put(x), *w.on, 64, acc, rows, 256, 20)
+    want = x.astype(np.float64) @ w.w64.T
+    assert np.abs(want).max() > 0
+    assert (np.abs(acc.to_numpy().reshape(rows, 20) - want) <= w.bound(x)).all()
 
 
 def test_views_and_a_replayed_graph():
