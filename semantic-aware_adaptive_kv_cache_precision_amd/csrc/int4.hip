@@ -133,6 +133,7 @@ namespace mi
       int groups;   // a row's
       int splits;   // waves an output's inputs are split over, a power of two
       int group_32; // log2 of a group's runs of 32
+      bool wide_meta; // whole chunks of groups a row, on their own alignment
     };
 
     // Eight codes, the first in the lowest bits, as fp16 in the order
@@ -432,13 +433,25 @@ namespace mi
 #pragma unroll
         for (int u = 0; u < FT; ++u)
         {
-#pragma unroll
-          for (int h = 0; h < Groups; ++h)
+          // A chunk's groups by one load, where a row's lie so.
+          if (Groups > 1 && a.wide_meta)
           {
-            const int group = chunk * Groups + h;
-            const std::size_t at = meta[u] + (group < a.groups ? group : 0);
-            to.s[u][h] = a.scales[at];
-            to.z[u][h] = a.zeros[at];
+            const std::size_t at = meta[u] + static_cast<std::size_t>(chunk) * Groups;
+            __builtin_memcpy(to.s[u], __builtin_assume_aligned(a.scales + at, 2 * Groups),
+                             2 * Groups);
+            __builtin_memcpy(to.z[u], __builtin_assume_aligned(a.zeros + at, 2 * Groups),
+                             2 * Groups);
+          }
+          else
+          {
+#pragma unroll
+            for (int h = 0; h < Groups; ++h)
+            {
+              const int group = chunk * Groups + h;
+              const std::size_t at = meta[u] + (group < a.groups ? group : 0);
+              to.s[u][h] = a.scales[at];
+              to.z[u][h] = a.zeros[at];
+            }
           }
         }
       };
@@ -597,11 +610,11 @@ namespace mi
 
     // The waves an output's inputs are split over: a power of two up to
     // `most`, while the waves would not fill the device twice over and each
-    // keeps two of its steps.
+    // keeps a step (a step is a trip to memory).
     int splits_of(int tiles, int steps, int most)
     {
       int splits = 1;
-      while (splits < most && static_cast<long long>(tiles) * splits < 4096 && steps >= 4 * splits)
+      while (splits < most && static_cast<long long>(tiles) * splits < 4096 && steps >= 2 * splits)
       {
         splits *= 2;
       }
@@ -653,25 +666,43 @@ namespace mi
     template <int Groups>
     void project(const Int4Args &a, Int4Out out, hipStream_t stream)
     {
-      if (a.rows <= 4)
+      // Four sets of outputs a wave where there are plenty. Three or four rows
+      // are the dot products' work only there: they read x a set at a time
+      // (8960 x 1536, three rows: 12.0 us, by tiles 6.7; 128256 x 2048: 72 and
+      // 84).
+      const bool many = a.features >= 16384;
+      if (a.rows == 1)
       {
-        // Four sets of outputs a wave where there are plenty.
-        const bool many = a.features >= 16384;
-        switch (a.rows)
-        {
-        case 1: many ? project_rows<1, 4>(a, out, stream) : project_rows<1, 1>(a, out, stream); break;
-        case 2: many ? project_rows<2, 4>(a, out, stream) : project_rows<2, 1>(a, out, stream); break;
-        default: many ? project_rows<4, 4>(a, out, stream) : project_rows<4, 1>(a, out, stream); break;
-        }
+        many ? project_rows<1, 4>(a, out, stream) : project_rows<1, 1>(a, out, stream);
         return;
       }
-      if (a.rows <= 16)
+      if (a.rows == 2)
+      {
+        many ? project_rows<2, 4>(a, out, stream) : project_rows<2, 1>(a, out, stream);
+        return;
+      }
+      if (a.rows <= 4 && many)
+      {
+        project_rows<4, 4>(a, out, stream);
+        return;
+      }
+      // A workgroup reads all its rows' x: few workgroups, each with many
+      // rows, are bound by what a CU takes in (27 rows 8960 -> 1536: 96
+      // workgroups of 32 rows 19.1 us, 192 of 16 13.1). Where there are
+      // plenty, four tiles of outputs a wave share each row of x.
+      const long long tiles = (a.features + 15) / 16;
+      const long long row_tiles = (a.rows + 15) / 16;
+      if (tiles * row_tiles <= 1024)
       {
         project_tiles<Groups, 1, 1, 16>(a, out, stream);
       }
+      else if (a.rows <= 16)
+      {
+        project_tiles<Groups, 1, 4, 8>(a, out, stream);
+      }
       else if (a.rows <= 32)
       {
-        project_tiles<Groups, 2, 1, 16>(a, out, stream);
+        project_tiles<Groups, 2, 4, 8>(a, out, stream);
       }
       else
       {
@@ -721,6 +752,8 @@ namespace mi
       a.in = in;
       a.features = features;
       a.groups = in / group;
+      a.wide_meta = in % kChunk == 0 && ((reinterpret_cast<std::uintptr_t>(scales) |
+                                          reinterpret_cast<std::uintptr_t>(zeros)) % 8) == 0;
       a.group_32 = group == 32 ? 0 : group == 64 ? 1 : 2;
       switch (group)
       {
