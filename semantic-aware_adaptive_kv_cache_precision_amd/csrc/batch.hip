@@ -11,7 +11,7 @@
 //
 // Layout. A sequence's visible pages (the sink pages, then the window's) are
 // one list; a workgroup takes a run of it, its eight waves sharing the run's
-// pages and the KV heads (up to eight) among them, so that the KV heads of a
+// pages and the KV heads (up to four) among them, so that the KV heads of a
 // page, which share its rows' lines, are read on one CU. A wave reads a page
 // of a KV head once for all the query heads of that KV head: the keys as M of
 // 16x16x32 products, the heads as N, codes made fp16 in registers (the page
@@ -46,12 +46,12 @@ namespace mi
     typedef const __attribute__((address_space(1))) unsigned *g_u32;
     typedef const __attribute__((address_space(1))) unsigned short *g_u16;
 
-    constexpr int kWaves = 8;
+    constexpr int kWaves = 4;
     constexpr int kThreads = 64 * kWaves;
     constexpr int kP = kBatchPageTokens;
     constexpr int kMaxGroup = 16;
-    constexpr int kMaxSplits = 1024; // the join keeps a weight of each in LDS
-    constexpr int kJoinWaves = 4;
+    constexpr int kMaxSplits = 1024;
+    constexpr int kJoinThreads = 512;
     // P is held x 2^14 (exact), so that its fp16 low part stays normal for
     // every weight above 2^-17 of the running maximum.
     constexpr float kPScale = 16384.0f;
@@ -68,18 +68,27 @@ namespace mi
       const unsigned long long *pages; // (batch, max_pages)
       const std::uint8_t *tiers;
       const int *lengths;
-      PageLayout lay[kTierCount];
       int max_pages;
       int heads;
       int kv_heads;
       int group;
-      int kv_block; // KV heads a workgroup takes: a power of two up to 8
+      int kv_block; // KV heads a workgroup takes: a power of two up to 4
       int window;   // 0: every token
       int sinks;
       int run_pages; // of the visible list a workgroup takes
       int splits;
       float scale; // log2 e / sqrt(hd): scores in base 2
-      BatchSequence held[kBatchHeld]; // the sequences themselves (kHeld)
+    };
+
+    // The sequences themselves, where the launch brings them (kHeld).
+    template <bool kHeld>
+    struct Sequences
+    {
+    };
+    template <>
+    struct Sequences<true>
+    {
+      BatchSequence of[kBatchHeld];
     };
 
     // A sequence's visible pages: [0, sink_pages) and [first, pages).
@@ -135,15 +144,19 @@ namespace mi
       return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
     }
 
+    // Loads from a base that is the same in every lane (scalar registers) and
+    // the lane's 32-bit offset.
+    typedef const __attribute__((address_space(1))) std::uint8_t *g_base;
+
     template <int Bytes>
-    __device__ inline void load_words(unsigned *w, const std::uint8_t *p)
+    __device__ inline void load_words(unsigned *w, g_base base, unsigned offset)
     {
       if constexpr (Bytes >= 16)
       {
 #pragma unroll
         for (int i = 0; i < Bytes / 16; ++i)
         {
-          const u32x4 v = *((g_u32x4)(p + 16 * i));
+          const u32x4 v = *((g_u32x4)(base + offset + 16 * i));
           w[4 * i + 0] = v.x;
           w[4 * i + 1] = v.y;
           w[4 * i + 2] = v.z;
@@ -152,13 +165,13 @@ namespace mi
       }
       else if constexpr (Bytes == 8)
       {
-        const u32x2 v = *((g_u32x2)(p));
+        const u32x2 v = *((g_u32x2)(base + offset));
         w[0] = v.x;
         w[1] = v.y;
       }
       else
       {
-        w[0] = *((g_u32)(p));
+        w[0] = *((g_u32)(base + offset));
       }
     }
 
@@ -178,9 +191,19 @@ namespace mi
       int g; // lane / 16: a quarter of the channels
       unsigned visible;
       float scale;
-      float *mass; // where head r's sum of the page goes, or null
+      bool scored;
+      unsigned mass_at; // where head r's sum of the page goes, from the KV head's rows
+      float *mass;
       float *mass_from;
     };
+
+    // The lane's first channel in row r of a page's keys, in elements. Opaque,
+    // so that no tier's offsets are kept in registers from page to page.
+    __device__ inline unsigned opaque(unsigned v)
+    {
+      asm volatile("" : "+v"(v));
+      return v;
+    }
 
     // The two 16-key accumulators as P (high, low), the running softmax
     // moved on. (Scores are scaled inside the subtraction of the maximum, by
@@ -192,11 +215,12 @@ namespace mi
     {
       if (c.visible != ~0u)
       {
+        const unsigned mine = c.visible >> (4 * c.g); // keys 16 b + 4 g + {0..3}
 #pragma unroll
         for (int e = 0; e < 8; ++e)
         {
-          const int t = e / 4 * 16 + 4 * c.g + e % 4;
-          acc[e / 4][e % 4] = (c.visible >> t) & 1u ? acc[e / 4][e % 4] : -INFINITY;
+          acc[e / 4][e % 4] =
+              mine & (1u << (e / 4 * 16 + e % 4)) ? acc[e / 4][e % 4] : -INFINITY;
         }
       }
       float top = acc[0][0];
@@ -217,10 +241,10 @@ namespace mi
         sum += p[e];
       }
       sum = lane_sum32(lane_sum16(sum));
-      if (c.mass != nullptr && c.g == 0)
+      if (c.scored && c.g == 0)
       {
-        *c.mass = sum;
-        *c.mass_from = from;
+        c.mass[c.mass_at] = sum;
+        c.mass_from[c.mass_at] = from;
       }
       run.l = run.l * keep + sum;
       if (__builtin_amdgcn_ballot_w64(!(top <= run.m)) != 0)
@@ -242,31 +266,49 @@ namespace mi
       }
     }
 
+    __device__ inline unsigned packed(float a, float b)
+    {
+      return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(a, b));
+    }
+
+    // The 0/1 matrix that picks channel r (lo) or 16 + r (hi) of 32: row
+    // 8 g + e, column r. Made anew for each page, not kept through it.
+    struct Pick
+    {
+      u32x4 lo;
+      u32x4 hi;
+      __device__ Pick(int lane_r, int g)
+      {
+        const unsigned r = opaque(lane_r);
+        const unsigned one = r & 1u ? 0x3C000000u : 0x00003C00u;
+        const unsigned word = r % 8 / 2;
+        const unsigned group = r / 8; // of lo; 2 more of hi
+#pragma unroll
+        for (unsigned w = 0; w < 4; ++w)
+        {
+          const unsigned v = w == word ? one : 0u;
+          lo[w] = static_cast<unsigned>(g) == group ? v : 0u;
+          hi[w] = static_cast<unsigned>(g) == group + 2 ? v : 0u;
+        }
+      }
+    };
+
     // P.V of 32 channels (8 of each quarter): V^T by products with a 0/1
     // matrix, whose K axis then is the lane's own keys.
     template <int HD>
-    __device__ inline void values_step(Running<HD> &run, int s, half8 v0, half8 v1, int r, int g,
+    __device__ inline void values_step(Running<HD> &run, int s, half8 v0, half8 v1, const Pick &p,
                                        half8 p_hi, half8 p_lo)
     {
       const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int h = 0; h < 2; ++h)
       {
-        half8 pick;
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-        {
-          pick[e] = static_cast<_Float16>(8 * g + e == r + 16 * h ? 1.0f : 0.0f);
-        }
+        const half8 pick = as_half8(h == 0 ? p.lo : p.hi);
         const f32x4 t0 = mfma(v0, pick, zero);
         const f32x4 t1 = mfma(v1, pick, zero);
-        half8 vt;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-        {
-          vt[i] = static_cast<_Float16>(t0[i]);
-          vt[4 + i] = static_cast<_Float16>(t1[i]);
-        }
+        // (Exact, so that any rounding is the same.)
+        const half8 vt = as_half8(u32x4{packed(t0[0], t0[1]), packed(t0[2], t0[3]),
+                                        packed(t1[0], t1[1]), packed(t1[2], t1[3])});
         run.o[2 * s + h] = mfma(vt, p_hi, run.o[2 * s + h]);
         run.o[2 * s + h] = mfma(vt, p_lo, run.o[2 * s + h]);
       }
@@ -281,25 +323,41 @@ namespace mi
 
     // A value row that is not visible may hold anything: it enters P.V as
     // zeros (its weight is zero, and zero times infinity is not).
-    __device__ inline half8 seen(half8 v, bool visible)
+    template <int S>
+    __device__ inline void hide_rows(half8 (&v)[2][S], const PageAt &c)
     {
-      return visible ? v : as_half8(u32x4{0u, 0u, 0u, 0u});
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+      {
+        if (!((c.visible >> (16 * b + c.r)) & 1u))
+        {
+#pragma unroll
+          for (int s = 0; s < S; ++s)
+          {
+            v[b][s] = as_half8(u32x4{0u, 0u, 0u, 0u});
+          }
+        }
+      }
     }
 
+    // A page of FP16 rows, keys then values. `own_row`, if it is not negative,
+    // is read from own_k and own_v (a token's row, not yet in the page).
     template <int HD>
     __device__ inline void fp16_page(Running<HD> &run, const PageAt &c, const half8 (&q)[HD / 32],
-                                     const std::uint16_t *const (&k_row)[2],
-                                     const std::uint16_t *const (&v_row)[2])
+                                     g_base page, unsigned elem, int width, int own_row = -1,
+                                     const std::uint16_t *own_k = nullptr,
+                                     const std::uint16_t *own_v = nullptr)
     {
       constexpr int S = HD / 32;
       half8 k[2][S], v[2][S];
+      const unsigned at = 2 * opaque(elem);
 #pragma unroll
       for (int b = 0; b < 2; ++b)
       {
 #pragma unroll
         for (int s = 0; s < S; ++s)
         {
-          k[b][s] = as_half8(*((g_u32x4)(k_row[b] + 8 * s)));
+          k[b][s] = as_half8(*((g_u32x4)(page + 32 * b * width + at + 16 * s)));
         }
       }
 #pragma unroll
@@ -308,7 +366,24 @@ namespace mi
 #pragma unroll
         for (int s = 0; s < S; ++s)
         {
-          v[b][s] = as_half8(*((g_u32x4)(v_row[b] + 8 * s)));
+          v[b][s] = as_half8(*((g_u32x4)(page + 2 * (kP + 16 * b) * width + at + 16 * s)));
+        }
+      }
+      if (own_row >= 0)
+      {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+        {
+          if (16 * b + c.r == own_row)
+          {
+            const unsigned chan = elem - c.r * width;
+#pragma unroll
+            for (int s = 0; s < S; ++s)
+            {
+              k[b][s] = as_half8(*((g_u32x4)(own_k + chan + 8 * s)));
+              v[b][s] = as_half8(*((g_u32x4)(own_v + chan + 8 * s)));
+            }
+          }
         }
       }
       f32x4 acc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
@@ -320,11 +395,15 @@ namespace mi
       }
       half8 p_hi, p_lo;
       softmax_page<HD>(acc, c, run, p_hi, p_lo);
-      const bool see0 = (c.visible >> c.r) & 1u, see1 = (c.visible >> (16 + c.r)) & 1u;
+      const Pick pick(c.r, c.g);
+      if (c.visible != ~0u)
+      {
+        hide_rows<S>(v, c);
+      }
 #pragma unroll
       for (int s = 0; s < S; ++s)
       {
-        values_step<HD>(run, s, seen(v[0][s], see0), seen(v[1][s], see1), c.r, c.g, p_hi, p_lo);
+        values_step<HD>(run, s, v[0][s], v[1][s], pick, p_hi, p_lo);
       }
     }
 
@@ -332,38 +411,43 @@ namespace mi
     // scales and zeros reach the 16 lanes that share them.
     template <int HD, int Bits>
     __device__ inline void quantised_page(Running<HD> &run, const PageAt &c,
-                                          const half8 (&q)[HD / 32], const std::uint8_t *page,
-                                          const PageLayout &L, int width, int kvh, int kv_heads,
-                                          int lane, unsigned *meta)
+                                          const half8 (&q)[HD / 32], g_base page, unsigned elem,
+                                          int width, int kvh, int kv_heads, int lane,
+                                          unsigned *meta)
     {
       constexpr int S = HD / 32;
       constexpr int kRun = HD / 4;
       constexpr int kRowBytes = kRun * Bits / 8;
       constexpr int kWords = kRowBytes / 4;
       constexpr int kMetaLanes = HD / 4; // 8 bytes a lane, scales then zeros
+      // The page's regions back to back, as page_layout lays them.
+      const unsigned value_codes = kP * width * Bits / 8;
+      const unsigned key_scales = 2 * value_codes;
+      const unsigned value_scales = key_scales + 4 * width;
+      const unsigned value_zeros = value_scales + 2 * kP * kv_heads;
       unsigned kc[2][kWords], vc[2][kWords];
       unsigned short vs[2], vz[2];
+      const unsigned at = opaque(elem) / (8 / Bits);
 #pragma unroll
       for (int b = 0; b < 2; ++b)
       {
-        const std::size_t at =
-            (static_cast<std::size_t>(16 * b + c.r) * width + kvh * HD + c.g * kRun) * Bits / 8;
-        load_words<kRowBytes>(kc[b], page + L.key_codes + at);
-        load_words<kRowBytes>(vc[b], page + L.value_codes + at);
+        load_words<kRowBytes>(kc[b], page + 16 * b * width * Bits / 8, at);
+        load_words<kRowBytes>(vc[b], page + value_codes + 16 * b * width * Bits / 8, at);
       }
       u32x2 km = {0u, 0u};
       if (lane < 2 * kMetaLanes)
       {
-        const std::size_t region = lane < kMetaLanes ? L.key_scales : L.key_zeros;
-        km = *((g_u32x2)(page + region + 2 * static_cast<std::size_t>(kvh) * HD +
-                         8 * (lane % kMetaLanes)));
+        // (The zeros lie behind the scales: a lane's eight bytes of a head's
+        // scales, or 2 width bytes on.)
+        const unsigned piece = 8 * (lane % kMetaLanes) + (lane < kMetaLanes ? 0 : 2 * width);
+        km = *((g_u32x2)(page + key_scales + 2 * kvh * HD + opaque(piece)));
       }
 #pragma unroll
       for (int b = 0; b < 2; ++b)
       {
-        const std::size_t row = static_cast<std::size_t>(16 * b + c.r) * kv_heads + kvh;
-        vs[b] = *((g_u16)(page + L.value_scales + 2 * row));
-        vz[b] = *((g_u16)(page + L.value_zeros + 2 * row));
+        const unsigned row = 2 * (opaque(c.r) * kv_heads);
+        vs[b] = *((g_u16)(page + value_scales + 2 * (16 * b * kv_heads + kvh) + row));
+        vz[b] = *((g_u16)(page + value_zeros + 2 * (16 * b * kv_heads + kvh) + row));
       }
       // One wave's LDS operations complete in order; the fences keep the
       // compiler from moving the reads above the write, and the write above
@@ -406,16 +490,18 @@ namespace mi
       }
       half8 p_hi, p_lo;
       softmax_page<HD>(acc, c, run, p_hi, p_lo);
+      const Pick pick(c.r, c.g);
       u32x4 s4[2], z4[2];
-      bool see[2];
 #pragma unroll
       for (int b = 0; b < 2; ++b)
       {
-        const unsigned sp = vs[b] | (static_cast<unsigned>(vs[b]) << 16);
-        const unsigned zp = vz[b] | (static_cast<unsigned>(vz[b]) << 16);
+        // (A row that is not visible: codes times zero and zero. Its scale and
+        // zero may be anything, its codes are finite.)
+        const bool see = c.visible == ~0u || ((c.visible >> (16 * b + c.r)) & 1u);
+        const unsigned sp = see ? vs[b] | (static_cast<unsigned>(vs[b]) << 16) : 0u;
+        const unsigned zp = see ? vz[b] | (static_cast<unsigned>(vz[b]) << 16) : 0u;
         s4[b] = u32x4{sp, sp, sp, sp};
         z4[b] = u32x4{zp, zp, zp, zp};
-        see[b] = (c.visible >> (16 * b + c.r)) & 1u;
       }
 #pragma unroll
       for (int s = 0; s < S; ++s)
@@ -424,10 +510,9 @@ namespace mi
 #pragma unroll
         for (int b = 0; b < 2; ++b)
         {
-          v[b] = seen(dequant_step<Bits>(word(vc[b], s, 0), word(vc[b], s, 1), s4[b], z4[b]),
-                      see[b]);
+          v[b] = dequant_step<Bits>(word(vc[b], s, 0), word(vc[b], s, 1), s4[b], z4[b]);
         }
-        values_step<HD>(run, s, v[0], v[1], c.r, c.g, p_hi, p_lo);
+        values_step<HD>(run, s, v[0], v[1], pick, p_hi, p_lo);
       }
     }
 
@@ -448,7 +533,8 @@ namespace mi
     }
 
     template <int HD, bool kHeld>
-    __global__ void __launch_bounds__(kThreads) batch_pages_kernel(BatchArgs a)
+    __global__ void __launch_bounds__(kThreads, HD == 64 ? 4 : 3) batch_pages_kernel(BatchArgs a,
+                                                                                    Sequences<kHeld> held)
     {
       constexpr int S = HD / 32;
       constexpr int kRun = HD / 4;
@@ -459,28 +545,45 @@ namespace mi
       const int g = lane >> 4;
       const int b = blockIdx.z;
       const int split = blockIdx.x;
-      const Reach reach = reach_of(a, kHeld ? a.held[b].length : a.lengths[b]);
-      const int count = reach.count();
+      const int phases = kWaves / a.kv_block;
+      const int phase = wave / a.kv_block;
       const int begin = split * a.run_pages;
+      BatchSequence sequence{};
+      if constexpr (kHeld)
+      {
+        sequence = held.of[b];
+      }
+      const unsigned long long *pages =
+          kHeld ? sequence.pages : a.pages + static_cast<std::size_t>(b) * a.max_pages;
+      const std::uint8_t *tiers =
+          kHeld ? sequence.tiers : a.tiers + static_cast<std::size_t>(b) * a.max_pages;
+      // Without a window the list is the table itself: the wave's first entries
+      // are asked for together with the length, which says whether they count.
+      unsigned long long first_address = 0;
+      int first_tier = kUnreadPage;
+      if (!kHeld && a.window == 0)
+      {
+        const long long entry = static_cast<long long>(begin) + phase + lane * phases;
+        if (lane * phases + phase < a.run_pages && entry < a.max_pages)
+        {
+          first_address = pages[entry];
+          first_tier = tiers[entry];
+        }
+      }
+      const Reach reach = reach_of(a, kHeld ? sequence.length : a.lengths[b]);
+      const int count = reach.count();
       if (split > 0 && begin >= count)
       {
         return; // the join reads no part of this split
       }
       const int end = min(begin + a.run_pages, count);
-      const int phases = kWaves / a.kv_block;
-      const int phase = wave / a.kv_block;
       const int kvh = blockIdx.y * a.kv_block + wave % a.kv_block;
       const int G = a.group;
       const int width = a.kv_heads * HD;
-      const std::size_t run_at = static_cast<std::size_t>(kvh) * HD + g * kRun;
 
-      const unsigned long long *pages =
-          kHeld ? a.held[b].pages : a.pages + static_cast<std::size_t>(b) * a.max_pages;
-      const std::uint8_t *tiers =
-          kHeld ? a.held[b].tiers : a.tiers + static_cast<std::size_t>(b) * a.max_pages;
       // The sequence's own page, where a cache that seals keeps it: the rows
       // before the token's in the page being filled, the token's as given.
-      const bool open = kHeld && a.held[b].open != nullptr;
+      const bool open = kHeld && sequence.open != nullptr;
       const int own_page = open ? (reach.length - 1) / kP : -1;
 
       // Columns past the group repeat its first head and are not stored.
@@ -501,61 +604,73 @@ namespace mi
         run.o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
       }
       unsigned *meta = reinterpret_cast<unsigned *>(lds) + wave * HD;
-      const std::size_t mass_at = (head0 + r) * a.max_pages;
+      const unsigned elem = static_cast<unsigned>(r * width + kvh * HD + g * kRun);
       const bool scored = a.mass != nullptr && r < G;
+      float *mass = a.mass + head0 * a.max_pages;
+      float *mass_from = a.mass_from + head0 * a.max_pages;
+      const unsigned mass_at = static_cast<unsigned>(r) * static_cast<unsigned>(a.max_pages);
 
-      for (int i = begin + phase; i < end; i += phases)
+      // The wave's pages, up to 64 at a time: their table entries are one
+      // lane's each, asked for together.
+      for (int first = begin + phase; first < end; first += 64 * phases)
       {
-        const int page = __builtin_amdgcn_readfirstlane(reach.page(i));
-        const PageAt c{r, g, visible_of(a, reach, page), a.scale,
-                       scored ? a.mass + mass_at + page : nullptr,
-                       scored ? a.mass_from + mass_at + page : nullptr};
-        if (kHeld && page == own_page)
+        unsigned long long address = 0;
+        int tier_of = kUnreadPage;
+        const int entry = first + lane * phases;
+        if (!kHeld && first == begin + phase && a.window == 0)
         {
-          const std::uint16_t *k_row[2], *v_row[2];
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-          {
-            const int row = 16 * h + r;
-            const bool own = page * kP + row == reach.length - 1;
-            k_row[h] = (own ? a.held[b].own_k : a.held[b].open + row * width) + run_at;
-            v_row[h] = (own ? a.held[b].own_v : a.held[b].open + (kP + row) * width) + run_at;
-          }
-          fp16_page<HD>(run, c, q, k_row, v_row);
-          continue;
+          address = first_address;
+          tier_of = first_tier;
         }
-        const unsigned long long address = pages[page];
-        const int tier = address == 0 ? static_cast<int>(kUnreadPage) : static_cast<int>(tiers[page]);
-        const auto *at = reinterpret_cast<const std::uint8_t *>(address);
-        switch (__builtin_amdgcn_readfirstlane(tier))
+        else if (entry < end && reach.page(entry) != own_page)
         {
-        case kFP16:
-        {
-          const std::uint16_t *k_row[2], *v_row[2];
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-          {
-            const auto *rows = reinterpret_cast<const std::uint16_t *>(at) + run_at;
-            k_row[h] = rows + (16 * h + r) * width;
-            v_row[h] = rows + (kP + 16 * h + r) * width;
-          }
-          fp16_page<HD>(run, c, q, k_row, v_row);
-          break;
+          // (The own page of a cache that seals has no entry to read: the
+          // table may end before it.)
+          address = pages[reach.page(entry)];
+          tier_of = tiers[reach.page(entry)];
         }
-        case kINT8:
-          quantised_page<HD, 8>(run, c, q, at, a.lay[kINT8], width, kvh, a.kv_heads, lane, meta);
-          break;
-        case kINT4:
-          quantised_page<HD, 4>(run, c, q, at, a.lay[kINT4], width, kvh, a.kv_heads, lane, meta);
-          break;
-        case kINT2:
-          quantised_page<HD, 2>(run, c, q, at, a.lay[kINT2], width, kvh, a.kv_heads, lane, meta);
-          break;
-        default:
-          if (c.mass != nullptr && g == 0)
+        if (entry >= end || address == 0)
+        {
+          tier_of = kUnreadPage;
+        }
+        const unsigned address_lo = static_cast<unsigned>(address);
+        const unsigned address_hi = static_cast<unsigned>(address >> 32);
+        const int here = min(64, (end - first + phases - 1) / phases);
+        for (int t = 0; t < here; ++t)
+        {
+          const int page = __builtin_amdgcn_readfirstlane(reach.page(first + t * phases));
+          const PageAt c{r, g, visible_of(a, reach, page), a.scale, scored, mass_at + page, mass,
+                         mass_from};
+          if (kHeld && page == own_page)
           {
-            *c.mass = 0.0f;
-            *c.mass_from = 0.0f;
+            fp16_page<HD>(run, c, q, (g_base)(sequence.open), elem, width,
+                          (reach.length - 1) % kP, sequence.own_k, sequence.own_v);
+            continue;
+          }
+          const unsigned long long page_address =
+              static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(address_lo), t)) |
+              static_cast<unsigned long long>(static_cast<unsigned>(
+                  __builtin_amdgcn_readlane(static_cast<int>(address_hi), t)))
+                  << 32;
+          const g_base at = (g_base)(page_address);
+          switch (__builtin_amdgcn_readlane(tier_of, t))
+          {
+          case kFP16: fp16_page<HD>(run, c, q, at, elem, width); break;
+          case kINT8:
+            quantised_page<HD, 8>(run, c, q, at, elem, width, kvh, a.kv_heads, lane, meta);
+            break;
+          case kINT4:
+            quantised_page<HD, 4>(run, c, q, at, elem, width, kvh, a.kv_heads, lane, meta);
+            break;
+          case kINT2:
+            quantised_page<HD, 2>(run, c, q, at, elem, width, kvh, a.kv_heads, lane, meta);
+            break;
+          default:
+            if (scored && g == 0)
+            {
+              mass[c.mass_at] = 0.0f;
+              mass_from[c.mass_at] = 0.0f;
+            }
           }
         }
       }
@@ -657,65 +772,71 @@ namespace mi
       }
     }
 
-    // A head's splits joined: weights 2^(m_s - max m), a wave every fourth
-    // split, a lane hd / 64 channels; then the masses of its pages.
+    // A head's splits joined, weights 2^(m_s - max m); then the masses of its
+    // pages.
     template <int HD, bool kHeld>
-    __global__ void __launch_bounds__(64 * kJoinWaves) batch_join_kernel(BatchArgs a)
+    __global__ void __launch_bounds__(kJoinThreads) batch_join_kernel(BatchArgs a, Sequences<kHeld> held)
     {
-      constexpr int C = HD / 64;
-      __shared__ float s_w[kMaxSplits];
-      __shared__ float s_o[kJoinWaves][HD];
-      __shared__ float s_x[kJoinWaves];
-      const int lane = threadIdx.x & 63;
-      const int wave = threadIdx.x >> 6;
+      __shared__ f32x2 s_ml[kJoinThreads / (HD / 4)];
+      __shared__ __align__(16) float s_o[kJoinThreads / (HD / 4)][HD];
       const int b = blockIdx.y;
       const std::size_t head = static_cast<std::size_t>(b) * a.heads + blockIdx.x;
-      const Reach reach = reach_of(a, kHeld ? a.held[b].length : a.lengths[b]);
+      int length;
+      if constexpr (kHeld)
+      {
+        length = held.of[b].length;
+      }
+      else
+      {
+        length = a.lengths[b];
+      }
+      const Reach reach = reach_of(a, length);
       const int live = (reach.count() + a.run_pages - 1) / a.run_pages;
-      const float *ml = a.parts_ml + 2 * head * a.splits;
-      float top = -INFINITY;
-      for (int s = threadIdx.x; s < live; s += 64 * kJoinWaves)
+      // Groups of lanes, sixteen bytes a lane of a split's outputs, each with a
+      // running maximum of its own, so that nothing waits for a first pass.
+      constexpr int kLanes = HD / 4, kGroups = kJoinThreads / kLanes;
+      const int group = threadIdx.x / kLanes;
+      const int d = 4 * (threadIdx.x % kLanes);
+      float m = -INFINITY, l = 0.0f;
+      f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+      for (int s = group; s < live; s += kGroups)
       {
-        top = fmaxf(top, ml[2 * s]);
+        const std::size_t part = head * a.splits + s;
+        const f32x2 ml = *reinterpret_cast<const f32x2 *>(a.parts_ml + 2 * part);
+        const f32x4 x = *reinterpret_cast<const f32x4 *>(a.parts_o + part * HD + d);
+        const float top = fmaxf(m, ml[0]);
+        const float from = top == -INFINITY ? 0.0f : top;
+        const float keep = __builtin_amdgcn_exp2f(m - from), w = __builtin_amdgcn_exp2f(ml[0] - from);
+        l = l * keep + ml[1] * w;
+        o = o * keep + x * w;
+        m = top;
       }
-      top = block_reduce<true>(top, s_x);
-      const float from = top == -INFINITY ? 0.0f : top;
-      float sum = 0.0f;
-      for (int s = threadIdx.x; s < live; s += 64 * kJoinWaves)
+      if (d == 0)
       {
-        const float w = __builtin_amdgcn_exp2f(ml[2 * s] - from);
-        s_w[s] = w;
-        sum += ml[2 * s + 1] * w;
+        s_ml[group] = f32x2{m, l};
       }
-      sum = block_reduce<false>(sum, s_x); // (its barriers order s_w too)
-      float o[C] = {};
-      const float *part = a.parts_o + head * a.splits * HD + lane;
-#pragma unroll 4
-      for (int s = wave; s < live; s += kJoinWaves)
-      {
-        const float w = s_w[s];
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-        {
-          o[c] += part[static_cast<std::size_t>(s) * HD + 64 * c] * w;
-        }
-      }
-#pragma unroll
-      for (int c = 0; c < C; ++c)
-      {
-        s_o[wave][lane + 64 * c] = o[c];
-      }
+      *reinterpret_cast<f32x4 *>(&s_o[group][d]) = o;
       __syncthreads();
-      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-      for (int d = threadIdx.x; d < HD; d += 64 * kJoinWaves)
-      {
-        float v = s_o[0][d];
+      float from = -INFINITY;
 #pragma unroll
-        for (int w = 1; w < kJoinWaves; ++w)
-        {
-          v += s_o[w][d];
-        }
-        a.out[head * HD + d] = __half_as_ushort(__float2half(v * inv));
+      for (int i = 0; i < kGroups; ++i)
+      {
+        from = fmaxf(from, s_ml[i][0]);
+      }
+      from = from == -INFINITY ? 0.0f : from;
+      float sum = 0.0f, out = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i)
+      {
+        const float w = __builtin_amdgcn_exp2f(s_ml[i][0] - from);
+        sum += s_ml[i][1] * w;
+        out += s_o[i][threadIdx.x % HD] * w;
+      }
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      if (threadIdx.x < HD)
+      {
+        a.out[head * HD + threadIdx.x] = __half_as_ushort(__float2half(out * inv));
       }
       if (a.mass == nullptr)
       {
@@ -723,7 +844,7 @@ namespace mi
       }
       float *mass = a.mass + head * a.max_pages;
       const float *held_from = a.mass_from + head * a.max_pages;
-      for (int p = threadIdx.x; p < a.max_pages; p += 64 * kJoinWaves)
+      for (int p = threadIdx.x; p < a.max_pages; p += kJoinThreads)
       {
         mass[p] = reach.has(p) ? mass_of(mass[p], held_from[p], from, inv) : 0.0f;
       }
@@ -753,8 +874,9 @@ namespace mi
                                              (static_cast<long long>(window) + kP - 2) / kP + 1);
       }
       most = std::max<long long>(most, 1);
-      // Four workgroups a CU over the batch, each wave at least a page.
-      constexpr long long kWorkgroups = 1024;
+      // Eight workgroups a CU over the batch if every sequence is as long as it
+      // can be, each wave at least a page.
+      constexpr long long kWorkgroups = 2048;
       const long long units = most * batch * (kv_heads / c.kv_block);
       long long run = std::max<long long>((units + kWorkgroups - 1) / kWorkgroups,
                                           (most + kMaxSplits - 1) / kMaxSplits);
@@ -796,19 +918,19 @@ namespace mi
     }
 
     template <int HD, bool kHeld>
-    void launch(BatchArgs a, int batch, hipStream_t stream)
+    void launch(const BatchArgs &a, const Sequences<kHeld> &held, int batch, hipStream_t stream)
     {
       const int phases = kWaves / a.kv_block;
       const std::size_t lds =
           sizeof(float) * (kMetaFloats<HD> + (phases - 1) * a.kv_block * kWaveFloats<HD> +
                            kHeadFloats);
       const dim3 grid(a.splits, a.kv_heads / a.kv_block, batch);
-      batch_pages_kernel<HD, kHeld><<<grid, kThreads, lds, stream>>>(a);
+      batch_pages_kernel<HD, kHeld><<<grid, kThreads, lds, stream>>>(a, held);
       hip_check(hipGetLastError(), "batch_pages_kernel");
       if (a.splits > 1)
       {
         batch_join_kernel<HD, kHeld>
-            <<<dim3(a.heads, batch), 64 * kJoinWaves, 0, stream>>>(a);
+            <<<dim3(a.heads, batch), kJoinThreads, 0, stream>>>(a, held);
         hip_check(hipGetLastError(), "batch_join_kernel");
       }
     }
@@ -888,14 +1010,10 @@ namespace mi
       parts = a.parts_ml + rows * cut.splits * 2;
     }
     a.mass_from = parts;
-    for (int tier = kINT8; tier < kTierCount; ++tier)
-    {
-      a.lay[tier] = page_layout(tier, kP, t.kv_heads, t.head_dim);
-    }
     if (t.held == nullptr)
     {
-      t.head_dim == 64 ? launch<64, false>(a, t.batch, stream)
-                       : launch<128, false>(a, t.batch, stream);
+      t.head_dim == 64 ? launch<64, false>(a, {}, t.batch, stream)
+                       : launch<128, false>(a, {}, t.batch, stream);
       return;
     }
     // The sequences go with the launch, kBatchHeld at a time.
@@ -911,8 +1029,10 @@ namespace mi
         part.mass += at * per * t.max_pages;
         part.mass_from += at * per * t.max_pages;
       }
-      std::copy(t.held + at, t.held + at + n, part.held);
-      t.head_dim == 64 ? launch<64, true>(part, n, stream) : launch<128, true>(part, n, stream);
+      Sequences<true> held{};
+      std::copy(t.held + at, t.held + at + n, held.of);
+      t.head_dim == 64 ? launch<64, true>(part, held, n, stream)
+                       : launch<128, true>(part, held, n, stream);
     }
   }
 
