@@ -380,8 +380,9 @@ namespace mi
               const f32x2 w = {
                   __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][j][i], a.scale, -from)),
                   __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][j][i + 1], a.scale, -from))};
-              sum += w[0] + w[1];
               const half2v h = __builtin_convertvector(w, half2v);
+              const _Float16 one = static_cast<_Float16>(1.0f);
+              sum = __builtin_amdgcn_fdot2(h, half2v{one, one}, sum, false);
               p[t][j][i / 8][i % 8] = h[0];
               p[t][j][i / 8][i % 8 + 1] = h[1];
             }
@@ -557,7 +558,7 @@ namespace mi
 
     constexpr int kFewRows = 32, kFewKeys = 32, kManyKeys = 64, kManyWaves = 4;
     template <int HD>
-    constexpr int kRowTiles = HD == 64 ? 2 : 1;
+    constexpr int kRowTiles = 1;
 
     Cut cut_of(const WindowAttention &t, bool may_split)
     {
