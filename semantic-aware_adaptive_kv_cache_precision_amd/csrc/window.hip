@@ -6,11 +6,11 @@
 // sqrt(hd)) v over those; every query sees itself at least.
 //
 // A workgroup takes one KV head and consecutive (query, head) rows of its
-// group, query by query, so that its rows' windows nearly coincide; 32 * RT
-// rows a wave. Steps of kKeys keys, of which only those some row of the
-// workgroup sees are taken (the sink steps, then the window's), pass through
-// LDS, double buffered, copied there directly from memory. In the matrix
-// cores' terms, with keys as M and rows as N:
+// group, query by query, so that its rows' windows nearly coincide; 32 rows a
+// wave. Steps of kKeys keys, of which only those some row of the workgroup
+// sees are taken (the sink steps, then the window's), pass through LDS, double
+// buffered, copied there directly from memory. In the matrix cores' terms,
+// with keys as M and rows as N:
 //   S^T (32 keys x 32 rows) = K . Q^T      lane l holds row l % 32
 //   O^T (32 channels x 32 rows) += V^T . P^T  P from the lane's own scores,
 //                                             V^T by transposing LDS reads
@@ -22,13 +22,27 @@
 // pieces), meet no bank twice.
 //
 // P is rounded to fp16 once (half a step is 2^-11 of a weight, as much as the
-// output's own rounding; the sums are of the unrounded weights), held against
-// a reference that is moved up only when a score passes it by 2^kRise: P is at
-// most 2^(kRise + kProb) = 2^14, and a weight keeps its 11 bits down to 2^-22
-// of the reference.
+// output's own rounding; the sums are of the rounded weights, so that the
+// output stays an average of the values), held against a reference that is
+// moved up only when a score passes it by 2^kRise: P is at most
+// 2^(kRise + kProb) = 2^14, and a weight keeps its 11 bits down to 2^-22 of
+// the reference.
 //
 // With few rows the range of keys is split over workgroups, whose parts a
 // second launch joins.
+//
+// Bound by a SIMD's two waves taking turns at the matrix cores and the softmax
+// (exponentials 20%, sums 10%, first product 25% of the time, which add up).
+// 2,048 queries x 32 heads at 14,336 behind a 4,096-token window with 4 sinks,
+// head_dim 64: 110 us, 622 TFLOP/s, the matrix cores busy 62% of it. A prompt
+// of 4,096 x 12 heads of 128 behind 1,024: 57 us, 396 TFLOP/s, its 384
+// workgroups leaving half the CUs one instead of two. 100 queries x 14 heads
+// of 64: 9.4 us, two launches. Measured and not taken: 64 rows a wave (158 us
+// for the first of these, one wave a SIMD), the next step's first product
+// beside this step's exponentials (the same at head_dim 64; 90 us for the
+// second, out of registers), addresses a lane keeps instead of making (the
+// same), KV heads first in the order of workgroups (the same, 95% of reads
+// meet the L2 either way).
 
 #include "common.hpp"
 #include "kernels.hpp"
@@ -171,13 +185,13 @@ namespace mi
       }
     };
 
-    template <int HD, int RT, int NW, int kKeys>
+    template <int HD, int NW, int kKeys>
     __global__ void __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) window_kernel(WindowArgs a)
     {
       constexpr int kPieces = HD / 8;          // 16-byte pieces a row
       constexpr int kTile = kKeys * HD;        // halves of a step's keys
       constexpr int kStage = 2 * kTile;        // keys, then values
-      constexpr int kRows = 32 * RT * NW;      // rows a workgroup
+      constexpr int kRows = 32 * NW;           // rows a workgroup
       constexpr int N = kKeys / 32;
       extern __shared__ __align__(16) std::uint16_t stages[]; // two of kStage
 
@@ -206,43 +220,36 @@ namespace mi
       const int begin = min(split * per, steps.count);
       const int end = min(begin + per, steps.count);
 
-      bool valid[RT];
-      int pos[RT];
-      std::size_t row_at[RT]; // query * heads + head
-      half8 q[RT][HD / 16];
-      Rows<HD> run[RT];
-#pragma unroll
-      for (int t = 0; t < RT; ++t)
-      {
-        const long long row = row0 + 32 * (RT * wave + t) + n;
-        valid[t] = row < all_rows;
-        const int query = valid[t] ? static_cast<int>(row / G) : 0;
-        const int head = kvh * G + (valid[t] ? static_cast<int>(row % G) : 0);
-        pos[t] = past + query;
-        row_at[t] = static_cast<std::size_t>(query) * a.heads + head;
-        const std::uint16_t *from = a.q + query * a.q_stride + head * HD + 8 * half;
-#pragma unroll
-        for (int c = 0; c < HD / 16; ++c)
-        {
-          q[t][c] = as_half8(*reinterpret_cast<const u32x4 *>(from + 16 * c));
-        }
-        run[t].m = -INFINITY;
-        run[t].l = 0.0f;
-#pragma unroll
-        for (int d = 0; d < HD / 32; ++d)
-        {
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-          {
-            run[t].o[d][i] = 0.0f;
-          }
-        }
-      }
-      // The wave's positions (a wave past the rows computes nothing).
-      const long long wave_row = row0 + 32 * RT * wave;
+      // The wave's rows (a wave past the last computes nothing), and the lane's.
+      const long long wave_row = row0 + 32 * wave;
       const bool computes = wave_row < all_rows;
       const int wave_lo = past + static_cast<int>(min(wave_row, all_rows - 1) / G);
-      const int wave_hi = past + static_cast<int>((min(wave_row + 32 * RT, all_rows) - 1) / G);
+      const int wave_hi = past + static_cast<int>((min(wave_row + 32, all_rows) - 1) / G);
+      const long long row = wave_row + n;
+      const bool valid = row < all_rows;
+      const int query = valid ? static_cast<int>(row / G) : 0;
+      const int head = kvh * G + (valid ? static_cast<int>(row % G) : 0);
+      const int pos = past + query;
+      const std::size_t row_at = static_cast<std::size_t>(query) * a.heads + head;
+      half8 q[HD / 16];
+      const std::uint16_t *q_row = a.q + query * a.q_stride + head * HD + 8 * half;
+#pragma unroll
+      for (int c = 0; c < HD / 16; ++c)
+      {
+        q[c] = as_half8(*reinterpret_cast<const u32x4 *>(q_row + 16 * c));
+      }
+      Rows<HD> run;
+      run.m = -INFINITY;
+      run.l = 0.0f;
+#pragma unroll
+      for (int d = 0; d < HD / 32; ++d)
+      {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+        {
+          run.o[d][i] = 0.0f;
+        }
+      }
 
       // A step's rows to LDS, 16 bytes a lane; rows past the last repeat it.
       const auto copy = [&](int step, int buf) {
@@ -254,12 +261,12 @@ namespace mi
           const int place = (i * NW + wave) * 64 + lane;
           const int t = place / kPieces;
           const int c = (place % kPieces) ^ swizzle<HD>(t);
-          const long long row = min(key0 + t, a.seq_k - 1);
+          const long long key = min(key0 + t, a.seq_k - 1);
           std::uint16_t *to = stage + (i * NW + wave) * 512;
           __builtin_amdgcn_global_load_lds(
-              (global_void)(a.k + row * a.k_stride + kvh * HD + 8 * c), (lds_void)(to), 16, 0, 0);
+              (global_void)(a.k + key * a.k_stride + kvh * HD + 8 * c), (lds_void)(to), 16, 0, 0);
           __builtin_amdgcn_global_load_lds(
-              (global_void)(a.v + row * a.v_stride + kvh * HD + 8 * c), (lds_void)(to + kTile), 16,
+              (global_void)(a.v + key * a.v_stride + kvh * HD + 8 * c), (lds_void)(to + kTile), 16,
               0, 0);
         }
       };
@@ -289,18 +296,14 @@ namespace mi
         }
         const std::uint16_t *keys = stages + buf * kStage;
         const std::uint16_t *values = keys + kTile;
-        f32x16 s[RT][N];
+        f32x16 s[N];
 #pragma unroll
-        for (int t = 0; t < RT; ++t)
+        for (int j = 0; j < N; ++j)
         {
 #pragma unroll
-          for (int j = 0; j < N; ++j)
+          for (int i = 0; i < 16; ++i)
           {
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-            {
-              s[t][j][i] = 0.0f;
-            }
+            s[j][i] = 0.0f;
           }
         }
 #pragma unroll
@@ -312,11 +315,7 @@ namespace mi
             const int t0 = 32 * j + n;
             const half8 k = as_half8(*reinterpret_cast<const u32x4 *>(
                 keys + t0 * HD + 8 * ((2 * c + half) ^ swizzle<HD>(t0))));
-#pragma unroll
-            for (int t = 0; t < RT; ++t)
-            {
-              s[t][j] = mfma32(k, q[t][c], s[t][j]);
-            }
+            s[j] = mfma32(k, q[c], s[j]);
           }
         }
         // Whether some row of the wave does not see some key of the step.
@@ -325,70 +324,62 @@ namespace mi
                            key0 + kKeys > a.sinks);
         if (edge)
         {
-#pragma unroll
-          for (int t = 0; t < RT; ++t)
-          {
-            const int from = a.window > 0 ? pos[t] - a.window : -1; // keys after it are seen
-#pragma unroll
-            for (int j = 0; j < N; ++j)
-            {
-#pragma unroll
-              for (int i = 0; i < 16; ++i)
-              {
-                const int key = key0 + 32 * j + 8 * (i / 4) + 4 * half + i % 4;
-                const bool seen = key <= pos[t] && (key > from || key < a.sinks);
-                s[t][j][i] = seen ? s[t][j][i] : -INFINITY;
-              }
-            }
-          }
-        }
-        half8 p[RT][N][2];
-#pragma unroll
-        for (int t = 0; t < RT; ++t)
-        {
-          float top = s[t][0][0];
+          const int from = a.window > 0 ? pos - a.window : -1; // keys after it are seen
 #pragma unroll
           for (int j = 0; j < N; ++j)
           {
 #pragma unroll
             for (int i = 0; i < 16; ++i)
             {
-              top = fmaxf(top, s[t][j][i]);
+              const int key = key0 + 32 * j + 8 * (i / 4) + 4 * half + i % 4;
+              const bool seen = key <= pos && (key > from || key < a.sinks);
+              s[j][i] = seen ? s[j][i] : -INFINITY;
             }
           }
-          top = lane_max32(top) * a.scale;
-          if (__any(top > run[t].m + kRise))
-          {
-            const float m = fmaxf(run[t].m, top);
-            const float keep = run[t].m == m ? 1.0f : __builtin_amdgcn_exp2f(run[t].m - m);
-            run[t].m = m;
-            run[t].l *= keep;
-#pragma unroll
-            for (int d = 0; d < HD / 32; ++d)
-            {
-              run[t].o[d] *= keep;
-            }
-          }
-          const float from = (run[t].m == -INFINITY ? 0.0f : run[t].m) - kProb;
-          float sum = 0.0f;
-#pragma unroll
-          for (int j = 0; j < N; ++j)
-          {
-#pragma unroll
-            for (int i = 0; i < 16; i += 2)
-            {
-              const f32x2 w = {
-                  __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][j][i], a.scale, -from)),
-                  __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][j][i + 1], a.scale, -from))};
-              const half2v h = __builtin_convertvector(w, half2v);
-              const _Float16 one = static_cast<_Float16>(1.0f);
-              sum = __builtin_amdgcn_fdot2(h, half2v{one, one}, sum, false);
-              p[t][j][i / 8][i % 8] = h[0];
-              p[t][j][i / 8][i % 8 + 1] = h[1];
-            }
-          }
-          run[t].l += sum;
         }
+        half8 p[N][2];
+        float top = s[0][0];
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+        {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+          {
+            top = fmaxf(top, s[j][i]);
+          }
+        }
+        top = lane_max32(top) * a.scale;
+        if (__any(top > run.m + kRise))
+        {
+          const float m = fmaxf(run.m, top);
+          const float keep = run.m == m ? 1.0f : __builtin_amdgcn_exp2f(run.m - m);
+          run.m = m;
+          run.l *= keep;
+#pragma unroll
+          for (int d = 0; d < HD / 32; ++d)
+          {
+            run.o[d] *= keep;
+          }
+        }
+        const float from = (run.m == -INFINITY ? 0.0f : run.m) - kProb;
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+        {
+#pragma unroll
+          for (int i = 0; i < 16; i += 2)
+          {
+            const f32x2 w = {
+                __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][i], a.scale, -from)),
+                __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][i + 1], a.scale, -from))};
+            const half2v h = __builtin_convertvector(w, half2v);
+            const _Float16 one = static_cast<_Float16>(1.0f);
+            sum = __builtin_amdgcn_fdot2(h, half2v{one, one}, sum, false);
+            p[j][i / 8][i % 8] = h[0];
+            p[j][i / 8][i % 8 + 1] = h[1];
+          }
+        }
+        run.l += sum;
         // A value some row does not see may be anything: if one of an edge
         // step's is not finite, the products take it as zero, and the rows
         // that do see it add it after them.
@@ -420,11 +411,7 @@ namespace mi
               {
                 vt = finite_only(vt);
               }
-#pragma unroll
-              for (int t = 0; t < RT; ++t)
-              {
-                run[t].o[d] = mfma32(vt, p[t][j][u], run[t].o[d]);
-              }
+              run.o[d] = mfma32(vt, p[j][u], run.o[d]);
             }
           }
         }
@@ -432,7 +419,7 @@ namespace mi
         {
           for (int key = key0; key < min(key0 + kKeys, a.seq_k); ++key)
           {
-            const std::uint16_t *row = values + (key - key0) * HD;
+            const std::uint16_t *spoilt_row = values + (key - key0) * HD;
             const int swap = swizzle<HD>(key - key0);
 #pragma unroll
             for (int d = 0; d < HD / 32; ++d)
@@ -441,70 +428,61 @@ namespace mi
               for (int i = 0; i < 16; ++i)
               {
                 const int ch = 32 * d + 8 * (i / 4) + 4 * half + i % 4;
-                const std::uint16_t v = row[8 * ((ch / 8) ^ swap) + ch % 8];
-#pragma unroll
-                for (int t = 0; t < RT; ++t)
-                {
-                  const bool seen = key <= pos[t] && (a.window == 0 || key > pos[t] - a.window ||
-                                                      key < a.sinks);
-                  run[t].o[d][i] += seen && !is_finite(v) ? h2f(v) : 0.0f;
-                }
+                const std::uint16_t v = spoilt_row[8 * ((ch / 8) ^ swap) + ch % 8];
+                const bool seen = key <= pos && (a.window == 0 || key > pos - a.window ||
+                                                 key < a.sinks);
+                run.o[d][i] += seen && !is_finite(v) ? h2f(v) : 0.0f;
               }
             }
           }
         }
       }
 
-#pragma unroll
-      for (int t = 0; t < RT; ++t)
+      const float sum = lane_sum32(run.l) * kProbUnscale;
+      if (!valid)
       {
-        const float sum = lane_sum32(run[t].l) * kProbUnscale;
-        if (!valid[t])
-        {
-          continue;
-        }
-        if (a.splits == 1)
-        {
-          const float inv = kProbUnscale / sum;
-          std::uint16_t *out = a.out + row_at[t] * HD + 4 * half;
-#pragma unroll
-          for (int d = 0; d < HD / 32; ++d)
-          {
-#pragma unroll
-            for (int b = 0; b < 4; ++b)
-            {
-              const f32x16 &o = run[t].o[d];
-              const half2v x = {static_cast<_Float16>(o[4 * b] * inv),
-                                static_cast<_Float16>(o[4 * b + 1] * inv)};
-              const half2v y = {static_cast<_Float16>(o[4 * b + 2] * inv),
-                                static_cast<_Float16>(o[4 * b + 3] * inv)};
-              *reinterpret_cast<u32x2 *>(out + 32 * d + 8 * b) =
-                  u32x2{__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, y)};
-            }
-          }
-          continue;
-        }
-        const std::size_t at =
-            static_cast<std::size_t>(split) * a.seq_q * a.heads + row_at[t];
-        if (half == 0)
-        {
-          *reinterpret_cast<f32x2 *>(a.part_ml + 2 * at) = f32x2{run[t].m, sum};
-        }
-        float *out = a.part_o + at * HD + 4 * half;
+        return;
+      }
+      if (a.splits == 1)
+      {
+        const float inv = kProbUnscale / sum;
+        std::uint16_t *out = a.out + row_at * HD + 4 * half;
 #pragma unroll
         for (int d = 0; d < HD / 32; ++d)
         {
 #pragma unroll
           for (int b = 0; b < 4; ++b)
           {
-            f32x4 x;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-            {
-              x[i] = run[t].o[d][4 * b + i] * kProbUnscale;
-            }
-            *reinterpret_cast<f32x4 *>(out + 32 * d + 8 * b) = x;
+            const f32x16 &o = run.o[d];
+            const half2v x = {static_cast<_Float16>(o[4 * b] * inv),
+                              static_cast<_Float16>(o[4 * b + 1] * inv)};
+            const half2v y = {static_cast<_Float16>(o[4 * b + 2] * inv),
+                              static_cast<_Float16>(o[4 * b + 3] * inv)};
+            *reinterpret_cast<u32x2 *>(out + 32 * d + 8 * b) =
+                u32x2{__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, y)};
           }
+        }
+        return;
+      }
+      const std::size_t at = static_cast<std::size_t>(split) * a.seq_q * a.heads + row_at;
+      if (half == 0)
+      {
+        *reinterpret_cast<f32x2 *>(a.part_ml + 2 * at) = f32x2{run.m, sum};
+      }
+      float *out = a.part_o + at * HD + 4 * half;
+#pragma unroll
+      for (int d = 0; d < HD / 32; ++d)
+      {
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+        {
+          f32x4 x;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+          {
+            x[i] = run.o[d][4 * b + i] * kProbUnscale;
+          }
+          *reinterpret_cast<f32x4 *>(out + 32 * d + 8 * b) = x;
         }
       }
     }
@@ -557,8 +535,6 @@ namespace mi
     };
 
     constexpr int kFewRows = 32, kFewKeys = 32, kManyKeys = 64, kManyWaves = 4;
-    template <int HD>
-    constexpr int kRowTiles = 1;
 
     Cut cut_of(const WindowAttention &t, bool may_split)
     {
@@ -567,8 +543,7 @@ namespace mi
       Cut c{};
       const long long few = (rows + kFewRows - 1) / kFewRows;
       c.few = few * t.kv_heads <= 512;
-      const int tiles = t.head_dim == 64 ? kRowTiles<64> : kRowTiles<128>;
-      c.rows = c.few ? kFewRows : 32 * tiles * kManyWaves;
+      c.rows = c.few ? kFewRows : 32 * kManyWaves;
       c.keys = c.few ? kFewKeys : kManyKeys;
       c.blocks = static_cast<int>((rows + c.rows - 1) / c.rows);
       c.splits = 1;
@@ -622,11 +597,11 @@ namespace mi
       }
     }
 
-    template <int HD, int RT, int NW, int kKeys>
+    template <int HD, int NW, int kKeys>
     void launch(const WindowArgs &a, const Cut &c, hipStream_t stream)
     {
       const std::size_t lds = sizeof(std::uint16_t) * 2 * 2 * kKeys * HD;
-      window_kernel<HD, RT, NW, kKeys>
+      window_kernel<HD, NW, kKeys>
           <<<dim3(c.blocks, a.kv_heads, c.splits), 64 * NW, lds, stream>>>(a);
       hip_check(hipGetLastError(), "window_kernel");
     }
@@ -636,11 +611,11 @@ namespace mi
     {
       if (c.few)
       {
-        launch<HD, 1, 1, kFewKeys>(a, c, stream);
+        launch<HD, 1, kFewKeys>(a, c, stream);
       }
       else
       {
-        launch<HD, kRowTiles<HD>, kManyWaves, kManyKeys>(a, c, stream);
+        launch<HD, kManyWaves, kManyKeys>(a, c, stream);
       }
       if (c.splits > 1)
       {

@@ -63,7 +63,7 @@ def test_an_empty_batch_is_done_and_caches_must_match_their_positions():
 def test_partials_grow_with_what_is_asked():
     from microinfer import _microinfer as m
     need = m.device.attention_batch_partials
-    assert need(4, 4, 4, 2, 64) == 0  # one run a sequence
+    assert need(4, 2, 4, 2, 64) == 0  # one run a sequence
     assert need(1, 1024, 12, 2, 128) > 0
     assert need(1, 1024, 12, 2, 128, mass=True) == need(1, 1024, 12, 2, 128) + 12 * 1024
     assert need(1, 1024, 12, 2, 128, window=64, sinks=4) < need(1, 1024, 12, 2, 128)
