@@ -51,6 +51,7 @@
 #include <algorithm>
 #include <cmath>
 #include <string>
+#include <type_traits>
 
 namespace mi
 {
@@ -185,18 +186,25 @@ namespace mi
       }
     };
 
-    template <int HD, int NW, int kKeys>
-    __global__ void __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) window_kernel(WindowArgs a)
+    template <int HD, int kTiles, int kWays>
+    constexpr int kWavesASimd = HD == 64 && kTiles > 1 ? 2 * kWays : kTiles > 1 ? 2 : 1;
+
+    template <int HD, int kTiles, int kWays, int kKeys>
+    __global__ void __launch_bounds__(64 * kTiles * kWays, (kWavesASimd<HD, kTiles, kWays>))
+        window_kernel(WindowArgs a)
     {
+      constexpr int NW = kTiles * kWays;
       constexpr int kPieces = HD / 8;          // 16-byte pieces a row
       constexpr int kTile = kKeys * HD;        // halves of a step's keys
       constexpr int kStage = 2 * kTile;        // keys, then values
-      constexpr int kRows = 32 * NW;           // rows a workgroup
-      constexpr int N = kKeys / 32;
+      constexpr int kRows = 32 * kTiles;       // rows a workgroup
+      constexpr int kWayKeys = kKeys / kWays;
+      constexpr int N = kWayKeys / 32;
       extern __shared__ __align__(16) std::uint16_t stages[]; // two of kStage
 
       const int lane = threadIdx.x & 63;
       const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+      const int way = wave / kTiles;
       const int n = lane & 31;
       const int half = lane >> 5;
       const int kvh = blockIdx.y;
@@ -221,7 +229,7 @@ namespace mi
       const int end = min(begin + per, steps.count);
 
       // The wave's rows (a wave past the last computes nothing), and the lane's.
-      const long long wave_row = row0 + 32 * wave;
+      const long long wave_row = row0 + 32 * (wave % kTiles);
       const bool computes = wave_row < all_rows;
       const int wave_lo = past + static_cast<int>(min(wave_row, all_rows - 1) / G);
       const int wave_hi = past + static_cast<int>((min(wave_row + 32, all_rows) - 1) / G);
@@ -286,15 +294,15 @@ namespace mi
         {
           copy(step + 1, buf ^ 1);
         }
-        const int key0 = steps.key(step, kKeys);
+        const int key0 = steps.key(step, kKeys) + way * kWayKeys;
         const bool sees = key0 <= wave_hi &&
-                          (a.window == 0 || key0 + kKeys - 1 > wave_lo - a.window ||
+                          (a.window == 0 || key0 + kWayKeys - 1 > wave_lo - a.window ||
                            key0 < a.sinks);
         if (!computes || !sees)
         {
           continue;
         }
-        const std::uint16_t *keys = stages + buf * kStage;
+        const std::uint16_t *keys = stages + buf * kStage + way * kWayKeys * HD;
         const std::uint16_t *values = keys + kTile;
         f32x16 s[N];
 #pragma unroll
@@ -319,9 +327,9 @@ namespace mi
           }
         }
         // Whether some row of the wave does not see some key of the step.
-        const bool edge = key0 + kKeys - 1 > wave_lo ||
+        const bool edge = key0 + kWayKeys - 1 > wave_lo ||
                           (a.window > 0 && key0 <= wave_hi - a.window &&
-                           key0 + kKeys > a.sinks);
+                           key0 + kWayKeys > a.sinks);
         if (edge)
         {
           const int from = a.window > 0 ? pos - a.window : -1; // keys after it are seen
@@ -383,7 +391,7 @@ namespace mi
         // A value some row does not see may be anything: if one of an edge
         // step's is not finite, the products take it as zero, and the rows
         // that do see it add it after them.
-        const bool spoilt = edge && !finite_values<HD, kKeys>(values, lane);
+        const bool spoilt = edge && !finite_values<HD, kWayKeys>(values, lane);
         // Lane l's P of a 16-key product: keys 8 e + 4 half + {0..3}, e = 0, 1.
 #pragma unroll
         for (int j = 0; j < N; ++j)
@@ -417,7 +425,7 @@ namespace mi
         }
         if (spoilt)
         {
-          for (int key = key0; key < min(key0 + kKeys, a.seq_k); ++key)
+          for (int key = key0; key < min(key0 + kWayKeys, a.seq_k); ++key)
           {
             const std::uint16_t *spoilt_row = values + (key - key0) * HD;
             const int swap = swizzle<HD>(key - key0);
@@ -438,6 +446,59 @@ namespace mi
         }
       }
 
+      if constexpr (kWays > 1)
+      {
+        // The ways' sums joined by the first way's wave.
+        constexpr int kHeld = (HD / 2 + 2) * 64; // floats a wave leaves
+        float *left = reinterpret_cast<float *>(stages);
+        __syncthreads();
+        if (way > 0)
+        {
+          float *to = left + (wave - kTiles) * kHeld + lane;
+          to[0] = run.m;
+          to[64] = run.l;
+#pragma unroll
+          for (int i = 0; i < HD / 2; ++i)
+          {
+            to[64 * (2 + i)] = run.o[i / 16][i % 16];
+          }
+        }
+        __syncthreads();
+        if (way > 0)
+        {
+          return;
+        }
+        float m[kWays];
+        m[0] = run.m;
+        float top = run.m;
+#pragma unroll
+        for (int w = 1; w < kWays; ++w)
+        {
+          m[w] = left[((w - 1) * kTiles + wave) * kHeld + lane];
+          top = fmaxf(top, m[w]);
+        }
+        const float keep = m[0] == top ? 1.0f : __builtin_amdgcn_exp2f(m[0] - top);
+        run.m = top;
+        run.l *= keep;
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d)
+        {
+          run.o[d] *= keep;
+        }
+#pragma unroll
+        for (int w = 1; w < kWays; ++w)
+        {
+          const float *from = left + ((w - 1) * kTiles + wave) * kHeld + lane;
+          const float weight = m[w] == top ? 1.0f : __builtin_amdgcn_exp2f(m[w] - top);
+          run.l = __builtin_fmaf(from[64], weight, run.l);
+#pragma unroll
+          for (int i = 0; i < HD / 2; ++i)
+          {
+            run.o[i / 16][i % 16] =
+                __builtin_fmaf(from[64 * (2 + i)], weight, run.o[i / 16][i % 16]);
+          }
+        }
+      }
       const float sum = lane_sum32(run.l) * kProbUnscale;
       if (!valid)
       {
@@ -523,43 +584,49 @@ namespace mi
           u32x2{__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, y)};
     }
 
-    // How a launch is cut: the rows and keys of a workgroup's tile, and the
-    // workgroups a row's keys are split over.
+    // A launch's form: the row tiles of a workgroup, the waves that share a
+    // tile's keys, and the keys a step.
+    template <int kTiles_, int kWays_, int kKeys_>
+    struct Form
+    {
+      static constexpr int tiles = kTiles_, ways = kWays_, keys = kKeys_, rows = 32 * kTiles_;
+    };
+    using Few = Form<1, 4, 128>;
+    using Many64 = Form<4, 2, 64>;
+    using Many128 = Form<4, 1, 64>;
+
+    // How a launch is cut.
     struct Cut
     {
-      bool few; // a wave of 32 rows a workgroup, 32 keys a step
-      int rows;
+      bool few;
+      int rows; // a workgroup's rows, and keys a step
       int keys;
       int blocks; // workgroups over the rows, a KV head
-      int splits;
+      int splits; // workgroups over a row's keys
     };
-
-    constexpr int kFewRows = 32, kFewKeys = 32, kManyKeys = 64, kManyWaves = 4;
 
     Cut cut_of(const WindowAttention &t, bool may_split)
     {
       const int group = t.heads / t.kv_heads;
       const long long rows = static_cast<long long>(t.seq_q) * group;
       Cut c{};
-      const long long few = (rows + kFewRows - 1) / kFewRows;
-      c.few = few * t.kv_heads <= 512;
-      c.rows = c.few ? kFewRows : 32 * kManyWaves;
-      c.keys = c.few ? kFewKeys : kManyKeys;
+      c.few = (rows + Few::rows - 1) / Few::rows * t.kv_heads <= 512;
+      c.rows = c.few ? Few::rows : t.head_dim == 64 ? Many64::rows : Many128::rows;
+      c.keys = c.few ? Few::keys : t.head_dim == 64 ? Many64::keys : Many128::keys;
       c.blocks = static_cast<int>((rows + c.rows - 1) / c.rows);
       c.splits = 1;
       if (may_split && c.blocks > 0)
       {
         // The most steps a workgroup takes.
-        long long steps = (t.seq_k + c.keys - 1) / c.keys;
+        long long steps = (static_cast<long long>(t.seq_k) + c.keys - 1) / c.keys;
         if (t.window > 0)
         {
           const long long span = static_cast<long long>(t.window) + (c.rows - 1) / group + 1;
           steps = std::min(steps, (span + c.keys - 1) / c.keys + 1 +
                                       (static_cast<long long>(t.sinks) + c.keys - 1) / c.keys);
         }
-        // Four workgroups of a wave, or one of four, a CU, each with four
-        // steps to take.
-        const long long fill = (c.few ? 1024 : 256) / (static_cast<long long>(c.blocks) * t.kv_heads);
+        // A workgroup a CU, each with four steps to take.
+        const long long fill = 256 / (static_cast<long long>(c.blocks) * t.kv_heads);
         c.splits = static_cast<int>(
             std::max<long long>(1, std::min<long long>({fill, steps / 4, kMaxSplits})));
       }
@@ -597,12 +664,20 @@ namespace mi
       }
     }
 
-    template <int HD, int NW, int kKeys>
+    template <int HD, typename F>
     void launch(const WindowArgs &a, const Cut &c, hipStream_t stream)
     {
-      const std::size_t lds = sizeof(std::uint16_t) * 2 * 2 * kKeys * HD;
-      window_kernel<HD, NW, kKeys>
-          <<<dim3(c.blocks, a.kv_heads, c.splits), 64 * NW, lds, stream>>>(a);
+      constexpr std::size_t lds = std::max(sizeof(std::uint16_t) * 2 * 2 * F::keys * HD,
+                                       sizeof(float) * (F::ways - 1) * F::tiles * (HD / 2 + 2) * 64);
+      auto kernel = window_kernel<HD, F::tiles, F::ways, F::keys>;
+      if constexpr (lds > 64 * 1024)
+      {
+        hip_check(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
+                                      hipFuncAttributeMaxDynamicSharedMemorySize,
+                                      static_cast<int>(lds)),
+                  "hipFuncSetAttribute window LDS");
+      }
+      kernel<<<dim3(c.blocks, a.kv_heads, c.splits), 64 * F::tiles * F::ways, lds, stream>>>(a);
       hip_check(hipGetLastError(), "window_kernel");
     }
 
@@ -611,11 +686,11 @@ namespace mi
     {
       if (c.few)
       {
-        launch<HD, 1, kFewKeys>(a, c, stream);
+        launch<HD, Few>(a, c, stream);
       }
       else
       {
-        launch<HD, kManyWaves, kManyKeys>(a, c, stream);
+        launch<HD, std::conditional_t<HD == 64, Many64, Many128>>(a, c, stream);
       }
       if (c.splits > 1)
       {
