@@ -6,8 +6,9 @@
 // sqrt(hd)) v over those; every query sees itself at least.
 //
 // A workgroup takes one KV head and consecutive (query, head) rows of its
-// group, query by query, so that its rows' windows nearly coincide; 32 rows a
-// wave. Steps of kKeys keys, of which only those some row of the workgroup
+// group, query by query, so that its rows' windows nearly coincide, in tiles of
+// 32; a tile's waves share the keys of a step and join their sums at the end.
+// Steps of kKeys keys, of which only those some row of the workgroup
 // sees are taken (the sink steps, then the window's), pass through LDS, double
 // buffered, copied there directly from memory. In the matrix cores' terms,
 // with keys as M and rows as N:
@@ -31,18 +32,19 @@
 // With few rows the range of keys is split over workgroups, whose parts a
 // second launch joins.
 //
-// Bound by a SIMD's two waves taking turns at the matrix cores and the softmax
-// (exponentials 20%, sums 10%, first product 25% of the time, which add up).
-// 2,048 queries x 32 heads at 14,336 behind a 4,096-token window with 4 sinks,
-// head_dim 64: 110 us, 622 TFLOP/s, the matrix cores busy 62% of it. A prompt
-// of 4,096 x 12 heads of 128 behind 1,024: 57 us, 396 TFLOP/s, its 384
-// workgroups leaving half the CUs one instead of two. 100 queries x 14 heads
-// of 64: 9.4 us, two launches. Measured and not taken: 64 rows a wave (158 us
-// for the first of these, one wave a SIMD), the next step's first product
-// beside this step's exponentials (the same at head_dim 64; 90 us for the
-// second, out of registers), addresses a lane keeps instead of making (the
-// same), KV heads first in the order of workgroups (the same, 95% of reads
-// meet the L2 either way).
+// Bound by the vector units beside the matrix cores: a 32 x 32 tile's weights
+// at head_dim 64 take some 450 cycles of a SIMD (16 exponentials a lane at a
+// quarter of the rate are 256 of them), its products 256, and the two overlap
+// only across waves. 2,048 queries x 32 heads at 14,336 behind a 4,096-token
+// window with 4 sinks, head_dim 64: 100.5 us, 684 TFLOP/s. A prompt of 4,096 x
+// 12 heads of 128 behind 1,024: 57.5 us, 394 TFLOP/s, its 384 workgroups
+// leaving half the CUs one instead of two. 100 queries x 14 heads of 64:
+// 5.9 us, a launch and a chain of loads. Measured and not taken: 64 rows a
+// wave (158 us for the first of these, one wave a SIMD), the next step's first
+// product beside this step's exponentials (the same at head_dim 64; 90 us for
+// the second, out of registers), addresses a lane keeps instead of making, KV
+// heads first in the order of workgroups (the same; 95% of reads meet the L2
+// either way).
 
 #include "common.hpp"
 #include "kernels.hpp"
@@ -186,11 +188,13 @@ namespace mi
       }
     };
 
-    template <int HD, int kTiles, int kWays>
-    constexpr int kWavesASimd = HD == 64 && kTiles > 1 ? 2 * kWays : kTiles > 1 ? 2 : 1;
+    // Waves a SIMD that a form's registers are held to: four at head_dim 64
+    // (128 registers), two at 128 (256); few rows leave a wave alone anyway.
+    template <int HD, int kTiles>
+    constexpr int kWavesASimd = kTiles == 1 ? 1 : HD == 64 ? 4 : 2;
 
     template <int HD, int kTiles, int kWays, int kKeys>
-    __global__ void __launch_bounds__(64 * kTiles * kWays, (kWavesASimd<HD, kTiles, kWays>))
+    __global__ void __launch_bounds__(64 * kTiles * kWays, (kWavesASimd<HD, kTiles>))
         window_kernel(WindowArgs a)
     {
       constexpr int NW = kTiles * kWays;
@@ -585,14 +589,22 @@ namespace mi
     }
 
     // A launch's form: the row tiles of a workgroup, the waves that share a
-    // tile's keys, and the keys a step.
+    // tile's keys, and the keys a step. Few rows are a matter of latency, so
+    // four waves take a quarter of a step's keys each (100 queries x 14 heads
+    // of 64 by one wave 9.1 us, by four 5.9). Many at head_dim 64 have the
+    // registers for four waves a SIMD, two to a tile, and one barrier in 128
+    // keys (2,048 queries x 32 heads at 14K behind 4,096: one wave to a tile
+    // and 64 keys a step 110 us, two 104, and 128 keys 100.5). At 128 a wave's
+    // output and queries allow two a SIMD, and tiles of half the rows, or
+    // three waves a SIMD, cost more than they balance (4,096 x 12 heads behind
+    // 1,024: 57.5 us, 65.6 and 124).
     template <int kTiles_, int kWays_, int kKeys_>
     struct Form
     {
       static constexpr int tiles = kTiles_, ways = kWays_, keys = kKeys_, rows = 32 * kTiles_;
     };
     using Few = Form<1, 4, 128>;
-    using Many64 = Form<4, 2, 64>;
+    using Many64 = Form<4, 2, 128>;
     using Many128 = Form<4, 1, 64>;
 
     // How a launch is cut.
@@ -610,25 +622,36 @@ namespace mi
       const int group = t.heads / t.kv_heads;
       const long long rows = static_cast<long long>(t.seq_q) * group;
       Cut c{};
-      c.few = (rows + Few::rows - 1) / Few::rows * t.kv_heads <= 512;
+      // The keys that a row sees, and the sink steps beside them.
+      const long long span =
+          t.window > 0 ? std::min<long long>(t.seq_k, static_cast<long long>(t.window) + t.sinks)
+                       : t.seq_k;
+      // Few: what leaves no CU two of those workgroups; at head_dim 64, whose
+      // stages leave room, twice as many for short spans (measured in us, few
+      // against many: 1,024 x 14 heads behind 64 keys 11 and 15, 512 x 32 with
+      // 512 keys 10.7 and 12.9, with 4,096 keys 56 and 43; 768 x 12 of 128
+      // behind 1,024 keys 23.2 and 21.5, 512 of them 13.2 and 19.3).
+      const long long few = (rows + Few::rows - 1) / Few::rows * t.kv_heads;
+      c.few = few <= 256 || (t.head_dim == 64 && few <= 512 && span <= 1024);
       c.rows = c.few ? Few::rows : t.head_dim == 64 ? Many64::rows : Many128::rows;
       c.keys = c.few ? Few::keys : t.head_dim == 64 ? Many64::keys : Many128::keys;
       c.blocks = static_cast<int>((rows + c.rows - 1) / c.rows);
       c.splits = 1;
       if (may_split && c.blocks > 0)
       {
-        // The most steps a workgroup takes.
-        long long steps = (static_cast<long long>(t.seq_k) + c.keys - 1) / c.keys;
-        if (t.window > 0)
-        {
-          const long long span = static_cast<long long>(t.window) + (c.rows - 1) / group + 1;
-          steps = std::min(steps, (span + c.keys - 1) / c.keys + 1 +
-                                      (static_cast<long long>(t.sinks) + c.keys - 1) / c.keys);
-        }
-        // A workgroup a CU, each with four steps to take.
-        const long long fill = 256 / (static_cast<long long>(c.blocks) * t.kv_heads);
-        c.splits = static_cast<int>(
-            std::max<long long>(1, std::min<long long>({fill, steps / 4, kMaxSplits})));
+        // About the steps a workgroup takes.
+        const long long steps = (span + c.keys - 1) / c.keys;
+        // A workgroup a CU, each with two steps to take or more; two of those
+        // for many rows of head_dim 128, whose four waves leave half a CU
+        // idle, but no more than four parts to join (1,536 x 12 heads behind
+        // 1,024 keys: by one part 44 us, by three 33.5; 768 of them by seven
+        // 23.5, by four 22). At head_dim 64 a workgroup has the CU's waves
+        // busy by itself (1,024 x 32: one part 19.5 us, two 26).
+        const bool two = !c.few && t.head_dim == 128;
+        const long long fill =
+            (two ? 512 : 256) / (static_cast<long long>(c.blocks) * t.kv_heads);
+        c.splits = static_cast<int>(std::max<long long>(
+            1, std::min<long long>({fill, steps / 2, two ? 4 : kMaxSplits})));
       }
       return c;
     }
@@ -668,7 +691,7 @@ namespace mi
     void launch(const WindowArgs &a, const Cut &c, hipStream_t stream)
     {
       constexpr std::size_t lds = std::max(sizeof(std::uint16_t) * 2 * 2 * F::keys * HD,
-                                       sizeof(float) * (F::ways - 1) * F::tiles * (HD / 2 + 2) * 64);
+                                           sizeof(float) * (F::ways - 1) * F::tiles * (HD / 2 + 2) * 64);
       auto kernel = window_kernel<HD, F::tiles, F::ways, F::keys>;
       if constexpr (lds > 64 * 1024)
       {
