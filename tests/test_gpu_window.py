@@ -73,7 +73,8 @@ def test_windows_and_sinks(window, sinks, hd):
 
 @pytest.mark.parametrize("heads,kv,hd,seq_q,seq_k,window,sinks", [
     (32, 8, 64, 700, 900, 300, 4), (32, 8, 64, 601, 601, 0, 0), (12, 2, 128, 1500, 1500, 257, 70),
-    (14, 2, 64, 1301, 1400, 64, 0), (28, 4, 128, 700, 703, 1, 0)])
+    (14, 2, 64, 1301, 1400, 64, 0), (28, 4, 128, 700, 703, 1, 0), (32, 8, 64, 300, 1500, 0, 0),
+    (32, 8, 64, 301, 1501, 1200, 130)])
 def test_many_rows(heads, kv, hd, seq_q, seq_k, window, sinks):
     """Prompts of the kernel's large tiles: ragged last tiles, waves with no rows."""
     rng = np.random.default_rng(seq_q)
@@ -164,11 +165,12 @@ def test_what_a_query_does_not_see_may_be_anything(heads, kv, hd, seq_q):
             assert not np.isfinite(got[seen[:, j]][:, :, i]).any()
 
 
-def test_replayed_graphs_and_repeats_to_the_bit():
+@pytest.mark.parametrize("hd", [64, 128])
+def test_replayed_graphs_and_repeats_to_the_bit(hd):
     m = mi()
     d = m.device
     rng = np.random.default_rng(12)
-    seq_q, seq_k, heads, kv, hd = 5, 3000, 8, 2, 64
+    seq_q, seq_k, heads, kv = 5, 3000, 8, 2
     q, k, v = inputs(rng, seq_q, seq_k, heads, kv, hd)
     dq, dk, dv = d.empty(q.size), put(k), put(v)
     stream = m.Stream()
