@@ -371,14 +371,6 @@ namespace mi
 
     // NT tiles of 16 rows, FT tiles of 16 outputs a wave; Groups: groups in a
     // chunk.
-    template <int Groups, int FT>
-    struct TileFetch
-    {
-      u32x4 w[FT];
-      std::uint16_t s[FT][Groups];
-      std::uint16_t z[FT][Groups];
-    };
-
     template <int Groups, int NT, int FT, int Waves, Int4Out Out>
     __global__ void __launch_bounds__(64 * Waves) int4_tiles_kernel(Int4Args a)
     {
@@ -422,48 +414,79 @@ namespace mi
       const half8 ones = {one, one, one, one, one, one, one, one};
       const f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f};
       const int chunks = (a.in + kChunk - 1) / kChunk;
-      const auto fetch = [&](TileFetch<Groups, FT> &to, int chunk) {
-        // (Inputs past the last, and groups: the first's, which no product takes.)
+      // (Inputs past the last, and groups: the first's, which no product takes.)
+      const auto fetch = [&](u32x4 (&to)[FT], int chunk) {
         const int k = chunk * kChunk + 32 * g;
 #pragma unroll
         for (int u = 0; u < FT; ++u)
         {
-          to.w[u] = *reinterpret_cast<const u32x4 *>(codes[u] + (k < a.in ? k : 0) / 2);
+          to[u] = *reinterpret_cast<const u32x4 *>(codes[u] + (k < a.in ? k : 0) / 2);
         }
+      };
+      // Scales (low) and zeros of four chunks, lanes g those of chunk + g: a
+      // load is paid by the lines it touches, and a row's lie together.
+      const auto fetch_meta = [&](unsigned (&to)[FT][Groups], int chunk) {
+        const int at_chunk = min(chunk + g, chunks - 1);
 #pragma unroll
         for (int u = 0; u < FT; ++u)
         {
-          // A chunk's groups by one load, where a row's lie so.
+          std::uint16_t sc[Groups], ze[Groups];
+          const std::size_t at = meta[u] + static_cast<std::size_t>(at_chunk) * Groups;
           if (Groups > 1 && a.wide_meta)
           {
-            const std::size_t at = meta[u] + static_cast<std::size_t>(chunk) * Groups;
-            __builtin_memcpy(to.s[u], __builtin_assume_aligned(a.scales + at, 2 * Groups),
-                             2 * Groups);
-            __builtin_memcpy(to.z[u], __builtin_assume_aligned(a.zeros + at, 2 * Groups),
-                             2 * Groups);
+            __builtin_memcpy(sc, __builtin_assume_aligned(a.scales + at, 2 * Groups), 2 * Groups);
+            __builtin_memcpy(ze, __builtin_assume_aligned(a.zeros + at, 2 * Groups), 2 * Groups);
           }
           else
           {
 #pragma unroll
             for (int h = 0; h < Groups; ++h)
             {
-              const int group = chunk * Groups + h;
-              const std::size_t at = meta[u] + (group < a.groups ? group : 0);
-              to.s[u][h] = a.scales[at];
-              to.z[u][h] = a.zeros[at];
+              const int group = at_chunk * Groups + h;
+              const std::size_t one = meta[u] + (group < a.groups ? group : 0);
+              sc[h] = a.scales[one];
+              ze[h] = a.zeros[one];
             }
+          }
+#pragma unroll
+          for (int h = 0; h < Groups; ++h)
+          {
+            to[u][h] = sc[h] | static_cast<unsigned>(ze[h]) << 16;
           }
         }
       };
-      TileFetch<Groups, FT> next;
-      if (split < chunks)
+      const int per = (chunks + a.splits - 1) / a.splits;
+      const int begin = split * per;
+      const int end = min(begin + per, chunks);
+      u32x4 next[FT];
+      unsigned four[FT][Groups], next_four[FT][Groups];
+      if (begin < end)
       {
-        fetch(next, split);
+        fetch(next, begin);
+        fetch_meta(next_four, begin);
       }
-      for (int chunk = split; chunk < chunks; chunk += a.splits)
+      for (int chunk = begin; chunk < end; ++chunk)
       {
-        TileFetch<Groups, FT> now = next;
-        fetch(next, min(chunk + a.splits, chunks - 1));
+        const int of_four = (chunk - begin) & 3;
+        u32x4 now[FT];
+#pragma unroll
+        for (int u = 0; u < FT; ++u)
+        {
+          now[u] = next[u];
+#pragma unroll
+          for (int h = 0; h < Groups; ++h)
+          {
+            four[u][h] = of_four == 0 ? next_four[u][h] : four[u][h];
+          }
+        }
+        if (chunk + 1 < end)
+        {
+          fetch(next, chunk + 1);
+          if (of_four == 3)
+          {
+            fetch_meta(next_four, chunk + 1);
+          }
+        }
         const int k0 = chunk * kChunk;
         u32x4 xa[NT][4];
 #pragma unroll
@@ -478,7 +501,7 @@ namespace mi
 #pragma unroll
         for (int u = 0; u < FT; ++u)
         {
-          transpose_words(now.w[u]);
+          transpose_words(now[u]);
         }
 #pragma unroll
         for (int h = 0; h < Groups; ++h)
@@ -502,7 +525,7 @@ namespace mi
 #pragma unroll
             for (int u = 0; u < FT; ++u)
             {
-              const unsigned word = now.w[u][h * kPer + j];
+              const unsigned word = now[u][h * kPer + j];
               const half8 q = codes_as_half(word);
 #pragma unroll
               for (int t = 0; t < NT; ++t)
@@ -515,7 +538,10 @@ namespace mi
 #pragma unroll
           for (int u = 0; u < FT; ++u)
           {
-            const float s = h2f(now.s[u][h]), z = h2f(now.z[u][h]);
+            const unsigned both = static_cast<unsigned>(__builtin_amdgcn_ds_bpermute(
+                4 * (16 * of_four + n), static_cast<int>(four[u][h])));
+            const float s = h2f(static_cast<std::uint16_t>(both));
+            const float z = h2f(static_cast<std::uint16_t>(both >> 16));
 #pragma unroll
             for (int t = 0; t < NT; ++t)
             {
