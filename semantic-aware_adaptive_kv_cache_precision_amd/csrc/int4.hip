@@ -375,7 +375,8 @@ namespace mi
     __global__ void __launch_bounds__(64 * Waves) int4_tiles_kernel(Int4Args a)
     {
       constexpr int kPer = 4 / Groups; // instructions a group
-      extern __shared__ __align__(16) f32x4 parts[];
+      constexpr int kStage = NT * 256; // 16-byte pieces of a wave's x
+      extern __shared__ __align__(16) u32x4 stages[];
       const int lane = threadIdx.x & 63;
       const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
       const int n = lane & 15;
@@ -394,11 +395,18 @@ namespace mi
         codes[u] = a.codes + static_cast<std::size_t>(row) * (a.in / 2);
         meta[u] = static_cast<std::size_t>(row) * a.groups;
       }
-      const std::uint16_t *x[NT]; // (a row past the last repeats it)
+      // x comes in whole lines, four rows' chunks a load, and turns through the
+      // wave's own LDS, piece p of row r at place p ^ r % 16 of its row.
+      u32x4 *stage = stages + wave * kStage;
+      const std::uint16_t *x[NT][4]; // (a row past the last repeats it)
 #pragma unroll
       for (int t = 0; t < NT; ++t)
       {
-        x[t] = a.x + static_cast<std::size_t>(row0 + min(16 * t + n, rows - 1)) * a.in + 8 * g;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+        {
+          x[t][i] = a.x + static_cast<std::size_t>(row0 + min(16 * t + 4 * i + g, rows - 1)) * a.in;
+        }
       }
       f32x4 y[NT][FT];
 #pragma unroll
@@ -421,6 +429,21 @@ namespace mi
         for (int u = 0; u < FT; ++u)
         {
           to[u] = *reinterpret_cast<const u32x4 *>(codes[u] + (k < a.in ? k : 0) / 2);
+        }
+      };
+      const auto fetch_x = [&](u32x4 (&to)[NT][4], int chunk) {
+        const int k = chunk * kChunk + 8 * n;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+        {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+          {
+            if (16 * t + 4 * i < rows)
+            {
+              to[t][i] = *reinterpret_cast<const u32x4 *>(x[t][i] + (k < a.in ? k : 0));
+            }
+          }
         }
       };
       // Scales (low) and zeros of four chunks, lanes g those of chunk + g: a
@@ -458,11 +481,12 @@ namespace mi
       const int per = (chunks + a.splits - 1) / a.splits;
       const int begin = split * per;
       const int end = min(begin + per, chunks);
-      u32x4 next[FT];
+      u32x4 next[FT], next_x[NT][4] = {};
       unsigned four[FT][Groups], next_four[FT][Groups];
       if (begin < end)
       {
         fetch(next, begin);
+        fetch_x(next_x, begin);
         fetch_meta(next_four, begin);
       }
       for (int chunk = begin; chunk < end; ++chunk)
@@ -479,25 +503,26 @@ namespace mi
             four[u][h] = of_four == 0 ? next_four[u][h] : four[u][h];
           }
         }
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+        {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+          {
+            const int row = 4 * i + g; // (products of rows past the last are left)
+            stage[t * 256 + 16 * row + (n ^ row)] = turned(next_x[t][i]);
+          }
+        }
         if (chunk + 1 < end)
         {
           fetch(next, chunk + 1);
+          fetch_x(next_x, chunk + 1);
           if (of_four == 3)
           {
             fetch_meta(next_four, chunk + 1);
           }
         }
         const int k0 = chunk * kChunk;
-        u32x4 xa[NT][4];
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-        {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-          {
-            xa[t][j] = *reinterpret_cast<const u32x4 *>(x[t] + (k0 + 32 * j < a.in ? k0 + 32 * j : 0));
-          }
-        }
 #pragma unroll
         for (int u = 0; u < FT; ++u)
         {
@@ -518,7 +543,8 @@ namespace mi
 #pragma unroll
             for (int t = 0; t < NT; ++t)
             {
-              xt[t] = __builtin_bit_cast(half8, turned(xa[t][h * kPer + j]));
+              xt[t] = __builtin_bit_cast(
+                  half8, stage[t * 256 + 16 * n + ((4 * (h * kPer + j) + g) ^ n)]);
               sum[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xt[t], ones, j ? sum[t] : none, 0, 0,
                                                               0);
             }
@@ -559,6 +585,8 @@ namespace mi
       // The splits' sums, added by the tile's first wave in wave order.
       if (a.splits > 1)
       {
+        static_assert(FT <= 4, "a wave's sums in its stage");
+        f32x4 *parts = reinterpret_cast<f32x4 *>(stages);
         if (split > 0)
         {
 #pragma unroll
@@ -567,7 +595,7 @@ namespace mi
 #pragma unroll
             for (int u = 0; u < FT; ++u)
             {
-              parts[((wave * NT + t) * FT + u) * 64 + lane] = y[t][u];
+              parts[wave * kStage + (t * FT + u) * 64 + lane] = y[t][u];
             }
           }
         }
@@ -584,7 +612,7 @@ namespace mi
 #pragma unroll
             for (int u = 0; u < FT; ++u)
             {
-              y[t][u] += parts[(((wave + p) * NT + t) * FT + u) * 64 + lane];
+              y[t][u] += parts[(wave + p) * kStage + (t * FT + u) * 64 + lane];
             }
           }
         }
@@ -675,17 +703,18 @@ namespace mi
                            (a.in + kChunk - 1) / kChunk, Waves);
       const int per = Waves / a.splits;
       const dim3 grid((tiles + per - 1) / per, row_tiles);
-      const std::size_t lds = a.splits > 1 ? sizeof(f32x4) * Waves * NT * FT * 64 : 0;
-      if (out == Int4Out::kHalf)
+      constexpr std::size_t lds = sizeof(u32x4) * Waves * NT * 256;
+      auto kernel = out == Int4Out::kHalf
+                        ? int4_tiles_kernel<Groups, NT, FT, Waves, Int4Out::kHalf>
+                        : int4_tiles_kernel<Groups, NT, FT, Waves, Int4Out::kAccumulate>;
+      if constexpr (lds > 64 * 1024)
       {
-        int4_tiles_kernel<Groups, NT, FT, Waves, Int4Out::kHalf>
-            <<<grid, 64 * Waves, lds, stream>>>(a);
+        hip_check(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
+                                      hipFuncAttributeMaxDynamicSharedMemorySize,
+                                      static_cast<int>(lds)),
+                  "hipFuncSetAttribute int4 LDS");
       }
-      else
-      {
-        int4_tiles_kernel<Groups, NT, FT, Waves, Int4Out::kAccumulate>
-            <<<grid, 64 * Waves, lds, stream>>>(a);
-      }
+      kernel<<<grid, 64 * Waves, lds, stream>>>(a);
       hip_check(hipGetLastError(), "int4_tiles_kernel");
     }
 
