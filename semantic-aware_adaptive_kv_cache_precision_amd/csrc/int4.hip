@@ -386,26 +386,32 @@ namespace mi
           (static_cast<int>(blockIdx.x) * (Waves / a.splits) + wave / a.splits) * FT * 16;
       const int row0 = static_cast<int>(blockIdx.y) * 16 * NT;
       const int rows = min(a.rows - row0, 16 * NT);
-      const std::uint8_t *codes[FT];
-      std::size_t meta[FT];
+      // Addresses: a scalar base and 32 bits a lane (in is held to kMostInputs).
+      const int base = min(tile0, a.features - 1); // (a wave past the last output repeats it)
+      const std::uint8_t *codes = a.codes + static_cast<std::size_t>(base) * (a.in / 2);
+      const char *scales =
+          reinterpret_cast<const char *>(a.scales + static_cast<std::size_t>(base) * a.groups);
+      const char *zeros =
+          reinterpret_cast<const char *>(a.zeros + static_cast<std::size_t>(base) * a.groups);
+      unsigned of[FT];
 #pragma unroll
       for (int u = 0; u < FT; ++u)
       {
-        const int row = min(tile0 + 16 * u + n, a.features - 1);
-        codes[u] = a.codes + static_cast<std::size_t>(row) * (a.in / 2);
-        meta[u] = static_cast<std::size_t>(row) * a.groups;
+        of[u] = min(16 * u + n, a.features - 1 - base);
       }
       // x comes in whole lines, four rows' chunks a load, and turns through the
       // wave's own LDS, piece p of row r at place p ^ r % 16 of its row.
       u32x4 *stage = stages + wave * kStage;
-      const std::uint16_t *x[NT][4]; // (a row past the last repeats it)
+      const char *x =
+          reinterpret_cast<const char *>(a.x + static_cast<std::size_t>(row0) * a.in);
+      unsigned x_at[NT][4]; // (a row past the last repeats it)
 #pragma unroll
       for (int t = 0; t < NT; ++t)
       {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
         {
-          x[t][i] = a.x + static_cast<std::size_t>(row0 + min(16 * t + 4 * i + g, rows - 1)) * a.in;
+          x_at[t][i] = 2u * min(16 * t + 4 * i + g, rows - 1) * static_cast<unsigned>(a.in);
         }
       }
       f32x4 y[NT][FT];
@@ -428,7 +434,8 @@ namespace mi
 #pragma unroll
         for (int u = 0; u < FT; ++u)
         {
-          to[u] = *reinterpret_cast<const u32x4 *>(codes[u] + (k < a.in ? k : 0) / 2);
+          to[u] = *reinterpret_cast<const u32x4 *>(
+              codes + (of[u] * static_cast<unsigned>(a.in) + (k < a.in ? k : 0)) / 2);
         }
       };
       const auto fetch_x = [&](u32x4 (&to)[NT][4], int chunk) {
@@ -441,7 +448,8 @@ namespace mi
           {
             if (16 * t + 4 * i < rows)
             {
-              to[t][i] = *reinterpret_cast<const u32x4 *>(x[t][i] + (k < a.in ? k : 0));
+              to[t][i] = *reinterpret_cast<const u32x4 *>(
+                  x + (x_at[t][i] + 2u * (k < a.in ? k : 0)));
             }
           }
         }
@@ -454,11 +462,12 @@ namespace mi
         for (int u = 0; u < FT; ++u)
         {
           std::uint16_t sc[Groups], ze[Groups];
-          const std::size_t at = meta[u] + static_cast<std::size_t>(at_chunk) * Groups;
+          const unsigned row = of[u] * a.groups;
           if (Groups > 1 && a.wide_meta)
           {
-            __builtin_memcpy(sc, __builtin_assume_aligned(a.scales + at, 2 * Groups), 2 * Groups);
-            __builtin_memcpy(ze, __builtin_assume_aligned(a.zeros + at, 2 * Groups), 2 * Groups);
+            const unsigned at = 2u * (row + at_chunk * Groups);
+            __builtin_memcpy(sc, __builtin_assume_aligned(scales + at, 2 * Groups), 2 * Groups);
+            __builtin_memcpy(ze, __builtin_assume_aligned(zeros + at, 2 * Groups), 2 * Groups);
           }
           else
           {
@@ -466,9 +475,9 @@ namespace mi
             for (int h = 0; h < Groups; ++h)
             {
               const int group = at_chunk * Groups + h;
-              const std::size_t one = meta[u] + (group < a.groups ? group : 0);
-              sc[h] = a.scales[one];
-              ze[h] = a.zeros[one];
+              const unsigned at = 2u * (row + (group < a.groups ? group : 0));
+              sc[h] = *reinterpret_cast<const std::uint16_t *>(scales + at);
+              ze[h] = *reinterpret_cast<const std::uint16_t *>(zeros + at);
             }
           }
 #pragma unroll
@@ -749,7 +758,10 @@ namespace mi
       const long long row_tiles = (a.rows + 15) / 16;
       if (tiles * row_tiles <= 1024)
       {
-        project_tiles<Groups, 1, 1, 16>(a, out, stream);
+        const int steps = (a.in + kChunk - 1) / kChunk;
+        splits_of(static_cast<int>(tiles * row_tiles), steps, 16) > 8
+            ? project_tiles<Groups, 1, 1, 16>(a, out, stream)
+            : project_tiles<Groups, 1, 1, 8>(a, out, stream);
       }
       else if (a.rows <= 16)
       {
@@ -791,6 +803,15 @@ namespace mi
       {
         throw InvalidArgument("rows " + std::to_string(rows) + " are more than an int4 projection's " +
                               std::to_string(kMostRows));
+      }
+      // 64 rows of x within 32 bits, a grid's threads too.
+      constexpr int kMostInputs = 1 << 24, kMostOutputs = 1 << 27;
+      if (in > kMostInputs || features > kMostOutputs)
+      {
+        throw InvalidArgument("an int4 projection takes at most " + std::to_string(kMostInputs) +
+                              " in_features and " + std::to_string(kMostOutputs) +
+                              " out_features, got " + std::to_string(in) + " and " +
+                              std::to_string(features));
       }
       if (in == 0)
       {
