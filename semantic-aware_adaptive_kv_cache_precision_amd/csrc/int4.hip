@@ -730,38 +730,39 @@ namespace mi
     template <int Groups>
     void project(const Int4Args &a, Int4Out out, hipStream_t stream)
     {
-      // Four sets of outputs a wave where there are plenty. Three or four rows
-      // are the dot products' work only there: they read x a set at a time
-      // (8960 x 1536, three rows: 12.0 us, by tiles 6.7; 128256 x 2048: 72 and
-      // 84).
+      const long long tiles = (a.features + 15) / 16;
+      const long long work = tiles * ((a.rows + 15) / 16);
+      const int steps = (a.in + kChunk - 1) / kChunk;
+      // Whether it takes more than eight waves a tile to make the device full.
+      const bool wide = work <= 4096 && splits_of(static_cast<int>(work), steps, 16) > 8;
+      // One row by dot products, and two of plenty of outputs or a wide tile
+      // (128256 x 2048, two rows 41 us, by tiles 50; 1536 x 8960 7.3 and 7.7;
+      // but 8960 x 1536 7.1 and 5.2); four sets of outputs a wave where there
+      // are plenty.
       const bool many = a.features >= 16384;
       if (a.rows == 1)
       {
         many ? project_rows<1, 4>(a, out, stream) : project_rows<1, 1>(a, out, stream);
-        return;
       }
-      if (a.rows == 2)
+      else if (a.rows == 2 && (many || wide))
       {
         many ? project_rows<2, 4>(a, out, stream) : project_rows<2, 1>(a, out, stream);
-        return;
       }
-      if (a.rows <= 4 && many)
+      // Little work: a tile a wave, its inputs split over as many waves as
+      // make the device full, in workgroups of eight where that is enough
+      // (8960 x 1536, 16 rows, in us: sixteen waves 8.3, eight 5.7; 48 rows
+      // 10.0, by the tiles below 15.7; 64 rows of 8192 x 2048 13.8 and 12.0).
+      // Where workgroups of sixteen waves, one a CU, would take two turns, two
+      // row tiles a wave share the codes (1536 x 8960: 64 rows 16.4 and 13.2,
+      // 32 rows, one turn, 9.3). Much work: tiles of outputs share x.
+      else if (wide && work * steps <= 40960)
       {
-        project_rows<4, 4>(a, out, stream);
-        return;
+        work > 256 ? project_tiles<Groups, 2, 1, 16>(a, out, stream)
+                   : project_tiles<Groups, 1, 1, 16>(a, out, stream);
       }
-      // A workgroup reads all its rows' x: few workgroups, each with many
-      // rows, are bound by what a CU takes in (27 rows 8960 -> 1536: 96
-      // workgroups of 32 rows 19.1 us, 192 of 16 13.1). Where there are
-      // plenty, four tiles of outputs a wave share each row of x.
-      const long long tiles = (a.features + 15) / 16;
-      const long long row_tiles = (a.rows + 15) / 16;
-      if (tiles * row_tiles <= 1024)
+      else if (!wide && (work <= 1024 || work * steps <= 28672))
       {
-        const int steps = (a.in + kChunk - 1) / kChunk;
-        splits_of(static_cast<int>(tiles * row_tiles), steps, 16) > 8
-            ? project_tiles<Groups, 1, 1, 16>(a, out, stream)
-            : project_tiles<Groups, 1, 1, 8>(a, out, stream);
+        project_tiles<Groups, 1, 1, 8>(a, out, stream);
       }
       else if (a.rows <= 16)
       {
