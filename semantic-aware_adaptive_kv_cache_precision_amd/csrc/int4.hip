@@ -371,7 +371,9 @@ namespace mi
 
     // NT tiles of 16 rows, FT tiles of 16 outputs a wave; Groups: groups in a
     // chunk.
-    template <int Groups, int NT, int FT, int Waves, Int4Out Out>
+    // Shared: the waves' tiles of outputs are all different, and x goes through
+    // LDS once for all of them, double buffered.
+    template <int Groups, int NT, int FT, int Waves, bool Shared, Int4Out Out>
     __global__ void __launch_bounds__(64 * Waves) int4_tiles_kernel(Int4Args a)
     {
       constexpr int kPer = 4 / Groups; // instructions a group
@@ -401,18 +403,16 @@ namespace mi
       }
       // x comes in whole lines, four rows' chunks a load, and turns through the
       // wave's own LDS, piece p of row r at place p ^ r % 16 of its row.
-      u32x4 *stage = stages + wave * kStage;
+      u32x4 *stage = stages + (Shared ? 0 : wave * kStage);
       const char *x =
           reinterpret_cast<const char *>(a.x + static_cast<std::size_t>(row0) * a.in);
-      unsigned x_at[NT][4]; // (a row past the last repeats it)
+      constexpr int kFetches = Shared ? (4 * NT + Waves - 1) / Waves : 4 * NT; // of four rows
+      const auto four_of = [&](int i) { return Shared ? wave + Waves * i : i; };
+      unsigned x_at[kFetches]; // (a row past the last repeats it)
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+      for (int i = 0; i < kFetches; ++i)
       {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-        {
-          x_at[t][i] = 2u * min(16 * t + 4 * i + g, rows - 1) * static_cast<unsigned>(a.in);
-        }
+        x_at[i] = 2u * min(4 * four_of(i) + g, rows - 1) * static_cast<unsigned>(a.in);
       }
       f32x4 y[NT][FT];
 #pragma unroll
@@ -438,19 +438,27 @@ namespace mi
               codes + (of[u] * static_cast<unsigned>(a.in) + (k < a.in ? k : 0)) / 2);
         }
       };
-      const auto fetch_x = [&](u32x4 (&to)[NT][4], int chunk) {
+      const auto fetch_x = [&](u32x4 (&to)[kFetches], int chunk) {
         const int k = chunk * kChunk + 8 * n;
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+        for (int i = 0; i < kFetches; ++i)
         {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
+          if (4 * four_of(i) < rows)
           {
-            if (16 * t + 4 * i < rows)
-            {
-              to[t][i] = *reinterpret_cast<const u32x4 *>(
-                  x + (x_at[t][i] + 2u * (k < a.in ? k : 0)));
-            }
+            to[i] = *reinterpret_cast<const u32x4 *>(x + (x_at[i] + 2u * (k < a.in ? k : 0)));
+          }
+        }
+      };
+      // (Products of rows past the last are left.)
+      const auto stage_x = [&](u32x4 *to, const u32x4 (&from)[kFetches]) {
+#pragma unroll
+        for (int i = 0; i < kFetches; ++i)
+        {
+          const int four = four_of(i);
+          if (!Shared || four < 4 * NT)
+          {
+            const int row = 4 * (four % 4) + g;
+            to[four / 4 * 256 + 16 * row + (n ^ row)] = turned(from[i]);
           }
         }
       };
@@ -490,13 +498,17 @@ namespace mi
       const int per = (chunks + a.splits - 1) / a.splits;
       const int begin = split * per;
       const int end = min(begin + per, chunks);
-      u32x4 next[FT], next_x[NT][4] = {};
+      u32x4 next[FT], next_x[kFetches] = {};
       unsigned four[FT][Groups], next_four[FT][Groups];
       if (begin < end)
       {
         fetch(next, begin);
         fetch_x(next_x, begin);
         fetch_meta(next_four, begin);
+        if constexpr (Shared)
+        {
+          stage_x(stage, next_x);
+        }
       }
       for (int chunk = begin; chunk < end; ++chunk)
       {
@@ -512,15 +524,14 @@ namespace mi
             four[u][h] = of_four == 0 ? next_four[u][h] : four[u][h];
           }
         }
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
+        if constexpr (Shared)
         {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-          {
-            const int row = 4 * i + g; // (products of rows past the last are left)
-            stage[t * 256 + 16 * row + (n ^ row)] = turned(next_x[t][i]);
-          }
+          stage = stages + ((chunk - begin) & 1) * kStage;
+          __syncthreads();
+        }
+        else
+        {
+          stage_x(stage, next_x);
         }
         if (chunk + 1 < end)
         {
@@ -589,12 +600,19 @@ namespace mi
             }
           }
         }
+        if constexpr (Shared)
+        {
+          if (chunk + 1 < end)
+          {
+            stage_x(stages + ((chunk + 1 - begin) & 1) * kStage, next_x);
+          }
+        }
       }
 
       // The splits' sums, added by the tile's first wave in wave order.
       if (a.splits > 1)
       {
-        static_assert(FT <= 4, "a wave's sums in its stage");
+        static_assert(Shared || FT <= 4, "a wave's sums in its stage");
         f32x4 *parts = reinterpret_cast<f32x4 *>(stages);
         if (split > 0)
         {
@@ -702,20 +720,20 @@ namespace mi
       hip_check(hipGetLastError(), "int4_rows_kernel");
     }
 
-    template <int Groups, int NT, int FT, int Waves>
+    template <int Groups, int NT, int FT, int Waves, bool Shared = false>
     void project_tiles(Int4Args a, Int4Out out, hipStream_t stream)
     {
       const int tiles = (a.features + 16 * FT - 1) / (16 * FT);
       const int row_tiles = (a.rows + 16 * NT - 1) / (16 * NT);
       a.splits = splits_of(static_cast<int>(std::min<long long>(
                                static_cast<long long>(tiles) * row_tiles, 1 << 20)),
-                           (a.in + kChunk - 1) / kChunk, Waves);
+                           (a.in + kChunk - 1) / kChunk, Shared ? 1 : Waves);
       const int per = Waves / a.splits;
       const dim3 grid((tiles + per - 1) / per, row_tiles);
-      constexpr std::size_t lds = sizeof(u32x4) * Waves * NT * 256;
+      constexpr std::size_t lds = sizeof(u32x4) * (Shared ? 2 : Waves) * NT * 256;
       auto kernel = out == Int4Out::kHalf
-                        ? int4_tiles_kernel<Groups, NT, FT, Waves, Int4Out::kHalf>
-                        : int4_tiles_kernel<Groups, NT, FT, Waves, Int4Out::kAccumulate>;
+                        ? int4_tiles_kernel<Groups, NT, FT, Waves, Shared, Int4Out::kHalf>
+                        : int4_tiles_kernel<Groups, NT, FT, Waves, Shared, Int4Out::kAccumulate>;
       if constexpr (lds > 64 * 1024)
       {
         hip_check(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
@@ -733,6 +751,10 @@ namespace mi
       const long long tiles = (a.features + 15) / 16;
       const long long work = tiles * ((a.rows + 15) / 16);
       const int steps = (a.in + kChunk - 1) / kChunk;
+      const auto groups_of = [&](int outputs, int rows) { // workgroups of tiles of these
+        return static_cast<long long>((a.features + outputs - 1) / outputs) *
+               ((a.rows + rows - 1) / rows);
+      };
       // Whether it takes more than eight waves a tile to make the device full.
       const bool wide = work <= 4096 && splits_of(static_cast<int>(work), steps, 16) > 8;
       // One row by dot products, and two of plenty of outputs or a wide tile
@@ -764,17 +786,35 @@ namespace mi
       {
         project_tiles<Groups, 1, 1, 8>(a, out, stream);
       }
+      // Where workgroups of eight different tiles fill most of the device, x
+      // goes through LDS once for all of them (128256 x 2048: 16 rows 55 us
+      // and shared 49, 32 rows 72 and 57, 64 rows 109 and 80, 1,024 rows 1386
+      // and 1073, 501 TFLOP/s; but 64 rows of 16384 x 2048, 64 workgroups, 23
+      // and 37).
       else if (a.rows <= 16)
       {
-        project_tiles<Groups, 1, 4, 8>(a, out, stream);
+        groups_of(64 * 4, 16) >= 192 ? project_tiles<Groups, 1, 4, 4, true>(a, out, stream)
+                                     : project_tiles<Groups, 1, 4, 8>(a, out, stream);
       }
       else if (a.rows <= 32)
       {
-        project_tiles<Groups, 2, 4, 8>(a, out, stream);
+        groups_of(32 * 8, 32) >= 192 ? project_tiles<Groups, 2, 2, 8, true>(a, out, stream)
+                                     : project_tiles<Groups, 2, 4, 8>(a, out, stream);
+      }
+      else if (groups_of(32 * 8, 64) < 192)
+      {
+        project_tiles<Groups, 4, 2, 8>(a, out, stream);
+      }
+      // One workgroup a CU at a time: tiles of twice the outputs unless they
+      // take more turns for it (1,024 rows 8192 x 2048, 256 workgroups: 72 us,
+      // the smaller tiles 77; 8960 x 1536, 288: 111 and 76).
+      else if (2 * ((groups_of(64 * 8, 64) + 255) / 256) <= (groups_of(32 * 8, 64) + 255) / 256)
+      {
+        project_tiles<Groups, 4, 4, 8, true>(a, out, stream);
       }
       else
       {
-        project_tiles<Groups, 4, 2, 8>(a, out, stream);
+        project_tiles<Groups, 4, 2, 8, true>(a, out, stream);
       }
     }
 

@@ -115,7 +115,10 @@ def test_linear_against_float64(rows, out, n_in, group):
 
 @pytest.mark.parametrize("rows,out,n_in,group", [
     (1, 1536, 8960, 128), (27, 1536, 8960, 128), (64, 72, 24608, 32), (1, 33, 24608, 32),
-    (1, 40001, 2048, 64), (3, 151936, 896, 32), (16, 8192, 2048, 64)])
+    (1, 40001, 2048, 64), (3, 151936, 896, 32), (16, 8192, 2048, 64), (2, 40001, 160, 32),
+    (9, 50001, 160, 32), (30, 50001, 320, 64), (64, 60001, 384, 128), (300, 65000, 96, 32),
+    (40, 16400, 2176, 128), (40, 1000, 8960, 64), (10, 20000, 4096, 64), (20, 20000, 4096, 64),
+    (700, 8200, 256, 64)])
 def test_linear_at_the_models_sizes(rows, out, n_in, group):
     d = mi().device
     rng = np.random.default_rng(rows + out)
