@@ -216,7 +216,8 @@ namespace mi
       const int G = a.group;
       const int past = a.seq_k - a.seq_q;
       const long long all_rows = static_cast<long long>(a.seq_q) * G;
-      const long long row0 = static_cast<long long>(blockIdx.x) * kRows;
+      // The last queries, whose ranges are longest, go first.
+      const long long row0 = static_cast<long long>(gridDim.x - 1 - blockIdx.x) * kRows;
 
       // The workgroup's positions, and the steps they see.
       const int lo_pos = past + static_cast<int>(row0 / G);
