@@ -256,9 +256,10 @@ int mi_linear_f32(const void *x, const void *weight, float *out, int accumulate,
  * whose 15 steps reach the group's range, codes rounded half to even.
  * mi_linear_int4: out (rows, out) fp16 = x (rows, in) W^T + bias (out fp16, or
  * null), fp32 sums rounded once. mi_linear_int4_accumulate: out (rows, out)
- * fp32 += x W^T. The sums' order depends on the sizes alone. For a decode
- * row or the rows of some sequences' steps; many rows (a prompt's) are better
- * multiplied by mi_linear against fp16 weights. */
+ * fp32 += x W^T. The sums' order depends on the sizes alone. At most 2^24
+ * in_features and 2^27 out_features. For a decode row or the rows of some
+ * sequences' steps; a prompt's many rows are faster by mi_linear against fp16
+ * weights, where those are kept. */
 int mi_quantise_int4(const void *weight, void *codes, void *scales, void *zeros, int group,
                      int in_features, int out_features, void *stream);
 int mi_linear_int4(const void *x, const void *codes, const void *scales, const void *zeros,

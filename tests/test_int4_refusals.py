@@ -41,6 +41,10 @@ def test_linear_int4_refuses(change, word):
 @pytest.mark.parametrize("change,word", [
     (dict(in_features=0, x=On(0), codes=On(0), scales=On(0), zeros=On(0)), "at least one group"),
     (dict(rows=65535 * 64 + 1, x=On(1 << 40), out=On(1 << 40, 0x20000)), "rows"),
+    (dict(in_features=(1 << 24) + 128, x=On(1 << 40), codes=On(1 << 40, item=1),
+          scales=On(1 << 40), zeros=On(1 << 40)), "16777216 in_features"),
+    (dict(out_features=(1 << 27) + 1, codes=On(1 << 40, item=1), scales=On(1 << 40),
+          zeros=On(1 << 40), bias=None, out=On(1 << 40, 0x20000)), "134217728 out_features"),
 ])
 def test_linear_int4_refuses_sizes(change, word):
     from microinfer import _microinfer as m
