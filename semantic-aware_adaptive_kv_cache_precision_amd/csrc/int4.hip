@@ -363,19 +363,6 @@ namespace mi
 
     // ---- more rows ----------------------------------------------------------
 
-    // Words j of lanes g = 0..3 (lane / 16) to word g of lanes j.
-    __device__ inline void transpose_words(u32x4 &w)
-    {
-      unsigned a = w.x, b = w.y, c = w.z, d = w.w;
-      // The upper lanes' a and the lower lanes' c change places, and b's and d's;
-      // then the odd row groups' a and the even ones' b.
-      asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(a), "+v"(c));
-      asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(b), "+v"(d));
-      asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b));
-      asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(c), "+v"(d));
-      w = u32x4{a, b, c, d};
-    }
-
     constexpr int kChunk = 128; // inputs a wave takes at a time
 
     // NT tiles of 16 rows, FT tiles of 16 outputs a wave; Groups: groups in a
@@ -386,7 +373,8 @@ namespace mi
     __global__ void __launch_bounds__(64 * Waves) int4_tiles_kernel(Int4Args a)
     {
       constexpr int kPer = 4 / Groups; // instructions a group
-      constexpr int kStage = NT * 256; // 16-byte pieces of a wave's x
+      constexpr int kStage = NT * 256;               // 16-byte pieces of x
+      constexpr int kWaveStage = kStage + 64 * FT;   // and of a wave's codes
       extern __shared__ __align__(16) u32x4 stages[];
       const int lane = threadIdx.x & 63;
       const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
@@ -404,15 +392,20 @@ namespace mi
           reinterpret_cast<const char *>(a.scales + static_cast<std::size_t>(base) * a.groups);
       const char *zeros =
           reinterpret_cast<const char *>(a.zeros + static_cast<std::size_t>(base) * a.groups);
+      // Codes, scales and zeros are loaded by the lane's fourth: four lanes an
+      // output.
+      const int quarter = lane & 3;
       unsigned of[FT];
 #pragma unroll
       for (int u = 0; u < FT; ++u)
       {
-        of[u] = min(16 * u + n, a.features - 1 - base);
+        of[u] = min(16 * u + (lane >> 2), a.features - 1 - base);
       }
+      unsigned *words = reinterpret_cast<unsigned *>(
+          stages + (Shared ? 2 * kStage + wave * FT * 64 : wave * kWaveStage + kStage));
       // x comes in whole lines, four rows' chunks a load, and turns through the
       // wave's own LDS, piece p of row r at place p ^ r % 16 of its row.
-      u32x4 *stage = stages + (Shared ? 0 : wave * kStage);
+      u32x4 *stage = stages + (Shared ? 0 : wave * kWaveStage);
       const char *x =
           reinterpret_cast<const char *>(a.x + static_cast<std::size_t>(row0) * a.in);
       constexpr int kFetches = Shared ? (4 * NT + Waves - 1) / Waves : 4 * NT; // of four rows
@@ -439,7 +432,7 @@ namespace mi
       const int chunks = (a.in + kChunk - 1) / kChunk;
       // (Inputs past the last, and groups: the first's, which no product takes.)
       const auto fetch = [&](u32x4 (&to)[FT], int chunk) {
-        const int k = chunk * kChunk + 32 * g;
+        const int k = chunk * kChunk + 32 * quarter;
 #pragma unroll
         for (int u = 0; u < FT; ++u)
         {
@@ -471,10 +464,9 @@ namespace mi
           }
         }
       };
-      // Scales (low) and zeros of four chunks, lanes g those of chunk + g: a
-      // load is paid by the lines it touches, and a row's lie together.
+      // Scales (low) and zeros of four chunks, quarters q those of chunk + q.
       const auto fetch_meta = [&](unsigned (&to)[FT][Groups], int chunk) {
-        const int at_chunk = min(chunk + g, chunks - 1);
+        const int at_chunk = min(chunk + quarter, chunks - 1);
 #pragma unroll
         for (int u = 0; u < FT; ++u)
         {
@@ -522,11 +514,12 @@ namespace mi
       for (int chunk = begin; chunk < end; ++chunk)
       {
         const int of_four = (chunk - begin) & 3;
-        u32x4 now[FT];
+        // The codes, run p of 32 of output o at place p ^ o / 4 of its four.
 #pragma unroll
         for (int u = 0; u < FT; ++u)
         {
-          now[u] = next[u];
+          const int o = lane >> 2;
+          reinterpret_cast<u32x4 *>(words)[u * 64 + 4 * o + (quarter ^ (o >> 2))] = next[u];
 #pragma unroll
           for (int h = 0; h < Groups; ++h)
           {
@@ -553,11 +546,6 @@ namespace mi
         }
         const int k0 = chunk * kChunk;
 #pragma unroll
-        for (int u = 0; u < FT; ++u)
-        {
-          transpose_words(now[u]);
-        }
-#pragma unroll
         for (int h = 0; h < Groups; ++h)
         {
           if (h > 0 && k0 + 32 * kPer * h >= a.in)
@@ -580,7 +568,8 @@ namespace mi
 #pragma unroll
             for (int u = 0; u < FT; ++u)
             {
-              const unsigned word = now[u][h * kPer + j];
+              const unsigned word =
+                  words[u * 256 + 16 * n + 4 * ((h * kPer + j) ^ (n >> 2)) + g];
               const half8 q = codes_as_half(word);
 #pragma unroll
               for (int t = 0; t < NT; ++t)
@@ -594,7 +583,7 @@ namespace mi
           for (int u = 0; u < FT; ++u)
           {
             const unsigned both = static_cast<unsigned>(__builtin_amdgcn_ds_bpermute(
-                4 * (16 * of_four + n), static_cast<int>(four[u][h])));
+                4 * (4 * n + of_four), static_cast<int>(four[u][h])));
             const float s = h2f(static_cast<std::uint16_t>(both));
             const float z = h2f(static_cast<std::uint16_t>(both >> 16));
 #pragma unroll
@@ -631,7 +620,7 @@ namespace mi
 #pragma unroll
             for (int u = 0; u < FT; ++u)
             {
-              parts[wave * kStage + (t * FT + u) * 64 + lane] = y[t][u];
+              parts[wave * kWaveStage + (t * FT + u) * 64 + lane] = y[t][u];
             }
           }
         }
@@ -648,7 +637,7 @@ namespace mi
 #pragma unroll
             for (int u = 0; u < FT; ++u)
             {
-              y[t][u] += parts[(wave + p) * kStage + (t * FT + u) * 64 + lane];
+              y[t][u] += parts[(wave + p) * kWaveStage + (t * FT + u) * 64 + lane];
             }
           }
         }
@@ -739,7 +728,8 @@ namespace mi
                            (a.in + kChunk - 1) / kChunk, Shared ? 1 : Waves);
       const int per = Waves / a.splits;
       const dim3 grid((tiles + per - 1) / per, row_tiles);
-      constexpr std::size_t lds = sizeof(u32x4) * (Shared ? 2 : Waves) * NT * 256;
+      constexpr std::size_t lds =
+          sizeof(u32x4) * ((Shared ? 2 : Waves) * NT * 256 + Waves * FT * 64);
       auto kernel = out == Int4Out::kHalf
                         ? int4_tiles_kernel<Groups, NT, FT, Waves, Shared, Int4Out::kHalf>
                         : int4_tiles_kernel<Groups, NT, FT, Waves, Shared, Int4Out::kAccumulate>;
