@@ -425,6 +425,8 @@ int mi_kv_fold_kept(mi_kv_pages *kv, float *mass, long long mass_stride, float *
  * mass can be asked for. Calls that may overlap need partials of their own.
  * head_dim 64 or 128; at most 16 query heads a KV head; q, out and partials
  * 16-byte aligned, pages as an allocator's. Keys hold their bias, if any.
+ * Values are expected finite: one that is not, and is seen, may spoil 32
+ * channels of the heads that see it.
  * mi_kv_attention_batch: the same for `count` caches of one shape, the query
  * of cache i at position seq_k[i] - 1 of `layer` (seq_k in host memory; 0: no
  * token), its row stored before, as mi_kv_attention takes it: a cache that

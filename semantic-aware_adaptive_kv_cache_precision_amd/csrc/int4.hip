@@ -17,19 +17,17 @@
 //
 // More rows (int4_tiles_kernel): the matrix cores form x . codes (A: 16 rows of
 // x, B: 16 outputs' codes as fp16 integers, exact) and sum(x) (B: ones) of 32
-// inputs an instruction in fp32, and two fmas an output scale a group. A lane
-// loads 16 bytes of its output's codes, 32 inputs of the 128 its three
-// neighbours (lane ^ 16, 32, 48) complete; lane swaps transpose the four
-// words, so that an instruction's inputs are 32 in a row: of one group,
-// whatever its size.
-//
-// Those loads are paid by the lines they touch, about four cycles of a CU
-// each, before the bytes: so scales and zeros come four chunks at a load, x in
-// whole lines, four rows at a load, turned through LDS, and nothing is fetched
-// that is not used (of 16 rows of 2048 x 8192 each took 3 us of 16). 27 rows
-// of 8960 -> 1536: 9.1 us, 192 workgroups of two dependent trips of loads to a
-// step; 64 rows of 128256 x 2048: 80 us, a third of the matrix cores' rate,
-// the vector units making fp16 of codes beside them.
+// inputs an instruction in fp32, and two fmas an output scale a group. A step
+// is 128 inputs: their codes, 64 bytes an output, come four lanes an output
+// and turn through the wave's own LDS to a word an instruction, its inputs 32
+// in a row: of one group, whatever its size. x comes sixteen lanes a row and
+// turns the same way; scales and zeros come four steps at a load. (The lanes
+// of an operand lie along the rows, where each sixteen bytes are a request of
+// their own, and requests are what a CU runs out of: loaded so, and the next
+// step's fetched past the last, 16 rows of 2048 x 8192 took 16.1 us, now 8.0.)
+// 27 rows of 8960 -> 1536: 8.5 us, five dependent steps a wave; 64 rows of
+// 128256 x 2048: 79 us, a third of the matrix cores' rate, the vector units
+// making fp16 of codes beside them.
 //
 // A code becomes fp16 by the mask that splices it under the exponent of 1024
 // (or, four bits up, 1024 + 16 code): nine instructions for eight, which
