@@ -202,8 +202,9 @@ int mi_attention_paged_causal_noalloc(const void *q, const unsigned long long *s
  * sees key j <= p where window is 0, or j > p - window, or j < sinks. out
  * (seq_q, heads, head_dim) contiguous. head_dim 64 or 128, any whole number of
  * query heads a KV head; rows 16-byte aligned (strides multiples of 8).
- * partials: mi_attention_window_partials floats, the caller's until the launch
- * is done, which let few rows' keys be split over the device; or NULL. Calls
+ * partials: mi_attention_window_partials floats (of these sizes: others, smaller
+ * ones too, may ask for more), the caller's until the launch is done, which
+ * let few rows' keys be split over the device; or NULL. Calls
  * that may overlap need partials of their own. */
 int mi_attention_window_partials(int seq_q, int seq_k, int heads, int kv_heads, int head_dim,
                                  int window, int sinks, size_t *floats);
@@ -419,8 +420,8 @@ int mi_kv_fold_kept(mi_kv_pages *kv, float *mass, long long mass_stride, float *
  * out (batch, heads, head_dim) fp16; a sequence with nothing to see (length 0)
  * gives zeros. mass (batch, heads, max_pages) fp32 or NULL: each page's share
  * of each head's softmax, 0 for pages not read. partials:
- * mi_attention_batch_partials floats (for sequences of up to max_pages pages;
- * 0 where one launch does), the caller's until the launch is done, or NULL:
+ * mi_attention_batch_partials floats (for up to `batch` sequences of up to
+ * max_pages pages; 0 where one launch does), the caller's until the launch is done, or NULL:
  * then a sequence's pages are walked by one workgroup a few KV heads, and no
  * mass can be asked for. Calls that may overlap need partials of their own.
  * head_dim 64 or 128; at most 16 query heads a KV head; q, out and partials

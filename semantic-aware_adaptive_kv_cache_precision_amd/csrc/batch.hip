@@ -868,11 +868,14 @@ namespace mi
       int kv_block;
       int run_pages;
       int splits;
+      long long most_parts; // of a head over the batch, of partials
     };
+
+    constexpr long long kWorkgroups = 2048;
 
     Cut cut_of(int batch, int max_pages, int kv_heads, int window, int sinks)
     {
-      Cut c{1, 1, 1};
+      Cut c{1, 1, 1, 0};
       while (c.kv_block < kWaves && kv_heads % (2 * c.kv_block) == 0)
       {
         c.kv_block *= 2;
@@ -890,13 +893,18 @@ namespace mi
       // can be, each wave at least a page: a ragged batch fills half of them,
       // and more only adds parts to join (32 behind a window, in us: 1,024
       // workgroups 35.5, 2,048 29.8, 4,096 30.3; 16 to 32K 40.9, 36.8, 37.2).
-      constexpr long long kWorkgroups = 2048;
       const long long units = most * batch * (kv_heads / c.kv_block);
       long long run = std::max<long long>((units + kWorkgroups - 1) / kWorkgroups,
                                           (most + kMaxSplits - 1) / kMaxSplits);
       run = (run + phases - 1) / phases * phases;
       c.run_pages = static_cast<int>(std::min<long long>(run, 0x7fffffc0));
       c.splits = static_cast<int>((most + run - 1) / run);
+      // What no cut of fewer sequences or pages passes: a part a wave's page,
+      // and the workgroups that fill the device with one more a sequence.
+      const long long paged = std::min<long long>((most + phases - 1) / phases, kMaxSplits);
+      c.most_parts = paged <= 1 ? 0
+                                : std::min(batch * paged,
+                                           kWorkgroups / (kv_heads / c.kv_block) + batch);
       return c;
     }
 
@@ -955,7 +963,7 @@ namespace mi
     check_batch(t);
     const std::size_t rows = static_cast<std::size_t>(t.batch) * t.heads;
     const Cut cut = cut_of(t.batch, t.max_pages, t.kv_heads, t.window, t.sinks);
-    return (cut.splits > 1 ? rows * cut.splits * (t.head_dim + 2) : 0) +
+    return static_cast<std::size_t>(cut.most_parts) * t.heads * (t.head_dim + 2) +
            (with_mass ? rows * t.max_pages : 0);
   }
 

@@ -1399,7 +1399,8 @@ def _device_attention_window(q, k, v, out, seq_q, seq_k, heads, kv_heads, head_d
 @functools.lru_cache(maxsize=256, typed=True)
 def _attention_batch_partials(batch: int, max_pages: int, heads: int, kv_heads: int, head_dim: int,
                               window: int = 0, sinks: int = 0, mass: bool = False) -> int:
-    """Floats of partials attention_batch needs for these sizes."""
+    """Floats of partials attention_batch needs for up to these many sequences
+    and pages."""
     out = C.c_size_t()
     _check(lib.mi_attention_batch_partials(batch, max_pages, heads, kv_heads, head_dim, window,
                                            sinks, int(bool(mass)), C.byref(out)))

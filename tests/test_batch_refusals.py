@@ -69,3 +69,17 @@ def test_partials_grow_with_what_is_asked():
     assert need(1, 1024, 12, 2, 128, window=64, sinks=4) < need(1, 1024, 12, 2, 128)
     with pytest.raises(ValueError):
         need(1, 1024, 12, 2, 96)
+
+
+@pytest.mark.parametrize("heads,kv,hd", [(14, 2, 64), (12, 2, 128), (32, 8, 64), (6, 3, 64)])
+def test_partials_for_the_longest_and_most_do_for_less(heads, kv, hd):
+    """A buffer made for a serving run's largest step: no shorter or smaller one asks for more."""
+    from microinfer import _microinfer as m
+    need = m.device.attention_batch_partials
+    for window in (0, 700):
+        for batch in (1, 3, 8, 48, 300):
+            by_pages = [need(batch, p, heads, kv, hd, window, 4) for p in range(0, 1200, 7)]
+            assert by_pages == sorted(by_pages)
+    for pages in (1, 2, 3, 40, 1000):
+        by_batch = [need(b, pages, heads, kv, hd) for b in range(0, 400)]
+        assert by_batch == sorted(by_batch)
