@@ -766,9 +766,9 @@ namespace mi
     {
       throw InvalidArgument("window attention's rows and partials must be 16-byte aligned");
     }
-    if (t.out == t.q)
+    if (t.out == t.q || t.out == t.k || t.out == t.v)
     {
-      throw InvalidArgument("window attention cannot write over its queries");
+      throw InvalidArgument("window attention cannot write over its queries, keys or values");
     }
     const Cut c = cut_of(t, t.partials != nullptr);
     if (t.partials != nullptr && t.partials_floats < window_attention_floats(t))

@@ -30,6 +30,8 @@ def args(**change):
     (dict(q=On(768, 0x10008)), "aligned"),
     (dict(partials=On(100, 0x50008, 4)), "aligned"),
     (dict(out=On(768)), "over its queries"),
+    (dict(out=On(768, 0x20000)), "keys or values"),
+    (dict(out=On(768, 0x30000)), "keys or values"),
     (dict(head_dim=32), "head_dim 64 or 128"),
     (dict(kv_heads=3, k=On(10**6, 0x20000), v=On(10**6, 0x30000)), "whole number"),
     (dict(seq_k=0x7fffff01, k=On(1 << 50, 0x20000), v=On(1 << 50, 0x30000)), "exceeds window"),
