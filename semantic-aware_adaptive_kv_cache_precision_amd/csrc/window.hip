@@ -76,6 +76,7 @@ namespace mi
     constexpr float kProb = 8.0f; // P x 2^8
     constexpr float kProbUnscale = 1.0f / 256.0f;
     constexpr int kMaxSplits = 256;
+    constexpr int kFewSplits = 8; // that a lane joins one after another
 
     struct WindowArgs
     {
@@ -589,6 +590,61 @@ namespace mi
           u32x2{__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, y)};
     }
 
+    // The same for many splits: a workgroup a row, its groups of lanes each
+    // taking some, with maxima of their own (one query over 7,000 keys, 56 splits:
+    // 17.8 us in all with the kernel above, 9.9 with this).
+    template <int HD>
+    __global__ void __launch_bounds__(256) window_join_row_kernel(WindowArgs a, std::size_t rows)
+    {
+      constexpr int kLanes = HD / 4, kGroups = 256 / kLanes;
+      __shared__ f32x2 s_ml[kGroups];
+      __shared__ __align__(16) float s_o[kGroups][HD];
+      const std::size_t row = blockIdx.x;
+      const int group = threadIdx.x / kLanes;
+      const int d = 4 * static_cast<int>(threadIdx.x % kLanes);
+      float m = -INFINITY, l = 0.0f;
+      f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+      for (int s = group; s < a.splits; s += kGroups)
+      {
+        const f32x2 ml = *reinterpret_cast<const f32x2 *>(a.part_ml + 2 * (s * rows + row));
+        const f32x4 x = *reinterpret_cast<const f32x4 *>(a.part_o + (s * rows + row) * HD + d);
+        const float top = fmaxf(m, ml[0]);
+        const float from = top == -INFINITY ? 0.0f : top;
+        const float keep = __builtin_amdgcn_exp2f(m - from), w = __builtin_amdgcn_exp2f(ml[0] - from);
+        l = l * keep + ml[1] * w;
+        o = o * keep + x * w;
+        m = top;
+      }
+      if (d == 0)
+      {
+        s_ml[group] = f32x2{m, l};
+      }
+      *reinterpret_cast<f32x4 *>(&s_o[group][d]) = o;
+      __syncthreads();
+      if (threadIdx.x >= HD)
+      {
+        return;
+      }
+      float from = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i)
+      {
+        from = fmaxf(from, s_ml[i][0]);
+      }
+      from = from == -INFINITY ? 0.0f : from;
+      float sum = 0.0f, out = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i)
+      {
+        const float w = __builtin_amdgcn_exp2f(s_ml[i][0] - from);
+        sum += s_ml[i][1] * w;
+        out += s_o[i][threadIdx.x] * w;
+      }
+      a.out[row * HD + threadIdx.x] =
+          __builtin_bit_cast(std::uint16_t, static_cast<_Float16>(out / sum));
+    }
+
     // A launch's form: the row tiles of a workgroup, the waves that share a
     // tile's keys, and the keys a step. Few rows are a matter of latency, so
     // four waves take a quarter of a step's keys each (100 queries x 14 heads
@@ -627,13 +683,17 @@ namespace mi
       const long long span =
           t.window > 0 ? std::min<long long>(t.seq_k, static_cast<long long>(t.window) + t.sinks)
                        : t.seq_k;
-      // Few: what leaves no CU two of those workgroups; at head_dim 64, whose
-      // stages leave room, twice as many for short spans (measured in us, few
-      // against many: 1,024 x 14 heads behind 64 keys 11 and 15, 512 x 32 with
-      // 512 keys 10.7 and 12.9, with 4,096 keys 56 and 43; 768 x 12 of 128
-      // behind 1,024 keys 23.2 and 21.5, 512 of them 13.2 and 19.3).
+      // Few: what leaves no CU two of those workgroups; over long spans, where
+      // 32 rows are too few to share a step's copies, a half or a quarter of
+      // that; at head_dim 64, whose stages leave room, twice as many for short
+      // ones. Measured in us, few against many: 1,024 x 14 heads of 64 behind
+      // 64 keys 11 and 15; 512 x 32 over 512 keys 10.7 and 12.9; 256 x 32 over
+      // 1,256 16.7 and 18.2, over 3,256 34.5 and 23.2; 400 x 12 of 128 over 400
+      // 12.7 and 17.6, over 3,400 48.7 and 38.3; 256 x 12 over 3,256 32.3 and
+      // 35.6.
       const long long few = (rows + Few::rows - 1) / Few::rows * t.kv_heads;
-      c.few = few <= 256 || (t.head_dim == 64 && few <= 512 && span <= 1024);
+      const bool narrow = t.head_dim == 64;
+      c.few = few <= (span <= 1024 && narrow ? 512 : span <= 2048 ? 256 : narrow ? 64 : 128);
       c.rows = c.few ? Few::rows : t.head_dim == 64 ? Many64::rows : Many128::rows;
       c.keys = c.few ? Few::keys : t.head_dim == 64 ? Many64::keys : Many128::keys;
       c.blocks = static_cast<int>((rows + c.rows - 1) / c.rows);
@@ -641,18 +701,26 @@ namespace mi
       if (may_split && c.blocks > 0)
       {
         // About the steps a workgroup takes.
-        const long long steps = (span + c.keys - 1) / c.keys;
-        // A workgroup a CU, each with two steps to take or more; two of those
-        // for many rows of head_dim 128, whose four waves leave half a CU
-        // idle, but no more than four parts to join (1,536 x 12 heads behind
-        // 1,024 keys: by one part 44 us, by three 33.5; 768 of them by seven
-        // 23.5, by four 22). At head_dim 64 a workgroup has the CU's waves
-        // busy by itself (1,024 x 32: one part 19.5 us, two 26).
+        const long long reach = t.seq_k - t.seq_q / 2;
+        const long long steps = t.window > 0 && span < reach
+                                    ? (t.window + c.keys - 1) / c.keys + 1 +
+                                          (t.sinks + c.keys - 1) / c.keys
+                                    : (reach + c.keys - 1) / c.keys;
+        // A workgroup a CU, down to a step each for few rows, a chain of trips
+        // otherwise (one query x 14 heads of 64 over 1,000 keys: two steps each
+        // 10.2 us, one 9.8; 16 x 12 of 128 over 500 14.5 and 12.9), unless the
+        // chain is as short as the join (over 300: whole 8.0, in parts 9.7),
+        // and two or more steps for many. Two workgroups a CU for many rows of
+        // head_dim 128, whose four waves leave half of it idle, but no more
+        // than four parts to join (1,536 x 12 heads behind 1,024 keys: by one
+        // part 44 us, by three 33.5; 768 of them by seven 23.5, by four 22). At
+        // head_dim 64 a workgroup has the CU's waves busy by itself (1,024 x
+        // 32: one part 19.5 us, two 26).
         const bool two = !c.few && t.head_dim == 128;
         const long long fill =
             (two ? 512 : 256) / (static_cast<long long>(c.blocks) * t.kv_heads);
         c.splits = static_cast<int>(std::max<long long>(
-            1, std::min<long long>({fill, steps / 2, two ? 4 : kMaxSplits})));
+            1, std::min<long long>({fill, c.few ? (steps < 4 ? 1 : steps) : steps / 2, two ? 4 : kMaxSplits})));
       }
       return c;
     }
@@ -719,6 +787,12 @@ namespace mi
       if (c.splits > 1)
       {
         const std::size_t rows = static_cast<std::size_t>(a.seq_q) * a.heads;
+        if (c.splits > kFewSplits)
+        {
+          window_join_row_kernel<HD><<<static_cast<unsigned>(rows), 256, 0, stream>>>(a, rows);
+          hip_check(hipGetLastError(), "window_join_row_kernel");
+          return;
+        }
         const std::size_t blocks = (rows * (HD / 4) + 255) / 256;
         window_join_kernel<HD><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(a, rows);
         hip_check(hipGetLastError(), "window_join_kernel");
