@@ -715,10 +715,15 @@ namespace mi
         // than four parts to join (1,536 x 12 heads behind 1,024 keys: by one
         // part 44 us, by three 33.5; 768 of them by seven 23.5, by four 22). At
         // head_dim 64 a workgroup has the CU's waves busy by itself (1,024 x
-        // 32: one part 19.5 us, two 26).
+        // 32: one part 19.5 us, two 26), and a second part pays over long spans
+        // alone (680 x 32 behind 4,096: one 66 us, two 56; 1,400 x 14 over
+        // 4,400 57 and 51).
         const bool two = !c.few && t.head_dim == 128;
+        const long long groups = static_cast<long long>(c.blocks) * t.kv_heads;
         const long long fill =
-            (two ? 512 : 256) / (static_cast<long long>(c.blocks) * t.kv_heads);
+            !c.few && narrow && span > 2048 && groups > 128 && groups <= 256
+                ? 2
+                : (two ? 512 : 256) / groups;
         c.splits = static_cast<int>(std::max<long long>(
             1, std::min<long long>({fill, c.few ? (steps < 4 ? 1 : steps) : steps / 2, two ? 4 : kMaxSplits})));
       }

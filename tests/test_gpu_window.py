@@ -74,7 +74,7 @@ def test_windows_and_sinks(window, sinks, hd):
 @pytest.mark.parametrize("heads,kv,hd,seq_q,seq_k,window,sinks", [
     (32, 8, 64, 700, 900, 300, 4), (32, 8, 64, 601, 601, 0, 0), (12, 2, 128, 1500, 1500, 257, 70),
     (14, 2, 64, 1301, 1400, 64, 0), (28, 4, 128, 700, 703, 1, 0), (32, 8, 64, 300, 1500, 0, 0),
-    (32, 8, 64, 301, 1501, 1200, 130)])
+    (32, 8, 64, 301, 1501, 1200, 130), (32, 8, 64, 530, 2500, 0, 0), (14, 2, 64, 160, 2600, 2400, 33)])
 def test_many_rows(heads, kv, hd, seq_q, seq_k, window, sinks):
     """Prompts of the kernel's large tiles: ragged last tiles, waves with no rows."""
     rng = np.random.default_rng(seq_q)
