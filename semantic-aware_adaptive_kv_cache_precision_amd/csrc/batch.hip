@@ -872,8 +872,7 @@ namespace mi
     };
 
     constexpr long long kWorkgroups = 2048;
-
-    Cut cut_of(int batch, int max_pages, int kv_heads, int window, int sinks)
+    Cut cut_of(int batch, int max_pages, int kv_heads, int head_dim, int window, int sinks)
     {
       Cut c{1, 1, 1, 0};
       while (c.kv_block < kWaves && kv_heads % (2 * c.kv_block) == 0)
@@ -897,14 +896,22 @@ namespace mi
       long long run = std::max<long long>((units + kWorkgroups - 1) / kWorkgroups,
                                           (most + kMaxSplits - 1) / kMaxSplits);
       run = (run + phases - 1) / phases * phases;
+      // Pages a wave walks rather than have a second launch join them, in us (2
+      // KV heads): of 64, four pages 7.8 and 8.7, six 10.0 and 8.7; of 128, three
+      // 8.4 and 8.7, four 10.0 and 8.7.
+      const long long whole = head_dim == 64 ? 4 : 3;
+      const long long paged = std::min<long long>((most + phases - 1) / phases, kMaxSplits);
+      if (paged <= whole)
+      {
+        run = most;
+      }
       c.run_pages = static_cast<int>(std::min<long long>(run, 0x7fffffc0));
       c.splits = static_cast<int>((most + run - 1) / run);
       // What no cut of fewer sequences or pages passes: a part a wave's page,
       // and the workgroups that fill the device with one more a sequence.
-      const long long paged = std::min<long long>((most + phases - 1) / phases, kMaxSplits);
-      c.most_parts = paged <= 1 ? 0
-                                : std::min(batch * paged,
-                                           kWorkgroups / (kv_heads / c.kv_block) + batch);
+      c.most_parts = paged <= whole
+                         ? 0
+                         : std::min(batch * paged, kWorkgroups / (kv_heads / c.kv_block) + batch);
       return c;
     }
 
@@ -962,7 +969,7 @@ namespace mi
   {
     check_batch(t);
     const std::size_t rows = static_cast<std::size_t>(t.batch) * t.heads;
-    const Cut cut = cut_of(t.batch, t.max_pages, t.kv_heads, t.window, t.sinks);
+    const Cut cut = cut_of(t.batch, t.max_pages, t.kv_heads, t.head_dim, t.window, t.sinks);
     return static_cast<std::size_t>(cut.most_parts) * t.heads * (t.head_dim + 2) +
            (with_mass ? rows * t.max_pages : 0);
   }
@@ -993,7 +1000,7 @@ namespace mi
     {
       throw InvalidArgument("batch attention's masses need partials");
     }
-    Cut cut = cut_of(t.batch, t.max_pages, t.kv_heads, t.window, t.sinks);
+    Cut cut = cut_of(t.batch, t.max_pages, t.kv_heads, t.head_dim, t.window, t.sinks);
     if (t.partials == nullptr)
     {
       cut.run_pages = std::max(t.max_pages, 1);
