@@ -25,13 +25,14 @@
 // Bound by a page's chain, some 500 vector and 40 matrix instructions of a
 // SIMD that are busy 40% of the time, with the page's own trip to memory
 // before it: 16 sequences to 32,768 tokens (12 x 2 heads of 128, mixed tiers)
-// 36.5 us of which the join is 6, 2.4 TB/s; 32 to 16,640 behind a 4,096-token
-// window (32 x 8 heads of 64) 29 us, 2.7 TB/s; 8 to 5,000 with masses 14 us;
+// 30.4 us of which the join is 6, 2.9 TB/s; 32 to 16,640 behind a 4,096-token
+// window (32 x 8 heads of 64) 29 us, 2.7 TB/s; 8 to 5,000 with masses 12.9;
 // one of 33 tokens 5.5 us, one launch. Four waves a workgroup: eight took 54
 // and 38 us for the first two. Scalar page bases and 32-bit lane offsets, not
-// kept from page to page, leave four waves a SIMD at head_dim 64 and three at
-// 128. The next page fetched ahead, into registers or LDS, costs waves: 39 and
-// 34 us.
+// kept from page to page, leave four waves a SIMD at head_dim 64; two a SIMD,
+// evenly, are better than three at 128. The next page fetched ahead into LDS
+// costs waves at 64 (34 us) and saves nothing at 128, nor does memory: with
+// every page in the caches the first two take 33.8 of 36.6 and 27.5 of 28.3.
 
 #include "common.hpp"
 #include "dequant.hpp"
@@ -545,7 +546,7 @@ namespace mi
     }
 
     template <int HD, bool kHeld>
-    __global__ void __launch_bounds__(kThreads, HD == 64 ? 4 : 3) batch_pages_kernel(BatchArgs a,
+    __global__ void __launch_bounds__(kThreads, HD == 64 ? 4 : 2) batch_pages_kernel(BatchArgs a,
                                                                                     Sequences<kHeld> held)
     {
       constexpr int S = HD / 32;
@@ -871,7 +872,6 @@ namespace mi
       long long most_parts; // of a head over the batch, of partials
     };
 
-    constexpr long long kWorkgroups = 2048;
     Cut cut_of(int batch, int max_pages, int kv_heads, int head_dim, int window, int sinks)
     {
       Cut c{1, 1, 1, 0};
@@ -889,11 +889,13 @@ namespace mi
       }
       most = std::max<long long>(most, 1);
       // Eight workgroups a CU over the batch if every sequence is as long as it
-      // can be, each wave at least a page: a ragged batch fills half of them,
-      // and more only adds parts to join (32 behind a window, in us: 1,024
-      // workgroups 35.5, 2,048 29.8, 4,096 30.3; 16 to 32K 40.9, 36.8, 37.2).
+      // can be (six of head_dim 128, which has two at a time), each wave at
+      // least a page: a ragged batch fills half of them, and more only adds
+      // parts to join (32 behind a window, in us: 1,024 workgroups 35.5, 2,048
+      // 29, 4,096 30; of 128, 16 to 32K: 1,408 30.3, 1,536 30.4, 1,792 36.7).
+      const long long workgroups = head_dim == 64 ? 2048 : 1536;
       const long long units = most * batch * (kv_heads / c.kv_block);
-      long long run = std::max<long long>((units + kWorkgroups - 1) / kWorkgroups,
+      long long run = std::max<long long>((units + workgroups - 1) / workgroups,
                                           (most + kMaxSplits - 1) / kMaxSplits);
       run = (run + phases - 1) / phases * phases;
       // Pages a wave walks rather than have a second launch join them, in us (2
@@ -911,7 +913,7 @@ namespace mi
       // and the workgroups that fill the device with one more a sequence.
       c.most_parts = paged <= whole
                          ? 0
-                         : std::min(batch * paged, kWorkgroups / (kv_heads / c.kv_block) + batch);
+                         : std::min(batch * paged, workgroups / (kv_heads / c.kv_block) + batch);
       return c;
     }
 
@@ -950,9 +952,15 @@ namespace mi
     void launch(const BatchArgs &a, const Sequences<kHeld> &held, int batch, hipStream_t stream)
     {
       const int phases = kWaves / a.kv_block;
-      const std::size_t lds =
+      // At head_dim 128 LDS for no more than two workgroups a CU: the launch
+      // order gives some CUs three while others have one, and three take
+      // nearly twice two's time (16 to 32K 35.4 us, so 30.4; 8 to 5K 14.1 and
+      // 12.9).
+      constexpr std::size_t kThirdOfLds = HD == 64 ? 0 : 55 * 1024;
+      const std::size_t lds = std::max(
+          kThirdOfLds,
           sizeof(float) * (kMetaFloats<HD> + (phases - 1) * a.kv_block * kWaveFloats<HD> +
-                           kHeadFloats);
+                           kHeadFloats));
       const dim3 grid(a.splits, a.kv_heads / a.kv_block, batch);
       batch_pages_kernel<HD, kHeld><<<grid, kThreads, lds, stream>>>(a, held);
       hip_check(hipGetLastError(), "batch_pages_kernel");
