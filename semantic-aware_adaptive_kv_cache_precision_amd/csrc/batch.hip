@@ -792,6 +792,7 @@ namespace mi
     {
       __shared__ f32x2 s_ml[kJoinThreads / (HD / 4)];
       __shared__ __align__(16) float s_o[kJoinThreads / (HD / 4)][HD];
+      __shared__ f32x2 s_total;
       const int b = blockIdx.y;
       const std::size_t head = static_cast<std::size_t>(b) * a.heads + blockIdx.x;
       int length;
@@ -831,30 +832,37 @@ namespace mi
       }
       *reinterpret_cast<f32x4 *>(&s_o[group][d]) = o;
       __syncthreads();
-      float from = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < kGroups; ++i)
-      {
-        from = fmaxf(from, s_ml[i][0]);
-      }
-      from = from == -INFINITY ? 0.0f : from;
-      float sum = 0.0f, out = 0.0f;
-#pragma unroll
-      for (int i = 0; i < kGroups; ++i)
-      {
-        const float w = __builtin_amdgcn_exp2f(s_ml[i][0] - from);
-        sum += s_ml[i][1] * w;
-        out += s_o[i][threadIdx.x % HD] * w;
-      }
-      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      // (By the waves that have an output: the others' reads would be in the way.)
       if (threadIdx.x < HD)
       {
+        float from = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kGroups; ++i)
+        {
+          from = fmaxf(from, s_ml[i][0]);
+        }
+        from = from == -INFINITY ? 0.0f : from;
+        float sum = 0.0f, out = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kGroups; ++i)
+        {
+          const float w = __builtin_amdgcn_exp2f(s_ml[i][0] - from);
+          sum += s_ml[i][1] * w;
+          out += s_o[i][threadIdx.x] * w;
+        }
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         a.out[head * HD + threadIdx.x] = __half_as_ushort(__float2half(out * inv));
+        if (threadIdx.x == 0)
+        {
+          s_total = f32x2{from, inv};
+        }
       }
       if (a.mass == nullptr)
       {
         return;
       }
+      __syncthreads();
+      const float from = s_total[0], inv = s_total[1];
       float *mass = a.mass + head * a.max_pages;
       const float *held_from = a.mass_from + head * a.max_pages;
       for (int p = threadIdx.x; p < a.max_pages; p += kJoinThreads)
