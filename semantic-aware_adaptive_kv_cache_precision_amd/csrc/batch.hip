@@ -25,8 +25,8 @@
 // Bound by a page's chain, some 500 vector and 40 matrix instructions of a
 // SIMD that are busy 40% of the time, with the page's own trip to memory
 // before it: 16 sequences to 32,768 tokens (12 x 2 heads of 128, mixed tiers)
-// 30.4 us of which the join is 6, 2.9 TB/s; 32 to 16,640 behind a 4,096-token
-// window (32 x 8 heads of 64) 29 us, 2.7 TB/s; 8 to 5,000 with masses 12.9;
+// 29.5 us of which the join is 5, 3.0 TB/s; 32 to 16,640 behind a 4,096-token
+// window (32 x 8 heads of 64) 27.5 us, 2.8 TB/s; 8 to 5,000 with masses 12.8;
 // one of 33 tokens 5.5 us, one launch. Four waves a workgroup: eight took 54
 // and 38 us for the first two. Scalar page bases and 32-bit lane offsets, not
 // kept from page to page, leave four waves a SIMD at head_dim 64; two a SIMD,

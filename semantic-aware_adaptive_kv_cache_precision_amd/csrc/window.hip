@@ -36,7 +36,7 @@
 // at head_dim 64 take some 450 cycles of a SIMD (16 exponentials a lane at a
 // quarter of the rate are 256 of them), its products 256, and the two overlap
 // only across waves. 2,048 queries x 32 heads at 14,336 behind a 4,096-token
-// window with 4 sinks, head_dim 64: 100.5 us, 684 TFLOP/s. A prompt of 4,096 x
+// window with 4 sinks, head_dim 64: 102 us, 675 TFLOP/s. A prompt of 4,096 x
 // 12 heads of 128 behind 1,024: 57.5 us, 394 TFLOP/s, its 384 workgroups
 // leaving half the CUs one instead of two. 100 queries x 14 heads of 64:
 // 5.9 us, a launch and a chain of loads. Measured and not taken: 64 rows a
