@@ -36,8 +36,8 @@
 
 #include "common.hpp"
 #include "dequant.hpp"
-#include "kernels.hpp"
 #include "lane_ops.hpp"
+#include "serving.hpp"
 
 #include <algorithm>
 #include <cmath>

@@ -36,8 +36,8 @@
 // rounding of y. An output's inputs are split over up to sixteen waves, whose
 // sums meet in LDS in wave order: the bits do not depend on timing.
 
-#include "kernels.hpp"
 #include "quant_core.hpp"
+#include "serving.hpp"
 
 #include <algorithm>
 #include <string>

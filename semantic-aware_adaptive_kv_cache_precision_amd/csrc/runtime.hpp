@@ -14,6 +14,7 @@
 
 #include "common.hpp"
 #include "kernels.hpp"
+#include "serving.hpp"
 
 #include <array>
 #include <atomic>

@@ -47,8 +47,8 @@
 // either way).
 
 #include "common.hpp"
-#include "kernels.hpp"
 #include "lane_ops.hpp"
+#include "serving.hpp"
 
 #include <algorithm>
 #include <cmath>
