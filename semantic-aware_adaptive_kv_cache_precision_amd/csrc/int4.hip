@@ -25,7 +25,8 @@
 // of an operand lie along the rows, where each sixteen bytes are a request of
 // their own, and requests are what a CU runs out of: loaded so, and the next
 // step's fetched past the last, 16 rows of 2048 x 8192 took 16.1 us, now 8.0.)
-// 27 rows of 8960 -> 1536: 8.3 us, five dependent steps a wave; 64 rows of
+// 27 rows of 8960 -> 1536: 8.3 us, what a CU takes in (its 16 rows of x whole,
+// 287 KB; two steps fetched ahead 9.6); 64 rows of
 // 128256 x 2048: 79 us, a third of the matrix cores' rate, the vector units
 // making fp16 of codes beside them.
 //
