@@ -431,8 +431,11 @@ int mi_kv_fold_kept(mi_kv_pages *kv, float *mass, long long mass_stride, float *
  * mi_kv_attention_batch: the same for `count` caches of one shape, the query
  * of cache i at position seq_k[i] - 1 of `layer` (seq_k in host memory; 0: no
  * token), its row stored before, as mi_kv_attention takes it: a cache that
- * seals reads the row from keys, values (count, kv_width) fp16. A cache may be
- * named twice. mass (count, heads, mass_pages). partials: for max_pages =
+ * seals reads the row from keys, values (count, kv_width) fp16, and the rows
+ * before it in its page as they were stored, which it holds for the page being
+ * filled and for one that a store of a single row completed; a token of
+ * another page (one that a prompt's store completed, or an earlier one), but
+ * for a page's first, is refused. A cache may be named twice. mass (count, heads, mass_pages). partials: for max_pages =
  * mass_pages, or without mass the longest sequence's pages. On the runtime's
  * current stream; the caches' pages must not move while a captured one is
  * replayed. */

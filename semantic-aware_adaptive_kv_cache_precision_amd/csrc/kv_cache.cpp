@@ -210,6 +210,7 @@ namespace mi
     }
     current_open_.assign(layers, 0);
     attend_open_.assign(layers, 0);
+    open_rows_.assign(layers, OpenRows{});
     sealed_.assign(layers, 0);
     open_address_.assign(2 * static_cast<std::size_t>(layers), 0);
     allocator_.watch(this);
@@ -463,6 +464,7 @@ namespace mi
     const std::size_t half = static_cast<std::size_t>(page_tokens_) * W;
     const int cur = current_open_[layer];
     attend_open_[layer] = cur;
+    open_rows_[layer].end = start + n;
     const int first_span = start / page_tokens_;
     const int end = start + n;
     std::vector<RowJob> jobs;
@@ -489,6 +491,10 @@ namespace mi
       {
         // The page's last row is here: it is sealed from the rows the open
         // page holds before `a` and the rows brought from `a` on.
+        if (OpenRows &held = open_rows_[layer]; held.page == span)
+        {
+          held.rows = std::min(held.rows, a - span_start);
+        }
         const PageKey key{layer, span};
         const PageLocation at = allocator_.locate(key);
         const auto place = reinterpret_cast<unsigned long long>(allocator_.address_of(at));
@@ -541,6 +547,17 @@ namespace mi
         j.dst = reinterpret_cast<std::uint8_t *>(open_page(layer, which));
         j.tier = kFP16;
         current_open_[layer] = which;
+        OpenRows &held = open_rows_[layer];
+        if (a == span_start || (held.page == span && held.rows >= a - span_start))
+        {
+          held.page = span;
+          held.rows = b - span_start;
+        }
+        else if (held.page != kSomePage)
+        {
+          held.page = -1; // rows of a page whose first ones are elsewhere
+          held.rows = 0;
+        }
       }
       jobs.push_back(j);
     }
@@ -1258,6 +1275,19 @@ namespace mi
     {
       throw LogicError("attention before any position was reserved");
     }
+    const OpenRows &held = open_rows_[layer];
+    const int own_page = (seq_k - 1) / page_tokens_;
+    const int before = seq_k - 1 - own_page * page_tokens_;
+    if (seals_ && before > 0 && held.page != kSomePage &&
+        (held.page != own_page || held.rows < before))
+    {
+      throw InvalidArgument(
+          "a batch's token at position " + std::to_string(seq_k - 1) + " of layer " +
+          std::to_string(layer) + " reads its page's rows before it as they were stored, and this "
+          "cache holds " + std::to_string(held.rows) + " of page " + std::to_string(held.page) +
+          " so (a store of several rows that completes a page leaves those it brought at the "
+          "page's tier alone)");
+    }
     sync_tables(runtime_stream());
     const std::size_t row = static_cast<std::size_t>(layer) * table_.stride();
     s.length = seq_k;
@@ -1268,7 +1298,9 @@ namespace mi
     }
     if (seals_)
     {
-      s.open = open_page(layer, attend_open_[layer]);
+      // (The page being filled now: after a store over several pages the one
+      // that it ended in, where attention over its rows reads the one it began in.)
+      s.open = open_page(layer, current_open_[layer]);
       s.own_k = key;
       s.own_v = value;
     }
@@ -1445,6 +1477,7 @@ namespace mi
     st.kv_heads = kv_heads_;
     launch_step_store(st, head_dim_, stream);
     attend_open_[layer] = current_open_[layer];
+    open_rows_[layer].page = kSomePage;
   }
 
   void KVPages::rope_store(int layer, const void *qk, void *qk_out, int q_heads,
@@ -1587,6 +1620,7 @@ namespace mi
     st.tiers = table_.tiers() + row;
     st.kv_heads = kv_heads_;
     attend_open_[layer] = current_open_[layer];
+    open_rows_[layer].page = kSomePage;
     return st;
   }
 
@@ -1698,6 +1732,13 @@ namespace mi
     {
       sealed_[layer] = std::max(sealed_[layer], end / page_tokens_);
       attend_open_[layer] = current_open_[layer];
+      OpenRows &held = open_rows_[layer];
+      if (end > 0 && (held.page == kSomePage || held.end != end))
+      {
+        // (A row at a time: the one that completed a page is not in it.)
+        const int page = (end - 1) / page_tokens_;
+        held = {page, std::min(end - page * page_tokens_, page_tokens_ - 1), end};
+      }
     }
   }
 

@@ -592,7 +592,8 @@ namespace mi
     // Beyond the reference: this cache as one sequence of a batch's decode
     // (launch_batch_attention), its token at position seq_k - 1 (seq_k 0: no
     // token). A cache that seals reads the token's row from key and value
-    // (kv_width fp16 each). Good until the cache's next call.
+    // (kv_width fp16 each), and refuses a token whose page's rows before it
+    // it does not hold as they were stored. Good until the cache's next call.
     BatchSequence batch_sequence(int layer, int seq_k, int kv_heads, int head_dim,
                                  const std::uint16_t *key, const std::uint16_t *value);
     // Beyond the reference: the pieces of a decode step whose position lives
@@ -741,6 +742,17 @@ namespace mi
     bool open_pages_ = false;
     std::vector<int> current_open_;
     std::vector<int> attend_open_;
+    // A layer's open page as batch_sequence reads it: which page's rows the
+    // current one holds as they were stored, and how many from its first on.
+    // A page that a store completes keeps the rows before that store.
+    struct OpenRows
+    {
+      int page = -1; // none
+      int rows = 0;
+      int end = 0; // of the last store that the host knows
+    };
+    static constexpr int kSomePage = -2; // a step's, whose position the host does not know
+    std::vector<OpenRows> open_rows_;
     std::vector<int> sealed_;
     std::vector<unsigned long long> open_address_; // [layer][2]
     std::vector<std::uint8_t> flags_;              // [layer][flag_stride_]

@@ -1454,7 +1454,9 @@ def _device_attention_caches(caches, seq_k, layer, q, out, heads, kv_heads, head
                              partials=None):
     """attention_batch over KVPages: the query of caches[i] is at position
     seq_k[i] - 1 of `layer` (0: no token), stored before; caches that seal
-    read its row from keys and values (len(caches), kv_width). `mass` holds
+    read its row from keys and values (len(caches), kv_width) and refuse a
+    token whose page's rows they no longer hold as stored (one completed by a
+    store of several rows, or an earlier one). `mass` holds
     (len(caches), heads, mass_pages) floats, mass_pages the longest sequence's
     pages where it is not given."""
     n = len(caches)
