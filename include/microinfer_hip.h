@@ -257,7 +257,9 @@ int mi_linear_f32(const void *x, const void *weight, float *out, int accumulate,
  * whose 15 steps reach the group's range, codes rounded half to even.
  * mi_linear_int4: out (rows, out) fp16 = x (rows, in) W^T + bias (out fp16, or
  * null), fp32 sums rounded once. mi_linear_int4_accumulate: out (rows, out)
- * fp32 += x W^T. The sums' order depends on the sizes alone. At most 2^24
+ * fp32 += x W^T. The sums' order depends on the sizes alone. A row of x that
+ * holds infinities or NaN gives what its terms x (code * scale + zero) sum to,
+ * other rows theirs. At most 2^24
  * in_features and 2^27 out_features. For a decode row or the rows of some
  * sequences' steps; a prompt's many rows are faster by mi_linear against fp16
  * weights, where those are kept. */
