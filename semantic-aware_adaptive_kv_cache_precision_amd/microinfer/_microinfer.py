@@ -713,7 +713,8 @@ class FloatTensor:
 
 
 class DeviceIndex:
-    """int32 on the device: token ids or positions."""
+    """int32 on the device: token ids or positions, or the words of a table
+    (two an address, four tiers each: host arrays viewed as int32)."""
 
     def __init__(self, host):
         h = np.ascontiguousarray(host, np.int32).reshape(-1)
@@ -724,6 +725,10 @@ class DeviceIndex:
     @property
     def address(self) -> int:
         return self._storage.ptr
+
+    @property
+    def nbytes(self) -> int:
+        return 4 * self.count
 
 
 @functools.lru_cache(maxsize=64, typed=True)
@@ -1391,7 +1396,7 @@ def _device_attention_window(q, k, v, out, seq_q, seq_k, heads, kv_heads, head_d
     ka = _at(k, _strided(seq_k, k_stride, width), "k")
     va = _at(v, _strided(seq_k, v_stride, width), "v")
     oa = _at(out, seq_q * q_width, "out")
-    wa, floats = (partials.address, partials.numel) if partials is not None else (None, 0)
+    wa, floats = _scratch(partials)
     _check(lib.mi_attention_window(qa, ka, va, oa, q_stride, k_stride, v_stride, seq_q, seq_k, heads,
                                    kv_heads, head_dim, window, sinks, wa, floats, None))
 
@@ -1407,15 +1412,25 @@ def _attention_batch_partials(batch: int, max_pages: int, heads: int, kv_heads: 
     return out.value
 
 
-def _entries(x) -> int:
-    """The elements of a device array of any type."""
-    return x.numel if hasattr(x, "numel") else x.count
-
-
-def _held(x, count: int, what: str) -> int:
-    if _entries(x) < count:
-        raise ValueError(f"{what} holds {_entries(x)}, and the operation needs {count}")
+def _table(x, count: int, size: int, what: str) -> int:
+    """The address of a device array, of whatever elements, whose bytes must
+    hold `count` entries of `size` bytes."""
+    if x.nbytes < size * count:
+        raise ValueError(f"{what} holds {x.nbytes // size} entries of {size} bytes, and the "
+                         f"operation needs {count}")
     return x.address
+
+
+def _fp32_at(t, count: int, what: str) -> int:
+    """As _floats, by the buffer's bytes."""
+    if t.nbytes < 4 * count:
+        raise ValueError(f"{what} needs {count} floats; got {t.nbytes // 4}")
+    return t.address
+
+
+def _scratch(partials):
+    """The address and the floats of partials, or none."""
+    return (partials.address, partials.nbytes // 4) if partials is not None else (None, 0)
 
 
 def _batch_sizes(batch, max_pages, heads, head_dim, q, out, mass):
@@ -1425,7 +1440,7 @@ def _batch_sizes(batch, max_pages, heads, head_dim, q, out, mass):
     per = batch * heads
     qa = _at(q, per * head_dim, "q")
     oa = _at(out, per * head_dim, "out")
-    ma = _floats(mass, per * max_pages, "mass") if mass is not None else None
+    ma = _fp32_at(mass, per * max_pages, "mass") if mass is not None else None
     return qa, oa, ma
 
 
@@ -1435,16 +1450,17 @@ def _device_attention_batch(q, pages, tiers, lengths, out, batch, max_pages, hea
     mixed-precision caches. q and out hold (batch, heads, head_dim) fp16;
     `pages` (batch, max_pages) 64-bit device addresses of 32-token pages,
     `tiers` their tiers (bytes; 255: not read) and `lengths` (batch) int32 each
-    sequence's tokens, the query's own counted, all device arrays read when
-    the kernels run. With `window`, a query sees its last `window` tokens and
+    sequence's tokens, the query's own counted, all device arrays (of any
+    elements: a DeviceIndex of the host table's int32 words) read when the
+    kernels run. With `window`, a query sees its last `window` tokens and
     the first `sinks`. `mass` (batch, heads, max_pages) floats takes each
     page's share of the softmax. `partials` holds attention_batch_partials
     floats and lets a sequence be read by several workgroups; masses need it."""
     qa, oa, ma = _batch_sizes(batch, max_pages, heads, head_dim, q, out, mass)
-    pa = _held(pages, batch * max_pages, "pages")
-    ta = _held(tiers, batch * max_pages, "tiers")
-    la = _held(lengths, batch, "lengths")
-    wa, floats = (partials.address, partials.numel) if partials is not None else (None, 0)
+    pa = _table(pages, batch * max_pages, 8, "pages")
+    ta = _table(tiers, batch * max_pages, 1, "tiers")
+    la = _table(lengths, batch, 4, "lengths")
+    wa, floats = _scratch(partials)
     _check(lib.mi_attention_batch(qa, pa, ta, la, batch, max_pages, P_DEFAULT, oa, heads, kv_heads,
                                   head_dim, window, sinks, ma, wa, floats, None))
 
@@ -1472,7 +1488,7 @@ def _device_attention_caches(caches, seq_k, layer, q, out, heads, kv_heads, head
     qa, oa, ma = _batch_sizes(n, mass_pages, heads, head_dim, q, out, mass)
     ka = _at(keys, n * width, "keys") if keys is not None else None
     va = _at(values, n * width, "values") if values is not None else None
-    wa, floats = (partials.address, partials.numel) if partials is not None else (None, 0)
+    wa, floats = _scratch(partials)
     _check(lib.mi_kv_attention_batch((_vp * n)(*(c._h for c in caches)), (C.c_int * n)(*seq_k), n,
                                      layer, qa, oa, heads, kv_heads, head_dim, ka, va, window, sinks,
                                      ma, mass_pages, wa, floats))
@@ -1601,7 +1617,7 @@ def _device_linear_int4_accumulate(x, codes, scales, zeros, group, out: FloatTen
     _non_negative(rows, "rows")
     ca, sa, za = _int4_at(codes, scales, zeros, group, in_features, out_features)
     xa = _at(x, rows * in_features, "x")
-    oa = _floats(out, rows * out_features, "out")
+    oa = _fp32_at(out, rows * out_features, "out")
     _check(lib.mi_linear_int4_accumulate(xa, ca, sa, za, group, oa, rows, in_features,
                                          out_features, None))
 
