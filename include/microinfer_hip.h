@@ -201,7 +201,9 @@ int mi_attention_paged_causal_noalloc(const void *q, const unsigned long long *s
  * that the three may lie in one projection's rows. The query at position p
  * sees key j <= p where window is 0, or j > p - window, or j < sinks. out
  * (seq_q, heads, head_dim) contiguous. head_dim 64 or 128, any whole number of
- * query heads a KV head; rows 16-byte aligned (strides multiples of 8).
+ * query heads a KV head; rows 16-byte aligned (strides multiples of 8). What is
+ * written (out, partials) may share no byte with what is read, or is refused:
+ * so too in the batch's and the 4-bit operators.
  * partials: mi_attention_window_partials floats (of these sizes: others, smaller
  * ones too, may ask for more), the caller's until the launch is done, which
  * let few rows' keys be split over the device; or NULL. Calls

@@ -981,6 +981,42 @@ namespace mi
     }
   } // namespace
 
+  namespace
+  {
+    void check_overlaps(const BatchAttention &t)
+    {
+      const std::size_t rows = static_cast<std::size_t>(t.batch) * t.heads;
+      const std::size_t entries = static_cast<std::size_t>(t.batch) * t.max_pages;
+      const Extent q{t.q, 2 * rows * t.head_dim}, out{t.out, 2 * rows * t.head_dim};
+      const Extent mass{t.mass, sizeof(float) * rows * t.max_pages};
+      const Extent parts{t.partials, t.partials == nullptr
+                                         ? 0
+                                         : sizeof(float) *
+                                               batch_attention_floats(t, t.mass != nullptr)};
+      const Extent pages{t.pages, 8 * entries}, tiers{t.tiers, entries};
+      const Extent lengths{t.lengths, sizeof(int) * static_cast<std::size_t>(t.batch)};
+      const std::size_t row = 2 * static_cast<std::size_t>(t.kv_heads) * t.head_dim;
+      for (const Extent &written : {out, mass, parts})
+      {
+        bool over = overlaps(written, q) || overlaps(written, pages) || overlaps(written, tiers) ||
+                    overlaps(written, lengths);
+        for (int b = 0; t.held != nullptr && b < t.batch; ++b)
+        {
+          over = over || overlaps(written, {t.held[b].own_k, row}) ||
+                 overlaps(written, {t.held[b].own_v, row});
+        }
+        if (over)
+        {
+          throw InvalidArgument("batch attention cannot write over its queries, tables or rows");
+        }
+      }
+      if (overlaps(out, mass) || overlaps(out, parts) || overlaps(mass, parts))
+      {
+        throw InvalidArgument("batch attention's output, masses and partials write over one another");
+      }
+    }
+  } // namespace
+
   std::size_t batch_attention_floats(const BatchAttention &t, bool with_mass)
   {
     check_batch(t);
@@ -1008,10 +1044,6 @@ namespace mi
     {
       throw InvalidArgument("batch attention's q, out and partials must be 16-byte aligned");
     }
-    if (t.q == t.out)
-    {
-      throw InvalidArgument("batch attention cannot write over its queries");
-    }
     if (t.mass != nullptr && t.partials == nullptr && t.max_pages > 0)
     {
       throw InvalidArgument("batch attention's masses need partials");
@@ -1029,6 +1061,7 @@ namespace mi
                             " floats; got " +
                             std::to_string(t.partials_floats));
     }
+    check_overlaps(t);
     BatchArgs a{};
     a.q = static_cast<const std::uint16_t *>(t.q);
     a.out = static_cast<std::uint16_t *>(t.out);

@@ -934,6 +934,18 @@ namespace mi
       {
         throw InvalidArgument("an int4 projection needs at least one group of inputs");
       }
+      const std::size_t outputs = static_cast<std::size_t>(features);
+      const std::size_t meta = 2 * outputs * (in / group);
+      const Extent written{out, (kind == Int4Out::kHalf ? 2 : 4) * outputs * rows};
+      for (const Extent &read : {Extent{x, 2 * static_cast<std::size_t>(rows) * in},
+                                 Extent{codes, outputs * (in / 2)}, Extent{scales, meta},
+                                 Extent{zeros, meta}, Extent{bias, 2 * outputs}})
+      {
+        if (overlaps(written, read))
+        {
+          throw InvalidArgument("an int4 projection cannot write over its input or weight");
+        }
+      }
       Int4Args a{};
       a.x = static_cast<const std::uint16_t *>(x);
       a.codes = static_cast<const std::uint8_t *>(codes);
@@ -974,6 +986,15 @@ namespace mi
     if (blocks > 0x7fffffffull)
     {
       throw InvalidArgument("a weight of " + std::to_string(8 * count) + " values is too large");
+    }
+    const std::size_t meta = 16 * count / group;
+    const Extent read{weight, 16 * count}, code_bytes{codes, 4 * count};
+    const Extent scale_bytes{scales, meta}, zero_bytes{zeros, meta};
+    if (overlaps(code_bytes, read) || overlaps(scale_bytes, read) || overlaps(zero_bytes, read) ||
+        overlaps(code_bytes, scale_bytes) || overlaps(code_bytes, zero_bytes) ||
+        overlaps(scale_bytes, zero_bytes))
+    {
+      throw InvalidArgument("codes, scales and zeros cannot write over the weight or one another");
     }
     const dim3 grid(static_cast<unsigned>(blocks));
     const auto *w = static_cast<const std::uint16_t *>(weight);

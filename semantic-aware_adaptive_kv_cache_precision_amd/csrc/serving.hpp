@@ -5,8 +5,39 @@
 
 #include "common.hpp"
 
+#include <cstddef>
+#include <cstdint>
+
 namespace mi
 {
+
+  // ---- what a launch may not write over ----------------------------------------------
+  // Memory that a launch reads or writes: `bytes` from `at`, or rows of them
+  // `stride` bytes apart. (Null, or no bytes: none.)
+  struct Extent
+  {
+    const void *at;
+    std::size_t bytes;
+    std::size_t rows = 1;
+    std::size_t stride = 0;
+  };
+  // Whether `a`, one run of bytes, shares a byte with some row of `b`.
+  inline bool overlaps(const Extent &a, const Extent &b)
+  {
+    if (a.at == nullptr || b.at == nullptr || a.bytes == 0 || b.bytes == 0 || b.rows == 0)
+    {
+      return false;
+    }
+    const auto from = reinterpret_cast<std::uintptr_t>(a.at), to = from + a.bytes;
+    const auto first = reinterpret_cast<std::uintptr_t>(b.at);
+    // The first row that ends behind `from`.
+    std::size_t row = 0;
+    if (first + b.bytes <= from && b.stride > 0)
+    {
+      row = (from - first - b.bytes) / b.stride + 1;
+    }
+    return row < b.rows && first + row * b.stride + b.bytes > from && first + row * b.stride < to;
+  }
 
   // ---- 4-bit weights (int4.hip) -----------------------------------------------------
   // A weight (out, in) as codes (out, in / 2) bytes, two a byte, the first in

@@ -845,16 +845,31 @@ namespace mi
     {
       throw InvalidArgument("window attention's rows and partials must be 16-byte aligned");
     }
-    if (t.out == t.q || t.out == t.k || t.out == t.v)
-    {
-      throw InvalidArgument("window attention cannot write over its queries, keys or values");
-    }
     const Cut c = cut_of(t, t.partials != nullptr);
     if (t.partials != nullptr && t.partials_floats < window_attention_floats(t))
     {
       throw InvalidArgument("window attention's partials need " +
                             std::to_string(window_attention_floats(t)) + " floats; got " +
                             std::to_string(t.partials_floats));
+    }
+    const auto rows_of = [](const void *at, long long width, int tokens, long long stride) {
+      return Extent{at, 2 * static_cast<std::size_t>(width), static_cast<std::size_t>(tokens),
+                    2 * static_cast<std::size_t>(stride)};
+    };
+    const Extent out{t.out, 2 * static_cast<std::size_t>(t.seq_q) * q_width};
+    const Extent parts{t.partials, t.partials != nullptr ? sizeof(float) * window_attention_floats(t) : 0};
+    for (const Extent &read : {rows_of(t.q, q_width, t.seq_q, q_stride),
+                               rows_of(t.k, width, t.seq_k, k_stride),
+                               rows_of(t.v, width, t.seq_k, v_stride)})
+    {
+      if (overlaps(out, read) || overlaps(parts, read))
+      {
+        throw InvalidArgument("window attention cannot write over its queries, keys or values");
+      }
+    }
+    if (overlaps(parts, out))
+    {
+      throw InvalidArgument("window attention's partials lie over its output");
     }
     WindowArgs a{};
     a.q = static_cast<const std::uint16_t *>(t.q);

@@ -1605,8 +1605,6 @@ def _device_linear_int4(x, codes, scales, zeros, group, bias, out, rows, in_feat
     xa = _at(x, rows * in_features, "x")
     ba = _at(bias, out_features, "bias") if bias is not None else None
     oa = _at(out, rows * out_features, "out")
-    if oa == xa:
-        raise ValueError("an int4 projection cannot write over its input")
     _check(lib.mi_linear_int4(xa, ca, sa, za, group, ba, oa, rows, in_features, out_features,
                               None))
 
