@@ -759,6 +759,12 @@ namespace mi
         throw InvalidArgument("window attention takes a whole number of query heads a KV head, got " +
                               std::to_string(t.heads) + " and " + std::to_string(t.kv_heads));
       }
+      // A head's offset in its token is 32 bits.
+      if (static_cast<long long>(t.heads) * t.head_dim > 0x7fffffff)
+      {
+        throw InvalidArgument("window attention takes fewer than 2^31 query elements a token, got " +
+                              std::to_string(t.heads) + " heads of " + std::to_string(t.head_dim));
+      }
     }
 
     template <int HD, typename F>
