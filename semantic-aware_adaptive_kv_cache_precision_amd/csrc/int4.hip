@@ -402,6 +402,16 @@ namespace mi
 
     constexpr int kChunk = 128; // inputs a wave takes at a time
 
+    // Between one wave's writes of LDS and its reads of them by other lanes, and
+    // between those reads and the next writes: the wave's operations complete in
+    // order, and this keeps the compiler to it. (No instruction.)
+    __device__ inline void wave_exchange()
+    {
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+
     // NT tiles of 16 rows, FT tiles of 16 outputs a wave; Groups: groups in a
     // chunk.
     // Shared: the waves' tiles of outputs are all different, and x goes through
@@ -551,6 +561,7 @@ namespace mi
       for (int chunk = begin; chunk < end; ++chunk)
       {
         const int of_four = (chunk - begin) & 3;
+        wave_exchange();
         // The codes, run p of 32 of output o at place p ^ o / 4 of its four.
 #pragma unroll
         for (int u = 0; u < FT; ++u)
@@ -571,6 +582,7 @@ namespace mi
         else
         {
           stage_x(stage, next_x);
+          wave_exchange();
         }
         if (chunk + 1 < end)
         {
@@ -649,6 +661,7 @@ namespace mi
       {
         static_assert(Shared || FT <= 4, "a wave's sums in its stage");
         f32x4 *parts = reinterpret_cast<f32x4 *>(stages);
+        wave_exchange();
         if (split > 0)
         {
 #pragma unroll
