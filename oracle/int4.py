@@ -43,3 +43,30 @@ def linear_bound(x, codes, scales, zeros, group: int) -> np.ndarray:
     z = np.repeat(np.abs(np.asarray(zeros, np.float64)), group, axis=1)
     size = np.abs(np.asarray(x, np.float64)) @ (codes * s + z).T
     return (codes.shape[1] + 4) * 2.0**-23 * size
+
+
+def linear_limit(x, codes, scales, zeros, group: int) -> np.ndarray:
+    """How far the fp32 sums may be from float64's, by the steps they are
+    formed in (linear_bound knows the terms alone, which at thousands of inputs
+    leaves room for a lost group):
+
+    - within a group: x . code and sum(x), of `group` exact terms each, added in
+      any order by an adder that may truncate: at most group 2^-23 of the terms'
+      magnitudes;
+    - over the groups: two fmas a run of 32 inputs (the finest the sums are
+      taken in) and the joins of lanes and waves (fewer than 32), each rounding
+      a sum of some runs by 2^-24. Such a sum is at most the runs' own
+      |s dot + z sum| and, between the two fmas, one run's |z sum| beside them.
+    """
+    x = np.asarray(x, np.float64)
+    rows, n = x.shape
+    s, z = (np.asarray(a, np.float64) for a in (scales, zeros))
+    sizes = np.abs(x) @ (codes * np.repeat(s, group, axis=1) + np.repeat(np.abs(z), group, axis=1)).T
+    # (runs, rows, out): each run's x . code and sum(x), with its group's scale and zero.
+    runs = n // 32
+    xr = x.reshape(rows, runs, 32).transpose(1, 0, 2)
+    dot = xr @ codes.reshape(len(codes), runs, 32).astype(np.float64).transpose(1, 2, 0)
+    of = np.arange(runs) * 32 // group
+    zsum = xr.sum(2)[:, :, None] * z.T[of][:, None]
+    reach = (np.abs(s.T[of][:, None] * dot + zsum) + np.abs(zsum)).sum(0)
+    return group * 2.0**-23 * sizes + (2 * runs + 32) * 2.0**-24 * reach
