@@ -204,10 +204,15 @@ int mi_attention_paged_causal_noalloc(const void *q, const unsigned long long *s
  * query heads a KV head; rows 16-byte aligned (strides multiples of 8). What is
  * written (out, partials) may share no byte with what is read, or is refused:
  * so too in the batch's and the 4-bit operators.
- * partials: mi_attention_window_partials floats (of these sizes: others, smaller
- * ones too, may ask for more), the caller's until the launch is done, which
- * let few rows' keys be split over the device; or NULL. Calls
- * that may overlap need partials of their own. */
+ * partials: mi_attention_window_partials floats of these sizes, the caller's
+ * until the launch is done, which let few rows' keys be split over the device;
+ * or NULL. Other sizes, smaller ones too, may ask for more, but none for more
+ * than 65,536 (head_dim + 2) floats: a buffer of those serves every call. Fewer
+ * than the call's are refused. Calls that may overlap need partials of their
+ * own. Weights are rounded to fp16 before they meet the values (half a step is
+ * 2^-11 of a weight; the sums that divide them are of the rounded ones, in
+ * fp32), where mi_attention keeps some 22 bits of them. Values that a query
+ * sees are expected finite: one that is not makes its channel so. */
 int mi_attention_window_partials(int seq_q, int seq_k, int heads, int kv_heads, int head_dim,
                                  int window, int sinks, size_t *floats);
 int mi_attention_window(const void *q, const void *k, const void *v, void *out, long long q_stride,

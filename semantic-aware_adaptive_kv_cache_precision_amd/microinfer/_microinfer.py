@@ -1367,7 +1367,8 @@ def _device_attention(q, k, v, k_bias, rope_table, out, seq_q, seq_k, heads, kv_
 @functools.lru_cache(maxsize=256, typed=True)
 def _attention_window_partials(seq_q: int, seq_k: int, heads: int, kv_heads: int, head_dim: int,
                                window: int = 0, sinks: int = 0) -> int:
-    """Floats of partials attention_window uses at these sizes."""
+    """Floats of partials attention_window uses at these sizes (at any: no more
+    than 65,536 * (head_dim + 2))."""
     out = C.c_size_t()
     _check(lib.mi_attention_window_partials(seq_q, seq_k, heads, kv_heads, head_dim, window, sinks,
                                             C.byref(out)))
@@ -1385,7 +1386,8 @@ def _device_attention_window(q, k, v, out, seq_q, seq_k, heads, kv_heads, head_d
     (p - window, p] and the first `sinks` (every key up to its own where
     `window` is 0). q holds the last seq_q of the seq_k positions of k and v;
     strides are elements between tokens (0: contiguous). `partials`
-    (attention_window_partials floats) lets few rows' keys be split."""
+    (attention_window_partials floats) lets few rows' keys be split. The
+    softmax's weights are rounded to fp16 before they meet the values."""
     for value, what in ((seq_q, "seq_q"), (q_stride, "q_stride"), (k_stride, "k_stride"),
                         (v_stride, "v_stride")):
         _non_negative(value, what)
