@@ -539,10 +539,11 @@ namespace mi
     constexpr int kHeadFloats = kWaves * kMaxGroup * 2;
 
     // One page's mass from the sum held against `held_from`, given the row's
-    // maximum and sum.
+    // maximum and sum. (A page that was not read is held against 0, which may
+    // lie further above the maximum than 2^x reaches: its zero stays one.)
     __device__ inline float mass_of(float sum, float held_from, float top, float inv)
     {
-      return sum * __builtin_amdgcn_exp2f(held_from - top) * inv;
+      return sum == 0.0f ? 0.0f : sum * __builtin_amdgcn_exp2f(held_from - top) * inv;
     }
 
     template <int HD, bool kHeld>
