@@ -22,17 +22,18 @@
 // run a sequence writes its outputs itself. A visible value that is not finite
 // makes the 32 channels of its step not finite in the heads that see it.
 //
-// Bound by a page's chain, some 500 vector and 40 matrix instructions of a
-// SIMD that are busy 40% of the time, with the page's own trip to memory
-// before it: 16 sequences to 32,768 tokens (12 x 2 heads of 128, mixed tiers)
-// 29.5 us of which the join is 5, 3.0 TB/s; 32 to 16,640 behind a 4,096-token
-// window (32 x 8 heads of 64) 27.5 us, 2.8 TB/s; 8 to 5,000 with masses 12.8;
-// one of 33 tokens 5.5 us, one launch. Four waves a workgroup: eight took 54
+// Bound by the latency of a page's one dependent chain, some 500 vector and 40
+// matrix instructions (a SIMD is busy 40% of the time), with the page's own
+// trip to memory before it: 16 sequences to 32,768 tokens (12 x 2 heads of 128,
+// mixed tiers) 30 us of which the join is 5, 2.9 TB/s; 32 to 16,640 behind a
+// 4,096-token window (32 x 8 heads of 64) 27.5 us, 2.8 TB/s; 8 to 5,000 with
+// masses 12.8; one of 33 tokens 5.4 us, one launch. Four waves a workgroup: eight took 54
 // and 38 us for the first two. Scalar page bases and 32-bit lane offsets, not
 // kept from page to page, leave four waves a SIMD at head_dim 64; two a SIMD,
 // evenly, are better than three at 128. The next page fetched ahead into LDS
-// costs waves at 64 (34 us) and saves nothing at 128, nor does memory: with
-// every page in the caches the first two take 33.8 of 36.6 and 27.5 of 28.3.
+// costs waves at 64 (34 us) and saves nothing at 128, nor would faster memory
+// save much: with every page in the caches the first two take 28.7 of 31.0 us
+// and 26.2 of 27.0, each pair from one run.
 
 #include "common.hpp"
 #include "dequant.hpp"

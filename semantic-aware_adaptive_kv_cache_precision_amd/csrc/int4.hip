@@ -13,7 +13,7 @@
 // takes 32 codes, 16 bytes, of one output; sixteen lanes take 256 bytes of a
 // row and a wave 4 R rows at a time, so that every line is asked for once and
 // whole; v_dot2 multiplies pairs into fp32. 128256 x 2048 in groups of 64, a
-// row: 31 us, 4.8 TB/s; 128 x 896: 4.7 us, a launch.
+// row: 30 us, 4.9 TB/s; 128 x 896: 5.0 us, a launch.
 //
 // More rows (int4_tiles_kernel): the matrix cores form x . codes (A: 16 rows of
 // x, B: 16 outputs' codes as fp16 integers, exact) and sum(x) (B: ones) of 32
@@ -26,7 +26,7 @@
 // their own, and requests are what a CU runs out of: loaded so, and the next
 // step's fetched past the last, 16 rows of 2048 x 8192 took 16.1 us, now 8.0.)
 // 27 rows of 8960 -> 1536: 8.3 us, what a CU takes in (its 16 rows of x whole,
-// 287 KB; two steps fetched ahead 9.6); 64 rows of
+// 287 KB, and 72 KB of codes; two steps fetched ahead 9.6); 64 rows of
 // 128256 x 2048: 79 us, a third of the matrix cores' rate, the vector units
 // making fp16 of codes beside them.
 //

@@ -32,13 +32,15 @@
 // With few rows the range of keys is split over workgroups, whose parts a
 // second launch joins.
 //
-// Bound by the vector units beside the matrix cores: a 32 x 32 tile's weights
-// at head_dim 64 take some 450 cycles of a SIMD (16 exponentials a lane at a
-// quarter of the rate are 256 of them), its products 256, and the two overlap
-// only across waves. 2,048 queries x 32 heads at 14,336 behind a 4,096-token
-// window with 4 sinks, head_dim 64: 102 us, 675 TFLOP/s. A prompt of 4,096 x
-// 12 heads of 128 behind 1,024: 57.5 us, 394 TFLOP/s, its 384 workgroups
-// leaving half the CUs one instead of two. 100 queries x 14 heads of 64:
+// Bound by vector and matrix work that take turns. 2,048 queries x 32 heads at
+// 14,336 behind a 4,096-token window with 4 sinks, head_dim 64: 103 us, 668
+// TFLOP/s; of the 253 M SIMD cycles in it vector instructions take some 166 M
+// (28.8 M of them, 4 cycles each, the exponentials, 16 a lane of a 32 x 32 tile,
+// at a quarter of that rate) and the products 69 M, together nearly all: the
+// waves of a SIMD pass the step's barrier together and do the same kind of work
+// at the same time. A prompt of 4,096 x 12 heads of 128 behind 1,024: 57.6 us,
+// 393 TFLOP/s, vector work 43 M and products 25 M of 141 M cycles, its 384
+// workgroups of unequal ranges leaving half the CUs one instead of two. 100 queries x 14 heads of 64:
 // 5.9 us, a launch and a chain of loads. Measured and not taken: 64 rows a
 // wave (158 us for the first of these, one wave a SIMD), the next step's first
 // product beside this step's exponentials (the same at head_dim 64; 90 us for
