@@ -446,8 +446,10 @@ int mi_kv_fold_kept(mi_kv_pages *kv, float *mass, long long mass_stride, float *
  * another page (one that a prompt's store completed, or an earlier one), but
  * for a page's first, is refused. A cache may be named twice. mass (count, heads, mass_pages). partials: for max_pages =
  * mass_pages, or without mass the longest sequence's pages. On the runtime's
- * current stream; the caches' pages must not move while a captured one is
- * replayed. */
+ * current stream. A captured one holds the positions and the caches' pages as
+ * they were: no page may move while it is replayed, and the caches' page
+ * tables must be on the device before (a call outside the capture, after
+ * pages were reserved or moved, puts them there; else it is refused). */
 int mi_attention_batch_partials(int batch, int max_pages, int heads, int kv_heads, int head_dim,
                                 int window, int sinks, int with_mass, size_t *floats);
 int mi_attention_batch(const void *q, const unsigned long long *pages, const uint8_t *tiers,

@@ -110,6 +110,18 @@ namespace mi
     }
     else if (!marked_.empty())
     {
+      // (A capture would keep the address of the edits, which go with this call.)
+      hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
+      if (stream != nullptr)
+      {
+        hip_check(hipStreamIsCapturing(stream, &capturing), "hipStreamIsCapturing");
+      }
+      if (capturing != hipStreamCaptureStatusNone)
+      {
+        throw LogicError("pages were reserved, moved or evicted since this cache's last call: run "
+                         "the calls once before they are captured, so that the page table is on "
+                         "the device");
+      }
       std::vector<TableEdit> edits;
       edits.reserve(marked_.size());
       for (const std::uint32_t at : marked_)
