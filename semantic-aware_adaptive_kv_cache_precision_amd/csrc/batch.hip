@@ -56,6 +56,8 @@ namespace mi
     typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
     typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
     typedef const __attribute__((address_space(1))) u32x4 *g_u32x4;
+    typedef u32x4 u32x4_anywhere __attribute__((aligned(2))); // a token's row: any view's
+    typedef const __attribute__((address_space(1))) u32x4_anywhere *g_u32x4_anywhere;
     typedef const __attribute__((address_space(1))) u32x2 *g_u32x2;
     typedef const __attribute__((address_space(1))) unsigned *g_u32;
     typedef const __attribute__((address_space(1))) unsigned short *g_u16;
@@ -394,8 +396,8 @@ namespace mi
 #pragma unroll
             for (int s = 0; s < S; ++s)
             {
-              k[b][s] = as_half8(*((g_u32x4)(own_k + chan + 8 * s)));
-              v[b][s] = as_half8(*((g_u32x4)(own_v + chan + 8 * s)));
+              k[b][s] = as_half8(*((g_u32x4_anywhere)(own_k + chan + 8 * s)));
+              v[b][s] = as_half8(*((g_u32x4_anywhere)(own_v + chan + 8 * s)));
             }
           }
         }

@@ -126,3 +126,25 @@ def test_a_page_s_first_token_needs_no_rows_before_it():
     q = fp16_exact(rng.standard_normal((3, 14, 64)))
     announce("first tokens")
     check([held] * 3, [1, 33, 193], q, 0, "a page's first token")
+
+
+@pytest.mark.parametrize("offset", [1, 4])
+def test_own_rows_on_any_alignment(offset):
+    """keys and values as views that begin between 16-byte lines."""
+    d = mi().device
+    rng = np.random.default_rng(offset)
+    heads, kv, hd = 12, 2, 128
+    held = [Stored(rng, kv, hd, e) for e in ((70,), (63, 64), (97,))]
+    lengths = [70, 64, 97]
+    q = fp16_exact(rng.standard_normal((3, heads, hd)))
+    rows = [np.stack([getattr(h, x)[0, n - 1] for h, n in zip(held, lengths)]).reshape(-1)
+            for x in "kv"]
+    buffers = [put(np.concatenate([np.full(offset, np.nan), r])) for r in rows]
+    out = d.empty(3 * heads * hd)
+    announce("own rows at", offset)
+    d.attention_caches([h.cache for h in held], lengths, 0, put(q), out, heads, kv, hd,
+                       *(d.view(b, offset, 3 * kv * hd) for b in buffers))
+    got = out.to_numpy().reshape(3, heads, hd)
+    for i, (h, n) in enumerate(zip(held, lengths)):
+        want, _, bound = h.want(q[i], 0, n)
+        assert_attention_close(got[i], want, f"offset {offset} {n}", bound)
