@@ -1394,10 +1394,10 @@ def _device_attention_window(q, k, v, out, seq_q, seq_k, heads, kv_heads, head_d
     if seq_q > seq_k:
         raise ValueError(f"seq_q {seq_q} exceeds seq_k {seq_k}")
     width, q_width = kv_heads * head_dim, heads * head_dim
-    qa = _at(q, _strided(seq_q, q_stride, q_width), "q")
-    ka = _at(k, _strided(seq_k, k_stride, width), "k")
-    va = _at(v, _strided(seq_k, v_stride, width), "v")
-    oa = _at(out, seq_q * q_width, "out")
+    qa = _fp16_at(q, _strided(seq_q, q_stride, q_width), "q")
+    ka = _fp16_at(k, _strided(seq_k, k_stride, width), "k")
+    va = _fp16_at(v, _strided(seq_k, v_stride, width), "v")
+    oa = _fp16_at(out, seq_q * q_width, "out")
     wa, floats = _scratch(partials)
     _check(lib.mi_attention_window(qa, ka, va, oa, q_stride, k_stride, v_stride, seq_q, seq_k, heads,
                                    kv_heads, head_dim, window, sinks, wa, floats, None))
@@ -1412,6 +1412,14 @@ def _attention_batch_partials(batch: int, max_pages: int, heads: int, kv_heads: 
     _check(lib.mi_attention_batch_partials(batch, max_pages, heads, kv_heads, head_dim, window,
                                            sinks, int(bool(mass)), C.byref(out)))
     return out.value
+
+
+def _fp16_at(x, count: int, what: str) -> int:
+    """As _at, by a tensor's bytes too."""
+    held = x.count if isinstance(x, Span) else min(x.numel, x.nbytes // 2)
+    if held < count:
+        raise ValueError(f"{what} holds {held}, and the operation needs {count}")
+    return x.address
 
 
 def _table(x, count: int, size: int, what: str) -> int:
@@ -1440,8 +1448,8 @@ def _batch_sizes(batch, max_pages, heads, head_dim, q, out, mass):
     _non_negative(batch, "batch")
     _non_negative(max_pages, "max_pages")
     per = batch * heads
-    qa = _at(q, per * head_dim, "q")
-    oa = _at(out, per * head_dim, "out")
+    qa = _fp16_at(q, per * head_dim, "q")
+    oa = _fp16_at(out, per * head_dim, "out")
     ma = _fp32_at(mass, per * max_pages, "mass") if mass is not None else None
     return qa, oa, ma
 
@@ -1488,8 +1496,8 @@ def _device_attention_caches(caches, seq_k, layer, q, out, heads, kv_heads, head
     elif mass_pages is None:
         mass_pages = max(-(-k // P_DEFAULT) for k in seq_k)
     qa, oa, ma = _batch_sizes(n, mass_pages, heads, head_dim, q, out, mass)
-    ka = _at(keys, n * width, "keys") if keys is not None else None
-    va = _at(values, n * width, "values") if values is not None else None
+    ka = _fp16_at(keys, n * width, "keys") if keys is not None else None
+    va = _fp16_at(values, n * width, "values") if values is not None else None
     wa, floats = _scratch(partials)
     _check(lib.mi_kv_attention_batch((_vp * n)(*(c._h for c in caches)), (C.c_int * n)(*seq_k), n,
                                      layer, qa, oa, heads, kv_heads, head_dim, ka, va, window, sinks,
@@ -1593,7 +1601,7 @@ def _device_quantise_int4(weight, codes, scales, zeros, group, in_features, out_
     `group` (32, 64 or 128) inputs of a row; the weight at input i stands for
     code * scale + zero."""
     ca, sa, za = _int4_at(codes, scales, zeros, group, in_features, out_features)
-    wa = _at(weight, out_features * in_features, "weight")
+    wa = _fp16_at(weight, out_features * in_features, "weight")
     _check(lib.mi_quantise_int4(wa, ca, sa, za, group, in_features, out_features, None))
 
 
@@ -1604,9 +1612,9 @@ def _device_linear_int4(x, codes, scales, zeros, group, bias, out, rows, in_feat
     rows of a batch of sequences' steps."""
     _non_negative(rows, "rows")
     ca, sa, za = _int4_at(codes, scales, zeros, group, in_features, out_features)
-    xa = _at(x, rows * in_features, "x")
-    ba = _at(bias, out_features, "bias") if bias is not None else None
-    oa = _at(out, rows * out_features, "out")
+    xa = _fp16_at(x, rows * in_features, "x")
+    ba = _fp16_at(bias, out_features, "bias") if bias is not None else None
+    oa = _fp16_at(out, rows * out_features, "out")
     _check(lib.mi_linear_int4(xa, ca, sa, za, group, ba, oa, rows, in_features, out_features,
                               None))
 
@@ -1616,7 +1624,7 @@ def _device_linear_int4_accumulate(x, codes, scales, zeros, group, out: FloatTen
     """linear_accumulate through an int4 weight: out += x @ W.T in fp32."""
     _non_negative(rows, "rows")
     ca, sa, za = _int4_at(codes, scales, zeros, group, in_features, out_features)
-    xa = _at(x, rows * in_features, "x")
+    xa = _fp16_at(x, rows * in_features, "x")
     oa = _fp32_at(out, rows * out_features, "out")
     _check(lib.mi_linear_int4_accumulate(xa, ca, sa, za, group, oa, rows, in_features,
                                          out_features, None))

@@ -50,3 +50,28 @@ def test_a_table_in_int32_words_holds_half_as_many_addresses():
     assert Words(12, 0).nbytes == 48
     with pytest.raises(ValueError, match="tiers holds 4 entries"):
         m.device.attention_batch(**batch.args(pages=Words(12, 0x10000), tiers=Words(1, 0x30000)))
+
+
+@pytest.mark.parametrize("change,word", [
+    (dict(q=On(768, item=1)), "q holds 384"), (dict(k=On(640, 0x20000, 1)), "k holds 320"),
+    (dict(v=On(640, 0x30000, 1)), "v holds 320"), (dict(out=On(768, 0x40000, 1)), "out holds 384"),
+])
+def test_attention_window_refuses_bytes_for_halves(change, word):
+    from microinfer import _microinfer as m
+    with pytest.raises(ValueError, match=word):
+        m.device.attention_window(**window.args(**change))
+
+
+def test_the_others_refuse_bytes_for_halves():
+    import test_int4_refusals as int4
+    from microinfer import _microinfer as m
+    for name, count in (("q", 512), ("out", 512)):
+        with pytest.raises(ValueError, match=f"{name} holds {count // 2}"):
+            m.device.attention_batch(**batch.args(**{name: On(count, 0x20000, 1)}))
+    for name, count in (("x", 256), ("bias", 8), ("out", 16)):
+        with pytest.raises(ValueError, match=f"{name} holds {count // 2}"):
+            m.device.linear_int4(**int4.args(**{name: On(count, 0x20000, 1)}))
+    q = dict(weight=On(8 * 128, item=1), codes=On(512, item=1), scales=On(8), zeros=On(8), group=128,
+             in_features=128, out_features=8)
+    with pytest.raises(ValueError, match="weight holds 512"):
+        m.device.quantise_int4(**q)
