@@ -219,6 +219,24 @@ int mi_attention_window(const void *q, const void *k, const void *v, void *out, 
                         long long k_stride, long long v_stride, int seq_q, int seq_k, int heads,
                         int kv_heads, int head_dim, int window, int sinks, float *partials,
                         size_t partials_floats, void *stream);
+/* Beyond the reference: the attention of several prompts in one run of rows,
+ * causal. q (rows_q, heads, head_dim), k and v (rows_k, kv_heads, head_dim)
+ * fp16, token strides as above. offsets_q, offsets_k (batch + 1) int32 on the
+ * device, not decreasing, read when the kernels run: sequence s has the queries
+ * [offsets_q[s], offsets_q[s + 1]), the last positions of its keys
+ * [offsets_k[s], offsets_k[s + 1]); offsets_k NULL: the same. A query sees its
+ * sequence's keys up to its own position; one with none (fewer keys than
+ * queries) gives zeros. Rows of no sequence are left as they were. head_dim 64
+ * or 128; alignment, overlaps, the rounding of weights and values that are not
+ * finite as mi_attention_window's, and so the partials, those of
+ * mi_attention_packed_partials, never more than 65,536 (head_dim + 2) floats. */
+int mi_attention_packed_partials(int batch, int rows_q, int rows_k, int heads, int kv_heads,
+                                 int head_dim, size_t *floats);
+int mi_attention_packed(const void *q, const void *k, const void *v, void *out, long long q_stride,
+                        long long k_stride, long long v_stride, const int *offsets_q,
+                        const int *offsets_k, int batch, int rows_q, int rows_k, int heads,
+                        int kv_heads, int head_dim, float *partials, size_t partials_floats,
+                        void *stream);
 
 /* ---- pages, rows and scores ----------------------------------------------
  * reference: page_copy.cu:41-70, kv_pages.cu:47-60, importance_scores.cu:18-50. */
@@ -278,6 +296,47 @@ int mi_linear_int4(const void *x, const void *codes, const void *scales, const v
 int mi_linear_int4_accumulate(const void *x, const void *codes, const void *scales,
                               const void *zeros, int group, float *out, int rows, int in_features,
                               int out_features, void *stream);
+/* Beyond the reference: rows and weights in codes of 8 bits, for the projections
+ * of many rows. mi_quantise_rows_int8: x (rows, features) fp16, `stride`
+ * elements apart (0: features), as codes (rows, features) of a signed byte and
+ * an fp32 scale a row: scale = max |x| / 127, code = x / scale, both rounded in
+ * fp32, then to the nearest whole number, halves to even; a row of zeros has
+ * scale 0, one with a value that is not finite a NaN for its scale and codes 0.
+ * A weight (out, in) is quantised by its rows too.
+ * mi_linear_int8: out (rows, out) fp16 = x (rows, in) W^T + bias (out fp16, or
+ * NULL): whole-number sums, times the two scales and rounded once to fp16.
+ * mi_linear_int8_accumulate: out (rows, out) fp32 = residual + x W^T, residual
+ * NULL or out itself: in place. features and in multiples of 16, in below
+ * 131072 (the sums stay in 32 bits); x, codes, weight 16-byte aligned, stride a
+ * multiple of 8. */
+int mi_quantise_rows_int8(const void *x, long long stride, void *codes, float *scales, int rows,
+                          int features, void *stream);
+int mi_linear_int8(const void *x, const float *x_scales, const void *weight, const float *w_scales,
+                   const void *bias, void *out, int rows, int in_features, int out_features,
+                   void *stream);
+int mi_linear_int8_accumulate(const void *x, const float *x_scales, const void *weight,
+                              const float *w_scales, const float *residual, float *out, int rows,
+                              int in_features, int out_features, void *stream);
+/* Beyond the reference (whose engine takes the greedy token, argmax.cu): a
+ * token of every row of logits (rows, vocab), `stride` elements apart (0:
+ * vocab), fp32 or fp16, from a given number uniforms[row] in [0, 1). Token i
+ * weighs exp((l_i - max) / temperature), formed in fp64. Kept are the top_k
+ * largest (0 or less: all); of those the fewest largest whose weights sum to
+ * top_p of theirs (1 or more: all; at least one); of those the ones that weigh
+ * at least min_p of the largest (0 or less: all). Of equal logits the lower
+ * index is the larger. The token is the first, by index, whose kept weights up
+ * to and with its own exceed the uniform's share of all kept. A weight below
+ * 2^-40 of the largest is as good as none: a token of such is never chosen.
+ * temperature 0 or less: the largest logit. temperature, top_k, top_p, min_p
+ * (rows each) are device arrays or NULL: 1, all, all, all. NaN and -inf logits
+ * weigh nothing; +inf share the weight among them. A row with neither (nothing
+ * above -inf) gives `vocab`, as mi_argmax_rows does. vocab at most 2^20.
+ * scratch: mi_sample_scratch floats (never more for fewer rows, or for a
+ * smaller vocab), the caller's until the launch is done, 16-byte aligned. */
+int mi_sample_scratch(int rows, int vocab, size_t *floats);
+int mi_sample(const void *logits, int logits_are_f32, long long stride, const float *uniforms,
+              const float *temperature, const int *top_k, const float *top_p, const float *min_p,
+              int *tokens, int rows, int vocab, void *scratch, size_t scratch_floats, void *stream);
 /* reference: embed.cu:60-76, bindings_device.cpp:321-334 (embed_f32) and
  * :383-396 (embed): out (count, hidden) = table rows ids[i], fp16 or widened
  * to fp32 (out_is_f32); an id outside [0, vocab) gives a zero row. */
@@ -357,6 +416,12 @@ int mi_scores_info(mi_scores *s, int *layers, int *max_pages, float *alpha, size
 /* ---- RopeTable ----------------------------------------------------------------
  * reference: rope_table.h:25-44, bindings_device.cpp:529-566. */
 int mi_rope_table_create(int head_dim, double theta, mi_rope_table **out);
+/* Beyond the reference: a table of the angles position * frequencies[j] for
+ * j < head_dim / 2 (host doubles), cos and sin times `magnitude`: angles scaled
+ * for contexts past a model's own, or of part of a head. Everywhere a table is
+ * taken, with its head_dim. */
+int mi_rope_table_create_scaled(int head_dim, const double *frequencies, double magnitude,
+                                mi_rope_table **out);
 void mi_rope_table_destroy(mi_rope_table *t);
 int mi_rope_table_cover(mi_rope_table *t, int positions);
 int mi_rope_table_info(mi_rope_table *t, int *positions, const float **data);
@@ -460,6 +525,41 @@ int mi_kv_attention_batch(mi_kv_pages *const *kv, const int *seq_k, int count, i
                           const void *q, void *out, int heads, int kv_heads, int head_dim,
                           const void *keys, const void *values, int window, int sinks, float *mass,
                           int mass_pages, float *partials, size_t partials_floats);
+/* Beyond the reference: the rows of several sequences' new tokens put into
+ * their caches, queries and keys turned to their positions on the way. q
+ * (rows, heads, head_dim), k and v (rows, kv_heads, head_dim) fp16, token
+ * strides in elements (0: contiguous), so that the three may lie in one
+ * projection's rows. offsets (batch + 1) int32: sequence s has the rows
+ * [offsets[s], offsets[s + 1]), or none; NULL: one each, rows == batch. A row
+ * is at position lengths[s] less the rows of s from it on: lengths count the
+ * new tokens, as mi_attention_batch takes them. pages, tiers, lengths, offsets
+ * are device arrays, read when the kernel runs. A row's key and value go to
+ * their place in its FP16 page (32 key rows, 32 value rows); where its page's
+ * tier is not 0, its address 0 or its position past max_pages pages, nowhere.
+ * q_out (rows, heads, head_dim), and k_out, v_out (rows, kv_heads, head_dim) or
+ * NULL, take the rows beside. Rows of no sequence are left as they were.
+ * rope turns the first rope head_dim channels of a query or key head (NULL:
+ * none), pairs (j, j + half), or (2j, 2j + 1) where interleaved, and must cover
+ * max_pages pages. head_dim even, strides in whole elements; 16-byte aligned
+ * rows of whole sixteens of channels are faster. What is written may share no
+ * byte with what is read, pages not checked.
+ * mi_kv_append_batch: the same for `count` different caches of one shape, the
+ * counts[i] rows of cache i at positions [starts[i], starts[i] + counts[i]) of
+ * `layer` (host memory, as mi_kv_store takes them, reserved before). Caches
+ * that seal need k_out and v_out, which their pages are then filled and sealed
+ * from in a launch for all of them. On the runtime's current stream; what is
+ * refused is refused before the first launch. */
+int mi_append_batch(const void *q, const void *k, const void *v, void *q_out, void *k_out,
+                    void *v_out, long long q_stride, long long k_stride, long long v_stride,
+                    const unsigned long long *pages, const uint8_t *tiers, const int *lengths,
+                    const int *offsets, int batch, int max_pages, int page_tokens, int rows,
+                    int heads, int kv_heads, int head_dim, mi_rope_table *rope, int interleaved,
+                    void *stream);
+int mi_kv_append_batch(mi_kv_pages *const *kv, const int *starts, const int *counts, int count,
+                       int layer, const void *q, const void *k, const void *v, void *q_out,
+                       void *k_out, void *v_out, long long q_stride, long long k_stride,
+                       long long v_stride, int heads, int kv_heads, int head_dim,
+                       mi_rope_table *rope, int interleaved);
 /* Beyond the reference: the store and the decode of a step whose position
  * lives in device memory, what mi_decode_step's graph launches, for callers
  * that capture graphs of their own (the reference's KVPages.store and

@@ -58,6 +58,10 @@ struct mi_rope_table
 {
   mi::RopeTable impl;
   mi_rope_table(int hd, double theta) : impl(hd, theta) {}
+  mi_rope_table(int hd, std::vector<double> frequencies, double magnitude)
+      : impl(hd, std::move(frequencies), magnitude)
+  {
+  }
 };
 
 namespace
@@ -245,6 +249,34 @@ namespace
     t.mass = mass;
     t.partials = partials;
     t.partials_floats = partials_floats;
+    return t;
+  }
+  mi::AppendRows append_of(const void *q, const void *k, const void *v, void *q_out, void *k_out,
+                           void *v_out, long long q_stride, long long k_stride, long long v_stride,
+                           int rows, int heads, int kv_heads, int head_dim, mi_rope_table *rope,
+                           int interleaved)
+  {
+    mi::AppendRows t{};
+    t.q = q;
+    t.k = k;
+    t.v = v;
+    t.q_out = q_out;
+    t.k_out = k_out;
+    t.v_out = v_out;
+    t.q_stride = q_stride;
+    t.k_stride = k_stride;
+    t.v_stride = v_stride;
+    t.rows = rows;
+    t.heads = heads;
+    t.kv_heads = kv_heads;
+    t.head_dim = head_dim;
+    if (rope != nullptr)
+    {
+      t.table = rope->impl.data();
+      t.table_positions = rope->impl.positions();
+      t.rotary = rope->impl.head_dim();
+    }
+    t.interleaved = interleaved != 0;
     return t;
   }
 } // namespace
@@ -897,6 +929,55 @@ int mi_linear_int4_accumulate(const void *x, const void *codes, const void *scal
   });
 }
 
+int mi_quantise_rows_int8(const void *x, long long stride, void *codes, float *scales, int rows,
+                          int features, void *stream)
+{
+  return guarded([&] {
+    mi::launch_quantise_rows_int8(x, stride, codes, scales, rows, features, as_stream(stream));
+  });
+}
+
+int mi_linear_int8(const void *x, const float *x_scales, const void *weight, const float *w_scales,
+                   const void *bias, void *out, int rows, int in_features, int out_features,
+                   void *stream)
+{
+  return guarded([&] {
+    const mi::Int8Linear t{x,       x_scales, weight,      w_scales,    bias, out,
+                           nullptr, rows,     in_features, out_features};
+    mi::launch_linear_int8(t, as_stream(stream));
+  });
+}
+
+int mi_linear_int8_accumulate(const void *x, const float *x_scales, const void *weight,
+                              const float *w_scales, const float *residual, float *out, int rows,
+                              int in_features, int out_features, void *stream)
+{
+  return guarded([&] {
+    const mi::Int8Linear t{x,    x_scales,    weight,      w_scales, nullptr, out,
+                           residual != nullptr ? residual : out, rows, in_features, out_features};
+    mi::launch_linear_int8(t, as_stream(stream));
+  });
+}
+
+int mi_sample_scratch(int rows, int vocab, size_t *floats)
+{
+  return guarded([&] {
+    need(floats, "floats");
+    *floats = mi::sample_scratch_floats(rows, vocab);
+  });
+}
+
+int mi_sample(const void *logits, int logits_are_f32, long long stride, const float *uniforms,
+              const float *temperature, const int *top_k, const float *top_p, const float *min_p,
+              int *tokens, int rows, int vocab, void *scratch, size_t scratch_floats, void *stream)
+{
+  return guarded([&] {
+    const mi::Sampling t{logits, logits_are_f32 == 0, stride, uniforms, temperature, top_k,  top_p,
+                         min_p,  tokens,              rows,   vocab,    scratch,     scratch_floats};
+    mi::launch_sample(t, as_stream(stream));
+  });
+}
+
 int mi_embed(const int32_t *ids, int count, const void *table, void *out, int out_is_f32,
              int hidden, int vocab, void *stream)
 {
@@ -1191,6 +1272,21 @@ int mi_rope_table_create(int head_dim, double theta, mi_rope_table **out)
   return guarded([&] { *out = new mi_rope_table(head_dim, theta); });
 }
 
+int mi_rope_table_create_scaled(int head_dim, const double *frequencies, double magnitude,
+                                mi_rope_table **out)
+{
+  return guarded([&] {
+    need(out, "out");
+    if (head_dim > 0)
+    {
+      need(frequencies, "frequencies");
+    }
+    const std::size_t pairs = head_dim > 0 ? static_cast<std::size_t>(head_dim) / 2 : 0;
+    *out = new mi_rope_table(head_dim, std::vector<double>(frequencies, frequencies + pairs),
+                             magnitude);
+  });
+}
+
 void mi_rope_table_destroy(mi_rope_table *t) { delete t; }
 
 int mi_rope_table_cover(mi_rope_table *t, int positions)
@@ -1399,6 +1495,144 @@ int mi_kv_attention_batch(mi_kv_pages *const *kv, const int *seq_k, int count, i
                  head_dim, window, sinks, mass, partials, partials_floats);
     t.held = held.data();
     mi::launch_batch_attention(t, mi::runtime_stream());
+  });
+}
+
+int mi_append_batch(const void *q, const void *k, const void *v, void *q_out, void *k_out,
+                    void *v_out, long long q_stride, long long k_stride, long long v_stride,
+                    const unsigned long long *pages, const uint8_t *tiers, const int *lengths,
+                    const int *offsets, int batch, int max_pages, int page_tokens, int rows,
+                    int heads, int kv_heads, int head_dim, mi_rope_table *rope, int interleaved,
+                    void *stream)
+{
+  return guarded([&] {
+    if (page_tokens != mi::kBatchPageTokens)
+    {
+      throw mi::InvalidArgument("a batch's pages hold " + std::to_string(mi::kBatchPageTokens) +
+                                " tokens, got " + std::to_string(page_tokens));
+    }
+    mi::AppendRows t = append_of(q, k, v, q_out, k_out, v_out, q_stride, k_stride, v_stride, rows,
+                                 heads, kv_heads, head_dim, rope, interleaved);
+    t.pages = pages;
+    t.tiers = tiers;
+    t.lengths = lengths;
+    t.offsets = offsets;
+    t.batch = batch;
+    t.max_pages = max_pages;
+    t.page_tokens = page_tokens;
+    mi::launch_append(t, as_stream(stream));
+  });
+}
+
+int mi_kv_append_batch(mi_kv_pages *const *kv, const int *starts, const int *counts, int count,
+                       int layer, const void *q, const void *k, const void *v, void *q_out,
+                       void *k_out, void *v_out, long long q_stride, long long k_stride,
+                       long long v_stride, int heads, int kv_heads, int head_dim,
+                       mi_rope_table *rope, int interleaved)
+{
+  return guarded([&] {
+    if (count < 0)
+    {
+      throw mi::InvalidArgument("a batch of " + std::to_string(count) + " sequences");
+    }
+    if (count == 0)
+    {
+      return;
+    }
+    need(kv, "the caches");
+    need(starts, "starts");
+    need(counts, "counts");
+    // Everything that is refused is refused before the first launch.
+    std::vector<mi::AppendSequence> held(static_cast<std::size_t>(count));
+    std::vector<const mi_kv_pages *> seen;
+    long long rows = 0;
+    int end = 0;
+    bool seals = false;
+    for (int i = 0; i < count; ++i)
+    {
+      need(kv[i], "a cache");
+      held[i] = kv[i]->impl.append_sequence(layer, starts[i], counts[i], kv_heads, head_dim);
+      if (kv[i]->impl.page_tokens() != kv[0]->impl.page_tokens())
+      {
+        throw mi::InvalidArgument("the batch's caches have pages of one size");
+      }
+      seals = seals || (kv[i]->impl.seals() && counts[i] > 0);
+      rows += counts[i];
+      end = std::max(end, starts[i] + counts[i]);
+      seen.push_back(kv[i]);
+    }
+    std::sort(seen.begin(), seen.end());
+    if (std::adjacent_find(seen.begin(), seen.end()) != seen.end())
+    {
+      throw mi::InvalidArgument("a batch's append takes a cache once");
+    }
+    if (rows > 0x7fffffff)
+    {
+      throw mi::InvalidArgument("a batch's append takes fewer than 2^31 rows, got " +
+                                std::to_string(rows));
+    }
+    if (seals && (k_out == nullptr || v_out == nullptr))
+    {
+      throw mi::InvalidArgument("a cache that seals takes its rows from k_out and v_out; pass them");
+    }
+    mi::AppendRows t = append_of(q, k, v, q_out, k_out, v_out, q_stride, k_stride, v_stride,
+                                 static_cast<int>(rows), heads, kv_heads, head_dim, rope,
+                                 interleaved);
+    if (t.rotary > 0 && t.table_positions < end)
+    {
+      throw mi::InvalidArgument("the RoPE table covers " + std::to_string(t.table_positions) +
+                                " positions; the batch's rows end at " + std::to_string(end));
+    }
+    t.held = held.data();
+    t.batch = count;
+    t.page_tokens = kv[0]->impl.page_tokens();
+    const hipStream_t stream = mi::runtime_stream();
+    mi::launch_append(t, stream);
+    std::vector<mi::RowJob> jobs;
+    const std::size_t width = static_cast<std::size_t>(kv_heads) * head_dim;
+    std::size_t row = 0;
+    for (int i = 0; i < count; ++i)
+    {
+      kv[i]->impl.append_sealed(layer, static_cast<const std::uint16_t *>(k_out) + row * width,
+                                static_cast<const std::uint16_t *>(v_out) + row * width, starts[i],
+                                counts[i], jobs);
+      row += counts[i];
+    }
+    if (!jobs.empty())
+    {
+      mi::launch_row_jobs(jobs.data(), static_cast<int>(jobs.size()), t.page_tokens, kv_heads,
+                          head_dim, stream);
+    }
+  });
+}
+
+int mi_attention_packed_partials(int batch, int rows_q, int rows_k, int heads, int kv_heads,
+                                 int head_dim, size_t *floats)
+{
+  return guarded([&] {
+    need(floats, "floats");
+    mi::PackedAttention t{};
+    t.batch = batch;
+    t.rows_q = rows_q;
+    t.rows_k = rows_k;
+    t.heads = heads;
+    t.kv_heads = kv_heads;
+    t.head_dim = head_dim;
+    *floats = mi::packed_attention_floats(t);
+  });
+}
+
+int mi_attention_packed(const void *q, const void *k, const void *v, void *out, long long q_stride,
+                        long long k_stride, long long v_stride, const int *offsets_q,
+                        const int *offsets_k, int batch, int rows_q, int rows_k, int heads,
+                        int kv_heads, int head_dim, float *partials, size_t partials_floats,
+                        void *stream)
+{
+  return guarded([&] {
+    const mi::PackedAttention t{q,         k,        v,     out,    q_stride, k_stride, v_stride, offsets_q,
+                                offsets_k, batch,    rows_q, rows_k, heads,    kv_heads, head_dim, partials,
+                                partials_floats};
+    mi::launch_packed_attention(t, as_stream(stream));
   });
 }
 

@@ -470,7 +470,7 @@ namespace mi
   }
 
   void KVPages::store_sealed(int layer, const std::uint16_t *keys, const std::uint16_t *values,
-                             int start, int n)
+                             int start, int n, std::vector<RowJob> *together)
   {
     const std::size_t W = kv_width_;
     const std::size_t half = static_cast<std::size_t>(page_tokens_) * W;
@@ -578,10 +578,58 @@ namespace mi
       launch_row_run(run_keys, run_values, run.data(), static_cast<int>(run.size()), kv_heads_,
                      head_dim_, runtime_stream());
     }
-    if (!jobs.empty())
+    if (together != nullptr)
+    {
+      together->insert(together->end(), jobs.begin(), jobs.end());
+    }
+    else if (!jobs.empty())
     {
       launch_row_jobs(jobs.data(), static_cast<int>(jobs.size()), page_tokens_, kv_heads_,
                       head_dim_, runtime_stream());
+    }
+  }
+
+  AppendSequence KVPages::append_sequence(int layer, int start, int n, int kv_heads, int head_dim)
+  {
+    require_layer(layer);
+    if (kv_heads != kv_heads_ || head_dim != head_dim_)
+    {
+      throw InvalidArgument("the batch's sequences have " + std::to_string(kv_heads) +
+                            " KV heads of " + std::to_string(head_dim) + "; this cache holds " +
+                            std::to_string(kv_heads_) + " of " + std::to_string(head_dim_));
+    }
+    if (start < 0 || n < 0 || start > capacity_tokens() || n > capacity_tokens() - start)
+    {
+      throw OutOfRange("positions [" + std::to_string(start) + ", " +
+                       std::to_string(static_cast<long long>(start) + n) +
+                       ") are not all on pages; " + std::to_string(capacity_tokens()) +
+                       " positions are reserved");
+    }
+    AppendSequence s{nullptr, 0, n, start};
+    if (n == 0)
+    {
+      return s;
+    }
+    if (seals_)
+    {
+      for (int page = start / page_tokens_; page < (start + n) / page_tokens_; ++page)
+      {
+        allocator_.locate({layer, page}); // a page that these rows complete is held
+      }
+      return s;
+    }
+    sync_tables(runtime_stream());
+    s.pages = table_.addresses() + static_cast<std::size_t>(layer) * table_.stride();
+    s.page_count = pages_;
+    return s;
+  }
+
+  void KVPages::append_sealed(int layer, const std::uint16_t *keys, const std::uint16_t *values,
+                              int start, int n, std::vector<RowJob> &jobs)
+  {
+    if (seals_ && n > 0)
+    {
+      store_sealed(layer, keys, values, start, n, &jobs);
     }
   }
 

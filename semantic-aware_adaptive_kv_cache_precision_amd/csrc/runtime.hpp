@@ -14,6 +14,7 @@
 
 #include "common.hpp"
 #include "kernels.hpp"
+#include "ragged.hpp"
 #include "serving.hpp"
 
 #include <array>
@@ -444,6 +445,9 @@ namespace mi
   {
   public:
     RopeTable(int head_dim, double theta);
+    // The angles position * frequencies[pair] (head_dim / 2 of them), cos and
+    // sin times `magnitude`: scaled for contexts past a model's own.
+    RopeTable(int head_dim, std::vector<double> frequencies, double magnitude);
     void cover(int count);
     const float *data() const { return table_ ? table_->as<const float>() : nullptr; }
     // The angles of the first kAngleRows positions (a decode page's rows)
@@ -463,6 +467,8 @@ namespace mi
   private:
     int head_dim_;
     double theta_;
+    std::vector<double> frequencies_; // empty: theta's
+    double magnitude_ = 1.0;
     int positions_ = 0;
     std::unique_ptr<DeviceBuffer> table_;
     std::unique_ptr<DeviceBuffer> angles_;
@@ -596,6 +602,14 @@ namespace mi
     // it does not hold as they were stored. Good until the cache's next call.
     BatchSequence batch_sequence(int layer, int seq_k, int kv_heads, int head_dim,
                                  const std::uint16_t *key, const std::uint16_t *value);
+    // Beyond the reference: this cache as one sequence of a batch's append
+    // (launch_append), n rows from position `start` on, refused here or not at
+    // all. A cache that seals then takes them by append_sealed, from rows as
+    // they were appended (kv_width each): as store does, but the launches that
+    // fill and seal single pages are left to the caller, as jobs.
+    AppendSequence append_sequence(int layer, int start, int n, int kv_heads, int head_dim);
+    void append_sealed(int layer, const std::uint16_t *keys, const std::uint16_t *values, int start,
+                       int n, std::vector<RowJob> &jobs);
     // Beyond the reference: the pieces of a decode step whose position lives
     // on the device, so that one captured graph serves every step of a run.
     // store_step stores one row at *position (sealing the page it
@@ -699,8 +713,9 @@ namespace mi
     void refresh_entry(int layer, int page);
     void sync_tables(hipStream_t stream);
 
+    // The jobs of the store's single pages go to `together`, where given.
     void store_sealed(int layer, const std::uint16_t *keys, const std::uint16_t *values, int start,
-                      int n);
+                      int n, std::vector<RowJob> *together = nullptr);
     PageKey require_movable(int layer, int page, const char *verb) const;
     PageKey require_held(int layer, int page, const char *verb) const;
     // The tier moves of a batch: validated already, every page held.

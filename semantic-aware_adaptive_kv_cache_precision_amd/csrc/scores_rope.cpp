@@ -87,6 +87,31 @@ namespace mi
     }
   }
 
+  RopeTable::RopeTable(int head_dim, std::vector<double> frequencies, double magnitude)
+      : head_dim_(head_dim), theta_(0.0), frequencies_(std::move(frequencies)), magnitude_(magnitude)
+  {
+    if (head_dim <= 0 || head_dim % 2 != 0)
+    {
+      throw InvalidArgument("head_dim must be positive and even, got " + std::to_string(head_dim));
+    }
+    if (frequencies_.size() != static_cast<std::size_t>(head_dim) / 2)
+    {
+      throw InvalidArgument(std::to_string(frequencies_.size()) + " frequencies for " +
+                            std::to_string(head_dim / 2) + " pairs");
+    }
+    for (const double f : frequencies_)
+    {
+      if (!std::isfinite(f))
+      {
+        throw InvalidArgument("frequencies must be finite, got " + std::to_string(f));
+      }
+    }
+    if (!(magnitude > 0.0) || !std::isfinite(magnitude))
+    {
+      throw InvalidArgument("magnitude must be positive, got " + std::to_string(magnitude));
+    }
+  }
+
   void RopeTable::cover(int count)
   {
     if (count <= positions_)
@@ -96,7 +121,20 @@ namespace mi
     const int grown = std::max({count, 2 * positions_, kAngleRows});
     auto table = std::make_unique<DeviceBuffer>(static_cast<std::size_t>(grown) * head_dim_ *
                                                 sizeof(float));
-    launch_rope_table(table->as<float>(), grown, head_dim_, theta_, runtime_stream());
+    if (frequencies_.empty())
+    {
+      launch_rope_table(table->as<float>(), grown, head_dim_, theta_, runtime_stream());
+    }
+    else
+    {
+      const std::size_t bytes = frequencies_.size() * sizeof(double);
+      const DeviceBuffer held(bytes); // freed below, after the launch that reads it
+      hip_check(hipMemcpy(held.raw(), frequencies_.data(), bytes, hipMemcpyHostToDevice),
+                "hipMemcpy frequencies host-to-device");
+      launch_rope_frequencies(table->as<float>(), grown, held.as<const double>(), head_dim_ / 2,
+                              magnitude_, runtime_stream());
+      hip_check(hipStreamSynchronize(runtime_stream()), "hipStreamSynchronize frequencies");
+    }
     auto angles = std::make_unique<DeviceBuffer>(static_cast<std::size_t>(kAngleRows) * head_dim_ *
                                                  2 * sizeof(std::uint16_t));
     launch_rope_angles(table->as<const float>(), angles->as<std::uint16_t>(), kAngleRows,

@@ -84,6 +84,13 @@ SIGNATURES = {
                             _vp), C.c_int),
     "mi_kv_attention_batch": ((C.POINTER(_vp), _ip, _i, _i, _vp, _vp, _i, _i, _i, _vp, _vp, _i, _i,
                                _vp, _i, _vp, _sz), C.c_int),
+    "mi_append_batch": ((_vp, _vp, _vp, _vp, _vp, _vp, _ll, _ll, _ll, _vp, _vp, _vp, _vp, _i, _i, _i,
+                         _i, _i, _i, _i, _vp, _i, _vp), C.c_int),
+    "mi_kv_append_batch": ((C.POINTER(_vp), _ip, _ip, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _ll, _ll,
+                            _ll, _i, _i, _i, _vp, _i), C.c_int),
+    "mi_attention_packed_partials": ((_i, _i, _i, _i, _i, _i, _szp), C.c_int),
+    "mi_attention_packed": ((_vp, _vp, _vp, _vp, _ll, _ll, _ll, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp,
+                             _sz, _vp), C.c_int),
     "mi_kv_store_at": ((_vp, _i, _vp, _vp, _vp), C.c_int),
     "mi_kv_attention_at": ((_vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp), C.c_int),
     "mi_kv_stored_on_device": ((_vp, _i), C.c_int),
@@ -144,6 +151,11 @@ SIGNATURES = {
     "mi_quantise_int4": ((_vp, _vp, _vp, _vp, _i, _i, _i, _vp), C.c_int),
     "mi_linear_int4": ((_vp, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _vp), C.c_int),
     "mi_linear_int4_accumulate": ((_vp, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _vp), C.c_int),
+    "mi_quantise_rows_int8": ((_vp, _ll, _vp, _vp, _i, _i, _vp), C.c_int),
+    "mi_linear_int8": ((_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp), C.c_int),
+    "mi_linear_int8_accumulate": ((_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp), C.c_int),
+    "mi_sample_scratch": ((_i, _i, _szp), C.c_int),
+    "mi_sample": ((_vp, _i, _ll, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _sz, _vp), C.c_int),
     "mi_linear_f32": ((_vp, _vp, _vp, _i, _i, _i, _i, _vp), C.c_int),
     "mi_embed": ((_vp, _i, _vp, _vp, _i, _i, _i, _vp), C.c_int),
     "mi_argmax_rows": ((_vp, _i, _i, _vp, _vp), C.c_int),
@@ -185,6 +197,7 @@ SIGNATURES = {
     "mi_scores_layer_row": ((_vp, _i, C.POINTER(_vp)), C.c_int),
     "mi_scores_info": ((_vp, _ip, _ip, _fp, _szp), C.c_int),
     "mi_rope_table_create": ((_i, _d, C.POINTER(_vp)), C.c_int),
+    "mi_rope_table_create_scaled": ((_i, C.POINTER(_d), _d, C.POINTER(_vp)), C.c_int),
     "mi_rope_table_destroy": ((_vp,), None),
     "mi_rope_table_cover": ((_vp, _i), C.c_int),
     "mi_rope_table_info": ((_vp, _ip, C.POINTER(_vp)), C.c_int),
@@ -744,13 +757,75 @@ def _floats(t: FloatTensor | None, count: int, what: str):
     return t.address
 
 
+def rope_frequencies(head_dim: int, theta: float, scaling: dict | None = None):
+    """Beyond the reference: what a position turns each of head_dim / 2 pairs by,
+    float64, and the factor of cos and sin, for contexts scaled past a model's
+    own. `scaling`, as models' configurations give it:
+
+      kind "linear", factor: every frequency divided by factor;
+      kind "llama3", factor, low, high, original: pairs that turn fewer than
+        `low` times over `original` positions divided by factor, those that turn
+        more than `high` times as they are, between them by share;
+      kind "yarn", factor, original, fast (32), slow (1): the pairs between the
+        one that turns `fast` times over `original` positions and the one that
+        turns `slow` times by share, those below as they are, those above
+        divided; cos and sin times `magnitude` (0.1 ln factor + 1)."""
+    if head_dim <= 0 or head_dim % 2:
+        raise ValueError(f"head_dim must be positive and even, got {head_dim}")
+    if not theta > 0.0:
+        raise ValueError(f"theta must be positive, got {theta}")
+    f = float(theta) ** (-2.0 * np.arange(head_dim // 2) / head_dim)
+    if scaling is None:
+        return f, 1.0
+    known = {"linear": {"factor"}, "llama3": {"factor", "low", "high", "original"},
+             "yarn": {"factor", "original"}}
+    kind = scaling.get("kind")
+    if kind not in known:
+        raise ValueError(f"a rope scaling's kind is one of {sorted(known)}, got {kind!r}")
+    given = set(scaling) - {"kind"}
+    extra = {"fast", "slow", "magnitude"} if kind == "yarn" else set()
+    if not known[kind] <= given or given - known[kind] - extra:
+        raise ValueError(f"a {kind} scaling has {sorted(known[kind] | extra)}, got {sorted(given)}")
+    factor = float(scaling["factor"])
+    if not (factor >= 1.0 and np.isfinite(factor)):
+        raise ValueError(f"a rope scaling's factor is at least 1, got {factor}")
+    if kind == "linear":
+        return f / factor, 1.0
+    original = float(scaling["original"])
+    if not original > 0.0:
+        raise ValueError(f"a rope scaling's original context is positive, got {original}")
+    if kind == "llama3":
+        low, high = float(scaling["low"]), float(scaling["high"])
+        if not 0.0 < low < high:
+            raise ValueError(f"a llama3 scaling has 0 < low < high, got {low} and {high}")
+        whole = np.clip((original * f / (2 * np.pi) - low) / (high - low), 0.0, 1.0)
+        return f * (whole + (1.0 - whole) / factor), 1.0
+    fast, slow = float(scaling.get("fast", 32.0)), float(scaling.get("slow", 1.0))
+    if not (0.0 < slow <= fast and theta > 1.0):
+        raise ValueError(f"a yarn scaling has 0 < slow <= fast and theta > 1, got {slow}, {fast} "
+                         f"and {theta}")
+
+    def pair(turns):
+        return head_dim * np.log(original / (turns * 2 * np.pi)) / (2 * np.log(theta))
+
+    first, last = max(np.floor(pair(fast)), 0.0), min(np.ceil(pair(slow)), head_dim - 1.0)
+    part = np.clip((np.arange(head_dim // 2) - first) / max(last - first, 0.001), 0.0, 1.0)
+    magnitude = float(scaling.get("magnitude", 0.1 * np.log(factor) + 1.0))
+    return f * ((1.0 - part) + part / factor), magnitude
+
+
 class RopeTable:
     """cos and sin of every RoPE angle per position, fp32 on the device
-    (rope_table.h:25-44)."""
+    (rope_table.h:25-44). `scaling`, beyond the reference: rope_frequencies'."""
 
-    def __init__(self, head_dim: int, theta: float):
+    def __init__(self, head_dim: int, theta: float, scaling: dict | None = None):
         h = _vp()
-        _check(lib.mi_rope_table_create(head_dim, theta, C.byref(h)))
+        if scaling is None:
+            _check(lib.mi_rope_table_create(head_dim, theta, C.byref(h)))
+        else:
+            f, magnitude = rope_frequencies(head_dim, theta, scaling)
+            _check(lib.mi_rope_table_create_scaled(head_dim, (_d * len(f))(*f), magnitude,
+                                                   C.byref(h)))
         self._h = h.value
         self.head_dim, self.theta = head_dim, theta
         weakref.finalize(self, lib.mi_rope_table_destroy, self._h)
@@ -1504,6 +1579,105 @@ def _device_attention_caches(caches, seq_k, layer, q, out, heads, kv_heads, head
                                      ma, mass_pages, wa, floats))
 
 
+def _append_rows(q, k, v, q_out, k_out, v_out, rows, heads, kv_heads, head_dim, q_stride, k_stride,
+                 v_stride):
+    """The addresses of appended rows and of what they go to."""
+    for value, what in ((rows, "rows"), (heads, "heads"), (kv_heads, "kv_heads"),
+                        (head_dim, "head_dim"), (q_stride, "q_stride"), (k_stride, "k_stride"),
+                        (v_stride, "v_stride")):
+        _non_negative(value, what)
+    width, q_width = kv_heads * head_dim, heads * head_dim
+    return (_fp16_at(q, _strided(rows, q_stride, q_width), "q"),
+            _fp16_at(k, _strided(rows, k_stride, width), "k"),
+            _fp16_at(v, _strided(rows, v_stride, width), "v"),
+            _fp16_at(q_out, rows * q_width, "q_out"),
+            _fp16_at(k_out, rows * width, "k_out") if k_out is not None else None,
+            _fp16_at(v_out, rows * width, "v_out") if v_out is not None else None)
+
+
+def _device_append_batch(q, k, v, q_out, k_out, pages, tiers, lengths, offsets, batch, max_pages,
+                         rows, rope, heads, kv_heads, head_dim, interleaved=False, v_out=None,
+                         q_stride=0, k_stride=0, v_stride=0):
+    """Beyond the reference: the rows of several sequences' new tokens, queries
+    and keys turned to their positions, keys and values written into their FP16
+    pages. Sequence s has the rows [offsets[s], offsets[s + 1]) of q (rows,
+    heads, head_dim), k and v (rows, kv_heads, head_dim), the last of its
+    lengths[s] tokens (`offsets` None: a row each); pages, tiers (batch,
+    max_pages) and lengths as attention_batch takes them, all read when the
+    kernel runs. `rope` (a RopeTable that covers max_pages pages, of the
+    channels that turn, or None) pairs channels (j, j + half), or (2j, 2j + 1)
+    where `interleaved`. q_out, and k_out and v_out where not None, take the
+    rows (contiguous) for attention over them."""
+    _non_negative(batch, "batch")
+    _non_negative(max_pages, "max_pages")
+    rows_at = _append_rows(q, k, v, q_out, k_out, v_out, rows, heads, kv_heads, head_dim, q_stride,
+                           k_stride, v_stride)
+    pa = _table(pages, batch * max_pages, 8, "pages")
+    ta = _table(tiers, batch * max_pages, 1, "tiers")
+    la = _table(lengths, batch, 4, "lengths")
+    fa = _table(offsets, batch + 1, 4, "offsets") if offsets is not None else None
+    _check(lib.mi_append_batch(*rows_at, q_stride, k_stride, v_stride, pa, ta, la, fa, batch,
+                               max_pages, P_DEFAULT, rows, heads, kv_heads, head_dim,
+                               rope._h if rope is not None else None, int(bool(interleaved)), None))
+
+
+def _device_append_caches(caches, starts, counts, layer, q, k, v, q_out, k_out, v_out, rope, heads,
+                          kv_heads, head_dim, interleaved=False, q_stride=0, k_stride=0, v_stride=0):
+    """append_batch over KVPages: the counts[i] rows of caches[i] go to positions
+    [starts[i], starts[i] + counts[i]) of `layer`, reserved before, in place of
+    a rotation and a store each. No cache twice. Caches that seal need k_out and
+    v_out (of every row), which attention_caches then reads too."""
+    n = len(caches)
+    if len(starts) != n or len(counts) != n:
+        raise ValueError(f"{n} caches, {len(starts)} starts and {len(counts)} counts")
+    if n == 0:
+        return
+    for c in counts:
+        _non_negative(c, "a cache's rows")
+    rows_at = _append_rows(q, k, v, q_out, k_out, v_out, sum(counts), heads, kv_heads, head_dim,
+                           q_stride, k_stride, v_stride)
+    _check(lib.mi_kv_append_batch((_vp * n)(*(c._h for c in caches)), (C.c_int * n)(*starts),
+                                  (C.c_int * n)(*counts), n, layer, *rows_at, q_stride, k_stride,
+                                  v_stride, heads, kv_heads, head_dim,
+                                  rope._h if rope is not None else None, int(bool(interleaved))))
+
+
+@functools.lru_cache(maxsize=256, typed=True)
+def _attention_packed_partials(batch: int, rows_q: int, rows_k: int, heads: int, kv_heads: int,
+                               head_dim: int) -> int:
+    """Floats of partials attention_packed uses at these sizes (at any: no more
+    than 65,536 * (head_dim + 2))."""
+    out = C.c_size_t()
+    _check(lib.mi_attention_packed_partials(batch, rows_q, rows_k, heads, kv_heads, head_dim,
+                                            C.byref(out)))
+    return out.value
+
+
+def _device_attention_packed(q, k, v, out, offsets_q, offsets_k, batch, rows_q, rows_k, heads,
+                             kv_heads, head_dim, q_stride=0, k_stride=0, v_stride=0, partials=None):
+    """Beyond the reference: causal attention of several prompts in one run of
+    rows. Sequence s has the queries [offsets_q[s], offsets_q[s + 1]) of q, the
+    last positions of its keys [offsets_k[s], offsets_k[s + 1]) of k and v
+    (offsets_k None: the same); offsets are device arrays of batch + 1 int32,
+    read when the kernels run. Strides are elements between tokens (0:
+    contiguous). `partials` (attention_packed_partials floats) lets few rows'
+    keys be split. The softmax's weights are rounded to fp16 before they meet
+    the values. Rows of no sequence are left as they were."""
+    for value, what in ((batch, "batch"), (rows_q, "rows_q"), (rows_k, "rows_k"),
+                        (q_stride, "q_stride"), (k_stride, "k_stride"), (v_stride, "v_stride")):
+        _non_negative(value, what)
+    width, q_width = kv_heads * head_dim, heads * head_dim
+    qa = _fp16_at(q, _strided(rows_q, q_stride, q_width), "q")
+    ka = _fp16_at(k, _strided(rows_k, k_stride, width), "k")
+    va = _fp16_at(v, _strided(rows_k, v_stride, width), "v")
+    oa = _fp16_at(out, rows_q * q_width, "out")
+    fa = _table(offsets_q, batch + 1, 4, "offsets_q")
+    ga = _table(offsets_k, batch + 1, 4, "offsets_k") if offsets_k is not None else None
+    wa, floats = _scratch(partials)
+    _check(lib.mi_attention_packed(qa, ka, va, oa, q_stride, k_stride, v_stride, fa, ga, batch, rows_q,
+                                   rows_k, heads, kv_heads, head_dim, wa, floats, None))
+
+
 def _device_rmsnorm(x, weight, out, rows, hidden, eps):
     xa = _at(x, rows * hidden, "x")
     wa = _at(weight, hidden, "weight")
@@ -1628,6 +1802,98 @@ def _device_linear_int4_accumulate(x, codes, scales, zeros, group, out: FloatTen
     oa = _fp32_at(out, rows * out_features, "out")
     _check(lib.mi_linear_int4_accumulate(xa, ca, sa, za, group, oa, rows, in_features,
                                          out_features, None))
+
+
+def _int8_features(features, what):
+    if features < 0 or features % 16:
+        raise ValueError(f"{what} {features} must not be negative, and whole sixteens")
+
+
+def _device_quantise_rows_int8(x, codes, scales, rows, features, stride=0):
+    """Beyond the reference: fp16 rows as signed bytes with an fp32 scale each:
+    scale = max |x| / 127, code = x / scale rounded half to even. The rows of a
+    step before its projections; a weight (out, in) once, by its rows. `stride`
+    is elements between rows (0: features)."""
+    _non_negative(rows, "rows")
+    _non_negative(stride, "stride")
+    _int8_features(features, "features")
+    xa = _fp16_at(x, _strided(rows, stride, features), "x")
+    ca = _bytes_at(codes, rows * features, "codes")
+    sa = _fp32_at(scales, rows, "scales")
+    _check(lib.mi_quantise_rows_int8(xa, stride, ca, sa, rows, features, None))
+
+
+def _int8_at(x, x_scales, weight, w_scales, rows, in_features, out_features):
+    """The addresses of an int8 projection's operands."""
+    _non_negative(rows, "rows")
+    _non_negative(out_features, "out_features")
+    _int8_features(in_features, "in_features")
+    return (_bytes_at(x, rows * in_features, "x"), _fp32_at(x_scales, rows, "x_scales"),
+            _bytes_at(weight, out_features * in_features, "weight"),
+            _fp32_at(w_scales, out_features, "w_scales"))
+
+
+def _device_linear_int8(x, x_scales, weight, w_scales, bias, out, rows, in_features, out_features):
+    """linear in codes of 8 bits (beyond the reference): x and weight as
+    quantise_rows_int8 makes them, whole-number sums times the scales of their
+    rows, the bias added, rounded once. For the rows of prompts and batches."""
+    at = _int8_at(x, x_scales, weight, w_scales, rows, in_features, out_features)
+    ba = _fp16_at(bias, out_features, "bias") if bias is not None else None
+    oa = _fp16_at(out, rows * out_features, "out")
+    _check(lib.mi_linear_int8(*at, ba, oa, rows, in_features, out_features, None))
+
+
+def _device_linear_int8_accumulate(x, x_scales, weight, w_scales, out: FloatTensor, rows, in_features,
+                                   out_features, residual=None):
+    """linear_accumulate in codes of 8 bits: out = residual + x @ W.T in fp32,
+    residual out itself unless given."""
+    at = _int8_at(x, x_scales, weight, w_scales, rows, in_features, out_features)
+    oa = _fp32_at(out, rows * out_features, "out")
+    ra = _fp32_at(residual, rows * out_features, "residual") if residual is not None else None
+    _check(lib.mi_linear_int8_accumulate(*at, ra, oa, rows, in_features, out_features, None))
+
+
+@functools.lru_cache(maxsize=256, typed=True)
+def _sample_scratch(rows: int, vocab: int) -> int:
+    """Floats of scratch that sample takes (no fewer for more rows or a larger
+    vocab)."""
+    out = C.c_size_t()
+    _check(lib.mi_sample_scratch(rows, vocab, C.byref(out)))
+    return out.value
+
+
+def _sample(is_f32, logits, uniforms, tokens, rows, vocab, temperature, top_k, top_p, min_p, stride,
+            scratch):
+    for value, what in ((rows, "rows"), (vocab, "vocab"), (stride, "stride")):
+        _non_negative(value, what)
+    count = _strided(rows, stride, vocab)
+    la = (_fp32_at if is_f32 else _fp16_at)(logits, count, "logits")
+    ua = _fp32_at(uniforms, rows, "uniforms")
+    oa = _table(tokens, rows, 4, "tokens")
+    settings = [_table(x, rows, 4, what) if x is not None else None for x, what in (
+        (temperature, "temperature"), (top_k, "top_k"), (top_p, "top_p"), (min_p, "min_p"))]
+    wa, floats = _scratch(scratch)
+    _check(lib.mi_sample(la, int(is_f32), stride, ua, *settings, oa, rows, vocab, wa, floats, None))
+
+
+def _device_sample(logits, uniforms, tokens, rows, vocab, temperature=None, top_k=None, top_p=None,
+                   min_p=None, stride=0, scratch=None):
+    """Beyond the reference, whose engine takes the greedy token: a token of every
+    row of fp16 logits (rows, vocab) by the row's temperature, top_k, top_p and
+    min_p (device arrays of a value a row, int32 for top_k; None: off), from
+    uniforms[row] in [0, 1), into `tokens` (int32 on the device). `scratch`
+    holds sample_scratch floats. The weights are formed and summed in fp64; of
+    equal logits the lower index counts as the larger; temperature 0 is the
+    greedy token; a row with no logit above -inf gives `vocab`."""
+    _sample(False, logits, uniforms, tokens, rows, vocab, temperature, top_k, top_p, min_p, stride,
+            scratch)
+
+
+def _device_sample_f32(logits, uniforms, tokens, rows, vocab, temperature=None, top_k=None,
+                       top_p=None, min_p=None, stride=0, scratch=None):
+    """sample of fp32 logits."""
+    _sample(True, logits, uniforms, tokens, rows, vocab, temperature, top_k, top_p, min_p, stride,
+            scratch)
 
 
 def _device_embed(ids: DeviceIndex, table, out, hidden, vocab):
@@ -1791,6 +2057,9 @@ device = SimpleNamespace(
     quantise_int4=_device_quantise_int4,
     linear_int4=_device_linear_int4,
     linear_int4_accumulate=_device_linear_int4_accumulate,
+    quantise_rows_int8=_device_quantise_rows_int8,
+    linear_int8=_device_linear_int8,
+    linear_int8_accumulate=_device_linear_int8_accumulate,
     rmsnorm=_device_rmsnorm,
     rmsnorm_f32=_device_rmsnorm_f32,
     rope=_device_rope,
@@ -1804,7 +2073,15 @@ device = SimpleNamespace(
     attention_batch=_device_attention_batch,
     attention_batch_partials=_attention_batch_partials,
     attention_caches=_device_attention_caches,
+    attention_packed=_device_attention_packed,
+    attention_packed_partials=_attention_packed_partials,
+    append_batch=_device_append_batch,
+    append_caches=_device_append_caches,
     RopeTable=RopeTable,
+    rope_frequencies=rope_frequencies,
+    sample=_device_sample,
+    sample_f32=_device_sample_f32,
+    sample_scratch=_sample_scratch,
     add=_device_add,
     swiglu=_device_swiglu,
     copy=_device_copy,
