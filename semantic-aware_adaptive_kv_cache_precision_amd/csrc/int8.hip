@@ -330,7 +330,8 @@ namespace mi
     // step's copies have the time of two steps' products. Piece c (16 bytes)
     // of row t lies at place c ^ (t / 4 % 4) of its row: sixteen lanes that
     // read a piece of sixteen rows meet no bank twice.
-    template <int TM, int TN, bool kHalf>
+    // kTail: the last step is short, and what is past it counts as zeros.
+    template <int TM, int TN, bool kHalf, bool kTail>
     __global__ void __launch_bounds__(256, 2) int8_tiles_kernel(Int8Args a, int m_tiles, int n_tiles)
     {
       constexpr int kM = 64 * TM, kN = 64 * TN; // a workgroup's rows and outputs
@@ -368,7 +369,8 @@ namespace mi
       const int piece = (threadIdx.x % 4) ^ (threadIdx.x / 16 % 4);
       const int steps = (a.in + 63) / 64;
       const auto copy = [&](int step, int stage) {
-        // (Past the last input, of a short last step: any piece.)
+        // (Past the last input, of a short last step or the two after it: any
+        // piece.)
         const unsigned k = min(64 * step + 16 * piece, a.in - 16);
         std::uint8_t *to = stages + stage * kStage + wave * 1024;
 #pragma unroll
@@ -399,72 +401,53 @@ namespace mi
       const int x_row = (32 * TM * wm + n) * 64;
       const int w_row = (kM + 32 * TN * wn + n) * 64;
       const int turn = n / 4 % 4;
-      const auto multiply = [&](int stage, int inputs) {
+      copy(0, 0);
+      copy(1, 1);
+      int stage = 0;
+      for (int step = 0; step < steps; ++step)
+      {
+        // The step's copies have landed, the next one's may be on their way;
+        // every wave is done with the stage before, which the copies after
+        // those go to.
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kCopies) : "memory");
+        copy(step + 2, stage == 0 ? 2 : stage - 1);
         const std::uint8_t *at = stages + stage * kStage;
+        i32x4 x[2][TM], w[2][TN];
 #pragma unroll
         for (int c = 0; c < 2; ++c)
         {
           const int place = 16 * ((2 * c + half) ^ turn);
-          i32x4 x[TM], w[TN];
-#pragma unroll
-          for (int i = 0; i < TM; ++i)
-          {
-            x[i] = *reinterpret_cast<const i32x4 *>(at + x_row + 2048 * i + place);
-          }
 #pragma unroll
           for (int j = 0; j < TN; ++j)
           {
-            w[j] = *reinterpret_cast<const i32x4 *>(at + w_row + 2048 * j + place);
-            if (inputs < 64) // a short last step: what is past it counts as zeros
+            w[c][j] = *reinterpret_cast<const i32x4 *>(at + w_row + 2048 * j + place);
+            if constexpr (kTail)
             {
-              w[j] = 16 * (2 * c + half) < inputs ? w[j] : i32x4{0, 0, 0, 0};
+              w[c][j] = 64 * step + 16 * (2 * c + half) < a.in ? w[c][j] : i32x4{0, 0, 0, 0};
             }
           }
+#pragma unroll
+          for (int i = 0; i < TM; ++i)
+          {
+            x[c][i] = *reinterpret_cast<const i32x4 *>(at + x_row + 2048 * i + place);
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+        {
 #pragma unroll
           for (int j = 0; j < TN; ++j)
           {
 #pragma unroll
             for (int i = 0; i < TM; ++i)
             {
-              acc[j][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[j], x[i], acc[j][i], 0, 0, 0);
+              acc[j][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[c][j], x[c][i], acc[j][i], 0, 0, 0);
             }
           }
         }
-      };
-
-      copy(0, 0);
-      if (steps > 1)
-      {
-        copy(1, 1);
-      }
-      int stage = 0;
-      for (int step = 0; step < steps; ++step)
-      {
-        // The step's copies have landed, the next one's may be on their way;
-        // every wave is done with the stage before.
-        if (step + 1 < steps)
-        {
-          asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kCopies) : "memory");
-        }
-        else
-        {
-          asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        }
-        if (step + 2 < steps)
-        {
-          copy(step + 2, stage == 0 ? 2 : stage - 1);
-        }
-        const int inputs = a.in - 64 * step;
-        if (inputs >= 64)
-        {
-          multiply(stage, 64);
-        }
-        else
-        {
-          multiply(stage, inputs);
-        }
         stage = stage == 2 ? 0 : stage + 1;
       }
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); // the copies past the last
 
       // 32 rows at a time through the wave's own LDS, so that outputs leave
       // eight a lane in rows.
@@ -606,13 +589,13 @@ namespace mi
                              : want >= 4 ? rows_by<MT, 4>(a, stream) : rows_by<MT, 2>(a, stream);
     }
 
-    template <int TM, int TN, bool kHalf>
+    template <int TM, int TN, bool kHalf, bool kTail>
     void tiles_by(const Int8Args &a, hipStream_t stream)
     {
       constexpr std::size_t stages = 3 * (64 * TM + 64 * TN) * 64;
       constexpr std::size_t outs = 4 * 32 * (32 * TN * 4 + 16);
       constexpr std::size_t lds = std::max(stages, outs);
-      auto kernel = int8_tiles_kernel<TM, TN, kHalf>;
+      auto kernel = int8_tiles_kernel<TM, TN, kHalf, kTail>;
       if constexpr (lds > 64 * 1024)
       {
         hip_check(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
@@ -629,7 +612,16 @@ namespace mi
     template <int TM, int TN>
     void tiles_as(const Int8Args &a, hipStream_t stream)
     {
-      a.residual == nullptr ? tiles_by<TM, TN, true>(a, stream) : tiles_by<TM, TN, false>(a, stream);
+      if (a.in % 64 == 0)
+      {
+        a.residual == nullptr ? tiles_by<TM, TN, true, false>(a, stream)
+                              : tiles_by<TM, TN, false, false>(a, stream);
+      }
+      else
+      {
+        a.residual == nullptr ? tiles_by<TM, TN, true, true>(a, stream)
+                              : tiles_by<TM, TN, false, true>(a, stream);
+      }
     }
 
     void check_features(int features, const char *what)

@@ -3,15 +3,13 @@
 // [offsets_k[s], offsets_k[s + 1]) of their sequence. Query i of m, of e keys,
 // sees the first e - m + i + 1 of them; out = softmax(q . k / sqrt(hd)) v.
 //
-// Tiles are cut from the run of (query, head of the group) rows, whatever the
-// sequences' lengths: a row sees the keys [lo, hi] of the run of keys, and both
-// ends only rise along the run, so that a tile's keys are one range, from its
-// first row's lo to its last row's hi, and a short sequence costs a share of a
-// tile. Which sequence a row is of is found by a search of the offsets, held in
-// LDS before the first keys are.
+// A sequence's rows (query by query, the heads of a KV head's group) are cut into
+// tiles, and a workgroup takes a tile of one KV head. Which one, it finds from
+// the offsets, which are on the device: tiles with most keys first, as long as
+// the sequences are few enough to be ranked (a search for the length that as many
+// tiles reach as there are workgroups before this one); else in their order.
 //
-// A workgroup takes one KV head and consecutive rows, its waves 32 of them each;
-// the keys of a step pass through LDS, double buffered, copied there directly
+// The waves of a workgroup take 32 rows each; the keys of a step pass through LDS, double buffered, copied there directly
 // from memory; scores and output as attention_tiles.hpp has them, P rounded to
 // fp16 once (half a step is 2^-11 of a weight, as much as the output's own
 // rounding; the sums are of the rounded weights) against a reference that is
@@ -24,10 +22,8 @@
 #include "ragged.hpp"
 
 #include <algorithm>
-#include <climits>
 #include <cmath>
 #include <string>
-#include <type_traits>
 
 namespace mi
 {
@@ -36,7 +32,9 @@ namespace mi
     using namespace attention_tiles;
 
     constexpr int kMaxSplits = 256;
+    constexpr int kMfma = 0x8, kDsRead = 0x100; // instructions, to the scheduler
     constexpr int kOffsetsHeld = 4096; // offsets of each kind that LDS holds
+    constexpr int kRanked = 256;       // sequences whose tiles are ranked by their keys
 
     struct PackedArgs
     {
@@ -53,48 +51,13 @@ namespace mi
       int rows_q;
       int rows_k;
       int heads;
+      int kv_heads;
       int group;
       int splits;
       float scale;    // log2 e / sqrt(hd)
       float *part_ml; // splits > 1: [split][row] maximum and sum (row = query * heads + head),
       float *part_o;  // and hd outputs
     };
-
-    // The keys [lo, hi] that a query sees, none where hi is lo - 1; and whether
-    // it is a sequence's.
-    struct Seen
-    {
-      int lo;
-      int hi;
-      bool live;
-    };
-    template <typename Q, typename K>
-    __device__ inline Seen seen_by(int query, int batch, int rows_k, Q &&at_q, K &&at_k)
-    {
-      // The last sequence that begins at or before the query.
-      int from = 0, to = batch + 1;
-      while (from < to)
-      {
-        const int mid = (from + to) >> 1;
-        if (at_q(mid) <= query)
-        {
-          from = mid + 1;
-        }
-        else
-        {
-          to = mid;
-        }
-      }
-      const int s = from - 1;
-      if (s < 0 || s >= batch)
-      {
-        return {0, -1, false};
-      }
-      // (In 64 bits, and held within the keys: offsets may be anything.)
-      const long long begin = min(max(at_k(s), 0), rows_k), end = min(max(at_k(s + 1), 0), rows_k);
-      const long long last = end - 1 - (static_cast<long long>(at_q(s + 1)) - 1 - query);
-      return {static_cast<int>(begin), static_cast<int>(max(begin - 1, min(last, end - 1))), true};
-    }
 
     __device__ inline int wave_min(int v)
     {
@@ -106,6 +69,167 @@ namespace mi
       return __builtin_amdgcn_readfirstlane(v);
     }
     __device__ inline int wave_max(int v) { return -wave_min(-v); }
+
+    __device__ inline int wave_sum(int v)
+    {
+#pragma unroll
+      for (int offset = 1; offset < 64; offset *= 2)
+      {
+        v += __shfl_xor(v, offset);
+      }
+      return __builtin_amdgcn_readfirstlane(v);
+    }
+
+    // A sequence's rows and keys, whatever its offsets hold.
+    struct Sequence
+    {
+      int q0, queries, k0, keys;
+    };
+    template <typename Q, typename K>
+    __device__ inline Sequence sequence_of(const PackedArgs &a, int s, Q &&at_q, K &&at_k)
+    {
+      const int q0 = min(max(at_q(s), 0), a.rows_q), q1 = min(max(at_q(s + 1), 0), a.rows_q);
+      const int k0 = min(max(at_k(s), 0), a.rows_k), k1 = min(max(at_k(s + 1), 0), a.rows_k);
+      return {q0, max(q1 - q0, 0), k0, max(k1 - k0, 0)};
+    }
+    // The row tiles of a sequence, and how many of them (its last) see `keys`
+    // keys at least.
+    template <int kRows>
+    __device__ inline int tiles_of(const Sequence &s, int G)
+    {
+      return static_cast<int>((static_cast<long long>(s.queries) * G + kRows - 1) / kRows);
+    }
+    template <int kRows>
+    __device__ inline int tiles_that_see(const Sequence &s, int G, int keys)
+    {
+      // The first query that sees so many, and the tile that its last row is in
+      // or that reaches it.
+      const int query = keys - 1 - (s.keys - s.queries);
+      const int tiles = tiles_of<kRows>(s, G);
+      if (query <= 0 || keys <= 0)
+      {
+        return tiles;
+      }
+      return query >= s.queries
+                 ? 0
+                 : tiles - static_cast<int>(static_cast<long long>(query) * G / kRows);
+    }
+
+    // A workgroup's tile: its sequence, or none.
+    struct Tile
+    {
+      int sequence;
+      int tile;
+    };
+    // The index-th tile. Every wave finds it by itself.
+    template <int kRows, typename Q, typename K>
+    __device__ inline Tile tile_at(const PackedArgs &a, int index, Q &&at_q, K &&at_k)
+    {
+      const int lane = threadIdx.x & 63, G = a.group;
+      int least = -1; // keys that the tile sees, if they are ranked by them
+      if (a.batch <= kRanked)
+      {
+        Sequence mine[kRanked / 64];
+        int all = 0, most = 0;
+#pragma unroll
+        for (int i = 0; i < kRanked / 64; ++i)
+        {
+          const int s = lane + 64 * i;
+          mine[i] = s < a.batch ? sequence_of(a, s, at_q, at_k) : Sequence{0, 0, 0, 0};
+          all += tiles_of<kRows>(mine[i], G);
+          most = max(most, mine[i].keys);
+        }
+        if (index >= wave_sum(all))
+        {
+          return {-1, 0};
+        }
+        // The most keys that more than `index` tiles see: lo is, hi is not.
+        int lo = 0, hi = wave_max(most) + 1;
+        while (hi - lo > 1)
+        {
+          const int keys = lo + (hi - lo) / 2;
+          int see = 0;
+#pragma unroll
+          for (int i = 0; i < kRanked / 64; ++i)
+          {
+            see += tiles_that_see<kRows>(mine[i], G, keys);
+          }
+          (wave_sum(see) > index ? lo : hi) = keys;
+        }
+        int more = 0;
+#pragma unroll
+        for (int i = 0; i < kRanked / 64; ++i)
+        {
+          more += tiles_that_see<kRows>(mine[i], G, lo + 1);
+        }
+        index -= wave_sum(more); // among those that see so many and no more
+        least = lo;
+      }
+      for (int s0 = 0; s0 < a.batch; s0 += 64)
+      {
+        const int s = s0 + lane;
+        const Sequence mine = s < a.batch ? sequence_of(a, s, at_q, at_k) : Sequence{0, 0, 0, 0};
+        const int tiles = tiles_of<kRows>(mine, G);
+        const int see = least < 0 ? tiles : tiles_that_see<kRows>(mine, G, least);
+        const int count = least < 0 ? tiles : see - tiles_that_see<kRows>(mine, G, least + 1);
+        int upto = count;
+#pragma unroll
+        for (int offset = 1; offset < 64; offset *= 2)
+        {
+          const int before = __shfl_up(upto, offset);
+          upto = lane >= offset ? upto + before : upto;
+        }
+        const unsigned long long reached = __ballot(upto > index);
+        if (reached != 0)
+        {
+          const int at = __ffsll(reached) - 1;
+          const int tile = tiles - see + index - (upto - count);
+          return {s0 + at, __builtin_amdgcn_readfirstlane(__shfl(tile, at))};
+        }
+        index -= __builtin_amdgcn_readfirstlane(__shfl(upto, 63));
+      }
+      return {-1, 0};
+    }
+
+    // An LDS address as an instruction's operand has it.
+    __device__ inline unsigned lds_address(const void *p)
+    {
+      return static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(
+          reinterpret_cast<std::uintptr_t>((lds_void)(const_cast<void *>(p))))));
+    }
+    // `count` + 1 rows of `width` halves, `step` bytes apart, for buffer loads.
+    __device__ inline u32x4 rows_from(const std::uint16_t *at, int count, unsigned step, int width)
+    {
+      const auto address = reinterpret_cast<std::uintptr_t>(at);
+      const unsigned long long bytes = static_cast<unsigned long long>(count) * step + 2 * width;
+      return u32x4{static_cast<unsigned>(address), static_cast<unsigned>(address >> 32) & 0xFFFFu,
+                   static_cast<unsigned>(min(bytes, 0xFFFFFFFFull)), 0x00020000u};
+    }
+    // 16 bytes a lane from rows + at + more to the 1,024 bytes at LDS address `to`.
+    __device__ inline void copy_to_lds(unsigned to, unsigned at, u32x4 rows, unsigned more)
+    {
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                   :: "s"(to), "v"(at), "s"(rows), "s"(more)
+                   : "memory", "m0");
+    }
+
+    // A barrier for what waves leave each other in LDS, copies in flight or not.
+    __device__ inline void lds_barrier()
+    {
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    }
+    __device__ inline bool all_finite(half8 v)
+    {
+      const u32x4 bits = __builtin_bit_cast(u32x4, v);
+      bool fine = true;
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+      {
+        fine = fine && is_finite(static_cast<std::uint16_t>(bits[w])) &&
+               is_finite(static_cast<std::uint16_t>(bits[w] >> 16));
+      }
+      return fine;
+    }
 
     // Waves a SIMD that a form's registers are held to: four at head_dim 64
     // (128 registers), two at 128 (256); few rows leave a wave alone anyway.
@@ -124,34 +248,20 @@ namespace mi
       constexpr int kWayKeys = kKeys / kWays;
       constexpr int N = kWayKeys / 32;
       extern __shared__ __align__(16) std::uint16_t stages[]; // two of kStage
-      __shared__ int s_lo[NW], s_hi[NW];
+      __shared__ int s_fine[NW];
 
       const int lane = threadIdx.x & 63;
       const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
       const int way = wave / kTiles;
       const int n = lane & 31;
       const int half = lane >> 5;
-      const int kvh = blockIdx.y;
-      const int split = blockIdx.z;
+      const int kvh = blockIdx.x % a.kv_heads, index = blockIdx.x / a.kv_heads;
+      const int split = blockIdx.y;
       const int G = a.group;
-      const long long all_rows = static_cast<long long>(a.rows_q) * G;
-      // The last rows of the run go first: of one prompt, those with most keys.
-      const long long row0 = static_cast<long long>(gridDim.x - 1 - blockIdx.x) * kRows;
 
-      // The lane's row and what it sees.
-      const long long row = row0 + 32 * (wave % kTiles) + n;
-      const bool there = row < all_rows;
-      const int query = there ? static_cast<int>(row / G) : 0;
-      const int head = kvh * G + (there ? static_cast<int>(row % G) : 0);
-      const std::size_t row_at = static_cast<std::size_t>(query) * a.heads + head;
-      half8 q[HD / 16];
-      const std::uint16_t *q_row = a.q + query * a.q_stride + head * HD + 8 * half;
-#pragma unroll
-      for (int c = 0; c < HD / 16; ++c)
-      {
-        q[c] = as_half8(*reinterpret_cast<const u32x4 *>(q_row + 16 * c));
-      }
-      Seen seen;
+      // The tile, and its sequence.
+      Tile tile;
+      Sequence of;
       if (a.batch <= kOffsetsHeld)
       {
         int *held_q = reinterpret_cast<int *>(stages), *held_k = held_q + kOffsetsHeld + 1;
@@ -161,36 +271,52 @@ namespace mi
           held_k[i] = a.offsets_k[i];
         }
         __syncthreads();
-        seen = seen_by(query, a.batch, a.rows_k, [&](int i) { return held_q[i]; },
-                       [&](int i) { return held_k[i]; });
+        const auto at_q = [&](int i) { return held_q[i]; };
+        const auto at_k = [&](int i) { return held_k[i]; };
+        tile = tile_at<kRows>(a, index, at_q, at_k);
+        of = sequence_of(a, max(tile.sequence, 0), at_q, at_k);
+        __syncthreads(); // the offsets are read
       }
       else
       {
-        seen = seen_by(query, a.batch, a.rows_k, [&](int i) { return a.offsets_q[i]; },
-                       [&](int i) { return a.offsets_k[i]; });
+        const auto at_q = [&](int i) { return a.offsets_q[i]; };
+        const auto at_k = [&](int i) { return a.offsets_k[i]; };
+        tile = tile_at<kRows>(a, index, at_q, at_k);
+        of = sequence_of(a, max(tile.sequence, 0), at_q, at_k);
       }
-      const bool valid = there && seen.live;
-      const int lo = valid ? seen.lo : 0, hi = valid ? seen.hi : -1;
-      // The wave's keys, and those that every row of it sees.
-      const int wave_lo = wave_min(valid && hi >= lo ? lo : INT_MAX);
-      const int wave_hi = wave_max(hi);
-      const int all_lo = wave_max(valid ? lo : 0);
-      const int all_hi = wave_min(valid ? hi : INT_MAX);
-      if (lane == 0)
+      if (tile.sequence < 0)
       {
-        s_lo[wave] = wave_lo;
-        s_hi[wave] = wave_hi;
+        return;
       }
-      __syncthreads(); // (the offsets are read too)
-      int first = INT_MAX, last = -1;
+      const int q0 = __builtin_amdgcn_readfirstlane(of.q0), first = __builtin_amdgcn_readfirstlane(of.k0);
+      const int queries = __builtin_amdgcn_readfirstlane(of.queries);
+      const int past = __builtin_amdgcn_readfirstlane(of.keys) - queries; // less than none: blind queries
+
+      // The lane's row, and the last key it sees: one before the first, if none.
+      const long long rows = static_cast<long long>(queries) * G;
+      const long long tile_row = static_cast<long long>(tile.tile) * kRows;
+      const long long wave_row = tile_row + 32 * (wave % kTiles);
+      const long long row = wave_row + n;
+      const bool valid = row < rows;
+      const auto last_key = [&](long long r) {
+        return first + max(-1, past + static_cast<int>(min(r, rows - 1) / G));
+      };
+      const int query = q0 + (valid ? static_cast<int>(row / G) : 0);
+      const int head = kvh * G + (valid ? static_cast<int>(row % G) : 0);
+      const int hi = last_key(row);
+      const std::size_t row_at = static_cast<std::size_t>(query) * a.heads + head;
+      half8 q[HD / 16];
+      const std::uint16_t *q_row = a.q + query * a.q_stride + head * HD + 8 * half;
 #pragma unroll
-      for (int w = 0; w < NW; ++w)
+      for (int c = 0; c < HD / 16; ++c)
       {
-        first = min(first, s_lo[w]);
-        last = max(last, s_hi[w]);
+        q[c] = as_half8(*reinterpret_cast<const u32x4 *>(q_row + 16 * c));
       }
-      first = __builtin_amdgcn_readfirstlane(first);
-      last = __builtin_amdgcn_readfirstlane(last);
+      // The wave's last key, the last that all its rows see, and the workgroup's.
+      const int wave_hi = wave_row < rows ? last_key(wave_row + 31) : -1;
+      const int all_hi = last_key(wave_row);
+      const int block_hi = last_key(tile_row);
+      const int last = last_key(tile_row + kRows - 1);
       const int steps = last >= first ? (last - first) / kKeys + 1 : 0;
       const int per = (steps + a.splits - 1) / a.splits;
       const int begin = min(split * per, steps);
@@ -209,25 +335,36 @@ namespace mi
         }
       }
 
-      // A step's rows to LDS, 16 bytes a lane; rows past the last repeat it.
+      // A step's rows to LDS, 16 bytes a lane, asked for without the compiler's
+      // knowledge, whose wait for them would come before the first transposing
+      // read of the step before: buffer loads from the step's first row, with
+      // zeros for what lies past the last key.
+      constexpr int kCopies = kTile / 8 / (64 * NW);
+      constexpr int kCopyRows = 64 * NW / kPieces; // rows a copy of the workgroup
+      static_assert(kCopyRows % 16 == 0, "rows a copy apart have their pieces in the same places");
+      const int copy_row = static_cast<int>(threadIdx.x) / kPieces;
+      const int copy_piece = (static_cast<int>(threadIdx.x) % kPieces) ^ swizzle<HD>(copy_row);
+      const unsigned k_step = 2u * static_cast<unsigned>(a.k_stride), v_step = 2u * static_cast<unsigned>(a.v_stride);
+      const unsigned k_at = copy_row * k_step + 16 * copy_piece, v_at = copy_row * v_step + 16 * copy_piece;
       const auto copy = [&](int step, int buf) {
         const int key0 = first + step * kKeys;
-        std::uint16_t *stage = stages + buf * kStage;
+        const unsigned to = lds_address(stages + buf * kStage + wave * 512);
+        const u32x4 k_rows = rows_from(a.k + key0 * a.k_stride + kvh * HD, a.rows_k - 1 - key0, k_step, HD);
+        const u32x4 v_rows = rows_from(a.v + key0 * a.v_stride + kvh * HD, a.rows_k - 1 - key0, v_step, HD);
 #pragma unroll
-        for (int i = 0; i < kTile / 8 / (64 * NW); ++i)
+        for (int i = 0; i < kCopies; ++i)
         {
-          const int place = (i * NW + wave) * 64 + lane;
-          const int t = place / kPieces;
-          const int c = (place % kPieces) ^ swizzle<HD>(t);
-          const long long key = min(key0 + t, a.rows_k - 1);
-          std::uint16_t *to = stage + (i * NW + wave) * 512;
-          __builtin_amdgcn_global_load_lds(
-              (global_void)(a.k + key * a.k_stride + kvh * HD + 8 * c), (lds_void)(to), 16, 0, 0);
-          __builtin_amdgcn_global_load_lds(
-              (global_void)(a.v + key * a.v_stride + kvh * HD + 8 * c), (lds_void)(to + kTile), 16,
-              0, 0);
+          copy_to_lds(to + 1024 * NW * i, k_at, k_rows, i * kCopyRows * k_step);
+          copy_to_lds(to + 2 * kTile + 1024 * NW * i, v_at, v_rows, i * kCopyRows * v_step);
         }
       };
+      // (The queries are there before the loop: a wait for them inside it would
+      // wait for the copies too.)
+#pragma unroll
+      for (int c = 0; c < HD / 16; ++c)
+      {
+        asm volatile("" : "+v"(q[c]));
+      }
       if (begin < end)
       {
         copy(begin, 0);
@@ -235,17 +372,76 @@ namespace mi
       for (int step = begin; step < end; ++step)
       {
         const int buf = (step - begin) & 1;
-        // This step's copies have landed (a wave waits for its own before the
-        // barrier), and every wave is done with the other buffer.
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_s_waitcnt(0x0F70); // vmcnt(0)
-        __syncthreads();
+        // This step's copies have landed, and every wave is done with the other
+        // buffer.
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         if (step + 1 < end)
         {
           copy(step + 1, buf ^ 1);
         }
-        const int key0 = first + step * kKeys + way * kWayKeys;
-        if (key0 > wave_hi || key0 + kWayKeys - 1 < wave_lo)
+        const int step0 = first + step * kKeys;
+        // A value that some row does not see may be anything: where one of such
+        // a step's is not finite, the rows that see it add it here, and the
+        // products take it as zero.
+        if (step0 + kKeys - 1 > block_hi)
+        {
+          std::uint16_t *brought = stages + buf * kStage + kTile + 8 * threadIdx.x;
+          bool fine = true;
+#pragma unroll
+          for (int i = 0; i < kCopies; ++i)
+          {
+            const half8 v = as_half8(*reinterpret_cast<const u32x4 *>(brought + 512 * NW * i));
+            fine = fine && all_finite(v);
+          }
+          if (lane == 0)
+          {
+            s_fine[wave] = 1;
+          }
+          if (!__all(fine) && lane == 0)
+          {
+            s_fine[wave] = 0;
+          }
+          lds_barrier();
+          bool all = true;
+#pragma unroll
+          for (int w = 0; w < NW; ++w)
+          {
+            all = all && s_fine[w] != 0;
+          }
+          if (!all)
+          {
+            if (way == step % kWays) // the ways' sums are added up: one of them adds it
+            {
+              for (int t = 0; t < min(kKeys, a.rows_k - step0); ++t)
+              {
+                const std::uint16_t *spoilt_row = stages + buf * kStage + kTile + t * HD;
+                const int swap = swizzle<HD>(t);
+                const bool sees = step0 + t <= hi;
+#pragma unroll
+                for (int d = 0; d < HD / 32; ++d)
+                {
+#pragma unroll
+                  for (int i = 0; i < 16; ++i)
+                  {
+                    const int ch = 32 * d + 8 * (i / 4) + 4 * half + i % 4;
+                    const std::uint16_t v = spoilt_row[8 * ((ch / 8) ^ swap) + ch % 8];
+                    run.o[d][i] += sees && !is_finite(v) ? h2f(v) : 0.0f;
+                  }
+                }
+              }
+            }
+            lds_barrier();
+#pragma unroll
+            for (int i = 0; i < kCopies; ++i)
+            {
+              u32x4 *at = reinterpret_cast<u32x4 *>(brought + 512 * NW * i);
+              *at = __builtin_bit_cast(u32x4, finite_only(as_half8(*at)));
+            }
+          }
+          lds_barrier();
+        }
+        const int key0 = step0 + way * kWayKeys;
+        if (key0 > wave_hi)
         {
           continue;
         }
@@ -273,8 +469,18 @@ namespace mi
             s[j] = mfma32(k, q[c], s[j]);
           }
         }
+        // Four reads ahead of the products.
+        constexpr int kReads = N * HD / 16;
+        __builtin_amdgcn_sched_group_barrier(kDsRead, 4, 0);
+#pragma unroll
+        for (int i = 4; i < kReads; ++i)
+        {
+          __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(kMfma, 4, 0);
         // Whether some row of the wave does not see some key of the step.
-        const bool edge = key0 + kWayKeys - 1 > all_hi || key0 < all_lo;
+        const bool edge = key0 + kWayKeys - 1 > all_hi;
         if (edge)
         {
 #pragma unroll
@@ -284,7 +490,7 @@ namespace mi
             for (int i = 0; i < 16; ++i)
             {
               const int key = key0 + 32 * j + 8 * (i / 4) + 4 * half + i % 4;
-              s[j][i] = key >= lo && key <= hi ? s[j][i] : -INFINITY;
+              s[j][i] = key <= hi ? s[j][i] : -INFINITY;
             }
           }
         }
@@ -331,10 +537,6 @@ namespace mi
           }
         }
         run.l += sum;
-        // A value some row does not see may be anything: if one of an edge
-        // step's is not finite, the products take it as zero, and the rows
-        // that do see it add it after them.
-        const bool spoilt = edge && !finite_values<HD, kWayKeys>(values, lane);
         // Lane l's P of a 16-key product: keys 8 e + 4 half + {0..3}, e = 0, 1.
 #pragma unroll
         for (int j = 0; j < N; ++j)
@@ -358,30 +560,7 @@ namespace mi
                 vt[4 * e + 2] = x[2];
                 vt[4 * e + 3] = x[3];
               }
-              if (spoilt)
-              {
-                vt = finite_only(vt);
-              }
               run.o[d] = mfma32(vt, p[j][u], run.o[d]);
-            }
-          }
-        }
-        if (spoilt)
-        {
-          for (int key = key0; key < min(key0 + kWayKeys, a.rows_k); ++key)
-          {
-            const std::uint16_t *spoilt_row = values + (key - key0) * HD;
-            const int swap = swizzle<HD>(key - key0);
-#pragma unroll
-            for (int d = 0; d < HD / 32; ++d)
-            {
-#pragma unroll
-              for (int i = 0; i < 16; ++i)
-              {
-                const int ch = 32 * d + 8 * (i / 4) + 4 * half + i % 4;
-                const std::uint16_t v = spoilt_row[8 * ((ch / 8) ^ swap) + ch % 8];
-                run.o[d][i] += key >= lo && key <= hi && !is_finite(v) ? h2f(v) : 0.0f;
-              }
             }
           }
         }
@@ -557,15 +736,14 @@ namespace mi
       static constexpr int tiles = kTiles_, ways = kWays_, keys = kKeys_, rows = 32 * kTiles_;
     };
     using Few = Form<1, 4, 128>;
-    using Many64 = Form<4, 2, 128>;
-    using Many128 = Form<4, 1, 64>;
+    using Many = Form<4, 1, 64>;
 
     // How a launch is cut. The lengths are on the device: what is known of them
     // here is how many rows and keys there are.
     struct Cut
     {
       bool few;
-      int blocks; // workgroups over the rows, a KV head
+      int blocks; // workgroups over the tiles there may be, a KV head
       int splits; // workgroups over a row's keys
     };
 
@@ -580,9 +758,9 @@ namespace mi
       Cut c{};
       const long long few = (rows + Few::rows - 1) / Few::rows * t.kv_heads;
       c.few = few <= (span <= 1024 && t.head_dim == 64 ? 512 : 256);
-      const int tile = c.few ? Few::rows : t.head_dim == 64 ? Many64::rows : Many128::rows;
-      const int keys = c.few ? Few::keys : t.head_dim == 64 ? Many64::keys : Many128::keys;
-      c.blocks = static_cast<int>((rows + tile - 1) / tile);
+      const int tile = c.few ? Few::rows : Many::rows;
+      const int keys = c.few ? Few::keys : Many::keys;
+      c.blocks = static_cast<int>(rows / tile + std::min(t.batch, t.rows_q)); // a short tile a sequence
       c.splits = 1;
       if (may_split && c.blocks > 0)
       {
@@ -605,10 +783,11 @@ namespace mi
                               std::to_string(t.rows_k));
       }
       constexpr int kMost = 0x7fffff00; // a step's last key stays an index
-      if (t.rows_q > kMost || t.rows_k > kMost || t.batch > kMost)
+      if (t.rows_q > kMost || t.rows_k > kMost || t.batch > 65535)
       {
-        throw InvalidArgument("batch, rows_q and rows_k exceed packed attention's " +
-                              std::to_string(kMost));
+        throw InvalidArgument("packed attention takes at most 65535 sequences and " +
+                              std::to_string(kMost) + " rows, got " + std::to_string(t.batch) + ", " +
+                              std::to_string(t.rows_q) + " and " + std::to_string(t.rows_k));
       }
       if (t.head_dim != 64 && t.head_dim != 128)
       {
@@ -620,18 +799,19 @@ namespace mi
         throw InvalidArgument("packed attention takes a whole number of query heads a KV head, got " +
                               std::to_string(t.heads) + " and " + std::to_string(t.kv_heads));
       }
-      // A head's offset in its token is 32 bits, and a launch's workgroups are.
+      // A head's offset in its token is 32 bits, and a launch's workgroups and
+      // a join's rows are.
       if (static_cast<long long>(t.heads) * t.head_dim > 0x7fffffff ||
-          static_cast<long long>(t.rows_q) * (t.heads / t.kv_heads) > 0x7fffffffll * 32)
+          static_cast<long long>(t.rows_q) * t.heads > 0x7fffffffll - 65535ll * t.kv_heads)
       {
         throw InvalidArgument("packed attention takes fewer than 2^31 query elements a token and "
-                              "2^36 rows a KV head, got " + std::to_string(t.heads) + " heads of " +
-                              std::to_string(t.head_dim));
+                              "(query, head) rows, got " + std::to_string(t.rows_q) + " rows of " +
+                              std::to_string(t.heads) + " heads of " + std::to_string(t.head_dim));
       }
     }
 
     template <int HD, typename F>
-    void launch(const PackedArgs &a, const Cut &c, int kv_heads, hipStream_t stream)
+    void launch(const PackedArgs &a, const Cut &c, hipStream_t stream)
     {
       constexpr std::size_t lds =
           std::max({sizeof(std::uint16_t) * 2 * 2 * F::keys * HD,
@@ -645,20 +825,20 @@ namespace mi
                                       static_cast<int>(lds)),
                   "hipFuncSetAttribute packed LDS");
       }
-      kernel<<<dim3(c.blocks, kv_heads, c.splits), 64 * F::tiles * F::ways, lds, stream>>>(a);
+      kernel<<<dim3(c.blocks * a.kv_heads, c.splits), 64 * F::tiles * F::ways, lds, stream>>>(a);
       hip_check(hipGetLastError(), "packed_kernel");
     }
 
     template <int HD>
-    void launch_any(const PackedArgs &a, const Cut &c, int kv_heads, hipStream_t stream)
+    void launch_any(const PackedArgs &a, const Cut &c, hipStream_t stream)
     {
       if (c.few)
       {
-        launch<HD, Few>(a, c, kv_heads, stream);
+        launch<HD, Few>(a, c, stream);
       }
       else
       {
-        launch<HD, std::conditional_t<HD == 64, Many64, Many128>>(a, c, kv_heads, stream);
+        launch<HD, Many>(a, c, stream);
       }
       if (c.splits > 1)
       {
@@ -703,12 +883,15 @@ namespace mi
     const long long q_stride = t.q_stride > 0 ? t.q_stride : q_width;
     const long long k_stride = t.k_stride > 0 ? t.k_stride : width;
     const long long v_stride = t.v_stride > 0 ? t.v_stride : width;
+    // (A step's rows within 32 bits.)
+    constexpr long long kMostStride = 1 << 24;
     if (t.q_stride < 0 || t.k_stride < 0 || t.v_stride < 0 || q_stride < q_width ||
-        k_stride < width || v_stride < width)
+        k_stride < width || v_stride < width || k_stride >= kMostStride || v_stride >= kMostStride)
     {
       throw InvalidArgument("packed attention's strides are of a token's " +
                             std::to_string(q_width) + " query and " + std::to_string(width) +
-                            " key and value elements at least (0: those); got " +
+                            " key and value elements at least (0: those), of keys and values below " +
+                            std::to_string(kMostStride) + "; got " +
                             std::to_string(t.q_stride) + ", " + std::to_string(t.k_stride) +
                             " and " + std::to_string(t.v_stride));
     }
@@ -762,6 +945,7 @@ namespace mi
     a.rows_q = t.rows_q;
     a.rows_k = t.rows_k;
     a.heads = t.heads;
+    a.kv_heads = t.kv_heads;
     a.group = t.heads / t.kv_heads;
     a.splits = c.splits;
     a.scale = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(t.head_dim)));
@@ -771,8 +955,8 @@ namespace mi
       a.part_o = t.partials;
       a.part_ml = t.partials + rows * c.splits * t.head_dim;
     }
-    t.head_dim == 64 ? launch_any<64>(a, c, t.kv_heads, stream)
-                     : launch_any<128>(a, c, t.kv_heads, stream);
+    t.head_dim == 64 ? launch_any<64>(a, c, stream)
+                     : launch_any<128>(a, c, stream);
   }
 
 } // namespace mi

@@ -9,14 +9,15 @@
 // uniform's share of all kept.
 //
 // Two launches. The first (a workgroup 4,096 logits of a row) finds its part's
-// largest logit and a histogram of the others below it: buckets of an eighth
-// of a nat, floor(8 l / T), on one grid for the whole row, each with its count
-// and its weights' sum. The second (a workgroup a row) adds the parts' up, and
-// knows from them the bucket that each border (k, p, min-p) falls into. Only
-// the logits of such a bucket are looked at again, in the parts that have any:
-// they are put in order, and the border found among them. With the kept part of
-// every bucket known, so is the part that the token is in, whose weights are
-// then added in turn.
+// largest logit and a histogram of the others below it: buckets of a
+// thirty-second of a nat, floor(32 l / T), on one grid for the whole row, each
+// with its count and its weights' sum. The second (a workgroup a row) adds the
+// parts' up, and knows from them the bucket that each border (k, p, min-p)
+// falls into. A bucket is a range of logits: only those are looked for again, in
+// the parts that have any, and the border found among them, by histograms of
+// their ranks until 64 are left to be put in order. With the kept part of every
+// bucket known, so is the part that the token is in, whose weights are then
+// added in turn.
 //
 // Sums: a bucket's weights are added as whole numbers of 2^-38 of the part's
 // largest, by LDS atomics of 64 bits (13 of them the count), so that the order
@@ -37,10 +38,11 @@ namespace mi
 
     constexpr int kPart = 4096;   // logits a part
     constexpr int kThreads = 256; // of a part's workgroup
-    constexpr int kBuckets = 256; // an eighth of a nat each: 32 nats below the largest
-    constexpr int kPerNat = 8;
-    constexpr int kRowThreads = 1024;
-    constexpr int kList = 2048;   // logits of a border's bucket held in LDS
+    constexpr int kBuckets = 1024; // 32 nats below the largest
+    constexpr int kPerNat = 32;
+    constexpr int kRowThreads = 1024; // a bucket each
+    constexpr int kList = 2048;       // logits of a border's bucket held in LDS
+    constexpr int kFew = 64;          // of them put in order
     constexpr int kMostVocab = 1 << 20;
     constexpr int kMostParts = kMostVocab / kPart;
     constexpr double kUnit = 0x1p38; // of a weight, in the histograms
@@ -60,6 +62,7 @@ namespace mi
       int vocab;
       int parts;
       unsigned long long *sums; // [row][part][bucket] count << 51 | weights
+      double *whole;            // [row][part] the weights of them all
       float *tops;              // [row][part] largest logit
       int *top_at;              // and its index, or vocab
     };
@@ -96,10 +99,10 @@ namespace mi
     __device__ inline bool counts(float l) { return l > -INFINITY; }
 
     // The bucket on the row's grid; larger for larger logits.
-    __device__ inline int on_grid(double eighths)
+    __device__ inline int on_grid(double steps)
     {
       constexpr double kFar = 1 << 29;
-      return static_cast<int>(fmin(fmax(floor(eighths), -kFar), kFar));
+      return static_cast<int>(fmin(fmax(floor(steps), -kFar), kFar));
     }
     __device__ inline int bucket_of(float l, double inv_t)
     {
@@ -134,7 +137,11 @@ namespace mi
         const int i = e * kThreads + threadIdx.x;
         l[e] = i < count ? logit_at<kHalf>(logits, first + i) : -INFINITY;
       }
-      s_sums[threadIdx.x] = 0;
+#pragma unroll
+      for (int b = 0; b < kBuckets; b += kThreads)
+      {
+        s_sums[b + threadIdx.x] = 0;
+      }
       // The largest, and the lowest index that has it.
       float top = -INFINITY;
       int at = a.vocab;
@@ -201,7 +208,29 @@ namespace mi
         }
       }
       __syncthreads();
-      a.sums[slot * kBuckets + threadIdx.x] = s_sums[threadIdx.x];
+      unsigned long long whole = 0;
+#pragma unroll
+      for (int b = 0; b < kBuckets; b += kThreads)
+      {
+        const unsigned long long v = s_sums[b + threadIdx.x];
+        a.sums[slot * kBuckets + b + threadIdx.x] = v;
+        whole += v & kSumMask;
+      }
+#pragma unroll
+      for (int offset = 1; offset < 64; offset *= 2)
+      {
+        whole += __shfl_xor(whole, offset);
+      }
+      __syncthreads();
+      if (threadIdx.x % 64 == 0)
+      {
+        s_sums[threadIdx.x / 64] = whole;
+      }
+      __syncthreads();
+      if (threadIdx.x == 0)
+      {
+        a.whole[slot] = static_cast<double>(s_sums[0] + s_sums[1] + s_sums[2] + s_sums[3]);
+      }
     }
 
     // ---- the row ------------------------------------------------------------------
@@ -250,20 +279,23 @@ namespace mi
 
     struct RowState
     {
-      int counts4[4][kBuckets]; // of quarters of the parts
-      double weights4[4][kBuckets];
       int count[kBuckets];      // of the row, up to and with each bucket
       double weight[kBuckets];
-      short with[kMostParts];   // the parts that have logits of a border's bucket
       double scale[kMostParts]; // of a part's weights in the row's
       short shift[kMostParts];  // a part's bucket 0 among the row's; kBuckets: none of it
+      short with[kMostParts];   // the parts that have logits of a border's bucket
       double kept[kMostParts];  // a part's kept weights
+      unsigned long long border[kMostParts]; // of the border's bucket
       unsigned long long list[kList];
-      unsigned long long bins[256]; // narrowing a border that is too wide for the list
+      unsigned long long bins[kRowThreads]; // histograms of ranks
+      int bin_counts[kRowThreads];
+      unsigned long long few[kFew];
       double waves[kRowThreads / 64];
       int int_waves[kRowThreads / 64];
       int ints[4];
+      unsigned long long rank;
       double value;
+      int listed;
     };
 
     // A border: everything in buckets before `bucket` is kept, and in it what
@@ -284,11 +316,33 @@ namespace mi
       double inv_t;
       float top;
       int highest;
+      int held = -1; // the bucket whose logits are all in the list
 
-      // Calls f(rank, logit) for the logits of buckets [b, end), by threads; the
-      // parts that have none are passed over.
+      // The least logit, as the upper half of a rank, of a bucket on the grid
+      // or above: by 64 pivots at a time.
+      __device__ unsigned first_key(int bucket) const
+      {
+        const unsigned lane = threadIdx.x & 63;
+        unsigned lo = 0x00800000u, hi = 0xFF800001u; // the least finite; past infinity
+        while (lo < hi)
+        {
+          const unsigned step = (hi - lo) / 64 + 1;
+          const unsigned long long at = lo + static_cast<unsigned long long>(lane) * step;
+          const bool reached =
+              at >= hi ||
+              bucket_of(logit_of(at << 32), inv_t) >= bucket;
+          const int before = __popcll(~__ballot(reached));
+          const unsigned long long next = lo + static_cast<unsigned long long>(before) * step;
+          lo = before > 0 ? static_cast<unsigned>(next - step + 1) : lo;
+          hi = static_cast<unsigned>(min(next, static_cast<unsigned long long>(hi)));
+        }
+        return __builtin_amdgcn_readfirstlane(lo);
+      }
+
+      // Calls f(rank, logit) for the row's logits of buckets [b, end), which
+      // are those from `least` to `most`; the parts that have none are passed over.
       template <typename F>
-      __device__ void each(int b, int end, F &&f) const
+      __device__ void each(int b, int end, float least, float most, F &&f) const
       {
         __syncthreads();
         if (threadIdx.x == 0)
@@ -316,200 +370,174 @@ namespace mi
         for (int i = threadIdx.x; i < all; i += kRowThreads)
         {
           const int part = s.with[i / kPart], at = part * kPart + i % kPart;
-          const float l = at < a.vocab ? logit_at<kHalf>(logits, at) : -INFINITY;
-          if (counts(l))
+          const float l = at < a.vocab ? logit_at<kHalf>(logits, at) : NAN;
+          if (l >= least && l <= most)
           {
-            const int below = highest - bucket_of(l, inv_t);
-            if (below >= b && below < end && below - s.shift[part] < kBuckets)
-            {
-              f(rank_of(l, at), l);
-            }
+            f(rank_of(l, at), l);
           }
         }
       }
 
-      // The list's first n ranks in order, largest first.
-      __device__ void sort(int n) const
+      // Of the ranks in [lo, hi], `source` calls back with each, those above the
+      // border are counted as taken, and [lo, hi] becomes the 1,024th of it that
+      // has the border. Returns how many are in it.
+      template <typename S>
+      __device__ int narrow(S &&source, long long most, double need, double least,
+                            unsigned long long &lo, unsigned long long &hi, long long &taken,
+                            double &weight) const
       {
-        int size = 64;
-        while (size < n)
-        {
-          size *= 2;
-        }
-        for (int i = n + threadIdx.x; i < size; i += kRowThreads)
-        {
-          s.list[i] = 0;
-        }
-        __syncthreads();
-        for (int k = 2; k <= size; k *= 2)
-        {
-          for (int j = k / 2; j > 0; j /= 2)
-          {
-            for (int i = threadIdx.x; i < size / 2; i += kRowThreads)
-            {
-              const int lo = 2 * j * (i / j) + i % j, hi = lo + j;
-              const unsigned long long x = s.list[lo], y = s.list[hi];
-              const bool down = (lo & k) == 0;
-              if ((x < y) == down)
-              {
-                s.list[lo] = y;
-                s.list[hi] = x;
-              }
-            }
-            __syncthreads();
-          }
-        }
-      }
-
-      // The border among the logits of buckets [b, end), of which the first are
-      // kept: as long as they are fewer than `most` and `reached` of their
-      // weights' sum so far (their own not in it) does not hold, and they weigh
-      // `least`. One of them is kept at least where `most` and `need` are
-      // positive. Returns the rank of the last kept (all ones: none), and to
-      // *sum the weights of the kept.
-      __device__ unsigned long long cut(int b, int end, long long most, double need, double least,
-                                        double *sum) const
-      {
-        // Ranks in [lo, hi] are looked at; what ranks above hi, within the
-        // buckets, is kept: `taken` logits of weight `weight`.
-        unsigned long long lo = 0, hi = ~0ull;
-        long long taken = 0;
-        double weight = 0.0;
-        for (;;)
-        {
-          if (threadIdx.x == 0)
-          {
-            s.ints[0] = 0;
-          }
-          __syncthreads();
-          each(b, end, [&](unsigned long long rank, float) {
-            if (rank >= lo && rank <= hi)
-            {
-              const int at = atomicAdd(&s.ints[0], 1);
-              if (at < kList)
-              {
-                s.list[at] = rank;
-              }
-            }
-          });
-          __syncthreads();
-          const int n = s.ints[0];
-          if (n <= kList)
-          {
-            sort(n);
-            // Two a thread, in order.
-            const int i0 = 2 * threadIdx.x;
-            double w[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-            {
-              w[e] = i0 + e < n ? weight_of(logit_of(s.list[i0 + e]), top, inv_t) : 0.0;
-            }
-            const double upto = scan(w[0] + w[1], s.waves);
-            double before = weight + (upto - (w[0] + w[1]));
-            if (threadIdx.x == 0)
-            {
-              s.ints[1] = 0;
-              s.value = 0.0;
-            }
-            __syncthreads();
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-            {
-              const int i = i0 + e;
-              if (i < n && taken + i < most && (before < need || taken + i == 0) && w[e] >= least)
-              {
-                atomicMax(&s.ints[1], i + 1);
-              }
-              before += w[e];
-            }
-            __syncthreads();
-            const int kept = s.ints[1];
-            before = weight + (upto - (w[0] + w[1]));
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-            {
-              before += w[e];
-              if (i0 + e == kept - 1)
-              {
-                s.value = before;
-              }
-            }
-            __syncthreads();
-            *sum = kept > 0 ? s.value : weight;
-            const unsigned long long rank = kept > 0 ? s.list[kept - 1] : hi == ~0ull ? ~0ull : hi + 1;
-            __syncthreads();
-            return rank;
-          }
-          // Too many: 256 equal ranges of [lo, hi], and the one with the border.
-          narrow(b, end, most, need, least, lo, hi, taken, weight);
-        }
-      }
-
-      __device__ void narrow(int b, int end, long long most, double need, double least,
-                             unsigned long long &lo, unsigned long long &hi, long long &taken,
-                             double &weight) const
-      {
-        // The ranks there are.
+        const unsigned long long step = (hi - lo) / kRowThreads + 1;
+        s.bins[threadIdx.x] = 0;
+        s.bin_counts[threadIdx.x] = 0;
         if (threadIdx.x == 0)
         {
-          s.bins[0] = ~0ull;
-          s.bins[1] = 0;
+          s.ints[1] = kRowThreads - 1;
         }
         __syncthreads();
-        each(b, end, [&](unsigned long long rank, float) {
-          if (rank >= lo && rank <= hi)
-          {
-            atomicMin(&s.bins[0], rank);
-            atomicMax(&s.bins[1], rank);
-          }
-        });
-        __syncthreads();
-        lo = s.bins[0];
-        hi = s.bins[1];
-        __syncthreads();
-        // (hi > lo: ranks differ, and there are many.)
-        const unsigned long long step = (hi - lo) / 256 + 1;
-        for (int i = threadIdx.x; i < 256; i += kRowThreads)
-        {
-          s.bins[i] = 0;
-        }
-        // Weights as whole numbers again; 2^20 of at most 2^38 stay below 2^58.
-        __shared__ int s_counts[256];
-        for (int i = threadIdx.x; i < 256; i += kRowThreads)
-        {
-          s_counts[i] = 0;
-        }
-        __syncthreads();
-        each(b, end, [&](unsigned long long rank, float l) {
+        source([&](unsigned long long rank, float l) {
           if (rank >= lo && rank <= hi)
           {
             const int bin = static_cast<int>((hi - rank) / step);
-            atomicAdd(&s_counts[bin], 1);
+            atomicAdd(&s.bin_counts[bin], 1);
+            // (2^20 of at most 2^38 stay below 2^58.)
             atomicAdd(&s.bins[bin],
                       static_cast<unsigned long long>(rint(weight_of(l, top, inv_t) * kUnit)));
           }
         });
         __syncthreads();
-        // The bin with the border: the first that cannot be kept whole.
-        int bin = 0;
-        for (; bin < 255; ++bin)
+        const int bin = threadIdx.x;
+        const int mine = s.bin_counts[bin];
+        const double own = static_cast<double>(s.bins[bin]) / kUnit;
+        const int count = scan(mine, s.int_waves);
+        const double sum = scan(own, s.waves);
+        // The first bin that cannot be kept whole has the border. (The least
+        // rank a bin may hold weighs too little: none after it can weigh enough.)
+        const unsigned long long end = step * (bin + 1) - 1;
+        const unsigned long long last = hi - lo < end ? lo : hi - end;
+        if (taken + count >= most || (taken + count > 0 && weight + sum >= need) ||
+            weight_of(logit_of(last), top, inv_t) < least)
         {
-          const long long with = taken + s_counts[bin];
-          const double sum = weight + static_cast<double>(s.bins[bin]) / kUnit;
-          // Its last logit's rank is at least hi - step (bin + 1) + 1: none weighs less.
-          const unsigned long long last = hi - lo < step * (bin + 1) - 1 ? lo : hi - (step * (bin + 1) - 1);
-          if (with >= most || sum >= need || weight_of(logit_of(last), top, inv_t) < least)
-          {
-            break;
-          }
-          taken = with;
-          weight = sum;
+          atomicMin(&s.ints[1], bin);
         }
-        const unsigned long long above = hi - step * bin;
+        __syncthreads();
+        const int at = s.ints[1];
+        if (bin == at)
+        {
+          s.ints[0] = count - mine;
+          s.ints[2] = mine;
+          s.value = sum - own;
+        }
+        __syncthreads();
+        taken += s.ints[0];
+        weight += s.value;
+        const unsigned long long above = hi - step * at;
         lo = above - lo < step ? lo : above - (step - 1);
         hi = above;
+        const int in = s.ints[2];
         __syncthreads();
+        return in;
+      }
+
+      // The border among the logits of buckets [b, end), of which the first are
+      // kept: as long as they are fewer than `most`, the weights before them
+      // less than `need`, and they weigh `least`; one at least if `need` is not
+      // more than nothing. Returns the rank of the last kept (all ones: none
+      // is), and to *sum the weights of the kept.
+      __device__ unsigned long long cut(int b, int end, long long most, double need, double least,
+                                        double *sum)
+      {
+        const unsigned key_lo = first_key(highest - end + 1);
+        const unsigned key_hi = b == 0 ? static_cast<unsigned>(rank_of(top, 0) >> 32)
+                                       : first_key(highest - b + 1) - 1;
+        const float from = logit_of(static_cast<unsigned long long>(key_lo) << 32);
+        const float to = logit_of(static_cast<unsigned long long>(key_hi) << 32);
+        unsigned long long lo = static_cast<unsigned long long>(key_lo) << 32;
+        unsigned long long hi = static_cast<unsigned long long>(key_hi) << 32 | 0xFFFFFFFFull;
+        long long taken = 0;
+        double weight = 0.0;
+        int n = s.count[end - 1] - (b > 0 ? s.count[b - 1] : 0);
+        const auto row = [&](auto &&f) { each(b, end, from, to, f); };
+        const bool whole = n <= kList && end == b + 1;
+        if (!(whole && held == b))
+        {
+          held = -1;
+          while (n > kList)
+          {
+            n = narrow(row, most, need, least, lo, hi, taken, weight);
+          }
+          if (threadIdx.x == 0)
+          {
+            s.listed = 0;
+          }
+          row([&](unsigned long long rank, float) {
+            if (rank >= lo && rank <= hi)
+            {
+              s.list[atomicAdd(&s.listed, 1)] = rank;
+            }
+          });
+          held = whole ? b : -1;
+          __syncthreads();
+        }
+        const int listed = s.listed;
+        const auto list = [&](auto &&f) {
+          for (int i = threadIdx.x; i < listed; i += kRowThreads)
+          {
+            f(s.list[i], logit_of(s.list[i]));
+          }
+        };
+        while (n > kFew)
+        {
+          n = narrow(list, most, need, least, lo, hi, taken, weight);
+        }
+        // The few in order, by each one's place among them.
+        if (threadIdx.x == 0)
+        {
+          s.ints[0] = 0;
+          s.ints[1] = 0;
+          s.value = weight;
+          s.rank = hi == ~0ull ? hi : hi + 1; // none of them: what ranks above
+        }
+        __syncthreads();
+        list([&](unsigned long long rank, float) {
+          if (rank >= lo && rank <= hi)
+          {
+            s.bins[atomicAdd(&s.ints[0], 1)] = rank;
+          }
+        });
+        __syncthreads();
+        if (threadIdx.x < 64)
+        {
+          const int lane = threadIdx.x;
+          const unsigned long long own = lane < n ? s.bins[lane] : 0;
+          int place = 0;
+          for (int i = 0; i < n; ++i)
+          {
+            place += s.bins[i] > own ? 1 : 0;
+          }
+          if (lane < n)
+          {
+            s.few[place] = own;
+          }
+        }
+        __syncthreads();
+        const int i = threadIdx.x;
+        const double w = i < n ? weight_of(logit_of(s.few[min(i, kFew - 1)]), top, inv_t) : 0.0;
+        const double upto = weight + scan(w, s.waves);
+        if (i < n && taken + i < most && (upto - w < need || taken + i == 0) && w >= least)
+        {
+          atomicMax(&s.ints[1], i + 1);
+        }
+        __syncthreads();
+        if (i == s.ints[1] - 1)
+        {
+          s.value = upto;
+          s.rank = s.few[i];
+        }
+        __syncthreads();
+        *sum = s.value;
+        const unsigned long long rank = s.rank;
+        __syncthreads();
+        return rank;
       }
     };
 
@@ -565,36 +593,21 @@ namespace mi
       }
       __syncthreads();
       {
-        const int bucket = threadIdx.x % kBuckets, quarter = threadIdx.x / kBuckets;
         int count = 0;
         double weight = 0.0;
 #pragma unroll 8
-        for (int p = quarter; p < a.parts; p += 4)
+        for (int p = 0; p < a.parts; ++p)
         {
-          const int of = bucket - s.shift[p];
+          const int of = static_cast<int>(threadIdx.x) - s.shift[p];
           const unsigned long long v =
               of >= 0 ? r.sums[static_cast<std::size_t>(p) * kBuckets + of] : 0;
           count += static_cast<int>(v >> kCountShift);
           weight += static_cast<double>(v & kSumMask) * s.scale[p];
         }
-        s.counts4[quarter][bucket] = count;
-        s.weights4[quarter][bucket] = weight;
-      }
-      __syncthreads();
-      {
-        const int b = threadIdx.x % kBuckets;
-        const bool mine = threadIdx.x < kBuckets;
-        const int count = mine ? s.counts4[0][b] + s.counts4[1][b] + s.counts4[2][b] + s.counts4[3][b] : 0;
-        const double weight = mine ? (s.weights4[0][b] + s.weights4[1][b]) +
-                                         (s.weights4[2][b] + s.weights4[3][b])
-                                   : 0.0;
         const int count_upto = scan(count, s.int_waves);
         const double weight_upto = scan(weight, s.waves);
-        if (mine)
-        {
-          s.count[b] = count_upto;
-          s.weight[b] = weight_upto;
-        }
+        s.count[threadIdx.x] = count_upto;
+        s.weight[threadIdx.x] = weight_upto;
       }
       __syncthreads();
       // The first bucket that a condition holds for, kBuckets if none: the
@@ -605,7 +618,7 @@ namespace mi
           s.ints[0] = kBuckets;
         }
         __syncthreads();
-        if (threadIdx.x < kBuckets && holds(static_cast<int>(threadIdx.x)))
+        if (holds(static_cast<int>(threadIdx.x)))
         {
           atomicMin(&s.ints[0], static_cast<int>(threadIdx.x));
         }
@@ -670,49 +683,71 @@ namespace mi
       // Each part's kept weights: those of the buckets before the border's, a
       // wave a part, and the border's own by their ranks.
       const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-      for (int q = wave; q < a.parts; q += kRowThreads / 64)
+      const double *whole = a.whole + static_cast<std::size_t>(row) * a.parts;
+      if (border.bucket >= kBuckets)
       {
-        double kept = 0.0;
-#pragma unroll
-        for (int c = 0; c < kBuckets / 64; ++c)
+        for (int q = threadIdx.x; q < a.parts; q += kRowThreads)
         {
-          const int of = lane + 64 * c;
-          const unsigned long long v = of + s.shift[q] < border.bucket
-                                           ? r.sums[static_cast<std::size_t>(q) * kBuckets + of]
-                                           : 0;
-          kept += static_cast<double>(v & kSumMask);
-        }
-#pragma unroll
-        for (int offset = 1; offset < 64; offset *= 2)
-        {
-          kept += __shfl_xor(kept, offset);
-        }
-        if (lane == 0)
-        {
-          s.kept[q] = kept * s.scale[q];
+          s.kept[q] = s.shift[q] < kBuckets ? whole[q] * s.scale[q] : 0.0;
+          s.border[q] = 0;
         }
       }
-      __shared__ unsigned long long s_border[kMostParts];
-      for (int q = threadIdx.x; q < a.parts; q += kRowThreads)
+      else
       {
-        s_border[q] = 0;
-      }
-      __syncthreads();
-      if (border.bucket < kBuckets)
-      {
-        r.each(border.bucket, border.bucket + 1, [&](unsigned long long rank, float l) {
+        for (int q = threadIdx.x; q < a.parts; q += kRowThreads)
+        {
+          s.border[q] = 0;
+        }
+        for (int q = wave; q < a.parts; q += kRowThreads / 64)
+        {
+          unsigned long long kept = 0;
+          const int before = border.bucket - s.shift[q];
+#pragma unroll 4
+          for (int of = lane; of < before; of += 64)
+          {
+            kept += r.sums[static_cast<std::size_t>(q) * kBuckets + of] & kSumMask;
+          }
+#pragma unroll
+          for (int offset = 1; offset < 64; offset *= 2)
+          {
+            kept += __shfl_xor(kept, offset);
+          }
+          if (lane == 0)
+          {
+            s.kept[q] = static_cast<double>(kept) * s.scale[q];
+          }
+        }
+        __syncthreads();
+        const auto add = [&](unsigned long long rank, float l) {
           if (rank >= border.rank)
           {
-            atomicAdd(&s_border[index_of(rank) / kPart],
+            atomicAdd(&s.border[index_of(rank) / kPart],
                       static_cast<unsigned long long>(rint(weight_of(l, top, inv_t) * kUnit)));
           }
-        });
+        };
+        if (r.held == border.bucket)
+        {
+          for (int i = threadIdx.x; i < s.listed; i += kRowThreads)
+          {
+            add(s.list[i], logit_of(s.list[i]));
+          }
+        }
+        else
+        {
+          // (What ranks at least the border's last, and lies in its bucket.)
+          const unsigned key_hi = border.bucket == 0
+                                      ? static_cast<unsigned>(rank_of(top, 0) >> 32)
+                                      : r.first_key(r.highest - border.bucket + 1) - 1;
+          const float to = logit_of(static_cast<unsigned long long>(key_hi) << 32);
+          const float from = border.rank == ~0ull ? INFINITY : logit_of(border.rank);
+          r.each(border.bucket, border.bucket + 1, from, to, add);
+        }
       }
       __syncthreads();
       // The part that holds the uniform's share.
       const double part_kept =
           static_cast<int>(threadIdx.x) < a.parts
-              ? s.kept[threadIdx.x] + static_cast<double>(s_border[threadIdx.x]) / kUnit
+              ? s.kept[threadIdx.x] + static_cast<double>(s.border[threadIdx.x]) / kUnit
               : 0.0;
       const double upto = scan(part_kept, s.waves);
       if (threadIdx.x == kRowThreads - 1)
@@ -810,7 +845,7 @@ namespace mi
   std::size_t sample_scratch_floats(int rows, int vocab)
   {
     check_sizes(rows, vocab);
-    return static_cast<std::size_t>(rows) * parts_of(vocab) * (2 * kBuckets + 2);
+    return static_cast<std::size_t>(rows) * parts_of(vocab) * (2 * kBuckets + 4);
   }
 
   void launch_sample(const Sampling &t, hipStream_t stream)
@@ -877,7 +912,8 @@ namespace mi
     a.parts = parts_of(t.vocab);
     const std::size_t slots = rows * a.parts;
     a.sums = static_cast<unsigned long long *>(t.scratch);
-    a.tops = reinterpret_cast<float *>(a.sums + slots * kBuckets);
+    a.whole = reinterpret_cast<double *>(a.sums + slots * kBuckets);
+    a.tops = reinterpret_cast<float *>(a.whole + slots);
     a.top_at = reinterpret_cast<int *>(a.tops + slots);
     const dim3 grid(a.parts, t.rows);
     if (t.half)
