@@ -8,16 +8,20 @@
 // the first by index whose kept weights, up to and with its own, exceed the
 // uniform's share of all kept.
 //
-// Two launches. The first (a workgroup 4,096 logits of a row) finds its part's
-// largest logit and a histogram of the others below it: buckets of a
-// thirty-second of a nat, floor(32 l / T), on one grid for the whole row, each
-// with its count and its weights' sum. The second (a workgroup a row) adds the
-// parts' up, and knows from them the bucket that each border (k, p, min-p)
-// falls into. A bucket is a range of logits: only those are looked for again, in
-// the parts that have any, and the border found among them, by histograms of
-// their ranks until 64 are left to be put in order. With the kept part of every
-// bucket known, so is the part that the token is in, whose weights are then
-// added in turn.
+// Four launches:
+//   parts   a workgroup 4,096 logits of a row: their largest, and a histogram of
+//           the others below it. Buckets of a sixteenth of a nat, floor(16 l / T),
+//           on one grid for the whole row, each with its count and its weights' sum.
+//   plan    a workgroup a row: the parts' histograms added up, and from them the
+//           bucket that each border (k, p, min-p) falls into, or the few it may.
+//   gather  a workgroup a part: the logits of those buckets, which are ranges of
+//           logits, into the row's list; its kept weights before them.
+//   choose  a workgroup a row: the borders, found in the list by histograms of its
+//           logits' places in the order until 64 are left to be put in order; with
+//           them each part's kept weights, the part that the token is in, and the
+//           token, by its weights in turn.
+// (One launch for the last three reads the row again by one CU: 27 us for a row
+// of 151,936 with 3,000 logits in a border's bucket.)
 //
 // Sums: a bucket's weights are added as whole numbers of 2^-38 of the part's
 // largest, by LDS atomics of 64 bits (13 of them the count), so that the order
@@ -28,6 +32,7 @@
 
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 namespace mi
 {
@@ -38,10 +43,10 @@ namespace mi
 
     constexpr int kPart = 4096;   // logits a part
     constexpr int kThreads = 256; // of a part's workgroup
-    constexpr int kBuckets = 1024; // 32 nats below the largest
-    constexpr int kPerNat = 32;
-    constexpr int kRowThreads = 1024; // a bucket each
-    constexpr int kList = 2048;       // logits of a border's bucket held in LDS
+    constexpr int kBuckets = 512; // 32 nats below the largest
+    constexpr int kPerNat = 16;
+    constexpr int kRowThreads = 512;  // a bucket each
+    constexpr int kList = 2048;       // of a row's list, held in LDS
     constexpr int kFew = 64;          // of them put in order
     constexpr int kMostVocab = 1 << 20;
     constexpr int kMostParts = kMostVocab / kPart;
@@ -53,6 +58,7 @@ namespace mi
     {
       const void *logits;
       long long stride;
+      bool aligned; // rows begin on 16 bytes
       const float *uniforms;
       const float *temperature;
       const int *top_k;
@@ -62,10 +68,18 @@ namespace mi
       int vocab;
       int parts;
       unsigned long long *sums; // [row][part][bucket] count << 51 | weights
-      double *whole;            // [row][part] the weights of them all
+      double *sure;             // [row][part] weights kept before the plan's first bucket
+      struct RowPlan *plans;    // [row]
+      unsigned long long *lists; // [row][vocab] ranks of the logits gathered
       float *tops;              // [row][part] largest logit
       int *top_at;              // and its index, or vocab
     };
+
+    // A whole number below 2^52.
+    __device__ inline double number_of(unsigned long long v)
+    {
+      return __builtin_bit_cast(double, v | __builtin_bit_cast(unsigned long long, 0x1p52)) - 0x1p52;
+    }
 
     template <bool kHalf>
     __device__ inline float logit_at(const void *row, int i)
@@ -77,6 +91,51 @@ namespace mi
       else
       {
         return static_cast<const float *>(row)[i];
+      }
+    }
+
+    // Logits a load of 16 bytes takes.
+    template <bool kHalf>
+    constexpr int kWide = kHalf ? 8 : 4;
+
+    // kWide logits from i on (a multiple of kWide), as they lie; -inf past the last.
+    template <bool kHalf>
+    __device__ inline u32x4 logits_at(const void *row, int i, int vocab, bool aligned)
+    {
+      if (aligned && i + kWide<kHalf> <= vocab)
+      {
+        return *reinterpret_cast<const u32x4 *>(static_cast<const std::uint8_t *>(row) +
+                                                static_cast<std::size_t>(i) * (16 / kWide<kHalf>));
+      }
+      unsigned v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+      {
+        if constexpr (kHalf)
+        {
+          const auto *at = static_cast<const std::uint16_t *>(row) + i + 2 * e;
+          const unsigned lo = i + 2 * e < vocab ? at[0] : 0xFC00u;
+          const unsigned hi = i + 2 * e + 1 < vocab ? at[1] : 0xFC00u;
+          v[e] = lo | hi << 16;
+        }
+        else
+        {
+          v[e] = i + e < vocab ? static_cast<const unsigned *>(row)[i + e] : 0xFF800000u;
+        }
+      }
+      return u32x4{v[0], v[1], v[2], v[3]};
+    }
+    template <bool kHalf>
+    __device__ inline float logit_in(u32x4 v, int e)
+    {
+      if constexpr (kHalf)
+      {
+        return h2f(static_cast<std::uint16_t>(v[e / 2] >> (16 * (e % 2))));
+      }
+      else
+      {
+        const unsigned bits = v[e]; // (a vector's element is no object to cast the bits of)
+        return __builtin_bit_cast(float, bits);
       }
     }
 
@@ -98,22 +157,61 @@ namespace mi
     // A logit that weighs anything.
     __device__ inline bool counts(float l) { return l > -INFINITY; }
 
-    // The bucket on the row's grid; larger for larger logits.
-    __device__ inline int on_grid(double steps)
+    // The bucket on the row's grid, floor(l steps) in fp32, with `steps` kPerNat
+    // / T: it never falls as l rises, which is all that is asked of it.
+    constexpr int kFar = 1 << 29;
+    __device__ inline int bucket_of(float l, float steps)
     {
-      constexpr double kFar = 1 << 29;
-      return static_cast<int>(fmin(fmax(floor(steps), -kFar), kFar));
+      return l == INFINITY ? 1 << 30
+                           : static_cast<int>(fminf(fmaxf(floorf(l * steps), -1.0f * kFar), 1.0f * kFar));
     }
-    __device__ inline int bucket_of(float l, double inv_t)
+    __device__ inline float steps_of(double inv_t)
     {
-      return l == INFINITY ? 1 << 30 : on_grid(kPerNat * (static_cast<double>(l) * inv_t));
+      return static_cast<float>(fmin(kPerNat * inv_t, 3e38));
+    }
+
+    // exp(x) for x <= 0 as 2^n exp(y), |y| <= ln 2 / 2, by the first N + 1 terms
+    // of exp's series: of 14, what is left out is 2^-57 of it, of 11 2^-40.
+    template <int N>
+    __device__ inline double exp_series(double y)
+    {
+      // 1 / N! .. 1 / 0!
+      constexpr double kInverse[] = {1.0, 1.0, 1.0 / 2, 1.0 / 6, 1.0 / 24, 1.0 / 120, 1.0 / 720,
+                                     1.0 / 5040, 1.0 / 40320, 1.0 / 362880, 1.0 / 3628800,
+                                     1.0 / 39916800, 1.0 / 479001600, 1.0 / 6227020800.0};
+      double p = kInverse[N];
+#pragma unroll
+      for (int i = N - 1; i >= 0; --i)
+      {
+        p = __builtin_fma(p, y, kInverse[i]);
+      }
+      return p;
+    }
+    constexpr double kLog2e = 1.4426950408889634;
+    constexpr double kLn2High = 0x1.62e42fefa38p-1, kLn2Low = 0x1.ef35793c7673p-45; // their sum ln 2
+    __device__ inline double exp_below(double x)
+    {
+      x = fmax(x, -1400.0); // (2^-1400 and less are 0)
+      const double n = rint(x * kLog2e);
+      const double y = __builtin_fma(n, -kLn2Low, __builtin_fma(n, -kLn2High, x));
+      return ldexp(exp_series<13>(y), static_cast<int>(n));
     }
 
     __device__ inline double weight_of(float l, float top, double inv_t)
     {
       return l == top          ? 1.0
              : top == INFINITY ? 0.0
-                               : exp((static_cast<double>(l) - static_cast<double>(top)) * inv_t);
+                               : exp_below((static_cast<double>(l) - static_cast<double>(top)) * inv_t);
+    }
+
+    // exp(x) as a whole number of kUnit.
+    __device__ inline unsigned long long whole_weight(double x)
+    {
+      const double t = fmax(x * kLog2e, -64.0);
+      const double n = rint(t);
+      // Added to 2^52, a number below it is rounded to a whole one, its low bits.
+      const double w = ldexp(exp_series<10>((t - n) * (kLn2High + kLn2Low)), static_cast<int>(n) + 38) + 0x1p52;
+      return __builtin_bit_cast(unsigned long long, w) & ((1ull << 52) - 1);
     }
 
     // ---- a part's histogram ---------------------------------------------------
@@ -127,16 +225,27 @@ namespace mi
       const int part = blockIdx.x, row = blockIdx.y;
       const void *logits = row_of<kHalf>(a, row);
       const int first = part * kPart;
-      const int count = min(kPart, a.vocab - first);
-      const double inv_t = inverse_temperature(a, row);
-      constexpr int kEach = kPart / kThreads;
-      float l[kEach];
-#pragma unroll
-      for (int e = 0; e < kEach; ++e)
+      constexpr int W = kWide<kHalf>, kLoads = kPart / kThreads / W;
+      float l[kLoads][W];
       {
-        const int i = e * kThreads + threadIdx.x;
-        l[e] = i < count ? logit_at<kHalf>(logits, first + i) : -INFINITY;
+        u32x4 raw[kLoads];
+#pragma unroll
+        for (int c = 0; c < kLoads; ++c)
+        {
+          raw[c] = logits_at<kHalf>(logits, first + W * (c * kThreads + static_cast<int>(threadIdx.x)),
+                                    a.vocab, a.aligned);
+        }
+#pragma unroll
+        for (int c = 0; c < kLoads; ++c)
+        {
+#pragma unroll
+          for (int e = 0; e < W; ++e)
+          {
+            l[c][e] = logit_in<kHalf>(raw[c], e);
+          }
+        }
       }
+      const double inv_t = inverse_temperature(a, row);
 #pragma unroll
       for (int b = 0; b < kBuckets; b += kThreads)
       {
@@ -146,12 +255,16 @@ namespace mi
       float top = -INFINITY;
       int at = a.vocab;
 #pragma unroll
-      for (int e = 0; e < kEach; ++e)
+      for (int c = 0; c < kLoads; ++c)
       {
-        if (l[e] > top)
+#pragma unroll
+        for (int e = 0; e < W; ++e)
         {
-          top = l[e];
-          at = first + e * kThreads + static_cast<int>(threadIdx.x);
+          if (l[c][e] > top)
+          {
+            top = l[c][e];
+            at = first + W * (c * kThreads + static_cast<int>(threadIdx.x)) + e;
+          }
         }
       }
 #pragma unroll
@@ -192,44 +305,33 @@ namespace mi
       }
       if (counts(top))
       {
-        const int highest = bucket_of(top, inv_t);
+        const float steps = steps_of(inv_t);
+        const int highest = bucket_of(top, steps);
+        const double high = static_cast<double>(top);
 #pragma unroll
-        for (int e = 0; e < kEach; ++e)
+        for (int c = 0; c < kLoads; ++c)
         {
-          if (counts(l[e]))
+#pragma unroll
+          for (int e = 0; e < W; ++e)
           {
-            const int below = highest - bucket_of(l[e], inv_t);
-            if (below < kBuckets)
+            if (counts(l[c][e]))
             {
-              const double w = weight_of(l[e], top, inv_t) * kUnit;
-              atomicAdd(&s_sums[below], (1ull << kCountShift) + static_cast<unsigned long long>(rint(w)));
+              const int below = highest - bucket_of(l[c][e], steps);
+              if (below < kBuckets)
+              {
+                // (Of an infinite largest, only its equals.)
+                const double x = l[c][e] == top ? 0.0 : (static_cast<double>(l[c][e]) - high) * inv_t;
+                atomicAdd(&s_sums[below], (1ull << kCountShift) + whole_weight(x));
+              }
             }
           }
         }
       }
       __syncthreads();
-      unsigned long long whole = 0;
 #pragma unroll
       for (int b = 0; b < kBuckets; b += kThreads)
       {
-        const unsigned long long v = s_sums[b + threadIdx.x];
-        a.sums[slot * kBuckets + b + threadIdx.x] = v;
-        whole += v & kSumMask;
-      }
-#pragma unroll
-      for (int offset = 1; offset < 64; offset *= 2)
-      {
-        whole += __shfl_xor(whole, offset);
-      }
-      __syncthreads();
-      if (threadIdx.x % 64 == 0)
-      {
-        s_sums[threadIdx.x / 64] = whole;
-      }
-      __syncthreads();
-      if (threadIdx.x == 0)
-      {
-        a.whole[slot] = static_cast<double>(s_sums[0] + s_sums[1] + s_sums[2] + s_sums[3]);
+        a.sums[slot * kBuckets + b + threadIdx.x] = s_sums[b + threadIdx.x];
       }
     }
 
@@ -252,310 +354,165 @@ namespace mi
       return static_cast<int>(~static_cast<unsigned>(rank));
     }
 
+    // v of the lane that a DPP pattern names, 0 where it names none.
+    template <int kPattern, int kRows>
+    __device__ inline int moved(int v)
+    {
+      return __builtin_amdgcn_update_dpp(0, v, kPattern, kRows, 0xF, false);
+    }
+    template <int kPattern, int kRows>
+    __device__ inline double moved(double v)
+    {
+      const auto bits = __builtin_bit_cast(unsigned long long, v);
+      const unsigned lo = moved<kPattern, kRows>(static_cast<int>(bits));
+      const unsigned hi = moved<kPattern, kRows>(static_cast<int>(bits >> 32));
+      return __builtin_bit_cast(double, static_cast<unsigned long long>(hi) << 32 | lo);
+    }
+    // Inclusive sums over a wave: within rows of 16 lanes, then the rows before.
+    template <typename T>
+    __device__ inline T wave_scan(T v)
+    {
+      v += moved<0x111, 0xF>(v); // row_shr:1, 2, 4, 8
+      v += moved<0x112, 0xF>(v);
+      v += moved<0x114, 0xF>(v);
+      v += moved<0x118, 0xF>(v);
+      v += moved<0x142, 0xA>(v); // row_bcast:15 to rows 1 and 3
+      v += moved<0x143, 0xC>(v); // row_bcast:31 to rows 2 and 3
+      return v;
+    }
     // Inclusive sums over the workgroup's threads, in thread order.
     template <typename T>
     __device__ inline T scan(T v, T *s_waves)
     {
       const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-      for (int offset = 1; offset < 64; offset *= 2)
-      {
-        const T before = __shfl_up(v, offset);
-        v = lane >= offset ? v + before : v;
-      }
+      v = wave_scan(v);
       __syncthreads(); // the last scan's sums are read
       if (lane == 63)
       {
         s_waves[wave] = v;
       }
       __syncthreads();
-      T before = 0;
-      for (int w = 0; w < wave; ++w)
-      {
-        before += s_waves[w];
-      }
-      return before + v;
+      const T before = wave_scan(lane < wave ? s_waves[lane] : T(0));
+      return v + __shfl(before, 63);
     }
 
-    struct RowState
+    // What the plan finds of a row.
+    struct RowPlan
     {
-      int count[kBuckets];      // of the row, up to and with each bucket
+      double inv_t;
+      float steps;
+      float top;   // the largest logit,
+      int highest; // and its bucket on the grid
+      int kind;
+      int k_bucket; // top_k's border's, kBuckets: none
+      int p_first;  // those that top_p's may be in, p_first > p_last: none
+      int p_last;
+      int first; // before it every bucket is kept: kBuckets where no border is
+      unsigned long long min_rank; // what min_p keeps ranks so at least
+      int min_bucket;
+      int listed; // logits gathered: those in these ranges
+      unsigned from[3]; // of top_k's bucket, top_p's, min_p's, as the upper half of
+      unsigned to[3];   // a rank; none where from > to
+      int count[kBuckets]; // of the row, up to and with each bucket
       double weight[kBuckets];
       double scale[kMostParts]; // of a part's weights in the row's
       short shift[kMostParts];  // a part's bucket 0 among the row's; kBuckets: none of it
-      short with[kMostParts];   // the parts that have logits of a border's bucket
-      double kept[kMostParts];  // a part's kept weights
-      unsigned long long border[kMostParts]; // of the border's bucket
-      unsigned long long list[kList];
-      unsigned long long bins[kRowThreads]; // histograms of ranks
-      int bin_counts[kRowThreads];
-      unsigned long long few[kFew];
-      double waves[kRowThreads / 64];
-      int int_waves[kRowThreads / 64];
-      int ints[4];
-      unsigned long long rank;
-      double value;
-      int listed;
+    };
+    enum : int
+    {
+      kChosen, // there is nothing to choose
+      kOpen,
     };
 
-    // A border: everything in buckets before `bucket` is kept, and in it what
-    // ranks at least `rank`.
-    struct Border
+    // The least logit, as the upper half of a rank, from which on a condition
+    // holds: by 64 pivots at a time.
+    template <typename F>
+    __device__ inline unsigned first_key(F &&holds)
     {
-      int bucket;
-      unsigned long long rank;
-    };
-
-    template <bool kHalf>
-    struct RowSampler
+      const unsigned lane = threadIdx.x & 63;
+      unsigned lo = 0x00800000u, hi = 0xFF800001u; // the least finite; past infinity
+      while (lo < hi)
+      {
+        const unsigned step = (hi - lo) / 64 + 1;
+        const unsigned long long at = lo + static_cast<unsigned long long>(lane) * step;
+        const bool reached = at >= hi || holds(logit_of(at << 32));
+        const int before = __popcll(~__ballot(reached));
+        const unsigned long long next = lo + static_cast<unsigned long long>(before) * step;
+        lo = before > 0 ? static_cast<unsigned>(next - step + 1) : lo;
+        hi = static_cast<unsigned>(min(next, static_cast<unsigned long long>(hi)));
+      }
+      return __builtin_amdgcn_readfirstlane(lo);
+    }
+    // The same near a logit that it should hold from: 64 of them at once.
+    template <typename F>
+    __device__ inline unsigned first_key(float near, F &&holds)
     {
-      const SampleArgs &a;
-      RowState &s;
-      const void *logits;
-      const unsigned long long *sums; // the row's histograms
-      double inv_t;
-      float top;
-      int highest;
-      int held = -1; // the bucket whose logits are all in the list
-
-      // The least logit, as the upper half of a rank, of a bucket on the grid
-      // or above: by 64 pivots at a time.
-      __device__ unsigned first_key(int bucket) const
+      if (near > -3e38f && near < 3e38f)
       {
-        const unsigned lane = threadIdx.x & 63;
-        unsigned lo = 0x00800000u, hi = 0xFF800001u; // the least finite; past infinity
-        while (lo < hi)
+        const unsigned from = static_cast<unsigned>(rank_of(near, 0) >> 32) - 32;
+        const unsigned long long reached =
+            __ballot(holds(logit_of(static_cast<unsigned long long>(from + (threadIdx.x & 63)) << 32)));
+        if ((reached & 1) == 0 && reached != 0)
         {
-          const unsigned step = (hi - lo) / 64 + 1;
-          const unsigned long long at = lo + static_cast<unsigned long long>(lane) * step;
-          const bool reached =
-              at >= hi ||
-              bucket_of(logit_of(at << 32), inv_t) >= bucket;
-          const int before = __popcll(~__ballot(reached));
-          const unsigned long long next = lo + static_cast<unsigned long long>(before) * step;
-          lo = before > 0 ? static_cast<unsigned>(next - step + 1) : lo;
-          hi = static_cast<unsigned>(min(next, static_cast<unsigned long long>(hi)));
-        }
-        return __builtin_amdgcn_readfirstlane(lo);
-      }
-
-      // Calls f(rank, logit) for the row's logits of buckets [b, end), which
-      // are those from `least` to `most`; the parts that have none are passed over.
-      template <typename F>
-      __device__ void each(int b, int end, float least, float most, F &&f) const
-      {
-        __syncthreads();
-        if (threadIdx.x == 0)
-        {
-          s.ints[3] = 0;
-        }
-        __syncthreads();
-        for (int part = threadIdx.x; part < a.parts; part += kRowThreads)
-        {
-          bool any = false;
-          for (int c = b; c < end; ++c)
-          {
-            const int of = c - s.shift[part];
-            any = any || (of >= 0 && of < kBuckets &&
-                          sums[static_cast<std::size_t>(part) * kBuckets + of] != 0);
-          }
-          if (any)
-          {
-            s.with[atomicAdd(&s.ints[3], 1)] = static_cast<short>(part);
-          }
-        }
-        __syncthreads();
-        const int all = s.ints[3] * kPart;
-#pragma unroll 4
-        for (int i = threadIdx.x; i < all; i += kRowThreads)
-        {
-          const int part = s.with[i / kPart], at = part * kPart + i % kPart;
-          const float l = at < a.vocab ? logit_at<kHalf>(logits, at) : NAN;
-          if (l >= least && l <= most)
-          {
-            f(rank_of(l, at), l);
-          }
+          return from + __ffsll(reached) - 1;
         }
       }
-
-      // Of the ranks in [lo, hi], `source` calls back with each, those above the
-      // border are counted as taken, and [lo, hi] becomes the 1,024th of it that
-      // has the border. Returns how many are in it.
-      template <typename S>
-      __device__ int narrow(S &&source, long long most, double need, double least,
-                            unsigned long long &lo, unsigned long long &hi, long long &taken,
-                            double &weight) const
-      {
-        const unsigned long long step = (hi - lo) / kRowThreads + 1;
-        s.bins[threadIdx.x] = 0;
-        s.bin_counts[threadIdx.x] = 0;
-        if (threadIdx.x == 0)
-        {
-          s.ints[1] = kRowThreads - 1;
-        }
-        __syncthreads();
-        source([&](unsigned long long rank, float l) {
-          if (rank >= lo && rank <= hi)
-          {
-            const int bin = static_cast<int>((hi - rank) / step);
-            atomicAdd(&s.bin_counts[bin], 1);
-            // (2^20 of at most 2^38 stay below 2^58.)
-            atomicAdd(&s.bins[bin],
-                      static_cast<unsigned long long>(rint(weight_of(l, top, inv_t) * kUnit)));
-          }
-        });
-        __syncthreads();
-        const int bin = threadIdx.x;
-        const int mine = s.bin_counts[bin];
-        const double own = static_cast<double>(s.bins[bin]) / kUnit;
-        const int count = scan(mine, s.int_waves);
-        const double sum = scan(own, s.waves);
-        // The first bin that cannot be kept whole has the border. (The least
-        // rank a bin may hold weighs too little: none after it can weigh enough.)
-        const unsigned long long end = step * (bin + 1) - 1;
-        const unsigned long long last = hi - lo < end ? lo : hi - end;
-        if (taken + count >= most || (taken + count > 0 && weight + sum >= need) ||
-            weight_of(logit_of(last), top, inv_t) < least)
-        {
-          atomicMin(&s.ints[1], bin);
-        }
-        __syncthreads();
-        const int at = s.ints[1];
-        if (bin == at)
-        {
-          s.ints[0] = count - mine;
-          s.ints[2] = mine;
-          s.value = sum - own;
-        }
-        __syncthreads();
-        taken += s.ints[0];
-        weight += s.value;
-        const unsigned long long above = hi - step * at;
-        lo = above - lo < step ? lo : above - (step - 1);
-        hi = above;
-        const int in = s.ints[2];
-        __syncthreads();
-        return in;
-      }
-
-      // The border among the logits of buckets [b, end), of which the first are
-      // kept: as long as they are fewer than `most`, the weights before them
-      // less than `need`, and they weigh `least`; one at least if `need` is not
-      // more than nothing. Returns the rank of the last kept (all ones: none
-      // is), and to *sum the weights of the kept.
-      __device__ unsigned long long cut(int b, int end, long long most, double need, double least,
-                                        double *sum)
-      {
-        const unsigned key_lo = first_key(highest - end + 1);
-        const unsigned key_hi = b == 0 ? static_cast<unsigned>(rank_of(top, 0) >> 32)
-                                       : first_key(highest - b + 1) - 1;
-        const float from = logit_of(static_cast<unsigned long long>(key_lo) << 32);
-        const float to = logit_of(static_cast<unsigned long long>(key_hi) << 32);
-        unsigned long long lo = static_cast<unsigned long long>(key_lo) << 32;
-        unsigned long long hi = static_cast<unsigned long long>(key_hi) << 32 | 0xFFFFFFFFull;
-        long long taken = 0;
-        double weight = 0.0;
-        int n = s.count[end - 1] - (b > 0 ? s.count[b - 1] : 0);
-        const auto row = [&](auto &&f) { each(b, end, from, to, f); };
-        const bool whole = n <= kList && end == b + 1;
-        if (!(whole && held == b))
-        {
-          held = -1;
-          while (n > kList)
-          {
-            n = narrow(row, most, need, least, lo, hi, taken, weight);
-          }
-          if (threadIdx.x == 0)
-          {
-            s.listed = 0;
-          }
-          row([&](unsigned long long rank, float) {
-            if (rank >= lo && rank <= hi)
-            {
-              s.list[atomicAdd(&s.listed, 1)] = rank;
-            }
-          });
-          held = whole ? b : -1;
-          __syncthreads();
-        }
-        const int listed = s.listed;
-        const auto list = [&](auto &&f) {
-          for (int i = threadIdx.x; i < listed; i += kRowThreads)
-          {
-            f(s.list[i], logit_of(s.list[i]));
-          }
-        };
-        while (n > kFew)
-        {
-          n = narrow(list, most, need, least, lo, hi, taken, weight);
-        }
-        // The few in order, by each one's place among them.
-        if (threadIdx.x == 0)
-        {
-          s.ints[0] = 0;
-          s.ints[1] = 0;
-          s.value = weight;
-          s.rank = hi == ~0ull ? hi : hi + 1; // none of them: what ranks above
-        }
-        __syncthreads();
-        list([&](unsigned long long rank, float) {
-          if (rank >= lo && rank <= hi)
-          {
-            s.bins[atomicAdd(&s.ints[0], 1)] = rank;
-          }
-        });
-        __syncthreads();
-        if (threadIdx.x < 64)
-        {
-          const int lane = threadIdx.x;
-          const unsigned long long own = lane < n ? s.bins[lane] : 0;
-          int place = 0;
-          for (int i = 0; i < n; ++i)
-          {
-            place += s.bins[i] > own ? 1 : 0;
-          }
-          if (lane < n)
-          {
-            s.few[place] = own;
-          }
-        }
-        __syncthreads();
-        const int i = threadIdx.x;
-        const double w = i < n ? weight_of(logit_of(s.few[min(i, kFew - 1)]), top, inv_t) : 0.0;
-        const double upto = weight + scan(w, s.waves);
-        if (i < n && taken + i < most && (upto - w < need || taken + i == 0) && w >= least)
-        {
-          atomicMax(&s.ints[1], i + 1);
-        }
-        __syncthreads();
-        if (i == s.ints[1] - 1)
-        {
-          s.value = upto;
-          s.rank = s.few[i];
-        }
-        __syncthreads();
-        *sum = s.value;
-        const unsigned long long rank = s.rank;
-        __syncthreads();
-        return rank;
-      }
-    };
-
-    template <bool kHalf>
-    __global__ void __launch_bounds__(kRowThreads) sample_rows_kernel(SampleArgs a)
+      return first_key(holds);
+    }
+    // The least and the largest logit of a bucket of the row.
+    __device__ inline unsigned least_key(const RowPlan &p, int b)
     {
-      __shared__ RowState s;
+      const int bucket = p.highest - b;
+      const float steps = p.steps;
+      return first_key(static_cast<float>(bucket) / steps,
+                       [&](float l) { return bucket_of(l, steps) >= bucket; });
+    }
+    __device__ inline unsigned most_key(const RowPlan &p, int b)
+    {
+      return b == 0 ? static_cast<unsigned>(rank_of(p.top, 0) >> 32) : least_key(p, b - 1) - 1;
+    }
+
+    // The first bucket that a condition holds for, kBuckets if none: the
+    // condition does not change back.
+    template <typename F>
+    __device__ inline int first_bucket(int *s_at, F &&holds)
+    {
+      __syncthreads();
+      if (threadIdx.x == 0)
+      {
+        *s_at = kBuckets;
+      }
+      __syncthreads();
+      if (holds(static_cast<int>(threadIdx.x)))
+      {
+        atomicMin(s_at, static_cast<int>(threadIdx.x));
+      }
+      __syncthreads();
+      return *s_at;
+    }
+
+    __global__ void __launch_bounds__(kRowThreads) sample_plan_kernel(SampleArgs a)
+    {
+      static_assert(kRowThreads == kBuckets, "a bucket a thread");
+      __shared__ double s_scale[kMostParts], s_waves[kRowThreads / 64], s_weight[kBuckets];
+      __shared__ int s_shift[kMostParts], s_int_waves[kRowThreads / 64], s_at;
+      __shared__ unsigned s_keys[7];
       const int row = blockIdx.x;
+      const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+      RowPlan &plan = a.plans[row];
       const double inv_t = inverse_temperature(a, row);
+      const int k = a.top_k != nullptr ? a.top_k[row] : 0;
+      const float p = a.top_p != nullptr ? a.top_p[row] : 1.0f;
+      const float m = a.min_p != nullptr ? a.min_p[row] : 0.0f;
       const float *tops = a.tops + static_cast<std::size_t>(row) * a.parts;
       const int *top_at = a.top_at + static_cast<std::size_t>(row) * a.parts;
       // The row's largest logit.
       float top = -INFINITY;
       int at = a.vocab;
-      for (int p = threadIdx.x & 63; p < a.parts; p += 64)
+      for (int q = threadIdx.x & 63; q < a.parts; q += 64)
       {
-        const float t = tops[p];
-        const int i = top_at[p];
+        const float t = tops[q];
+        const int i = top_at[q];
         if (t > top || (t == top && i < at))
         {
           top = t;
@@ -578,177 +535,476 @@ namespace mi
         if (threadIdx.x == 0)
         {
           a.tokens[row] = at;
+          plan.kind = kChosen;
         }
         return;
       }
-      RowSampler<kHalf> r{a, s, row_of<kHalf>(a, row),
-                          a.sums + static_cast<std::size_t>(row) * a.parts * kBuckets, inv_t, top,
-                          bucket_of(top, inv_t)};
-      for (int p = threadIdx.x; p < a.parts; p += kRowThreads)
+      RowPlan now;
+      now.inv_t = inv_t;
+      now.steps = steps_of(inv_t);
+      now.top = top;
+      now.highest = bucket_of(top, now.steps);
+      for (int q = threadIdx.x; q < a.parts; q += kRowThreads)
       {
-        const float t = tops[p];
-        const int shift = counts(t) ? r.highest - bucket_of(t, inv_t) : kBuckets;
-        s.shift[p] = static_cast<short>(min(shift, kBuckets));
-        s.scale[p] = counts(t) ? weight_of(t, top, inv_t) / kUnit : 0.0;
+        const float t = tops[q];
+        const int shift = counts(t) ? min(now.highest - bucket_of(t, now.steps), kBuckets) : kBuckets;
+        const double scale = counts(t) ? weight_of(t, top, inv_t) / kUnit : 0.0;
+        s_shift[q] = shift;
+        s_scale[q] = scale;
+        plan.shift[q] = static_cast<short>(shift);
+        plan.scale[q] = scale;
+      }
+      if (m > 0.0f && wave == kRowThreads / 64 - 1)
+      {
+        // The least logit that weighs enough for min_p, wherever it lies.
+        const double least = static_cast<double>(fminf(m, 1.0f));
+        const float near = static_cast<float>(static_cast<double>(top) + log(least) / inv_t);
+        s_keys[6] = first_key(
+            near, [&](float l) { return l >= top || weight_of(l, top, inv_t) >= least; });
       }
       __syncthreads();
+      // Twenty parts' counts asked for together.
+      const unsigned long long *sums = a.sums + static_cast<std::size_t>(row) * a.parts * kBuckets;
+      const int bucket = threadIdx.x;
+      int count = 0;
+      double weight = 0.0;
+      for (int q0 = 0; q0 < a.parts; q0 += 20)
       {
-        int count = 0;
-        double weight = 0.0;
-#pragma unroll 8
-        for (int p = 0; p < a.parts; ++p)
+        unsigned long long v[20];
+#pragma unroll
+        for (int i = 0; i < 20; ++i)
         {
-          const int of = static_cast<int>(threadIdx.x) - s.shift[p];
-          const unsigned long long v =
-              of >= 0 ? r.sums[static_cast<std::size_t>(p) * kBuckets + of] : 0;
-          count += static_cast<int>(v >> kCountShift);
-          weight += static_cast<double>(v & kSumMask) * s.scale[p];
+          const int of = q0 + i < a.parts ? bucket - s_shift[q0 + i] : -1;
+          v[i] = of >= 0 ? sums[static_cast<std::size_t>(q0 + i) * kBuckets + of] : 0;
         }
-        const int count_upto = scan(count, s.int_waves);
-        const double weight_upto = scan(weight, s.waves);
-        s.count[threadIdx.x] = count_upto;
-        s.weight[threadIdx.x] = weight_upto;
+#pragma unroll
+        for (int i = 0; i < 20; ++i)
+        {
+          count += static_cast<int>(v[i] >> kCountShift);
+          weight += number_of(v[i] & kSumMask) * s_scale[min(q0 + i, a.parts - 1)];
+        }
       }
-      __syncthreads();
-      // The first bucket that a condition holds for, kBuckets if none: the
-      // condition does not change back.
-      const auto first_bucket = [&](auto &&holds) {
-        if (threadIdx.x == 0)
-        {
-          s.ints[0] = kBuckets;
-        }
-        __syncthreads();
-        if (holds(static_cast<int>(threadIdx.x)))
-        {
-          atomicMin(&s.ints[0], static_cast<int>(threadIdx.x));
-        }
-        __syncthreads();
-        const int b = s.ints[0];
-        __syncthreads();
-        return b;
-      };
+      count = scan(count, s_int_waves);
+      weight = scan(weight, s_waves);
+      s_weight[bucket] = weight;
+      plan.count[bucket] = count;
+      plan.weight[bucket] = weight;
 
-      // The border so far: nothing left out.
-      Border border{kBuckets, 0};
-      const int k = a.top_k != nullptr ? a.top_k[row] : 0;
-      const float p = a.top_p != nullptr ? a.top_p[row] : 1.0f;
-      const float m = a.min_p != nullptr ? a.min_p[row] : 0.0f;
-      double total = s.weight[kBuckets - 1]; // of the weights kept by top_k
-      if (k > 0)
-      {
-        const int b = first_bucket([&](int i) { return s.count[i] >= k; });
-        if (b < kBuckets)
-        {
-          double kept = 0.0;
-          border.bucket = b;
-          border.rank = r.cut(b, b + 1, k - (b > 0 ? s.count[b - 1] : 0), INFINITY, 0.0, &kept);
-          total = (b > 0 ? s.weight[b - 1] : 0.0) + kept;
-        }
-      }
+      // The buckets to gather.
+      const int kb = k > 0 ? first_bucket(&s_at, [&](int) { return count >= k; }) : kBuckets;
+      now.k_bucket = kb;
+      now.p_first = kBuckets;
+      now.p_last = -1;
       if (p < 1.0f)
       {
-        const double need = static_cast<double>(fmaxf(p, 0.0f)) * total;
-        const int b = min(first_bucket([&](int i) { return s.weight[i] >= need; }),
-                          min(border.bucket, kBuckets - 1));
-        double kept = 0.0;
-        const unsigned long long rank =
-            r.cut(b, b + 1, 1ll << 40, need - (b > 0 ? s.weight[b - 1] : 0.0), 0.0, &kept);
-        if (b < border.bucket || rank > border.rank)
-        {
-          border.bucket = b;
-          border.rank = rank;
-        }
+        // top_p's share of what top_k keeps: all before its bucket, and some of
+        // that (by sums that may differ in their last places).
+        __syncthreads();
+        const double least = kb == 0 ? 0.0 : s_weight[(kb < kBuckets ? kb : kBuckets) - 1];
+        const double most = s_weight[min(kb, kBuckets - 1)];
+        const double share = static_cast<double>(fmaxf(p, 0.0f));
+        const int bound = min(kb, kBuckets - 1);
+        now.p_first = min(bound, first_bucket(&s_at, [&](int) { return weight >= share * least * (1 - 1e-9); }));
+        now.p_last = min(bound, first_bucket(&s_at, [&](int) { return weight >= share * most * (1 + 1e-9); }));
       }
+      now.min_rank = 0;
+      now.min_bucket = kBuckets;
       if (m > 0.0f)
       {
-        // The buckets that min_p's border may lie in: one, or two at an edge.
-        const double least = static_cast<double>(fminf(m, 1.0f));
-        const double edge = kPerNat * (static_cast<double>(top) * inv_t + log(least));
-        const int b = top == INFINITY ? 0 : max(r.highest - on_grid(edge + 1e-6), 0);
-        const int end = top == INFINITY ? 1 : min(max(r.highest - on_grid(edge - 1e-6), 0), kBuckets - 1) + 1;
-        if (b <= border.bucket && b < kBuckets)
+        now.min_rank = static_cast<unsigned long long>(s_keys[6]) << 32;
+        now.min_bucket = min(now.highest - bucket_of(logit_of(now.min_rank), now.steps), kBuckets);
+      }
+      now.first = min(min(kb, now.p_first), now.min_bucket);
+      // Their ranges, an end a wave (min_p's only where it may be the border).
+      const int reach = now.p_first < kBuckets ? now.p_last : kb;
+      const int from = wave % 3 == 0 ? kb : wave % 3 == 1 ? now.p_first : now.min_bucket;
+      const int to = wave % 3 == 1 ? now.p_last : from;
+      if (wave < 6)
+      {
+        const bool wanted = from < kBuckets && (wave % 3 < 2 || from <= reach);
+        s_keys[wave] = wave < 3 ? (wanted ? least_key(now, to) : 1u) : (wanted ? most_key(now, from) : 0u);
+      }
+      __syncthreads();
+      if (threadIdx.x == 0)
+      {
+        plan.inv_t = now.inv_t;
+        plan.steps = now.steps;
+        plan.top = now.top;
+        plan.highest = now.highest;
+        plan.k_bucket = now.k_bucket;
+        plan.p_first = now.p_first;
+        plan.p_last = now.p_last;
+        plan.first = now.first;
+        plan.min_rank = now.min_rank;
+        plan.min_bucket = now.min_bucket;
+        plan.listed = 0;
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
         {
-          double kept = 0.0;
-          const unsigned long long rank = r.cut(b, end, 1ll << 40, INFINITY, least, &kept);
-          // The last kept's bucket: with none kept in them, all before them are.
-          const int of = rank == ~0ull ? b : r.highest - bucket_of(logit_of(rank), inv_t);
-          if (of < border.bucket || (of == border.bucket && rank > border.rank))
-          {
-            border.bucket = of;
-            border.rank = rank;
-          }
+          plan.from[i] = s_keys[i];
+          plan.to[i] = s_keys[3 + i];
+        }
+        plan.kind = kOpen;
+      }
+    }
+
+    template <bool kHalf>
+    __global__ void __launch_bounds__(kThreads) sample_gather_kernel(SampleArgs a)
+    {
+      __shared__ double s_kept[kThreads / 64];
+      const int part = blockIdx.x, row = blockIdx.y;
+      RowPlan &plan = a.plans[row];
+      if (plan.kind == kChosen)
+      {
+        return;
+      }
+      const std::size_t slot = static_cast<std::size_t>(row) * a.parts + part;
+      // The part's weights before the plan's first bucket.
+      const int before = min(plan.first - plan.shift[part], kBuckets);
+      unsigned long long kept = 0;
+#pragma unroll
+      for (int b = 0; b < kBuckets; b += kThreads)
+      {
+        const int of = b + static_cast<int>(threadIdx.x);
+        kept += of < before ? a.sums[slot * kBuckets + of] & kSumMask : 0;
+      }
+      float from[3], to[3];
+      bool wanted = false;
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+      {
+        const bool any = plan.from[i] <= plan.to[i];
+        from[i] = any ? logit_of(static_cast<unsigned long long>(plan.from[i]) << 32) : INFINITY;
+        to[i] = any ? logit_of(static_cast<unsigned long long>(plan.to[i]) << 32) : -INFINITY;
+        wanted = wanted || a.tops[slot] >= from[i];
+      }
+      const double own = wave_scan(number_of(kept)); // (512 of at most 2^51 / 2^13)
+      if (threadIdx.x % 64 == 63)
+      {
+        s_kept[threadIdx.x / 64] = own;
+      }
+      __syncthreads();
+      if (threadIdx.x == 0)
+      {
+        a.sure[slot] = (s_kept[0] + s_kept[1] + s_kept[2] + s_kept[3]) * plan.scale[part];
+      }
+      if (!wanted)
+      {
+        return;
+      }
+      const void *logits = row_of<kHalf>(a, row);
+      constexpr int W = kWide<kHalf>, kLoads = kPart / kThreads / W;
+      const int i0 = part * kPart + W * static_cast<int>(threadIdx.x);
+      u32x4 raw[kLoads];
+#pragma unroll
+      for (int c = 0; c < kLoads; ++c)
+      {
+        raw[c] = logits_at<kHalf>(logits, i0 + W * kThreads * c, a.vocab, a.aligned);
+      }
+      unsigned found = 0;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+      {
+        const float l = logit_in<kHalf>(raw[i / W], i % W);
+        bool in = false;
+#pragma unroll
+        for (int j = 0; j < 3; ++j)
+        {
+          in = in || (l >= from[j] && l <= to[j]);
+        }
+        // (Buckets past the part's histogram are no part of any sum.)
+        in = in && plan.highest - bucket_of(l, plan.steps) - plan.shift[part] < kBuckets;
+        found |= (in ? 1u : 0u) << i;
+      }
+      if (__ballot(found != 0) == 0)
+      {
+        return;
+      }
+      // A wave's places in the list from one count.
+      const int mine = __popc(found);
+      const int upto = wave_scan(mine);
+      int at = 0;
+      if (threadIdx.x % 64 == 0)
+      {
+        at = atomicAdd(&plan.listed, __builtin_amdgcn_readlane(upto, 63));
+      }
+      at = __builtin_amdgcn_readfirstlane(at) + upto - mine;
+      unsigned long long *list = a.lists + static_cast<std::size_t>(row) * a.vocab;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+      {
+        if ((found >> i & 1) != 0)
+        {
+          list[at++] = rank_of(logit_in<kHalf>(raw[i / W], i % W), i0 + W * kThreads * (i / W) + i % W);
+        }
+      }
+    }
+
+    // The ranks of a bucket.
+    struct Ranks
+    {
+      unsigned long long lo;
+      unsigned long long hi;
+    };
+    __device__ inline Ranks ranks_of(unsigned from, unsigned to)
+    {
+      return {static_cast<unsigned long long>(from) << 32,
+              static_cast<unsigned long long>(to) << 32 | 0xFFFFFFFFull};
+    }
+    // A border: everything in buckets before `bucket` is kept, and in it what
+    // ranks at least `rank`.
+    struct Border
+    {
+      int bucket;
+      unsigned long long rank;
+      Ranks in;
+    };
+
+    struct RowState
+    {
+      unsigned long long list[kList];
+      unsigned long long bins[kRowThreads]; // histograms of ranks
+      int bin_counts[kRowThreads];
+      unsigned long long few[kFew];
+      unsigned long long border[kMostParts]; // each part's kept weights of the border's bucket
+      double waves[kRowThreads / 64];
+      int int_waves[kRowThreads / 64];
+      int ints[4];
+      unsigned long long rank;
+      double value;
+    };
+
+    struct RowSampler
+    {
+      RowState &s;
+      const RowPlan &plan;
+      const unsigned long long *list; // in LDS where it fits
+      int listed;
+
+      template <typename F>
+      __device__ void each(F &&f) const
+      {
+        for (int i = threadIdx.x; i < listed; i += kRowThreads)
+        {
+          f(list[i]);
         }
       }
 
-      // Each part's kept weights: those of the buckets before the border's, a
-      // wave a part, and the border's own by their ranks.
-      const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-      const double *whole = a.whole + static_cast<std::size_t>(row) * a.parts;
-      if (border.bucket >= kBuckets)
+      // Of the listed ranks in [lo, hi], those above the border are counted as
+      // taken, and [lo, hi] becomes the 512th of it that has the border. Returns
+      // how many are in it.
+      __device__ int narrow(long long most, double need, unsigned long long &lo,
+                            unsigned long long &hi, long long &taken, double &weight) const
       {
-        for (int q = threadIdx.x; q < a.parts; q += kRowThreads)
+        const unsigned long long step = (hi - lo) / kRowThreads + 1;
+        __syncthreads();
+        s.bins[threadIdx.x] = 0;
+        s.bin_counts[threadIdx.x] = 0;
+        if (threadIdx.x == 0)
         {
-          s.kept[q] = s.shift[q] < kBuckets ? whole[q] * s.scale[q] : 0.0;
-          s.border[q] = 0;
+          s.ints[1] = kRowThreads - 1;
         }
+        __syncthreads();
+        each([&](unsigned long long rank) {
+          if (rank >= lo && rank <= hi)
+          {
+            const int bin = static_cast<int>((hi - rank) / step);
+            atomicAdd(&s.bin_counts[bin], 1);
+            // (2^20 of at most 2^38 stay below 2^58.)
+            atomicAdd(&s.bins[bin], static_cast<unsigned long long>(rint(
+                                        weight_of(logit_of(rank), plan.top, plan.inv_t) * kUnit)));
+          }
+        });
+        __syncthreads();
+        const int bin = threadIdx.x;
+        const int mine = s.bin_counts[bin];
+        const double own = static_cast<double>(s.bins[bin]) / kUnit;
+        const int count = scan(mine, s.int_waves);
+        const double sum = scan(own, s.waves);
+        // The first bin that cannot be kept whole has the border.
+        if (taken + count >= most || (taken + count > 0 && weight + sum >= need))
+        {
+          atomicMin(&s.ints[1], bin);
+        }
+        __syncthreads();
+        const int at = s.ints[1];
+        if (bin == at)
+        {
+          s.ints[0] = count - mine;
+          s.ints[2] = mine;
+          s.value = sum - own;
+        }
+        __syncthreads();
+        taken += s.ints[0];
+        weight += s.value;
+        const unsigned long long above = hi - step * at;
+        lo = above - lo < step ? lo : above - (step - 1);
+        hi = above;
+        return s.ints[2];
       }
-      else
+
+      // The border among the logits of bucket b, of which the first are kept: as
+      // long as they are fewer than `most` and the weights before them less than
+      // `need`; one at least if `need` is not more than nothing. Returns the rank
+      // of the last kept (where none is, the one above the first), and to *sum
+      // the weights of the kept.
+      __device__ unsigned long long cut(int b, Ranks in, long long most, double need, double *sum) const
       {
-        for (int q = threadIdx.x; q < a.parts; q += kRowThreads)
+        unsigned long long lo = in.lo, hi = in.hi;
+        long long taken = 0;
+        double weight = 0.0;
+        int n = plan.count[b] - (b > 0 ? plan.count[b - 1] : 0);
+        while (n > kFew)
         {
-          s.border[q] = 0;
+          n = narrow(most, need, lo, hi, taken, weight);
         }
-        for (int q = wave; q < a.parts; q += kRowThreads / 64)
+        // The few in order, by each one's place among them.
+        __syncthreads();
+        if (threadIdx.x == 0)
         {
-          unsigned long long kept = 0;
-          const int before = border.bucket - s.shift[q];
-#pragma unroll 4
-          for (int of = lane; of < before; of += 64)
+          s.ints[0] = 0;
+          s.ints[1] = 0;
+          s.value = weight;
+          s.rank = hi == ~0ull ? hi : hi + 1; // none of them: what ranks above
+        }
+        __syncthreads();
+        each([&](unsigned long long rank) {
+          if (rank >= lo && rank <= hi)
           {
-            kept += r.sums[static_cast<std::size_t>(q) * kBuckets + of] & kSumMask;
+            s.bins[min(atomicAdd(&s.ints[0], 1), kFew - 1)] = rank;
           }
-#pragma unroll
-          for (int offset = 1; offset < 64; offset *= 2)
+        });
+        __syncthreads();
+        if (threadIdx.x < 64)
+        {
+          const int lane = threadIdx.x;
+          const unsigned long long own = lane < n ? s.bins[lane] : 0;
+          int place = 0;
+          for (int i = 0; i < n; ++i)
           {
-            kept += __shfl_xor(kept, offset);
+            place += s.bins[i] > own ? 1 : 0;
           }
-          if (lane == 0)
+          if (lane < n)
           {
-            s.kept[q] = static_cast<double>(kept) * s.scale[q];
+            s.few[min(place, kFew - 1)] = own;
           }
         }
         __syncthreads();
-        const auto add = [&](unsigned long long rank, float l) {
-          if (rank >= border.rank)
-          {
-            atomicAdd(&s.border[index_of(rank) / kPart],
-                      static_cast<unsigned long long>(rint(weight_of(l, top, inv_t) * kUnit)));
-          }
-        };
-        if (r.held == border.bucket)
+        if (threadIdx.x < 64)
         {
-          for (int i = threadIdx.x; i < s.listed; i += kRowThreads)
+          const int i = threadIdx.x;
+          const double w = i < n ? weight_of(logit_of(s.few[i]), plan.top, plan.inv_t) : 0.0;
+          const double upto = weight + wave_scan(w);
+          const bool kept = i < n && taken + i < most && (upto - w < need || taken + i == 0);
+          const unsigned long long all = __ballot(kept); // a run from the first on
+          if (kept && i == __popcll(all) - 1)
           {
-            add(s.list[i], logit_of(s.list[i]));
+            s.value = upto;
+            s.rank = s.few[i];
           }
         }
-        else
+        __syncthreads();
+        *sum = s.value;
+        return s.rank;
+      }
+    };
+
+    template <bool kHalf>
+    __global__ void __launch_bounds__(kRowThreads) sample_choose_kernel(SampleArgs a)
+    {
+      __shared__ RowState s;
+      const int row = blockIdx.x;
+      const RowPlan &plan = a.plans[row];
+      if (plan.kind == kChosen)
+      {
+        return;
+      }
+      const double inv_t = plan.inv_t;
+      const float top = plan.top;
+      const unsigned long long *list = a.lists + static_cast<std::size_t>(row) * a.vocab;
+      const int listed = plan.listed;
+      if (listed <= kList)
+      {
+        for (int i = threadIdx.x; i < listed; i += kRowThreads)
         {
-          // (What ranks at least the border's last, and lies in its bucket.)
-          const unsigned key_hi = border.bucket == 0
-                                      ? static_cast<unsigned>(rank_of(top, 0) >> 32)
-                                      : r.first_key(r.highest - border.bucket + 1) - 1;
-          const float to = logit_of(static_cast<unsigned long long>(key_hi) << 32);
-          const float from = border.rank == ~0ull ? INFINITY : logit_of(border.rank);
-          r.each(border.bucket, border.bucket + 1, from, to, add);
+          s.list[i] = list[i];
         }
+        list = s.list;
+      }
+      for (int q = threadIdx.x; q < a.parts; q += kRowThreads)
+      {
+        s.border[q] = 0;
       }
       __syncthreads();
+      const RowSampler r{s, plan, list, listed};
+
+      // The border so far: nothing left out.
+      Border border{kBuckets, 0, {0, 0}};
+      double total = plan.weight[kBuckets - 1]; // of the weights kept by top_k
+      const int k = a.top_k != nullptr ? a.top_k[row] : 0;
+      const float p = a.top_p != nullptr ? a.top_p[row] : 1.0f;
+      if (plan.k_bucket < kBuckets)
+      {
+        const int b = plan.k_bucket;
+        double kept = 0.0;
+        border.bucket = b;
+        border.in = ranks_of(plan.from[0], plan.to[0]);
+        border.rank = r.cut(b, border.in, k - (b > 0 ? plan.count[b - 1] : 0), INFINITY, &kept);
+        total = (b > 0 ? plan.weight[b - 1] : 0.0) + kept;
+      }
+      if (plan.p_first <= plan.p_last)
+      {
+        const double need = static_cast<double>(fmaxf(p, 0.0f)) * total;
+        int b = plan.p_first;
+        while (b < plan.p_last && plan.weight[b] < need)
+        {
+          ++b;
+        }
+        double kept = 0.0;
+        const Ranks in = plan.p_first == plan.p_last ? ranks_of(plan.from[1], plan.to[1])
+                                                     : ranks_of(least_key(plan, b), most_key(plan, b));
+        const unsigned long long rank =
+            r.cut(b, in, 1ll << 40, need - (b > 0 ? plan.weight[b - 1] : 0.0), &kept);
+        if (b < border.bucket || rank > border.rank)
+        {
+          border = {b, rank, in};
+        }
+      }
+      if (plan.min_bucket < border.bucket ||
+          (plan.min_bucket == border.bucket && plan.min_rank > border.rank))
+      {
+        border = {plan.min_bucket, plan.min_rank, ranks_of(plan.from[2], plan.to[2])};
+      }
+
+      // Each part's kept weights: those before the plan's first bucket, those of
+      // the buckets from there to the border's, and the border's own by their ranks.
+      if (border.bucket < kBuckets)
+      {
+        const unsigned long long lo = max(border.rank, border.in.lo);
+        r.each([&](unsigned long long rank) {
+          if (rank >= lo && rank <= border.in.hi)
+          {
+            atomicAdd(&s.border[index_of(rank) / kPart],
+                      static_cast<unsigned long long>(rint(weight_of(logit_of(rank), top, inv_t) * kUnit)));
+          }
+        });
+      }
+      __syncthreads();
+      double part_kept = 0.0;
+      const int mine = threadIdx.x;
+      const int shift = mine < a.parts ? plan.shift[mine] : kBuckets;
+      if (mine < a.parts)
+      {
+        const std::size_t slot = static_cast<std::size_t>(row) * a.parts + mine;
+        unsigned long long more = 0;
+        for (int b = max(plan.first, shift); b < border.bucket; ++b)
+        {
+          more += a.sums[slot * kBuckets + (b - shift)] & kSumMask;
+        }
+        part_kept = a.sure[slot] + static_cast<double>(more) * plan.scale[mine] +
+                    static_cast<double>(s.border[mine]) / kUnit;
+      }
       // The part that holds the uniform's share.
-      const double part_kept =
-          static_cast<int>(threadIdx.x) < a.parts
-              ? s.kept[threadIdx.x] + static_cast<double>(s.border[threadIdx.x]) / kUnit
-              : 0.0;
       const double upto = scan(part_kept, s.waves);
       if (threadIdx.x == kRowThreads - 1)
       {
@@ -760,11 +1016,11 @@ namespace mi
       const double share = (uniform > 0.0f ? fmin(static_cast<double>(uniform), 1.0) : 0.0) * s.value;
       if (part_kept > 0.0 && upto - part_kept <= share)
       {
-        atomicMax(&s.ints[2], static_cast<int>(threadIdx.x));
+        atomicMax(&s.ints[2], mine);
       }
       __syncthreads();
       const int part = s.ints[2];
-      if (static_cast<int>(threadIdx.x) == part)
+      if (mine == part)
       {
         s.value = share - (upto - part_kept);
         s.ints[3] = a.vocab;
@@ -772,31 +1028,32 @@ namespace mi
       }
       __syncthreads();
       const double left = s.value;
-      // Its weights in turn, four consecutive a thread.
-      double w[4], sum = 0.0;
-      const int i0 = part * kPart + 4 * static_cast<int>(threadIdx.x);
+      // Its weights in turn, eight consecutive a thread.
+      constexpr int kEach = kPart / kRowThreads, W = kWide<kHalf>;
+      const void *logits = row_of<kHalf>(a, row);
+      const int i0 = part * kPart + kEach * mine, part_shift = plan.shift[part];
+      u32x4 raw[kEach / W];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+      for (int c = 0; c < kEach / W; ++c)
       {
-        w[e] = 0.0;
-        if (i0 + e < a.vocab)
-        {
-          const float l = logit_at<kHalf>(r.logits, i0 + e);
-          if (counts(l))
-          {
-            const int below = r.highest - bucket_of(l, inv_t);
-            const bool kept = below < border.bucket ||
-                              (below == border.bucket && rank_of(l, i0 + e) >= border.rank);
-            w[e] = kept && below - s.shift[part] < kBuckets ? weight_of(l, top, inv_t) : 0.0;
-          }
-        }
+        raw[c] = logits_at<kHalf>(logits, i0 + W * c, a.vocab, a.aligned);
+      }
+      double w[kEach], sum = 0.0;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e)
+      {
+        const float l = logit_in<kHalf>(raw[e / W], e % W);
+        const int below = plan.highest - bucket_of(l, plan.steps);
+        const bool kept = counts(l) && below - part_shift < kBuckets &&
+                          (below < border.bucket ||
+                           (below == border.bucket && rank_of(l, i0 + e) >= border.rank));
+        w[e] = kept ? weight_of(l, top, inv_t) : 0.0;
         sum += w[e];
       }
-      const double all = scan(sum, s.waves);
-      double before = all - sum;
+      double before = scan(sum, s.waves) - sum;
       int found = a.vocab, last = -1;
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+      for (int e = 0; e < kEach; ++e)
       {
         before += w[e];
         if (w[e] > 0.0)
@@ -845,7 +1102,9 @@ namespace mi
   std::size_t sample_scratch_floats(int rows, int vocab)
   {
     check_sizes(rows, vocab);
-    return static_cast<std::size_t>(rows) * parts_of(vocab) * (2 * kBuckets + 4);
+    // In eight bytes: the list, the parts' histograms and numbers, the plan.
+    return 2 * static_cast<std::size_t>(rows) *
+           (vocab + static_cast<std::size_t>(parts_of(vocab)) * (kBuckets + 2) + sizeof(RowPlan) / 8);
   }
 
   void launch_sample(const Sampling &t, hipStream_t stream)
@@ -902,6 +1161,7 @@ namespace mi
     SampleArgs a{};
     a.logits = t.logits;
     a.stride = stride;
+    a.aligned = address(t.logits) % 16 == 0 && stride * static_cast<long long>(each) % 16 == 0;
     a.uniforms = t.uniforms;
     a.temperature = t.temperature;
     a.top_k = t.top_k;
@@ -910,22 +1170,23 @@ namespace mi
     a.tokens = t.tokens;
     a.vocab = t.vocab;
     a.parts = parts_of(t.vocab);
+    static_assert(sizeof(RowPlan) % 8 == 0, "plans lie one after another");
     const std::size_t slots = rows * a.parts;
     a.sums = static_cast<unsigned long long *>(t.scratch);
-    a.whole = reinterpret_cast<double *>(a.sums + slots * kBuckets);
-    a.tops = reinterpret_cast<float *>(a.whole + slots);
+    a.lists = a.sums + slots * kBuckets;
+    a.sure = reinterpret_cast<double *>(a.lists + rows * t.vocab);
+    a.plans = reinterpret_cast<RowPlan *>(a.sure + slots);
+    a.tops = reinterpret_cast<float *>(a.plans + rows);
     a.top_at = reinterpret_cast<int *>(a.tops + slots);
     const dim3 grid(a.parts, t.rows);
-    if (t.half)
-    {
-      sample_parts_kernel<true><<<grid, kThreads, 0, stream>>>(a);
-      sample_rows_kernel<true><<<t.rows, kRowThreads, 0, stream>>>(a);
-    }
-    else
-    {
-      sample_parts_kernel<false><<<grid, kThreads, 0, stream>>>(a);
-      sample_rows_kernel<false><<<t.rows, kRowThreads, 0, stream>>>(a);
-    }
+    const auto launch = [&](auto half) {
+      constexpr bool kHalf = decltype(half)::value;
+      sample_parts_kernel<kHalf><<<grid, kThreads, 0, stream>>>(a);
+      sample_plan_kernel<<<t.rows, kRowThreads, 0, stream>>>(a);
+      sample_gather_kernel<kHalf><<<grid, kThreads, 0, stream>>>(a);
+      sample_choose_kernel<kHalf><<<t.rows, kRowThreads, 0, stream>>>(a);
+    };
+    t.half ? launch(std::true_type{}) : launch(std::false_type{});
     hip_check(hipGetLastError(), "sample kernels");
   }
 

@@ -191,9 +191,12 @@ def test_int8_accumulate_and_quantise_refuse():
 
 # -- sampling ----------------------------------------------------------------------------
 
+SCRATCH = 1 << 16  # floats, more than three rows of 100 logits take
+
+
 def sample_args(**change):
     a = dict(logits=On(300, 0x10000, 4), uniforms=On(3, 0x20000, 4), tokens=On(3, 0x30000, 4), rows=3,
-             vocab=100, scratch=On(3 * 2052, 0x40000, 4))
+             vocab=100, scratch=On(SCRATCH, 0x40000, 4))
     a.update(change)
     return a
 
@@ -203,16 +206,16 @@ def sample_args(**change):
     (dict(logits=On(299, item=4)), "logits needs 300"), (dict(uniforms=On(2, item=4)), "uniforms needs 3"),
     (dict(tokens=On(2, item=4)), "tokens holds 2"), (dict(temperature=On(2, item=4)), "temperature holds"),
     (dict(top_k=On(2, item=4)), "top_k holds 2"), (dict(top_p=On(2, item=4)), "top_p holds 2"),
-    (dict(min_p=On(2, item=4)), "min_p holds 2"), (dict(scratch=None), "scratch needs 6156"),
-    (dict(scratch=On(6155, 0x40000, 4)), "scratch needs 6156"), (dict(stride=99), "apart"),
+    (dict(min_p=On(2, item=4)), "min_p holds 2"), (dict(scratch=None), "scratch needs"),
+    (dict(stride=99), "apart"),
     (dict(vocab=0), "a token at least"),
     (dict(vocab=(1 << 20) + 1, logits=On(1 << 30, item=4)), "1048576"),
     (dict(rows=65536, logits=On(1 << 30, item=4), uniforms=On(1 << 20, item=4),
           tokens=On(1 << 20, item=4)), "65535 rows"),
-    (dict(scratch=On(6156, 0x40008, 4)), "aligned"), (dict(logits=On(300, 0x10002, 4)), "aligned"),
+    (dict(scratch=On(SCRATCH, 0x40008, 4)), "aligned"), (dict(logits=On(300, 0x10002, 4)), "aligned"),
     (dict(top_k=On(3, 0x50002, 4)), "aligned"), (dict(tokens=On(3, 0x10000, 4)), "write over"),
     (dict(tokens=On(3, 0x20004, 4)), "write over"), (dict(top_p=On(3, 0x30008, 4)), "write over"),
-    (dict(scratch=On(6156, 0x10000, 4)), "write over"), (dict(scratch=On(6156, 0x30000 - 16, 4)), "lies over"),
+    (dict(scratch=On(SCRATCH, 0x10000, 4)), "write over"), (dict(scratch=On(SCRATCH, 0x30000 - 16, 4)), "lies over"),
 ])
 def test_sample_refuses(change, word):
     with pytest.raises(ValueError, match=word):
@@ -222,6 +225,10 @@ def test_sample_refuses(change, word):
 def test_sampling_scratch_grows_and_no_rows_are_done():
     d = device()
     assert d.sample_scratch(0, 1000) == 0
+    need = d.sample_scratch(3, 100)
+    assert need < SCRATCH
+    with pytest.raises(ValueError, match=f"scratch needs {need} floats; got {need - 1}"):
+        d.sample_f32(**sample_args(scratch=On(need - 1, 0x40000, 4)))
     sizes = [d.sample_scratch(3, v) for v in range(0, 60000, 511)]
     assert sizes == sorted(sizes)
     assert d.sample_scratch(4, 9000) > d.sample_scratch(3, 9000)
