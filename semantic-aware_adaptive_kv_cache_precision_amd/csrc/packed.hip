@@ -24,6 +24,7 @@
 #include <algorithm>
 #include <cmath>
 #include <string>
+#include <type_traits>
 
 namespace mi
 {
@@ -32,9 +33,11 @@ namespace mi
     using namespace attention_tiles;
 
     constexpr int kMaxSplits = 256;
+    constexpr int kFewSplits = 8; // that a lane joins by itself
     constexpr int kMfma = 0x8, kDsRead = 0x100; // instructions, to the scheduler
     constexpr int kOffsetsHeld = 4096; // offsets of each kind that LDS holds
     constexpr int kRanked = 256;       // sequences whose tiles are ranked by their keys
+    constexpr int kCus = 256;
 
     struct PackedArgs
     {
@@ -54,6 +57,8 @@ namespace mi
       int kv_heads;
       int group;
       int splits;
+      int ranked;     // whether workgroups take tiles by their keys, and so many of
+                      // the first are on the device together
       float scale;    // log2 e / sqrt(hd)
       float *part_ml; // splits > 1: [split][row] maximum and sum (row = query * heads + head),
       float *part_o;  // and hd outputs
@@ -127,7 +132,7 @@ namespace mi
     {
       const int lane = threadIdx.x & 63, G = a.group;
       int least = -1; // keys that the tile sees, if they are ranked by them
-      if (a.batch <= kRanked)
+      if (a.ranked > 0)
       {
         Sequence mine[kRanked / 64];
         int all = 0, most = 0;
@@ -255,7 +260,15 @@ namespace mi
       const int way = wave / kTiles;
       const int n = lane & 31;
       const int half = lane >> 5;
-      const int kvh = blockIdx.x % a.kv_heads, index = blockIdx.x / a.kv_heads;
+      // Of the workgroups on the device together, a CU's first, third .. come from
+      // the most keys on, its second, fourth .. the other way: 256 sums that are
+      // nearly alike (8 prompts of 12K rows: 1.11 of their mean at most, one way 1.35).
+      int block = blockIdx.x;
+      if ((block / kCus) % 2 == 1 && (block / kCus + 1) * kCus <= a.ranked)
+      {
+        block = (2 * (block / kCus) + 1) * kCus - 1 - block;
+      }
+      const int kvh = block % a.kv_heads, index = block / a.kv_heads;
       const int split = blockIdx.y;
       const int G = a.group;
 
@@ -369,9 +382,10 @@ namespace mi
       {
         copy(begin, 0);
       }
-      for (int step = begin; step < end; ++step)
-      {
-        const int buf = (step - begin) & 1;
+      // (Buffers in turn, as constants where registers allow: the places in them
+      // are then offsets of the reads' instructions.)
+      constexpr bool kInTurn = kTiles == 1 || HD == 128;
+      const auto take = [&](auto buf, int step) {
         // This step's copies have landed, and every wave is done with the other
         // buffer.
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -443,7 +457,7 @@ namespace mi
         const int key0 = step0 + way * kWayKeys;
         if (key0 > wave_hi)
         {
-          continue;
+          return;
         }
         const std::uint16_t *keys = stages + buf * kStage + way * kWayKeys * HD;
         const std::uint16_t *values = keys + kTile;
@@ -564,6 +578,19 @@ namespace mi
             }
           }
         }
+      };
+      for (int step = begin; step < end; step += kInTurn ? 2 : 1)
+      {
+        if constexpr (!kInTurn)
+        {
+          take((step - begin) & 1, step);
+          continue;
+        }
+        take(std::integral_constant<int, 0>{}, step);
+        if (step + 1 < end)
+        {
+          take(std::integral_constant<int, 1>{}, step + 1);
+        }
       }
 
       if constexpr (kWays > 1)
@@ -669,8 +696,54 @@ namespace mi
       }
     }
 
-    // The parts of a (query, head) row joined by a workgroup, its groups of
-    // lanes each taking some.
+    // The parts of a (query, head) row joined, four channels a thread.
+    template <int HD>
+    __global__ void __launch_bounds__(256) packed_join_few_kernel(PackedArgs a, std::size_t rows)
+    {
+      constexpr int kLanes = HD / 4;
+      const std::size_t i = static_cast<std::size_t>(blockIdx.x) * 256 + threadIdx.x;
+      const std::size_t row = i / kLanes;
+      const int d = 4 * static_cast<int>(i % kLanes);
+      const long long query = row / a.heads;
+      if (row >= rows || query < a.offsets_q[0] || query >= a.offsets_q[a.batch])
+      {
+        return; // of no sequence
+      }
+      float m[kFewSplits], l[kFewSplits];
+      f32x4 o[kFewSplits];
+      float top = -INFINITY;
+#pragma unroll
+      for (int s = 0; s < kFewSplits; ++s)
+      {
+        const std::size_t at = min(s, a.splits - 1) * rows + row;
+        const f32x2 ml = *reinterpret_cast<const f32x2 *>(a.part_ml + 2 * at);
+        o[s] = *reinterpret_cast<const f32x4 *>(a.part_o + at * HD + d);
+        m[s] = s < a.splits ? ml[0] : -INFINITY;
+        l[s] = ml[1];
+        top = fmaxf(top, m[s]);
+      }
+      const float from = top == -INFINITY ? 0.0f : top;
+      float sum = 0.0f;
+      f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int s = 0; s < kFewSplits; ++s)
+      {
+        if (s < a.splits)
+        {
+          const float w = __builtin_amdgcn_exp2f(m[s] - from);
+          sum += l[s] * w;
+          acc += o[s] * w;
+        }
+      }
+      const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f; // of no keys: zeros
+      const half2v x = {static_cast<_Float16>(acc[0] * inv), static_cast<_Float16>(acc[1] * inv)};
+      const half2v y = {static_cast<_Float16>(acc[2] * inv), static_cast<_Float16>(acc[3] * inv)};
+      *reinterpret_cast<u32x2 *>(a.out + row * HD + d) =
+          u32x2{__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, y)};
+    }
+
+    // The same for many parts: a workgroup a row, its groups of lanes each taking
+    // some.
     template <int HD>
     __global__ void __launch_bounds__(256) packed_join_kernel(PackedArgs a, std::size_t rows)
     {
@@ -736,7 +809,8 @@ namespace mi
       static constexpr int tiles = kTiles_, ways = kWays_, keys = kKeys_, rows = 32 * kTiles_;
     };
     using Few = Form<1, 4, 128>;
-    using Many = Form<4, 1, 64>;
+    using Many64 = Form<4, 2, 128>;
+    using Many128 = Form<4, 1, 64>;
 
     // How a launch is cut. The lengths are on the device: what is known of them
     // here is how many rows and keys there are.
@@ -756,20 +830,31 @@ namespace mi
       const long long batch = std::max(1, t.batch);
       const long long span = (t.rows_k - t.rows_q / 2 + batch - 1) / batch;
       Cut c{};
+      // Few rows over short spans: what leaves no CU two of those workgroups (at
+      // head_dim 64, whose stages leave room, four); a handful over long ones.
+      // Measured in us, few against many: 413 x 14 heads of 64 in nine chats 7.5 and
+      // 13; 256 x 12 of 128 over 2,000 keys 22.9 and 21.7; 512 x 12 of 128 over
+      // 8,192 87.6 and 54.8; 64 x 32 of 64 over 8,192 25.6 and 22.8.
       const long long few = (rows + Few::rows - 1) / Few::rows * t.kv_heads;
-      c.few = few <= (span <= 1024 && t.head_dim == 64 ? 512 : 256);
-      const int tile = c.few ? Few::rows : Many::rows;
-      const int keys = c.few ? Few::keys : Many::keys;
+      const bool narrow = t.head_dim == 64;
+      c.few = few <= (span <= 1024 && narrow ? 512 : span <= 2048 ? 256 : 32);
+      const int tile = c.few ? Few::rows : narrow ? Many64::rows : Many128::rows;
+      const int keys = c.few ? Few::keys : narrow ? Many64::keys : Many128::keys;
       c.blocks = static_cast<int>(rows / tile + std::min(t.batch, t.rows_q)); // a short tile a sequence
       c.splits = 1;
       if (may_split && c.blocks > 0)
       {
-        const long long steps = (2 * span + keys - 1) / keys;
+        // Few rows: a workgroup a CU, of two steps at least, unless the chain is as
+        // short as the join. Many: the device's workgroups, of eight steps at
+        // least, sixteen of the longer ones where they are no handful (512 x 12 of
+        // 128 over 8,192 keys: one part 153 us, four 54.8, eight 55.3; 8 x 64 over
+        // 2,000 each: one 43.9, three 26.0, eight 34; 8 x 64 x 32 of 64 over 2,000:
+        // one 29.2, two 40.5; 512 over 8,192 93.6, three 72.9).
+        const long long steps = (span + keys - 1) / keys;
         const long long groups = static_cast<long long>(c.blocks) * t.kv_heads;
-        const bool two = !c.few && t.head_dim == 128;
-        const long long fill = (two ? 512 : 256) / groups;
-        c.splits = static_cast<int>(std::max<long long>(
-            1, std::min<long long>({fill, steps < 4 ? 1 : steps / 2, two ? 4 : kMaxSplits})));
+        const long long parts = c.few ? std::min(256 / groups, steps < 4 ? 1 : steps / 2)
+                                      : std::min<long long>({512 / groups, steps / (narrow && groups >= 64 ? 16 : 8), 16});
+        c.splits = static_cast<int>(std::max<long long>(1, std::min<long long>(parts, kMaxSplits)));
       }
       return c;
     }
@@ -838,11 +923,18 @@ namespace mi
       }
       else
       {
-        launch<HD, Many>(a, c, stream);
+        launch<HD, std::conditional_t<HD == 64, Many64, Many128>>(a, c, stream);
       }
       if (c.splits > 1)
       {
         const std::size_t rows = static_cast<std::size_t>(a.rows_q) * a.heads;
+        if (c.splits <= kFewSplits)
+        {
+          const std::size_t blocks = (rows * (HD / 4) + 255) / 256;
+          packed_join_few_kernel<HD><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(a, rows);
+          hip_check(hipGetLastError(), "packed_join_few_kernel");
+          return;
+        }
         packed_join_kernel<HD><<<static_cast<unsigned>(rows), 256, 0, stream>>>(a, rows);
         hip_check(hipGetLastError(), "packed_join_kernel");
       }
@@ -948,6 +1040,10 @@ namespace mi
     a.kv_heads = t.kv_heads;
     a.group = t.heads / t.kv_heads;
     a.splits = c.splits;
+    // Where the device holds them all at once, tiles need no order.
+    const int held = 2 * kCus;
+    const long long groups = static_cast<long long>(c.blocks) * t.kv_heads;
+    a.ranked = t.batch <= kRanked && groups * c.splits > kCus ? static_cast<int>(std::min<long long>(held, groups)) : 0;
     a.scale = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(t.head_dim)));
     if (c.splits > 1)
     {
