@@ -326,21 +326,31 @@ namespace mi
     // two, takes 64 TM rows and 64 TN outputs, a wave 32 TM by 32 TN, with the
     // weight as the products' M and the rows as their N: a lane ends up with
     // four consecutive outputs of a row. Steps of 64 inputs pass through LDS,
-    // three of them, copied there directly from memory two ahead, so that a
-    // step's copies have the time of two steps' products. Piece c (16 bytes)
+    // kStages of them, copied there directly from memory, so that a step's
+    // copies have the time of kStages - 1 steps' products: two hide them under
+    // large tiles (a fourth stage costs a workgroup its place, 4,096 rows 1536
+    // -> 8960 84 -> 105 us), three under the smallest (8960 -> 1536 at 256 rows
+    // 27.8 -> 22.5). Piece c (16 bytes)
     // of row t lies at place c ^ (t / 4 % 4) of its row: sixteen lanes that
     // read a piece of sixteen rows meet no bank twice.
-    // kTail: the last step is short, and what is past it counts as zeros.
-    template <int TM, int TN, bool kHalf, bool kTail>
-    __global__ void __launch_bounds__(256, 2) int8_tiles_kernel(Int8Args a, int m_tiles, int n_tiles)
+    // Where that leaves the device workgroups too few, kGroups such sets of four
+    // waves share a tile's inputs, with stages of their own, and the first adds
+    // the others' sums up.
+    // kTail: the last step is short, or a group's steps end before the others':
+    // what is past the inputs counts as zeros.
+    template <int TM, int TN, int kGroups, int kStages, bool kHalf, bool kTail>
+    __global__ void __launch_bounds__(256 * kGroups, 2)
+        int8_tiles_kernel(Int8Args a, int m_tiles, int n_tiles)
     {
       constexpr int kM = 64 * TM, kN = 64 * TN; // a workgroup's rows and outputs
       constexpr int kStage = (kM + kN) * 64;    // bytes: rows, then the weight's
       constexpr int kCopies = kStage / 4096;    // 16-byte copies a lane a step
       constexpr int kPitch = 32 * TN * 4 + 16;  // bytes of a row of outputs in LDS
-      extern __shared__ __align__(16) std::uint8_t stages[];
-      const int lane = threadIdx.x & 63;
-      const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+      extern __shared__ __align__(16) std::uint8_t all_stages[];
+      const int lane = threadIdx.x & 63, thread = threadIdx.x % 256;
+      const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6)) % 4;
+      const int group = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x / 256));
+      std::uint8_t *stages = all_stages + group * kStages * kStage;
       // Workgroups go to the eight XCDs in turn: each XCD takes consecutive
       // tiles, columns of up to eight row tiles, so that its L2 holds the
       // rows and outputs its workgroups share.
@@ -361,17 +371,18 @@ namespace mi
 #pragma unroll
       for (int i = 0; i < kCopies; ++i)
       {
-        const int t = i * 64 + static_cast<int>(threadIdx.x) / 4;
+        const int t = i * 64 + thread / 4;
         const int r = i * 64 < kM ? min(t, a.rows - 1 - m0) : min(t - kM, a.features - 1 - n0);
         row_at[i] = static_cast<unsigned>(r) * a.in;
       }
       // The piece a lane copies: place % 4 of its row, turned by the row.
-      const int piece = (threadIdx.x % 4) ^ (threadIdx.x / 16 % 4);
-      const int steps = (a.in + 63) / 64;
+      const int piece = (thread % 4) ^ (thread / 16 % 4);
+      // The group's steps.
+      const int steps = ((a.in + 63) / 64 + kGroups - 1) / kGroups, begin = group * steps;
       const auto copy = [&](int step, int stage) {
-        // (Past the last input, of a short last step or the two after it: any
+        // (Past the last input, of a short last step or those after it: any
         // piece.)
-        const unsigned k = min(64 * step + 16 * piece, a.in - 16);
+        const unsigned k = min(64 * (begin + step) + 16 * piece, a.in - 16);
         std::uint8_t *to = stages + stage * kStage + wave * 1024;
 #pragma unroll
         for (int i = 0; i < kCopies; ++i)
@@ -401,16 +412,19 @@ namespace mi
       const int x_row = (32 * TM * wm + n) * 64;
       const int w_row = (kM + 32 * TN * wn + n) * 64;
       const int turn = n / 4 % 4;
-      copy(0, 0);
-      copy(1, 1);
+#pragma unroll
+      for (int i = 0; i < kStages - 1; ++i)
+      {
+        copy(i, i);
+      }
       int stage = 0;
       for (int step = 0; step < steps; ++step)
       {
-        // The step's copies have landed, the next one's may be on their way;
-        // every wave is done with the stage before, which the copies after
-        // those go to.
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kCopies) : "memory");
-        copy(step + 2, stage == 0 ? 2 : stage - 1);
+        // The step's copies have landed, those of the steps after it may be on
+        // their way; every wave is done with the stage before, which the next
+        // copies go to.
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kCopies * (kStages - 2)) : "memory");
+        copy(step + kStages - 1, stage == 0 ? kStages - 1 : stage - 1);
         const std::uint8_t *at = stages + stage * kStage;
         i32x4 x[2][TM], w[2][TN];
 #pragma unroll
@@ -423,7 +437,7 @@ namespace mi
             w[c][j] = *reinterpret_cast<const i32x4 *>(at + w_row + 2048 * j + place);
             if constexpr (kTail)
             {
-              w[c][j] = 64 * step + 16 * (2 * c + half) < a.in ? w[c][j] : i32x4{0, 0, 0, 0};
+              w[c][j] = 64 * (begin + step) + 16 * (2 * c + half) < a.in ? w[c][j] : i32x4{0, 0, 0, 0};
             }
           }
 #pragma unroll
@@ -445,13 +459,45 @@ namespace mi
             }
           }
         }
-        stage = stage == 2 ? 0 : stage + 1;
+        stage = stage == kStages - 1 ? 0 : stage + 1;
       }
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); // the copies past the last
 
+      __syncthreads();
+      if constexpr (kGroups > 1)
+      {
+        constexpr int kSums = 256 * 16 * TM * TN; // of a group
+        int *sums = reinterpret_cast<int *>(all_stages) + thread;
+        if (group > 0)
+        {
+          int *to = sums + (group - 1) * kSums;
+#pragma unroll
+          for (int e = 0; e < 16 * TM * TN; ++e)
+          {
+            to[256 * e] = acc[e / (16 * TM)][e / 16 % TM][e % 16];
+          }
+        }
+        __syncthreads();
+        if (group == 0)
+        {
+#pragma unroll
+          for (int g = 1; g < kGroups; ++g)
+          {
+#pragma unroll
+            for (int e = 0; e < 16 * TM * TN; ++e)
+            {
+              acc[e / (16 * TM)][e / 16 % TM][e % 16] += sums[(g - 1) * kSums + 256 * e];
+            }
+          }
+        }
+        __syncthreads(); // (the sums are read: their place is the outputs')
+        if (group > 0)
+        {
+          return;
+        }
+      }
       // 32 rows at a time through the wave's own LDS, so that outputs leave
       // eight a lane in rows.
-      __syncthreads();
       std::uint8_t *own = stages + wave * (32 * kPitch);
       constexpr int kRowLanes = 32 * TN / 8; // lanes a row
       constexpr int kRowsOnce = 64 / kRowLanes;
@@ -589,13 +635,14 @@ namespace mi
                              : want >= 4 ? rows_by<MT, 4>(a, stream) : rows_by<MT, 2>(a, stream);
     }
 
-    template <int TM, int TN, bool kHalf, bool kTail>
+    template <int TM, int TN, int kGroups, int kStages, bool kHalf, bool kTail>
     void tiles_by(const Int8Args &a, hipStream_t stream)
     {
-      constexpr std::size_t stages = 3 * (64 * TM + 64 * TN) * 64;
+      constexpr std::size_t stages = kGroups * kStages * (64 * TM + 64 * TN) * 64;
       constexpr std::size_t outs = 4 * 32 * (32 * TN * 4 + 16);
-      constexpr std::size_t lds = std::max(stages, outs);
-      auto kernel = int8_tiles_kernel<TM, TN, kHalf, kTail>;
+      constexpr std::size_t sums = (kGroups - 1) * sizeof(int) * 256 * 16 * TM * TN;
+      constexpr std::size_t lds = std::max({stages, outs, sums});
+      auto kernel = int8_tiles_kernel<TM, TN, kGroups, kStages, kHalf, kTail>;
       if constexpr (lds > 64 * 1024)
       {
         hip_check(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
@@ -605,22 +652,22 @@ namespace mi
       }
       const int m_tiles = (a.rows + 64 * TM - 1) / (64 * TM);
       const int n_tiles = (a.features + 64 * TN - 1) / (64 * TN);
-      kernel<<<static_cast<unsigned>(m_tiles) * n_tiles, 256, lds, stream>>>(a, m_tiles, n_tiles);
+      kernel<<<static_cast<unsigned>(m_tiles) * n_tiles, 256 * kGroups, lds, stream>>>(a, m_tiles, n_tiles);
       hip_check(hipGetLastError(), "int8_tiles_kernel");
     }
 
-    template <int TM, int TN>
+    template <int TM, int TN, int kGroups, int kStages>
     void tiles_as(const Int8Args &a, hipStream_t stream)
     {
-      if (a.in % 64 == 0)
+      if (a.in % (64 * kGroups) == 0)
       {
-        a.residual == nullptr ? tiles_by<TM, TN, true, false>(a, stream)
-                              : tiles_by<TM, TN, false, false>(a, stream);
+        a.residual == nullptr ? tiles_by<TM, TN, kGroups, kStages, true, false>(a, stream)
+                              : tiles_by<TM, TN, kGroups, kStages, false, false>(a, stream);
       }
       else
       {
-        a.residual == nullptr ? tiles_by<TM, TN, true, true>(a, stream)
-                              : tiles_by<TM, TN, false, true>(a, stream);
+        a.residual == nullptr ? tiles_by<TM, TN, kGroups, kStages, true, true>(a, stream)
+                              : tiles_by<TM, TN, kGroups, kStages, false, true>(a, stream);
       }
     }
 
@@ -770,27 +817,39 @@ namespace mi
     a.rows = t.rows;
     a.in = t.in;
     a.features = t.features;
-    const long long large = (t.rows + 255ll) / 256 * ((t.features + 127ll) / 128);
-    const long long small = (t.rows + 127ll) / 128 * ((t.features + 127ll) / 128);
-    if (t.rows <= 16)
+    // By the workgroups that a tile of 64 by 64 would make. Few tiles of few rows
+    // read the weight straight (us as rows and tiles: 1 row 1536 -> 8960 5.6 and
+    // 5.8, 8960 -> 1536 7.5 and 15.7, 32 rows 4096 -> 4096 8.0 and 9.8; but 24
+    // rows 2048 -> 8192 7.2 and 6.9, 16 rows 2048 -> 32000 17.5 and 14.1). As many
+    // workgroups as compute units or fewer want the smallest tile, its inputs
+    // shared by two groups (256 rows 8960 -> 1536 19.5, against 27.8 by one group
+    // and 31.4 by a tile twice as wide); then the tile grows as far as the device
+    // stays full: 64 by 128 (256 rows 1536 -> 8960 12.2, by 128 by 128 13.4;
+    // 1,000 rows 8960 -> 1536 33.3 and 43.6) also where 64 rows are all there are
+    // (60 rows 2048 -> 128256 50.4 and 54.1), 128 by 128 (2,048 rows 2048 -> 2048
+    // 15.2, by 64 by 128 17.8; 1,000 rows 1536 -> 8960 27.5 and by 128 by 256
+    // 30.7), and 128 by 256, which reads LDS least for its products (2,048 rows
+    // 2048 -> 8192 46.9 and by 128 by 128 48.9, 8192^3 583 and 685).
+    const long long tiles = (t.rows + 63ll) / 64 * ((t.features + 63ll) / 64);
+    if (t.rows <= 64 && t.rows * tiles <= 2048)
     {
-      rows_as<1>(a, stream);
+      t.rows <= 16 ? rows_as<1>(a, stream) : rows_as<2>(a, stream);
     }
-    else if (t.rows <= 32)
+    else if (tiles <= 256)
     {
-      rows_as<2>(a, stream);
+      tiles_as<1, 1, 2, 4>(a, stream);
     }
-    else if (t.rows <= 64 || small < 96)
+    else if (tiles <= 640 || t.rows <= 64)
     {
-      rows_as<4>(a, stream);
+      tiles_as<1, 2, 1, 3>(a, stream);
     }
-    else if (large >= 256)
+    else if (tiles <= 2560)
     {
-      tiles_as<4, 2>(a, stream);
+      tiles_as<2, 2, 1, 3>(a, stream);
     }
     else
     {
-      tiles_as<2, 2>(a, stream);
+      tiles_as<2, 4, 1, 3>(a, stream);
     }
   }
 

@@ -122,6 +122,16 @@ def test_many_rows(rows, n, out):
     check(rng, rows, n, out, f"{rows} x {n} -> {out}")
 
 
+@pytest.mark.parametrize("rows,n,out", [
+    (16, 128, 8256), (24, 2048, 8192), (33, 16, 8200), (64, 80, 4097), (256, 192, 1024), (70, 1536, 3000),
+    (65, 208, 16321), (60, 128, 20000), (640, 144, 4096), (700, 64, 15000), (1030, 128, 16500)])
+def test_tiles_between(rows, n, out):
+    """Between the choices of tiles: shared inputs whose last group has none, 64 rows of many outputs."""
+    rng = np.random.default_rng(rows + n)
+    announce("between", rows, n, out)
+    check(rng, rows, n, out, f"{rows} x {n} -> {out}")
+
+
 def test_sums_of_the_largest_codes():
     """-128 x -128 over the most inputs stays in 32 bits."""
     rng = np.random.default_rng(0)
