@@ -612,6 +612,10 @@ namespace mi
     }
     if (seals_)
     {
+      if (!open_pages_)
+      {
+        throw OutOfRange("no position of this cache is reserved");
+      }
       for (int page = start / page_tokens_; page < (start + n) / page_tokens_; ++page)
       {
         allocator_.locate({layer, page}); // a page that these rows complete is held
