@@ -380,20 +380,76 @@ namespace mi
       v += moved<0x143, 0xC>(v); // row_bcast:31 to rows 2 and 3
       return v;
     }
-    // Inclusive sums over the workgroup's threads, in thread order.
+    // Inclusive sums over the workgroup's threads, in thread order. (The caller
+    // has a barrier between two scans by the same s_waves.)
+    template <typename T>
+    __device__ inline T waves_before(const T *s_waves)
+    {
+      const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+      return __shfl(wave_scan(lane < wave ? s_waves[lane] : T(0)), 63);
+    }
     template <typename T>
     __device__ inline T scan(T v, T *s_waves)
     {
-      const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
       v = wave_scan(v);
-      __syncthreads(); // the last scan's sums are read
-      if (lane == 63)
+      if ((threadIdx.x & 63) == 63)
       {
-        s_waves[wave] = v;
+        s_waves[threadIdx.x >> 6] = v;
       }
       __syncthreads();
-      const T before = wave_scan(lane < wave ? s_waves[lane] : T(0));
-      return v + __shfl(before, 63);
+      return v + waves_before(s_waves);
+    }
+    __device__ inline void scan(int &count, double &sum, int *s_counts, double *s_sums)
+    {
+      count = wave_scan(count);
+      sum = wave_scan(sum);
+      if ((threadIdx.x & 63) == 63)
+      {
+        s_counts[threadIdx.x >> 6] = count;
+        s_sums[threadIdx.x >> 6] = sum;
+      }
+      __syncthreads();
+      count += waves_before(s_counts);
+      sum += waves_before(s_sums);
+    }
+
+    // The first thread of the row's workgroup that a condition holds for, `none`
+    // if none. (An LDS atomic of every thread takes 2 us: they share its address.
+    // Between two calls by the same s_waves the caller has a barrier.)
+    __device__ inline int first_of(bool holds, int none, int *s_waves)
+    {
+      const unsigned long long all = __ballot(holds);
+      if ((threadIdx.x & 63) == 0)
+      {
+        s_waves[threadIdx.x >> 6] =
+            all != 0 ? static_cast<int>(threadIdx.x) + __ffsll(all) - 1 : none;
+      }
+      __syncthreads();
+      int first = none;
+#pragma unroll
+      for (int w = kRowThreads / 64 - 1; w >= 0; --w)
+      {
+        first = s_waves[w] != none ? s_waves[w] : first;
+      }
+      return first;
+    }
+
+    // The last one, -1 if none.
+    __device__ inline int last_of(bool holds, int *s_waves)
+    {
+      const unsigned long long all = __ballot(holds);
+      if ((threadIdx.x & 63) == 0)
+      {
+        s_waves[threadIdx.x >> 6] = all != 0 ? static_cast<int>(threadIdx.x) + 63 - __clzll(all) : -1;
+      }
+      __syncthreads();
+      int last = -1;
+#pragma unroll
+      for (int w = 0; w < kRowThreads / 64; ++w)
+      {
+        last = max(last, s_waves[w]);
+      }
+      return last;
     }
 
     // What the plan finds of a row.
@@ -472,30 +528,12 @@ namespace mi
       return b == 0 ? static_cast<unsigned>(rank_of(p.top, 0) >> 32) : least_key(p, b - 1) - 1;
     }
 
-    // The first bucket that a condition holds for, kBuckets if none: the
-    // condition does not change back.
-    template <typename F>
-    __device__ inline int first_bucket(int *s_at, F &&holds)
-    {
-      __syncthreads();
-      if (threadIdx.x == 0)
-      {
-        *s_at = kBuckets;
-      }
-      __syncthreads();
-      if (holds(static_cast<int>(threadIdx.x)))
-      {
-        atomicMin(s_at, static_cast<int>(threadIdx.x));
-      }
-      __syncthreads();
-      return *s_at;
-    }
-
     __global__ void __launch_bounds__(kRowThreads) sample_plan_kernel(SampleArgs a)
     {
       static_assert(kRowThreads == kBuckets, "a bucket a thread");
       __shared__ double s_scale[kMostParts], s_waves[kRowThreads / 64], s_weight[kBuckets];
-      __shared__ int s_shift[kMostParts], s_int_waves[kRowThreads / 64], s_at;
+      __shared__ int s_shift[kMostParts], s_int_waves[kRowThreads / 64];
+      __shared__ int s_firsts[3][kRowThreads / 64];
       __shared__ unsigned s_keys[7];
       const int row = blockIdx.x;
       const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
@@ -563,35 +601,32 @@ namespace mi
             near, [&](float l) { return l >= top || weight_of(l, top, inv_t) >= least; });
       }
       __syncthreads();
-      // Twenty parts' counts asked for together.
+      // Forty parts' counts asked for together.
       const unsigned long long *sums = a.sums + static_cast<std::size_t>(row) * a.parts * kBuckets;
       const int bucket = threadIdx.x;
       int count = 0;
       double weight = 0.0;
-      for (int q0 = 0; q0 < a.parts; q0 += 20)
+      for (int q0 = 0; q0 < a.parts; q0 += 40)
       {
-        unsigned long long v[20];
+        unsigned long long v[40];
 #pragma unroll
-        for (int i = 0; i < 20; ++i)
+        for (int i = 0; i < 40; ++i)
         {
           const int of = q0 + i < a.parts ? bucket - s_shift[q0 + i] : -1;
           v[i] = of >= 0 ? sums[static_cast<std::size_t>(q0 + i) * kBuckets + of] : 0;
         }
 #pragma unroll
-        for (int i = 0; i < 20; ++i)
+        for (int i = 0; i < 40; ++i)
         {
           count += static_cast<int>(v[i] >> kCountShift);
           weight += number_of(v[i] & kSumMask) * s_scale[min(q0 + i, a.parts - 1)];
         }
       }
-      count = scan(count, s_int_waves);
-      weight = scan(weight, s_waves);
+      scan(count, weight, s_int_waves, s_waves);
       s_weight[bucket] = weight;
-      plan.count[bucket] = count;
-      plan.weight[bucket] = weight;
 
       // The buckets to gather.
-      const int kb = k > 0 ? first_bucket(&s_at, [&](int) { return count >= k; }) : kBuckets;
+      const int kb = k > 0 ? first_of(count >= k, kBuckets, s_firsts[0]) : kBuckets;
       now.k_bucket = kb;
       now.p_first = kBuckets;
       now.p_last = -1;
@@ -599,13 +634,13 @@ namespace mi
       {
         // top_p's share of what top_k keeps: all before its bucket, and some of
         // that (by sums that may differ in their last places).
-        __syncthreads();
+        __syncthreads(); // s_weight
         const double least = kb == 0 ? 0.0 : s_weight[(kb < kBuckets ? kb : kBuckets) - 1];
         const double most = s_weight[min(kb, kBuckets - 1)];
         const double share = static_cast<double>(fmaxf(p, 0.0f));
         const int bound = min(kb, kBuckets - 1);
-        now.p_first = min(bound, first_bucket(&s_at, [&](int) { return weight >= share * least * (1 - 1e-9); }));
-        now.p_last = min(bound, first_bucket(&s_at, [&](int) { return weight >= share * most * (1 + 1e-9); }));
+        now.p_first = min(bound, first_of(weight >= share * least * (1 - 1e-9), kBuckets, s_firsts[1]));
+        now.p_last = min(bound, first_of(weight >= share * most * (1 + 1e-9), kBuckets, s_firsts[2]));
       }
       now.min_rank = 0;
       now.min_bucket = kBuckets;
@@ -624,6 +659,8 @@ namespace mi
         const bool wanted = from < kBuckets && (wave % 3 < 2 || from <= reach);
         s_keys[wave] = wave < 3 ? (wanted ? least_key(now, to) : 1u) : (wanted ? most_key(now, from) : 0u);
       }
+      plan.count[bucket] = count;
+      plan.weight[bucket] = weight;
       __syncthreads();
       if (threadIdx.x == 0)
       {
@@ -654,13 +691,16 @@ namespace mi
       __shared__ double s_kept[kThreads / 64];
       const int part = blockIdx.x, row = blockIdx.y;
       RowPlan &plan = a.plans[row];
-      if (plan.kind == kChosen)
+      const std::size_t slot = static_cast<std::size_t>(row) * a.parts + part;
+      const int kind = plan.kind, shift = plan.shift[part];
+      const double scale = plan.scale[part];
+      const float part_top = a.tops[slot];
+      if (kind == kChosen)
       {
         return;
       }
-      const std::size_t slot = static_cast<std::size_t>(row) * a.parts + part;
       // The part's weights before the plan's first bucket.
-      const int before = min(plan.first - plan.shift[part], kBuckets);
+      const int before = min(plan.first - shift, kBuckets);
       unsigned long long kept = 0;
 #pragma unroll
       for (int b = 0; b < kBuckets; b += kThreads)
@@ -676,7 +716,7 @@ namespace mi
         const bool any = plan.from[i] <= plan.to[i];
         from[i] = any ? logit_of(static_cast<unsigned long long>(plan.from[i]) << 32) : INFINITY;
         to[i] = any ? logit_of(static_cast<unsigned long long>(plan.to[i]) << 32) : -INFINITY;
-        wanted = wanted || a.tops[slot] >= from[i];
+        wanted = wanted || part_top >= from[i];
       }
       const double own = wave_scan(number_of(kept)); // (512 of at most 2^51 / 2^13)
       if (threadIdx.x % 64 == 63)
@@ -686,7 +726,7 @@ namespace mi
       __syncthreads();
       if (threadIdx.x == 0)
       {
-        a.sure[slot] = (s_kept[0] + s_kept[1] + s_kept[2] + s_kept[3]) * plan.scale[part];
+        a.sure[slot] = (s_kept[0] + s_kept[1] + s_kept[2] + s_kept[3]) * scale;
       }
       if (!wanted)
       {
@@ -713,7 +753,7 @@ namespace mi
           in = in || (l >= from[j] && l <= to[j]);
         }
         // (Buckets past the part's histogram are no part of any sum.)
-        in = in && plan.highest - bucket_of(l, plan.steps) - plan.shift[part] < kBuckets;
+        in = in && plan.highest - bucket_of(l, plan.steps) - shift < kBuckets;
         found |= (in ? 1u : 0u) << i;
       }
       if (__ballot(found != 0) == 0)
@@ -769,6 +809,8 @@ namespace mi
       unsigned long long border[kMostParts]; // each part's kept weights of the border's bucket
       double waves[kRowThreads / 64];
       int int_waves[kRowThreads / 64];
+      int firsts[kRowThreads / 64];
+      int lasts[kRowThreads / 64];
       int ints[4];
       unsigned long long rank;
       double value;
@@ -800,10 +842,6 @@ namespace mi
         __syncthreads();
         s.bins[threadIdx.x] = 0;
         s.bin_counts[threadIdx.x] = 0;
-        if (threadIdx.x == 0)
-        {
-          s.ints[1] = kRowThreads - 1;
-        }
         __syncthreads();
         each([&](unsigned long long rank) {
           if (rank >= lo && rank <= hi)
@@ -819,15 +857,13 @@ namespace mi
         const int bin = threadIdx.x;
         const int mine = s.bin_counts[bin];
         const double own = static_cast<double>(s.bins[bin]) / kUnit;
-        const int count = scan(mine, s.int_waves);
-        const double sum = scan(own, s.waves);
+        int count = mine;
+        double sum = own;
+        scan(count, sum, s.int_waves, s.waves);
         // The first bin that cannot be kept whole has the border.
-        if (taken + count >= most || (taken + count > 0 && weight + sum >= need))
-        {
-          atomicMin(&s.ints[1], bin);
-        }
-        __syncthreads();
-        const int at = s.ints[1];
+        const int at = min(first_of(taken + count >= most || (taken + count > 0 && weight + sum >= need),
+                                    kRowThreads, s.firsts),
+                           kRowThreads - 1);
         if (bin == at)
         {
           s.ints[0] = count - mine;
@@ -913,19 +949,51 @@ namespace mi
     __global__ void __launch_bounds__(kRowThreads) sample_choose_kernel(SampleArgs a)
     {
       __shared__ RowState s;
+      __shared__ RowPlan plan;
       const int row = blockIdx.x;
-      const RowPlan &plan = a.plans[row];
+      const unsigned long long *list = a.lists + static_cast<std::size_t>(row) * a.vocab;
+      const int k = a.top_k != nullptr ? a.top_k[row] : 0;
+      const float p = a.top_p != nullptr ? a.top_p[row] : 1.0f;
+      const float uniform = a.uniforms[row];
+      // The plan, and the list as far as most go, asked for together.
+      {
+        constexpr int kWords = sizeof(RowPlan) / 8;
+        static_assert(sizeof(RowPlan) % 8 == 0, "in words");
+        const auto *from = reinterpret_cast<const unsigned long long *>(a.plans + row);
+        auto *to = reinterpret_cast<unsigned long long *>(&plan);
+        unsigned long long ranks[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+        {
+          const int at = i * kRowThreads + static_cast<int>(threadIdx.x);
+          ranks[i] = at < a.vocab ? list[at] : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < (kWords + kRowThreads - 1) / kRowThreads; ++i)
+        {
+          const int at = i * kRowThreads + static_cast<int>(threadIdx.x);
+          if (at < kWords)
+          {
+            to[at] = from[at];
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+        {
+          s.list[i * kRowThreads + threadIdx.x] = ranks[i];
+        }
+      }
+      __syncthreads();
       if (plan.kind == kChosen)
       {
         return;
       }
       const double inv_t = plan.inv_t;
       const float top = plan.top;
-      const unsigned long long *list = a.lists + static_cast<std::size_t>(row) * a.vocab;
       const int listed = plan.listed;
       if (listed <= kList)
       {
-        for (int i = threadIdx.x; i < listed; i += kRowThreads)
+        for (int i = 2 * kRowThreads + threadIdx.x; i < listed; i += kRowThreads)
         {
           s.list[i] = list[i];
         }
@@ -941,8 +1009,6 @@ namespace mi
       // The border so far: nothing left out.
       Border border{kBuckets, 0, {0, 0}};
       double total = plan.weight[kBuckets - 1]; // of the weights kept by top_k
-      const int k = a.top_k != nullptr ? a.top_k[row] : 0;
-      const float p = a.top_p != nullptr ? a.top_p[row] : 1.0f;
       if (plan.k_bucket < kBuckets)
       {
         const int b = plan.k_bucket;
@@ -1009,22 +1075,13 @@ namespace mi
       if (threadIdx.x == kRowThreads - 1)
       {
         s.value = upto;
-        s.ints[2] = 0;
       }
       __syncthreads();
-      const float uniform = a.uniforms[row];
       const double share = (uniform > 0.0f ? fmin(static_cast<double>(uniform), 1.0) : 0.0) * s.value;
-      if (part_kept > 0.0 && upto - part_kept <= share)
-      {
-        atomicMax(&s.ints[2], mine);
-      }
-      __syncthreads();
-      const int part = s.ints[2];
+      const int part = max(last_of(part_kept > 0.0 && upto - part_kept <= share, s.lasts), 0);
       if (mine == part)
       {
         s.value = share - (upto - part_kept);
-        s.ints[3] = a.vocab;
-        s.ints[1] = -1;
       }
       __syncthreads();
       const double left = s.value;
@@ -1065,19 +1122,12 @@ namespace mi
           }
         }
       }
-      if (found < a.vocab)
+      // (The share may pass the part's own sum by a rounding: then its last.)
+      const int by = first_of(found < a.vocab, kRowThreads, s.firsts);
+      const int end = last_of(last >= 0, s.lasts);
+      if (by < kRowThreads ? mine == by : mine == end)
       {
-        atomicMin(&s.ints[3], found);
-      }
-      if (last >= 0)
-      {
-        atomicMax(&s.ints[1], last);
-      }
-      __syncthreads();
-      if (threadIdx.x == 0)
-      {
-        // (The share may pass the part's own sum by a rounding: then its last.)
-        a.tokens[row] = s.ints[3] < a.vocab ? s.ints[3] : s.ints[1];
+        a.tokens[row] = by < kRowThreads ? found : last;
       }
     }
 
