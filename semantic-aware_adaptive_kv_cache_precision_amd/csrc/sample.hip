@@ -163,7 +163,7 @@ namespace mi
     __device__ inline int bucket_of(float l, float steps)
     {
       return l == INFINITY ? 1 << 30
-                           : static_cast<int>(fminf(fmaxf(floorf(l * steps), -1.0f * kFar), 1.0f * kFar));
+                           : static_cast<int>(__builtin_amdgcn_fmed3f(floorf(l * steps), -1.0f * kFar, 1.0f * kFar));
     }
     __device__ inline float steps_of(double inv_t)
     {
@@ -204,15 +204,48 @@ namespace mi
                                : exp_below((static_cast<double>(l) - static_cast<double>(top)) * inv_t);
     }
 
-    // exp(x) as a whole number of kUnit.
-    __device__ inline unsigned long long whole_weight(double x)
+    // A logit's entry of a histogram: one, and exp(x) as a whole number of kUnit.
+    // A double below 2^51 added to 1.5 x 2^52 is rounded to a whole one, its low
+    // bits: so n of exp(x) = 2^n 2^f, |f| <= 1/2, with which the exponent moves,
+    // and the number itself. 2^f by the polynomial of degree 8 with the least
+    // relative error, 2^-40.2, found by exchange of its extrema.
+    struct Entries
     {
-      const double t = fmax(x * kLog2e, -64.0);
-      const double n = rint(t);
-      // Added to 2^52, a number below it is rounded to a whole one, its low bits.
-      const double w = ldexp(exp_series<10>((t - n) * (kLn2High + kLn2Low)), static_cast<int>(n) + 38) + 0x1p52;
-      return __builtin_bit_cast(unsigned long long, w) & ((1ull << 52) - 1);
-    }
+      double c[9] = {0x1.ffffffffff7a3p-1,  0x1.62e42fef8615ep-1,  0x1.ebfbdff9319e1p-3,
+                     0x1.c6b08dd46d38fp-5,  0x1.3b2ab5c529251p-7,  0x1.5d87483855cbcp-10,
+                     0x1.430acca348ed9p-13, 0x1.00dad250347c9p-16, 0x1.61afceb9107ebp-20};
+      double log2e = kLog2e, least = -64.0, whole = 0x1.8p52 + 38 /* of kUnit */, one = 0x1p52;
+
+      // (In scalar registers: else every product takes its constant from two
+      // moves to vector ones.)
+      __device__ Entries()
+      {
+#pragma unroll
+        for (double &v : c)
+        {
+          asm volatile("" : "+s"(v));
+        }
+        asm volatile("" : "+s"(log2e), "+s"(least), "+s"(whole), "+s"(one));
+      }
+      __device__ unsigned long long of(double x) const
+      {
+        const double t = fmax(x * log2e, least);
+        const double m = t + whole;
+        const double f = t - (m - whole);
+        double p = __builtin_fma(c[8], f, c[7]);
+#pragma unroll
+        for (int i = 6; i >= 0; --i)
+        {
+          p = __builtin_fma(p, f, c[i]);
+        }
+        const auto n = static_cast<unsigned>(__builtin_bit_cast(unsigned long long, m)); // n + 38
+        const double w = __builtin_bit_cast(double, __builtin_bit_cast(unsigned long long, p) +
+                                                        (static_cast<unsigned long long>(n) << 52)) +
+                         one;
+        return __builtin_bit_cast(unsigned long long, w) -
+               (__builtin_bit_cast(unsigned long long, 0x1p52) - (1ull << kCountShift));
+      }
+    };
 
     // ---- a part's histogram ---------------------------------------------------
 
@@ -307,21 +340,36 @@ namespace mi
       {
         const float steps = steps_of(inv_t);
         const int highest = bucket_of(top, steps);
-        const double high = static_cast<double>(top);
+        // (Only the equals of an infinite largest are in its buckets: as the
+        // largest finite they weigh one.)
+        constexpr float kLargest = 0x1.fffffep127f;
+        const double high = static_cast<double>(fminf(top, kLargest));
+        const Entries entries;
 #pragma unroll
         for (int c = 0; c < kLoads; ++c)
         {
 #pragma unroll
-          for (int e = 0; e < W; ++e)
+          for (int e0 = 0; e0 < W; e0 += 4)
           {
-            if (counts(l[c][e]))
+            // (Four at a time, each for all lanes: their steps side by side.)
+            unsigned long long entry[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
             {
-              const int below = highest - bucket_of(l[c][e], steps);
-              if (below < kBuckets)
+              entry[e] = entries.of((static_cast<double>(fminf(l[c][e0 + e], kLargest)) - high) * inv_t);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+            {
+              asm volatile("" : "+v"(entry[e]));
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+            {
+              const int below = highest - bucket_of(l[c][e0 + e], steps);
+              if (counts(l[c][e0 + e]) && below < kBuckets)
               {
-                // (Of an infinite largest, only its equals.)
-                const double x = l[c][e] == top ? 0.0 : (static_cast<double>(l[c][e]) - high) * inv_t;
-                atomicAdd(&s_sums[below], (1ull << kCountShift) + whole_weight(x));
+                atomicAdd(&s_sums[below], entry[e]);
               }
             }
           }
