@@ -1582,10 +1582,11 @@ def _device_attention_caches(caches, seq_k, layer, q, out, heads, kv_heads, head
 def _append_rows(q, k, v, q_out, k_out, v_out, rows, heads, kv_heads, head_dim, q_stride, k_stride,
                  v_stride):
     """The addresses of appended rows and of what they go to."""
-    for value, what in ((rows, "rows"), (heads, "heads"), (kv_heads, "kv_heads"),
-                        (head_dim, "head_dim"), (q_stride, "q_stride"), (k_stride, "k_stride"),
-                        (v_stride, "v_stride")):
-        _non_negative(value, what)
+    if min(rows, heads, kv_heads, head_dim, q_stride, k_stride, v_stride) < 0:
+        for value, what in ((rows, "rows"), (heads, "heads"), (kv_heads, "kv_heads"),
+                            (head_dim, "head_dim"), (q_stride, "q_stride"), (k_stride, "k_stride"),
+                            (v_stride, "v_stride")):
+            _non_negative(value, what)
     width, q_width = kv_heads * head_dim, heads * head_dim
     return (_fp16_at(q, _strided(rows, q_stride, q_width), "q"),
             _fp16_at(k, _strided(rows, k_stride, width), "k"),
@@ -1663,9 +1664,10 @@ def _device_attention_packed(q, k, v, out, offsets_q, offsets_k, batch, rows_q, 
     contiguous). `partials` (attention_packed_partials floats) lets few rows'
     keys be split. The softmax's weights are rounded to fp16 before they meet
     the values. Rows of no sequence are left as they were."""
-    for value, what in ((batch, "batch"), (rows_q, "rows_q"), (rows_k, "rows_k"),
-                        (q_stride, "q_stride"), (k_stride, "k_stride"), (v_stride, "v_stride")):
-        _non_negative(value, what)
+    if min(batch, rows_q, rows_k, q_stride, k_stride, v_stride) < 0:
+        for value, what in ((batch, "batch"), (rows_q, "rows_q"), (rows_k, "rows_k"),
+                            (q_stride, "q_stride"), (k_stride, "k_stride"), (v_stride, "v_stride")):
+            _non_negative(value, what)
     width, q_width = kv_heads * head_dim, heads * head_dim
     qa = _fp16_at(q, _strided(rows_q, q_stride, q_width), "q")
     ka = _fp16_at(k, _strided(rows_k, k_stride, width), "k")
