@@ -325,25 +325,27 @@ namespace mi
     // Many rows: bound by the matrix cores. A workgroup of four waves, two by
     // two, takes 64 TM rows and 64 TN outputs, a wave 32 TM by 32 TN, with the
     // weight as the products' M and the rows as their N: a lane ends up with
-    // four consecutive outputs of a row. Steps of 64 inputs pass through LDS,
-    // kStages of them, copied there directly from memory, so that a step's
-    // copies have the time of kStages - 1 steps' products: two hide them under
-    // large tiles (a fourth stage costs a workgroup its place, 4,096 rows 1536
-    // -> 8960 84 -> 105 us), three under the smallest (8960 -> 1536 at 256 rows
-    // 27.8 -> 22.5). Piece c (16 bytes)
-    // of row t lies at place c ^ (t / 4 % 4) of its row: sixteen lanes that
-    // read a piece of sixteen rows meet no bank twice.
+    // four consecutive outputs of a row. Steps of 128 inputs, whole lines of
+    // memory (steps of 64 ask L2 for each line twice: 8192^3 577 us, and 507),
+    // pass through LDS, kStages of them, copied there directly: two stages where
+    // two workgroups to a CU hide the copies, three where one is alone (1,777
+    // rows 8192 -> 2048 36.8, by two 43.3). Piece c (16 bytes) of row t lies at
+    // place c ^ (t / 2 % 8) of its row: sixteen lanes that read a piece of
+    // sixteen rows meet no bank twice. A wave reads the operands of the next 32
+    // inputs while it multiplies these.
     // Where that leaves the device workgroups too few, kGroups such sets of four
     // waves share a tile's inputs, with stages of their own, and the first adds
     // the others' sums up.
     // kTail: the last step is short, or a group's steps end before the others':
     // what is past the inputs counts as zeros.
+    constexpr int kStep = 128; // inputs a step
     template <int TM, int TN, int kGroups, int kStages, bool kHalf, bool kTail>
     __global__ void __launch_bounds__(256 * kGroups, 2)
         int8_tiles_kernel(Int8Args a, int m_tiles, int n_tiles)
     {
       constexpr int kM = 64 * TM, kN = 64 * TN; // a workgroup's rows and outputs
-      constexpr int kStage = (kM + kN) * 64;    // bytes: rows, then the weight's
+      constexpr int kStage = (kM + kN) * kStep; // bytes: rows, then the weight's
+      constexpr int kPieces = kStep / 16, kCopyRows = 256 / kPieces, kSame = 256 / kStep;
       constexpr int kCopies = kStage / 4096;    // 16-byte copies a lane a step
       constexpr int kPitch = 32 * TN * 4 + 16;  // bytes of a row of outputs in LDS
       extern __shared__ __align__(16) std::uint8_t all_stages[];
@@ -371,23 +373,23 @@ namespace mi
 #pragma unroll
       for (int i = 0; i < kCopies; ++i)
       {
-        const int t = i * 64 + thread / 4;
-        const int r = i * 64 < kM ? min(t, a.rows - 1 - m0) : min(t - kM, a.features - 1 - n0);
+        const int t = i * kCopyRows + thread / kPieces;
+        const int r = i * kCopyRows < kM ? min(t, a.rows - 1 - m0) : min(t - kM, a.features - 1 - n0);
         row_at[i] = static_cast<unsigned>(r) * a.in;
       }
       // The piece a lane copies: place % 4 of its row, turned by the row.
-      const int piece = (thread % 4) ^ (thread / 16 % 4);
+      const int piece = (thread % kPieces) ^ (thread / kPieces / kSame % kPieces);
       // The group's steps.
-      const int steps = ((a.in + 63) / 64 + kGroups - 1) / kGroups, begin = group * steps;
+      const int steps = ((a.in + kStep - 1) / kStep + kGroups - 1) / kGroups, begin = group * steps;
       const auto copy = [&](int step, int stage) {
         // (Past the last input, of a short last step or those after it: any
         // piece.)
-        const unsigned k = min(64 * (begin + step) + 16 * piece, a.in - 16);
+        const unsigned k = min(kStep * (begin + step) + 16 * piece, a.in - 16);
         std::uint8_t *to = stages + stage * kStage + wave * 1024;
 #pragma unroll
         for (int i = 0; i < kCopies; ++i)
         {
-          const std::uint8_t *from = (i * 64 < kM ? x0 : w0) + (row_at[i] + k);
+          const std::uint8_t *from = (i * kCopyRows < kM ? x0 : w0) + (row_at[i] + k);
           __builtin_amdgcn_global_load_lds((global_void)from, (lds_void)(to + i * 4096), 16, 0, 0);
         }
       };
@@ -409,57 +411,72 @@ namespace mi
         }
       }
       // Where the lane's row lies in a stage, and its pieces' turn.
-      const int x_row = (32 * TM * wm + n) * 64;
-      const int w_row = (kM + 32 * TN * wn + n) * 64;
-      const int turn = n / 4 % 4;
+      const int x_row = (32 * TM * wm + n) * kStep;
+      const int w_row = (kM + 32 * TN * wn + n) * kStep;
+      const int turn = n / kSame % kPieces;
+      i32x4 x[2][TM], w[2][TN];
+      // Half c of a step's operands.
+      const auto read = [&](int c, int step, int stage) {
+        const std::uint8_t *at = stages + stage * kStage;
+        const int place = 16 * ((2 * c + half) ^ turn);
 #pragma unroll
-      for (int i = 0; i < kStages - 1; ++i)
+        for (int j = 0; j < TN; ++j)
+        {
+          i32x4 &codes = w[c % 2][j];
+          codes = *reinterpret_cast<const i32x4 *>(at + w_row + 32 * kStep * j + place);
+          if constexpr (kTail)
+          {
+            codes = kStep * (begin + step) + 16 * (2 * c + half) < a.in ? codes : i32x4{0, 0, 0, 0};
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+        {
+          x[c % 2][i] = *reinterpret_cast<const i32x4 *>(at + x_row + 32 * kStep * i + place);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      };
+      // Products [from, to) of half c.
+      const auto multiply = [&](int c, int from, int to) {
+#pragma unroll
+        for (int p = 0; p < TN * TM; ++p)
+        {
+          if (p >= from && p < to)
+          {
+            i32x16 &sums = acc[p / TM][p % TM];
+            sums = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[c % 2][p / TM], x[c % 2][p % TM], sums, 0, 0, 0);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      };
+#pragma unroll
+      for (int i = 0; i < kStages; ++i)
       {
         copy(i, i);
       }
+      asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(kCopies * (kStages - 1)) : "memory");
+      read(0, 0, 0);
       int stage = 0;
       for (int step = 0; step < steps; ++step)
       {
-        // The step's copies have landed, those of the steps after it may be on
-        // their way; every wave is done with the stage before, which the next
-        // copies go to.
+        // (Operands are asked for behind a first product: its wait for its own
+        // would be for them too.)
+#pragma unroll
+        for (int c = 0; c < kStep / 32 - 1; ++c)
+        {
+          multiply(c, 0, 1);
+          read(c + 1, step, stage);
+          multiply(c, 1, TN * TM);
+        }
+        // The next step's copies have landed, those of the steps after it may be
+        // on their way; every wave has its operands of this one, whose stage the
+        // next copies go to.
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kCopies * (kStages - 2)) : "memory");
-        copy(step + kStages - 1, stage == 0 ? kStages - 1 : stage - 1);
-        const std::uint8_t *at = stages + stage * kStage;
-        i32x4 x[2][TM], w[2][TN];
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-        {
-          const int place = 16 * ((2 * c + half) ^ turn);
-#pragma unroll
-          for (int j = 0; j < TN; ++j)
-          {
-            w[c][j] = *reinterpret_cast<const i32x4 *>(at + w_row + 2048 * j + place);
-            if constexpr (kTail)
-            {
-              w[c][j] = 64 * (begin + step) + 16 * (2 * c + half) < a.in ? w[c][j] : i32x4{0, 0, 0, 0};
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < TM; ++i)
-          {
-            x[c][i] = *reinterpret_cast<const i32x4 *>(at + x_row + 2048 * i + place);
-          }
-        }
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-        {
-#pragma unroll
-          for (int j = 0; j < TN; ++j)
-          {
-#pragma unroll
-            for (int i = 0; i < TM; ++i)
-            {
-              acc[j][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[c][j], x[c][i], acc[j][i], 0, 0, 0);
-            }
-          }
-        }
+        multiply(1, 0, 1);
+        copy(step + kStages, stage);
         stage = stage == kStages - 1 ? 0 : stage + 1;
+        read(0, step + 1, stage);
+        multiply(1, 1, TN * TM);
       }
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); // the copies past the last
 
@@ -500,7 +517,7 @@ namespace mi
       // eight a lane in rows.
       std::uint8_t *own = stages + wave * (32 * kPitch);
       constexpr int kRowLanes = 32 * TN / 8; // lanes a row
-      constexpr int kRowsOnce = 64 / kRowLanes;
+      constexpr int kRowsOnce = 64 / kRowLanes; // (of 12 lanes a row, four lanes take none)
       const int col = n0 + 32 * TN * wn + 8 * (lane % kRowLanes);
       const bool full = col + 8 <= a.features;
       const bool vector = full && a.features % 8 == 0;
@@ -528,16 +545,16 @@ namespace mi
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int p = 0; p < 32 / kRowsOnce; ++p)
+        for (int p = 0; p < (32 + kRowsOnce - 1) / kRowsOnce; ++p)
         {
           const int r = p * kRowsOnce + lane / kRowLanes;
           const int row = m0 + 32 * (TM * wm + i) + r;
-          const i32x4 lo = *reinterpret_cast<const i32x4 *>(own + r * kPitch + 32 * (lane % kRowLanes));
-          const i32x4 hi = *reinterpret_cast<const i32x4 *>(own + r * kPitch + 32 * (lane % kRowLanes) + 16);
-          if (row >= a.rows)
+          if ((64 % kRowLanes != 0 && (lane >= kRowsOnce * kRowLanes || r >= 32)) || row >= a.rows)
           {
             continue;
           }
+          const i32x4 lo = *reinterpret_cast<const i32x4 *>(own + r * kPitch + 32 * (lane % kRowLanes));
+          const i32x4 hi = *reinterpret_cast<const i32x4 *>(own + r * kPitch + 32 * (lane % kRowLanes) + 16);
           const float x_scale = a.x_scales[row];
           float y[8];
 #pragma unroll
@@ -638,7 +655,7 @@ namespace mi
     template <int TM, int TN, int kGroups, int kStages, bool kHalf, bool kTail>
     void tiles_by(const Int8Args &a, hipStream_t stream)
     {
-      constexpr std::size_t stages = kGroups * kStages * (64 * TM + 64 * TN) * 64;
+      constexpr std::size_t stages = kGroups * kStages * (64 * TM + 64 * TN) * kStep;
       constexpr std::size_t outs = 4 * 32 * (32 * TN * 4 + 16);
       constexpr std::size_t sums = (kGroups - 1) * sizeof(int) * 256 * 16 * TM * TN;
       constexpr std::size_t lds = std::max({stages, outs, sums});
@@ -659,7 +676,7 @@ namespace mi
     template <int TM, int TN, int kGroups, int kStages>
     void tiles_as(const Int8Args &a, hipStream_t stream)
     {
-      if (a.in % (64 * kGroups) == 0)
+      if (a.in % (kStep * kGroups) == 0)
       {
         a.residual == nullptr ? tiles_by<TM, TN, kGroups, kStages, true, false>(a, stream)
                               : tiles_by<TM, TN, kGroups, kStages, false, false>(a, stream);
@@ -822,14 +839,13 @@ namespace mi
     // 5.8, 8960 -> 1536 7.5 and 15.7, 32 rows 4096 -> 4096 8.0 and 9.8; but 24
     // rows 2048 -> 8192 7.2 and 6.9, 16 rows 2048 -> 32000 17.5 and 14.1). As many
     // workgroups as compute units or fewer want the smallest tile, its inputs
-    // shared by two groups (256 rows 8960 -> 1536 19.5, against 27.8 by one group
-    // and 31.4 by a tile twice as wide); then the tile grows as far as the device
-    // stays full: 64 by 128 (256 rows 1536 -> 8960 12.2, by 128 by 128 13.4;
-    // 1,000 rows 8960 -> 1536 33.3 and 43.6) also where 64 rows are all there are
-    // (60 rows 2048 -> 128256 50.4 and 54.1), 128 by 128 (2,048 rows 2048 -> 2048
-    // 15.2, by 64 by 128 17.8; 1,000 rows 1536 -> 8960 27.5 and by 128 by 256
-    // 30.7), and 128 by 256, which reads LDS least for its products (2,048 rows
-    // 2048 -> 8192 46.9 and by 128 by 128 48.9, 8192^3 583 and 685).
+    // shared by two groups (256 rows 8960 -> 1536 16.9, by 64 by 128 24.2); then
+    // the tile grows as far as it leaves every CU one: 64 by 128 (1,000 rows 8960
+    // -> 1536 26.5, by the smallest 33.1, by 128 by 128 47.2), also where 64 rows
+    // are all there are, 128 by 128 (2,048 rows 2048 -> 2048 13.9, by 64 by 128
+    // 14.3, by 128 by 192 18.3), and 128 by 192, two to a CU, which reads LDS less
+    // for its products (1,000 rows 1536 -> 8960 23.7, by 128 by 128 27.3, by 128 by
+    // 256 37; 4,096 rows 1536 -> 8960 69, 73 and 97; 8192^3 507, 554 and 615).
     const long long tiles = (t.rows + 63ll) / 64 * ((t.features + 63ll) / 64);
     if (t.rows <= 64 && t.rows * tiles <= 2048)
     {
@@ -837,19 +853,19 @@ namespace mi
     }
     else if (tiles <= 256)
     {
-      tiles_as<1, 1, 2, 4>(a, stream);
+      tiles_as<1, 1, 2, 3>(a, stream);
     }
     else if (tiles <= 640 || t.rows <= 64)
     {
       tiles_as<1, 2, 1, 3>(a, stream);
     }
-    else if (tiles <= 2560)
+    else if ((t.rows + 127ll) / 128 * ((t.features + 127ll) / 128) <= 256)
     {
       tiles_as<2, 2, 1, 3>(a, stream);
     }
     else
     {
-      tiles_as<2, 4, 1, 3>(a, stream);
+      tiles_as<2, 3, 1, 2>(a, stream);
     }
   }
 
