@@ -229,7 +229,8 @@ int mi_attention_window(const void *q, const void *k, const void *v, void *out, 
  * queries) gives zeros. Rows of no sequence are left as they were. head_dim 64
  * or 128; alignment, overlaps, the rounding of weights and values that are not
  * finite as mi_attention_window's, and so the partials, those of
- * mi_attention_packed_partials, never more than 65,536 (head_dim + 2) floats. */
+ * mi_attention_packed_partials, never more than 65,536 (head_dim + 2) floats.
+ * At most 65,535 sequences; strides of keys and values below 2^24. */
 int mi_attention_packed_partials(int batch, int rows_q, int rows_k, int heads, int kv_heads,
                                  int head_dim, size_t *floats);
 int mi_attention_packed(const void *q, const void *k, const void *v, void *out, long long q_stride,
@@ -320,13 +321,14 @@ int mi_linear_int8_accumulate(const void *x, const float *x_scales, const void *
 /* Beyond the reference (whose engine takes the greedy token, argmax.cu): a
  * token of every row of logits (rows, vocab), `stride` elements apart (0:
  * vocab), fp32 or fp16, from a given number uniforms[row] in [0, 1). Token i
- * weighs exp((l_i - max) / temperature), formed in fp64. Kept are the top_k
+ * weighs exp((l_i - max) / temperature); borders and sums hold to about 2^-30
+ * of the kept weights. Kept are the top_k
  * largest (0 or less: all); of those the fewest largest whose weights sum to
  * top_p of theirs (1 or more: all; at least one); of those the ones that weigh
  * at least min_p of the largest (0 or less: all). Of equal logits the lower
  * index is the larger. The token is the first, by index, whose kept weights up
  * to and with its own exceed the uniform's share of all kept. A weight below
- * 2^-40 of the largest is as good as none: a token of such is never chosen.
+ * 2^-39 of the largest may count as none.
  * temperature 0 or less: the largest logit. temperature, top_k, top_p, min_p
  * (rows each) are device arrays or NULL: 1, all, all, all. NaN and -inf logits
  * weigh nothing; +inf share the weight among them. A row with neither (nothing
@@ -548,7 +550,9 @@ int mi_kv_attention_batch(mi_kv_pages *const *kv, const int *seq_k, int count, i
  * `layer` (host memory, as mi_kv_store takes them, reserved before). Caches
  * that seal need k_out and v_out, which their pages are then filled and sealed
  * from in a launch for all of them. On the runtime's current stream; what is
- * refused is refused before the first launch. */
+ * refused is refused before the first launch. (mi_kv_attention_batch refuses a
+ * sealing cache's token whose page these rows completed with others, as after
+ * mi_kv_store: a prompt's attention reads k_out and v_out.) */
 int mi_append_batch(const void *q, const void *k, const void *v, void *q_out, void *k_out,
                     void *v_out, long long q_stride, long long k_stride, long long v_stride,
                     const unsigned long long *pages, const uint8_t *tiers, const int *lengths,

@@ -32,8 +32,9 @@ namespace mi::attention_tiles
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
 
-  // The place of piece c of row t (see above): for rows of 8 pieces two rows
-  // span the banks, so rows differ by t / 2; bits reversed, so that rows 0-3
+  // Piece c (16 bytes) of row t of a tile in LDS lies at place c ^ swizzle(t), so
+  // that lanes which read a piece of many rows meet no bank twice: for rows of 8
+  // pieces two rows span the banks, so rows differ by t / 2; bits reversed, so that rows 0-3
   // of a transposing read differ in the bits its four pieces do not use.
   template <int HD>
   __device__ inline int swizzle(int t)

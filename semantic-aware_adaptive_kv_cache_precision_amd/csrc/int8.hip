@@ -50,8 +50,10 @@ namespace mi
       return static_cast<int>(c);
     }
 
-    // Eight values a lane, kLanes lanes a row, kRuns times; rows of more are
-    // read twice (kRuns 0). Bound by memory: 2 bytes read, one written a value.
+    // Eight values a lane, kLanes lanes a row, kRuns times, held in registers
+    // between the largest and the codes; rows of more are read twice (kRuns 0).
+    // Bound by memory: 2 bytes read, one written a value (2,048 rows of 8,960 11.6
+    // us, 4.7 TB/s; five rows of 896 a launch, 4.5).
     template <int kLanes, int kRuns>
     __global__ void __launch_bounds__(256)
         quantise_rows_kernel(const std::uint16_t *__restrict__ x, long long stride,
@@ -204,7 +206,8 @@ namespace mi
     // 16 rows over its share of the inputs; the workgroup's waves share them,
     // 128 at a time, and meet in LDS. Operands straight from memory: lane l
     // holds the 32 bytes 32 (l / 16) .. of row l % 16 of a step, so that four
-    // lanes take a line and a product any 16 of a lane's bytes.
+    // lanes take a line and a product any 16 of a lane's bytes. (One row 1536 ->
+    // 8960 5.6 us, 2048 -> 128256 39, 6.7 TB/s with the weight in the caches.)
     template <int MT, int kWaves, bool kHalf>
     __global__ void __launch_bounds__(64 * kWaves) int8_rows_kernel(Int8Args a)
     {
@@ -332,7 +335,10 @@ namespace mi
     // rows 8192 -> 2048 36.8, by two 43.3). Piece c (16 bytes) of row t lies at
     // place c ^ (t / 2 % 8) of its row: sixteen lanes that read a piece of
     // sixteen rows meet no bank twice. A wave reads the operands of the next 32
-    // inputs while it multiplies these.
+    // inputs while it multiplies these. 8192^3 takes 507 us, 2,170 TOP/s, where the
+    // library's product reaches 2,069; 4,096 rows 1536 -> 8960 (1,504 tiles, 5.9 a
+    // CU) 69 to 77 us with the clocks; 1,777 rows 8192 -> 2048, 224 tiles for 256
+    // CUs with a wave a SIMD, 40, waiting for copies two fifths of it.
     // Where that leaves the device workgroups too few, kGroups such sets of four
     // waves share a tile's inputs, with stages of their own, and the first adds
     // the others' sums up.

@@ -1627,7 +1627,9 @@ def _device_append_caches(caches, starts, counts, layer, q, k, v, q_out, k_out, 
     """append_batch over KVPages: the counts[i] rows of caches[i] go to positions
     [starts[i], starts[i] + counts[i]) of `layer`, reserved before, in place of
     a rotation and a store each. No cache twice. Caches that seal need k_out and
-    v_out (of every row), which attention_caches then reads too."""
+    v_out (of every row); attention_caches takes a token's own row from them (and
+    refuses the last token of rows that completed a sealing cache's page: a
+    prompt's attention is attention_packed over k_out and v_out)."""
     n = len(caches)
     if len(starts) != n or len(counts) != n:
         raise ValueError(f"{n} caches, {len(starts)} starts and {len(counts)} counts")
@@ -1663,7 +1665,8 @@ def _device_attention_packed(q, k, v, out, offsets_q, offsets_k, batch, rows_q, 
     read when the kernels run. Strides are elements between tokens (0:
     contiguous). `partials` (attention_packed_partials floats) lets few rows'
     keys be split. The softmax's weights are rounded to fp16 before they meet
-    the values. Rows of no sequence are left as they were."""
+    the values. Rows of no sequence are left as they were. At most 65,535
+    sequences; strides of keys and values below 2^24."""
     if min(batch, rows_q, rows_k, q_stride, k_stride, v_stride) < 0:
         for value, what in ((batch, "batch"), (rows_q, "rows_q"), (rows_k, "rows_k"),
                             (q_stride, "q_stride"), (k_stride, "k_stride"), (v_stride, "v_stride")):
@@ -1884,8 +1887,8 @@ def _device_sample(logits, uniforms, tokens, rows, vocab, temperature=None, top_
     row of fp16 logits (rows, vocab) by the row's temperature, top_k, top_p and
     min_p (device arrays of a value a row, int32 for top_k; None: off), from
     uniforms[row] in [0, 1), into `tokens` (int32 on the device). `scratch`
-    holds sample_scratch floats. The weights are formed and summed in fp64; of
-    equal logits the lower index counts as the larger; temperature 0 is the
+    holds sample_scratch floats. Borders and sums hold to about 2^-30 of the kept
+    weights; of equal logits the lower index counts as the larger; temperature 0 is the
     greedy token; a row with no logit above -inf gives `vocab`."""
     _sample(False, logits, uniforms, tokens, rows, vocab, temperature, top_k, top_p, min_p, stride,
             scratch)
