@@ -73,26 +73,29 @@ namespace mi
       float *part_o;  // and hd outputs
     };
 
-    __device__ inline int wave_min(int v)
+    // A wave's sum and extrema: within rows of 16 lanes, then over the rows
+    // before, into the last lane. (Moves between registers: a search's steps
+    // each wait for one, and through LDS they take five times as long.)
+    template <typename F>
+    __device__ inline int wave_fold(int v, int none, F &&f)
     {
-#pragma unroll
-      for (int offset = 1; offset < 64; offset *= 2)
-      {
-        v = min(v, __shfl_xor(v, offset));
-      }
-      return __builtin_amdgcn_readfirstlane(v);
+      v = f(v, __builtin_amdgcn_update_dpp(none, v, 0x111, 0xF, 0xF, false)); // row_shr:1, 2, 4, 8
+      v = f(v, __builtin_amdgcn_update_dpp(none, v, 0x112, 0xF, 0xF, false));
+      v = f(v, __builtin_amdgcn_update_dpp(none, v, 0x114, 0xF, 0xF, false));
+      v = f(v, __builtin_amdgcn_update_dpp(none, v, 0x118, 0xF, 0xF, false));
+      v = f(v, __builtin_amdgcn_update_dpp(none, v, 0x142, 0xA, 0xF, false)); // row_bcast:15
+      v = f(v, __builtin_amdgcn_update_dpp(none, v, 0x143, 0xC, 0xF, false)); // row_bcast:31
+      return __builtin_amdgcn_readlane(v, 63);
     }
-    __device__ inline int wave_max(int v) { return -wave_min(-v); }
-
     __device__ inline int wave_sum(int v)
     {
-#pragma unroll
-      for (int offset = 1; offset < 64; offset *= 2)
-      {
-        v += __shfl_xor(v, offset);
-      }
-      return __builtin_amdgcn_readfirstlane(v);
+      return wave_fold(v, 0, [](int x, int y) { return x + y; });
     }
+    __device__ inline int wave_min(int v)
+    {
+      return wave_fold(v, 0x7fffffff, [](int x, int y) { return min(x, y); });
+    }
+    __device__ inline int wave_max(int v) { return -wave_min(-v); }
 
     // A sequence's rows and keys, whatever its offsets hold.
     struct Sequence
@@ -166,7 +169,10 @@ namespace mi
 #pragma unroll
           for (int i = 0; i < kRanked / 64; ++i)
           {
-            see += tiles_that_see<kRows>(mine[i], G, keys);
+            if (64 * i < a.batch)
+            {
+              see += tiles_that_see<kRows>(mine[i], G, keys);
+            }
           }
           (wave_sum(see) > index ? lo : hi) = keys;
         }
@@ -174,7 +180,10 @@ namespace mi
 #pragma unroll
         for (int i = 0; i < kRanked / 64; ++i)
         {
-          more += tiles_that_see<kRows>(mine[i], G, lo + 1);
+          if (64 * i < a.batch)
+          {
+            more += tiles_that_see<kRows>(mine[i], G, lo + 1);
+          }
         }
         index -= wave_sum(more); // among those that see so many and no more
         least = lo;
