@@ -52,6 +52,7 @@ namespace mi
     constexpr int kBuckets = 512; // 32 nats below the largest
     constexpr int kPerNat = 16;
     constexpr int kRowThreads = 512;  // a bucket each
+    constexpr int kBinBits = 9;       // and a bin
     constexpr int kList = 2048;       // of a row's list, held in LDS
     constexpr int kFew = 64;          // of them put in order
     constexpr int kMostVocab = 1 << 20;
@@ -85,6 +86,13 @@ namespace mi
     __device__ inline double number_of(unsigned long long v)
     {
       return __builtin_bit_cast(double, v | __builtin_bit_cast(unsigned long long, 0x1p52)) - 0x1p52;
+    }
+
+    // A weight, at most one, as the nearest whole number of kUnit.
+    __device__ inline unsigned long long units_of(double w)
+    {
+      return __builtin_bit_cast(unsigned long long, w * kUnit + 0x1p52) -
+             __builtin_bit_cast(unsigned long long, 0x1p52);
     }
 
     template <bool kHalf>
@@ -887,12 +895,14 @@ namespace mi
       }
 
       // Of the listed ranks in [lo, hi], those above the border are counted as
-      // taken, and [lo, hi] becomes the 512th of it that has the border. Returns
+      // taken, and [lo, hi] becomes the 512th of it (or the 256th) that has the border. Returns
       // how many are in it.
       __device__ int narrow(long long most, double need, unsigned long long &lo,
                             unsigned long long &hi, long long &taken, double &weight) const
       {
-        const unsigned long long step = (hi - lo) / kRowThreads + 1;
+        // (A power of two: a division of 64 bits a rank is most of a pass.)
+        const int shift = max(0, 64 - __clzll(hi - lo) - kBinBits);
+        const unsigned long long step = 1ull << shift;
         __syncthreads();
         s.bins[threadIdx.x] = 0;
         s.bin_counts[threadIdx.x] = 0;
@@ -900,11 +910,10 @@ namespace mi
         each([&](unsigned long long rank) {
           if (rank >= lo && rank <= hi)
           {
-            const int bin = static_cast<int>((hi - rank) / step);
+            const int bin = static_cast<int>((hi - rank) >> shift);
             atomicAdd(&s.bin_counts[bin], 1);
             // (2^20 of at most 2^38 stay below 2^58.)
-            atomicAdd(&s.bins[bin], static_cast<unsigned long long>(rint(
-                                        weight_of(logit_of(rank), plan.top, plan.inv_t) * kUnit)));
+            atomicAdd(&s.bins[bin], units_of(weight_of(logit_of(rank), plan.top, plan.inv_t)));
           }
         });
         __syncthreads();
@@ -1104,8 +1113,7 @@ namespace mi
         r.each([&](unsigned long long rank) {
           if (rank >= lo && rank <= border.in.hi)
           {
-            atomicAdd(&s.border[index_of(rank) / kPart],
-                      static_cast<unsigned long long>(rint(weight_of(logit_of(rank), top, inv_t) * kUnit)));
+            atomicAdd(&s.border[index_of(rank) / kPart], units_of(weight_of(logit_of(rank), top, inv_t)));
           }
         });
       }
