@@ -53,7 +53,7 @@ namespace mi
     constexpr int kPerNat = 16;
     constexpr int kRowThreads = 512;  // a bucket each
     constexpr int kBinBits = 9;       // and a bin
-    constexpr int kList = 2048;       // of a row's list, held in LDS
+    constexpr int kList = 4096;       // of a row's list, held in LDS
     constexpr int kFew = 64;          // of them put in order
     constexpr int kMostVocab = 1 << 20;
     constexpr int kMostParts = kMostVocab / kPart;
@@ -1056,9 +1056,21 @@ namespace mi
       const int listed = plan.listed;
       if (listed <= kList)
       {
-        for (int i = 2 * kRowThreads + threadIdx.x; i < listed; i += kRowThreads)
+        if (listed > 2 * kRowThreads)
         {
-          s.list[i] = list[i];
+          constexpr int kMore = kList / kRowThreads - 2;
+          unsigned long long ranks[kMore];
+#pragma unroll
+          for (int i = 0; i < kMore; ++i)
+          {
+            const int at = (i + 2) * kRowThreads + static_cast<int>(threadIdx.x);
+            ranks[i] = at < listed ? list[at] : 0;
+          }
+#pragma unroll
+          for (int i = 0; i < kMore; ++i)
+          {
+            s.list[(i + 2) * kRowThreads + threadIdx.x] = ranks[i];
+          }
         }
         list = s.list;
       }
