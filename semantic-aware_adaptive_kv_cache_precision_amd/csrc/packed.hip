@@ -24,8 +24,8 @@
 // most: a prompt of 16K runs at 855 TFLOP/s at head_dim 128, some 800 at 64,
 // where the exponentials and their sums are half of the time; a large product
 // reaches 1,323. Ragged ones lose a quarter more to CUs that end early: eight
-// prompts of 12K rows (12 heads of 128) 157 us, 830 TFLOP/s; new turns behind
-// prefixes (32 heads of 64) 190 us, 640. Nine chats of 413 rows take 7.1 us, a
+// prompts of 12K rows (12 heads of 128) 152 us, 866 TFLOP/s; new turns behind
+// prefixes (32 heads of 64) 188 us, 646. Nine chats of 413 rows take 7.1 us, a
 // launch and a chain of trips.
 #include "attention_tiles.hpp"
 #include "ragged.hpp"

@@ -29,9 +29,9 @@
 // below 2^-39 of its part's largest counts as none.
 //
 // One row of 128,256 takes 26 us, four launches that each are a chain of trips
-// and barriers (parts 5, plan 8, gather 5, choose 7); 48 rows of 151,936 47 us
+// and barriers (parts 5, plan 8, gather 5, choose 7); 48 rows of 151,936 44 us
 // (parts 14.5, where 29 MB are read and some 43 vector instructions a logit,
-// fp64 most, weigh as much as that; plan 9, gather 8, choose 16: borders in buckets of
+// fp64 most, weigh as much as that; plan 9, gather 8, choose 14: borders in buckets of
 // thousands, of the rows with high temperatures).
 #include "common.hpp"
 #include "ragged.hpp"
