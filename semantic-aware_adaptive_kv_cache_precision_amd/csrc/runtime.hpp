@@ -452,7 +452,8 @@ namespace mi
     const float *data() const { return table_ ? table_->as<const float>() : nullptr; }
     // The angles of the first kAngleRows positions (a decode page's rows)
     // as fp16 high and low parts, for the decode kernel's key bias:
-    // [position][hi | lo][head_dim], cos then sin. The table always covers
+    // [position][hi | lo][head_dim], cos then sin, without the magnitude (the
+    // kernel turns by the table first, which has it). The table always covers
     // that many positions.
     static constexpr int kAngleRows = 32;
     const std::uint16_t *angles() const

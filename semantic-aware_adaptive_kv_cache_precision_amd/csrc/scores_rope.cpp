@@ -121,24 +121,32 @@ namespace mi
     const int grown = std::max({count, 2 * positions_, kAngleRows});
     auto table = std::make_unique<DeviceBuffer>(static_cast<std::size_t>(grown) * head_dim_ *
                                                 sizeof(float));
+    auto angles = std::make_unique<DeviceBuffer>(static_cast<std::size_t>(kAngleRows) * head_dim_ *
+                                                 2 * sizeof(std::uint16_t));
     if (frequencies_.empty())
     {
       launch_rope_table(table->as<float>(), grown, head_dim_, theta_, runtime_stream());
+      launch_rope_angles(table->as<const float>(), angles->as<std::uint16_t>(), kAngleRows,
+                         head_dim_, runtime_stream());
     }
     else
     {
       const std::size_t bytes = frequencies_.size() * sizeof(double);
-      const DeviceBuffer held(bytes); // freed below, after the launch that reads it
+      const DeviceBuffer held(bytes);
+      // The rows of the angles without the magnitude: they turn what the table
+      // has turned to a page's first row, and scaled, before.
+      const DeviceBuffer rows(static_cast<std::size_t>(kAngleRows) * head_dim_ * sizeof(float));
       hip_check(hipMemcpy(held.raw(), frequencies_.data(), bytes, hipMemcpyHostToDevice),
                 "hipMemcpy frequencies host-to-device");
       launch_rope_frequencies(table->as<float>(), grown, held.as<const double>(), head_dim_ / 2,
                               magnitude_, runtime_stream());
+      launch_rope_frequencies(rows.as<float>(), kAngleRows, held.as<const double>(), head_dim_ / 2,
+                              1.0, runtime_stream());
+      launch_rope_angles(rows.as<const float>(), angles->as<std::uint16_t>(), kAngleRows, head_dim_,
+                         runtime_stream());
+      // `held` and `rows` go with this block, after the launches that read them.
       hip_check(hipStreamSynchronize(runtime_stream()), "hipStreamSynchronize frequencies");
     }
-    auto angles = std::make_unique<DeviceBuffer>(static_cast<std::size_t>(kAngleRows) * head_dim_ *
-                                                 2 * sizeof(std::uint16_t));
-    launch_rope_angles(table->as<const float>(), angles->as<std::uint16_t>(), kAngleRows,
-                       head_dim_, runtime_stream());
     table_ = std::move(table);
     angles_ = std::move(angles);
     positions_ = grown;
