@@ -28,6 +28,7 @@
 // prefixes (32 heads of 64) 188 us, 646. Nine chats of 413 rows take 7.1 us, a
 // launch and a chain of trips.
 #include "attention_tiles.hpp"
+#include "packed_copies.hpp"
 #include "ragged.hpp"
 
 #include <algorithm>
@@ -224,15 +225,14 @@ namespace mi
     __device__ inline u32x4 rows_from(const std::uint16_t *at, int count, unsigned step, int width)
     {
       const auto address = reinterpret_cast<std::uintptr_t>(at);
-      const unsigned long long bytes = static_cast<unsigned long long>(count) * step + 2 * width;
       return u32x4{static_cast<unsigned>(address), static_cast<unsigned>(address >> 32) & 0xFFFFu,
-                   static_cast<unsigned>(min(bytes, 0xFFFFFFFFull)), 0x00020000u};
+                   packed_copies::rows_bytes(count, step, width), 0x00020000u};
     }
-    // 16 bytes a lane from rows + at + more to the 1,024 bytes at LDS address `to`.
-    __device__ inline void copy_to_lds(unsigned to, unsigned at, u32x4 rows, unsigned more)
+    // 16 bytes a lane from rows + at to the 1,024 bytes at LDS address `to`.
+    __device__ inline void copy_to_lds(unsigned to, unsigned at, u32x4 rows)
     {
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-                   :: "s"(to), "v"(at), "s"(rows), "s"(more)
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                   :: "s"(to), "v"(at), "s"(rows)
                    : "memory", "m0");
     }
 
@@ -264,7 +264,7 @@ namespace mi
         packed_kernel(PackedArgs a)
     {
       constexpr int NW = kTiles * kWays;
-      constexpr int kPieces = HD / 8;    // 16-byte pieces a row
+      constexpr int kPieces = packed_copies::pieces(HD);
       constexpr int kTile = kKeys * HD;  // halves of a step's keys
       constexpr int kStage = 2 * kTile;  // keys, then values
       constexpr int kRows = 32 * kTiles; // rows a workgroup
@@ -369,14 +369,15 @@ namespace mi
       // A step's rows to LDS, 16 bytes a lane, asked for without the compiler's
       // knowledge, whose wait for them would come before the first transposing
       // read of the step before: buffer loads from the step's first row, with
-      // zeros for what lies past the last key.
-      constexpr int kCopies = kTile / 8 / (64 * NW);
-      constexpr int kCopyRows = 64 * NW / kPieces; // rows a copy of the workgroup
+      // zeros for what lies past the last key (packed_copies.hpp).
+      constexpr int kCopies = packed_copies::copies(HD, NW, kKeys);
+      constexpr int kCopyRows = packed_copies::rows_at_once(HD, NW);
       static_assert(kCopyRows % 16 == 0, "rows a copy apart have their pieces in the same places");
       const int copy_row = static_cast<int>(threadIdx.x) / kPieces;
       const int copy_piece = (static_cast<int>(threadIdx.x) % kPieces) ^ swizzle<HD>(copy_row);
       const unsigned k_step = 2u * static_cast<unsigned>(a.k_stride), v_step = 2u * static_cast<unsigned>(a.v_stride);
-      const unsigned k_at = copy_row * k_step + 16 * copy_piece, v_at = copy_row * v_step + 16 * copy_piece;
+      const unsigned k_at = packed_copies::lane_at(copy_row, copy_piece, k_step);
+      const unsigned v_at = packed_copies::lane_at(copy_row, copy_piece, v_step);
       const auto copy = [&](int step, int buf) {
         const int key0 = first + step * kKeys;
         const unsigned to = lds_address(stages + buf * kStage + wave * 512);
@@ -385,8 +386,9 @@ namespace mi
 #pragma unroll
         for (int i = 0; i < kCopies; ++i)
         {
-          copy_to_lds(to + 1024 * NW * i, k_at, k_rows, i * kCopyRows * k_step);
-          copy_to_lds(to + 2 * kTile + 1024 * NW * i, v_at, v_rows, i * kCopyRows * v_step);
+          copy_to_lds(to + 1024 * NW * i, packed_copies::copy_at(k_at, i, kCopyRows, k_step), k_rows);
+          copy_to_lds(to + 2 * kTile + 1024 * NW * i,
+                      packed_copies::copy_at(v_at, i, kCopyRows, v_step), v_rows);
         }
       };
       // (The queries are there before the loop: a wait for them inside it would
