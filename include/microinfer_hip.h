@@ -321,14 +321,15 @@ int mi_linear_int8_accumulate(const void *x, const float *x_scales, const void *
 /* Beyond the reference (whose engine takes the greedy token, argmax.cu): a
  * token of every row of logits (rows, vocab), `stride` elements apart (0:
  * vocab), fp32 or fp16, from a given number uniforms[row] in [0, 1). Token i
- * weighs exp((l_i - max) / temperature); borders and sums hold to about 2^-30
- * of the kept weights. Kept are the top_k
+ * weighs exp((l_i - max) / temperature). Kept are the top_k
  * largest (0 or less: all); of those the fewest largest whose weights sum to
  * top_p of theirs (1 or more: all; at least one); of those the ones that weigh
  * at least min_p of the largest (0 or less: all). Of equal logits the lower
  * index is the larger. The token is the first, by index, whose kept weights up
- * to and with its own exceed the uniform's share of all kept. A weight below
- * 2^-39 of the largest may count as none.
+ * to and with its own exceed the uniform's share of all kept. top_p's border
+ * holds to 2^-26 of the weights that top_k keeps at worst, the token's share to
+ * 2^-26 of all kept, and both to some 2^-30 where logits are spread; top_k and
+ * min_p are exact. A weight below 2^-39 of the largest may count as none.
  * temperature 0 or less: the largest logit. temperature, top_k, top_p, min_p
  * (rows each) are device arrays or NULL: 1, all, all, all. NaN and -inf logits
  * weigh nothing; +inf share the weight among them. A row with neither (nothing

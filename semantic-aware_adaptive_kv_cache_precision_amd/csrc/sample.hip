@@ -25,8 +25,12 @@
 //
 // Sums: a bucket's weights are added as whole numbers of 2^-38 of the part's
 // largest, by LDS atomics of 64 bits (13 of them the count), so that the order
-// of adding does not matter; everything else in fp64, in one order. A weight
-// below 2^-39 of its part's largest counts as none.
+// of adding does not matter: 4,096 weights are off by 2^-27 of the part's largest at
+// most, and so the sums of kept ones by 2^-27 of themselves, since a part that
+// has kept logits has its largest among them. A border's weights are added as
+// finer whole numbers, by what they are themselves (unit_exponent: off by 2^-31 of the
+// kept at most, however far below the row's largest they lie); everything else in
+// fp64, in one order. A weight below 2^-39 of its part's largest may count as none.
 //
 // One row of 128,256 takes 26 us, four launches that each are a chain of trips
 // and barriers (parts 5, plan 8, gather 5, choose 7); 48 rows of 151,936 44 us
@@ -88,13 +92,12 @@ namespace mi
       return __builtin_bit_cast(double, v | __builtin_bit_cast(unsigned long long, 0x1p52)) - 0x1p52;
     }
 
-    // A weight, at most one, as the nearest whole number of kUnit.
-    __device__ inline unsigned long long units_of(double w)
+    // The nearest whole number to one below 2^52.
+    __device__ inline unsigned long long units_of(double units)
     {
-      return __builtin_bit_cast(unsigned long long, w * kUnit + 0x1p52) -
+      return __builtin_bit_cast(unsigned long long, units + 0x1p52) -
              __builtin_bit_cast(unsigned long long, 0x1p52);
     }
-
     template <bool kHalf>
     __device__ inline float logit_at(const void *row, int i)
     {
@@ -216,6 +219,24 @@ namespace mi
       return l == top          ? 1.0
              : top == INFINITY ? 0.0
                                : exp_below((static_cast<double>(l) - static_cast<double>(top)) * inv_t);
+    }
+
+    // The power of two that a logit's weight does not pass.
+    __device__ inline int power_above(float l, float top, double inv_t)
+    {
+      return l >= top ? 0
+                      : static_cast<int>(ceil(
+                            fmax((static_cast<double>(l) - static_cast<double>(top)) * inv_t * kLog2e, -1400.0)));
+    }
+    // The units of 2^-e that n weights of at most 2^high each, some `mass` in all,
+    // are counted in: a weight is 2^51 of them at most, and all of them 2^62, by
+    // their mass, which may be too small by a factor of two, or by their number.
+    // What n halves of a unit make up is 2^-31 of a weight next to 2^high or 2^-42 of
+    // the mass at most. (From exponents alone: every pass of a border's search forms it.)
+    __device__ inline int unit_exponent(int n, double mass, int high)
+    {
+      const int many = max(0, min(32 - __clz(n), __builtin_amdgcn_frexp_exp(mass) - high));
+      return min(51, 62 - many) - high;
     }
 
     // A logit's entry of a histogram: one, and exp(x) as a whole number of kUnit.
@@ -876,6 +897,7 @@ namespace mi
       int ints[4];
       unsigned long long rank;
       double value;
+      double mass;
     };
 
     struct RowSampler
@@ -895,11 +917,14 @@ namespace mi
       }
 
       // Of the listed ranks in [lo, hi], those above the border are counted as
-      // taken, and [lo, hi] becomes the 512th of it (or the 256th) that has the border. Returns
-      // how many are in it.
-      __device__ int narrow(long long most, double need, unsigned long long &lo,
-                            unsigned long long &hi, long long &taken, double &weight) const
+      // taken, and [lo, hi] becomes the 512th of it (or the 256th) that has the border. n are in
+      // it, of some `mass`, before and after.
+      __device__ void narrow(long long most, double need, unsigned long long &lo,
+                             unsigned long long &hi, long long &taken, double &weight, int &n,
+                             double &mass) const
       {
+        const int units = unit_exponent(n, mass, power_above(logit_of(hi), plan.top, plan.inv_t));
+        const double scale = ldexp(1.0, units), unit = ldexp(1.0, -units);
         // (A power of two: a division of 64 bits a rank is most of a pass.)
         const int shift = max(0, 64 - __clzll(hi - lo) - kBinBits);
         const unsigned long long step = 1ull << shift;
@@ -912,14 +937,13 @@ namespace mi
           {
             const int bin = static_cast<int>((hi - rank) >> shift);
             atomicAdd(&s.bin_counts[bin], 1);
-            // (2^20 of at most 2^38 stay below 2^58.)
-            atomicAdd(&s.bins[bin], units_of(weight_of(logit_of(rank), plan.top, plan.inv_t)));
+            atomicAdd(&s.bins[bin], units_of(weight_of(logit_of(rank), plan.top, plan.inv_t) * scale));
           }
         });
         __syncthreads();
         const int bin = threadIdx.x;
         const int mine = s.bin_counts[bin];
-        const double own = static_cast<double>(s.bins[bin]) / kUnit;
+        const double own = static_cast<double>(s.bins[bin]) * unit;
         int count = mine;
         double sum = own;
         scan(count, sum, s.int_waves, s.waves);
@@ -932,14 +956,16 @@ namespace mi
           s.ints[0] = count - mine;
           s.ints[2] = mine;
           s.value = sum - own;
+          s.mass = own + mine * unit; // (a weight's rounding is half a unit)
         }
         __syncthreads();
         taken += s.ints[0];
         weight += s.value;
+        n = s.ints[2];
+        mass = s.mass;
         const unsigned long long above = hi - step * at;
         lo = above - lo < step ? lo : above - (step - 1);
         hi = above;
-        return s.ints[2];
       }
 
       // The border among the logits of bucket b, of which the first are kept: as
@@ -953,9 +979,11 @@ namespace mi
         long long taken = 0;
         double weight = 0.0;
         int n = plan.count[b] - (b > 0 ? plan.count[b - 1] : 0);
+        // (The plan's sums: each weight is off by 2^-39 of the row's largest at most.)
+        double mass = plan.weight[b] - (b > 0 ? plan.weight[b - 1] : 0.0) + n * 0x1p-38;
         while (n > kFew)
         {
-          n = narrow(most, need, lo, hi, taken, weight);
+          narrow(most, need, lo, hi, taken, weight, n, mass);
         }
         // The few in order, by each one's place among them.
         __syncthreads();
@@ -1119,13 +1147,18 @@ namespace mi
 
       // Each part's kept weights: those before the plan's first bucket, those of
       // the buckets from there to the border's, and the border's own by their ranks.
+      double unit = 1.0; // of the border's weights: a part has 4,096 of them at most
       if (border.bucket < kBuckets)
       {
         const unsigned long long lo = max(border.rank, border.in.lo);
+        const int units = 51 - power_above(logit_of(border.in.hi), top, inv_t);
+        const double scale = ldexp(1.0, units);
+        unit = ldexp(1.0, -units);
         r.each([&](unsigned long long rank) {
           if (rank >= lo && rank <= border.in.hi)
           {
-            atomicAdd(&s.border[index_of(rank) / kPart], units_of(weight_of(logit_of(rank), top, inv_t)));
+            atomicAdd(&s.border[index_of(rank) / kPart],
+                      units_of(weight_of(logit_of(rank), top, inv_t) * scale));
           }
         });
       }
@@ -1142,7 +1175,7 @@ namespace mi
           more += a.sums[slot * kBuckets + (b - shift)] & kSumMask;
         }
         part_kept = a.sure[slot] + static_cast<double>(more) * plan.scale[mine] +
-                    static_cast<double>(s.border[mine]) / kUnit;
+                    static_cast<double>(s.border[mine]) * unit;
       }
       // The part that holds the uniform's share.
       const double upto = scan(part_kept, s.waves);

@@ -1887,9 +1887,10 @@ def _device_sample(logits, uniforms, tokens, rows, vocab, temperature=None, top_
     row of fp16 logits (rows, vocab) by the row's temperature, top_k, top_p and
     min_p (device arrays of a value a row, int32 for top_k; None: off), from
     uniforms[row] in [0, 1), into `tokens` (int32 on the device). `scratch`
-    holds sample_scratch floats. Borders and sums hold to about 2^-30 of the kept
-    weights; of equal logits the lower index counts as the larger; temperature 0 is the
-    greedy token; a row with no logit above -inf gives `vocab`."""
+    holds sample_scratch floats. top_p's border and the token's share hold to
+    2^-26 of the kept weights at worst, to some 2^-30 where logits are spread; of equal
+    logits the lower index counts as the larger; temperature 0 is the greedy token; a
+    row with no logit above -inf gives `vocab`."""
     _sample(False, logits, uniforms, tokens, rows, vocab, temperature, top_k, top_p, min_p, stride,
             scratch)
 
