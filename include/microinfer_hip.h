@@ -544,8 +544,8 @@ int mi_kv_attention_batch(mi_kv_pages *const *kv, const int *seq_k, int count, i
  * rope turns the first rope head_dim channels of a query or key head (NULL:
  * none), pairs (j, j + half), or (2j, 2j + 1) where interleaved, and must cover
  * max_pages pages. head_dim even, strides in whole elements; 16-byte aligned
- * rows of whole sixteens of channels are faster. What is written may share no
- * byte with what is read, pages not checked.
+ * rows of whole sixteens of channels are faster. At most 32 (2^24 - 1) rows. What
+ * is written may share no byte with what is read, pages not checked.
  * mi_kv_append_batch: the same for `count` different caches of one shape, the
  * counts[i] rows of cache i at positions [starts[i], starts[i] + counts[i]) of
  * `layer` (host memory, as mi_kv_store takes them, reserved before). Caches

@@ -36,6 +36,7 @@ namespace mi
     constexpr int kThreads = 256;
     constexpr int kOffsetsHeld = 2048; // offsets that fit the workgroup's LDS
     constexpr int kRowsHeld = 32;      // rows of a workgroup
+    constexpr int kMostRows = 0xffffff * kRowsHeld; // a launch has fewer than 2^32 threads
 
     struct AppendArgs
     {
@@ -403,6 +404,11 @@ namespace mi
     {
       throw InvalidArgument("batch, max_pages and rows must not be negative, got " +
                             std::to_string(t.batch) + ", " + std::to_string(t.max_pages) + " and " +
+                            std::to_string(t.rows));
+    }
+    if (t.rows > kMostRows)
+    {
+      throw InvalidArgument("at most " + std::to_string(kMostRows) + " rows are appended at once, got " +
                             std::to_string(t.rows));
     }
     if (t.heads <= 0 || t.kv_heads <= 0 || t.head_dim <= 0 || t.head_dim % 2 != 0)

@@ -1,0 +1,18 @@
+"""Sizes past what one launch of a ragged batch's operators has threads for: refused
+before a launch, with no device call. A launch has fewer than 2^32 threads."""
+
+import pytest
+
+from test_int4_refusals import On
+from test_ragged_refusals import append_args, device
+
+FAR = 1 << 50  # bytes between buffers, more than any of them has
+
+
+def test_append_refuses_more_rows_than_a_launch_takes():
+    most = 0xFFFFFF * 32  # 32 rows to a workgroup of 256
+    sizes = dict(heads=1, kv_heads=1, head_dim=2, k_out=None,
+                 **{name: On(1 << 34, (i + 1) * FAR) for i, name in enumerate(("q", "k", "v", "q_out"))})
+    for rows in (most + 1, (1 << 31) - 1):
+        with pytest.raises(ValueError, match=f"at most {most} rows"):
+            device().append_batch(**append_args(rows=rows, **sizes))
