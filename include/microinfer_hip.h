@@ -309,7 +309,8 @@ int mi_linear_int4_accumulate(const void *x, const void *codes, const void *scal
  * mi_linear_int8_accumulate: out (rows, out) fp32 = residual + x W^T, residual
  * NULL or out itself: in place. features and in multiples of 16, in below
  * 131072 (the sums stay in 32 bits); x, codes, weight 16-byte aligned, stride a
- * multiple of 8. */
+ * multiple of 8. At most 4 (2^24 - 1) rows are quantised at once, of more than 2,048
+ * values 2^24 - 1. */
 int mi_quantise_rows_int8(const void *x, long long stride, void *codes, float *scales, int rows,
                           int features, void *stream);
 int mi_linear_int8(const void *x, const float *x_scales, const void *weight, const float *w_scales,

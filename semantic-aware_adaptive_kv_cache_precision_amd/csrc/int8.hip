@@ -727,6 +727,16 @@ namespace mi
     {
       throw InvalidArgument("rows to quantise need x, codes and scales");
     }
+    // A wave a row up to 2,048 values, else a workgroup; a launch has fewer than
+    // 2^32 threads.
+    const int runs = features / 8;
+    const int most_rows = 0xffffff * (runs <= 256 ? 4 : 1);
+    if (rows > most_rows)
+    {
+      throw InvalidArgument("at most " + std::to_string(most_rows) + " rows of " +
+                            std::to_string(features) + " values are quantised at once, got " +
+                            std::to_string(rows));
+    }
     stride = stride > 0 ? stride : features;
     if (stride < features || stride % 8 != 0)
     {
@@ -747,10 +757,8 @@ namespace mi
     }
     const auto *from = static_cast<const std::uint16_t *>(x);
     auto *to = static_cast<std::uint8_t *>(codes);
-    const int runs = features / 8;
     const unsigned blocks = static_cast<unsigned>(rows);
     const unsigned fours = (blocks + 3) / 4;
-    // A wave a row up to 2,048 values, else a workgroup.
     if (runs <= 64)
     {
       quantise_rows_kernel<64, 1><<<fours, 256, 0, stream>>>(from, stride, to, scales, rows, runs);

@@ -16,3 +16,10 @@ def test_append_refuses_more_rows_than_a_launch_takes():
     for rows in (most + 1, (1 << 31) - 1):
         with pytest.raises(ValueError, match=f"at most {most} rows"):
             device().append_batch(**append_args(rows=rows, **sizes))
+
+
+def test_quantise_refuses_more_rows_than_a_launch_takes():
+    for features, most in ((16, 4 * 0xFFFFFF), (2048, 4 * 0xFFFFFF), (2064, 0xFFFFFF), (65536, 0xFFFFFF)):
+        x, codes = On(1 << 46, FAR), On(1 << 46, 2 * FAR, 1)
+        with pytest.raises(ValueError, match=f"at most {most} rows of {features} values"):
+            device().quantise_rows_int8(x, codes, On(1 << 30, 3 * FAR, 4), most + 1, features)
