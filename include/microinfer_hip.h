@@ -230,7 +230,9 @@ int mi_attention_window(const void *q, const void *k, const void *v, void *out, 
  * or 128; alignment, overlaps, the rounding of weights and values that are not
  * finite as mi_attention_window's, and so the partials, those of
  * mi_attention_packed_partials, never more than 65,536 (head_dim + 2) floats.
- * At most 65,535 sequences; strides of keys and values below 2^24. */
+ * At most 65,535 sequences; strides of keys and values below 2^24; tiles of 128
+ * rows (a KV head's, and a sequence's short one) below 2^23 at head_dim 64, 2^24
+ * at 128. */
 int mi_attention_packed_partials(int batch, int rows_q, int rows_k, int heads, int kv_heads,
                                  int head_dim, size_t *floats);
 int mi_attention_packed(const void *q, const void *k, const void *v, void *out, long long q_stride,

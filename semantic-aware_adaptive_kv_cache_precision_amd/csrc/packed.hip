@@ -826,7 +826,8 @@ namespace mi
     template <int kTiles_, int kWays_, int kKeys_>
     struct Form
     {
-      static constexpr int tiles = kTiles_, ways = kWays_, keys = kKeys_, rows = 32 * kTiles_;
+      static constexpr int tiles = kTiles_, ways = kWays_, keys = kKeys_, rows = 32 * kTiles_,
+                           threads = 64 * kTiles_ * kWays_;
     };
     using Few = Form<1, 4, 128>;
     using Many64 = Form<4, 2, 128>;
@@ -930,7 +931,7 @@ namespace mi
                                       static_cast<int>(lds)),
                   "hipFuncSetAttribute packed LDS");
       }
-      kernel<<<dim3(c.blocks * a.kv_heads, c.splits), 64 * F::tiles * F::ways, lds, stream>>>(a);
+      kernel<<<dim3(c.blocks * a.kv_heads, c.splits), F::threads, lds, stream>>>(a);
       hip_check(hipGetLastError(), "packed_kernel");
     }
 
@@ -1016,6 +1017,15 @@ namespace mi
                             "offsets 4-byte");
     }
     const Cut c = cut_of(t, t.partials != nullptr);
+    const long long groups = static_cast<long long>(c.blocks) * t.kv_heads;
+    const int threads = c.few ? Few::threads : t.head_dim == 64 ? Many64::threads : Many128::threads;
+    if (groups * threads > 0xffffffffll) // (a launch's)
+    {
+      throw InvalidArgument("packed attention takes at most " + std::to_string(0xffffffffll / threads) +
+                            " tiles of rows and KV heads, got " + std::to_string(groups) + " of " +
+                            std::to_string(t.batch) + " sequences, " + std::to_string(t.rows_q) +
+                            " rows and " + std::to_string(t.kv_heads) + " KV heads");
+    }
     if (t.partials != nullptr && t.partials_floats < packed_attention_floats(t))
     {
       throw InvalidArgument("packed attention's partials need " +
@@ -1062,7 +1072,6 @@ namespace mi
     a.splits = c.splits;
     // Where the device holds them all at once, tiles need no order.
     const int held = 2 * kCus;
-    const long long groups = static_cast<long long>(c.blocks) * t.kv_heads;
     a.ranked = t.batch <= kRanked && groups * c.splits > kCus ? static_cast<int>(std::min<long long>(held, groups)) : 0;
     a.scale = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(t.head_dim)));
     if (c.splits > 1)

@@ -23,3 +23,13 @@ def test_quantise_refuses_more_rows_than_a_launch_takes():
         x, codes = On(1 << 46, FAR), On(1 << 46, 2 * FAR, 1)
         with pytest.raises(ValueError, match=f"at most {most} rows of {features} values"):
             device().quantise_rows_int8(x, codes, On(1 << 30, 3 * FAR, 4), most + 1, features)
+
+
+@pytest.mark.parametrize("hd,kv,most", [(64, 128, (1 << 23) - 1), (128, 256, (1 << 24) - 1)])
+def test_packed_attention_refuses_more_tiles_than_a_launch_takes(hd, kv, most):
+    """65,535 sequences of a token: a tile each of every KV head, and a 128th more."""
+    rows = 65535
+    far = lambda i: On(1 << 40, i * FAR)  # noqa: E731
+    with pytest.raises(ValueError, match=f"at most {most} tiles"):
+        device().attention_packed(far(1), far(2), far(3), far(4), On(rows + 1, 5 * FAR, 4), None, rows, rows,
+                                  rows, kv, kv, hd)
