@@ -543,7 +543,10 @@ int mi_kv_attention_batch(mi_kv_pages *const *kv, const int *seq_k, int count, i
  * their place in its FP16 page (32 key rows, 32 value rows); where its page's
  * tier is not 0, its address 0 or its position past max_pages pages, nowhere.
  * q_out (rows, heads, head_dim), and k_out, v_out (rows, kv_heads, head_dim) or
- * NULL, take the rows beside. Rows of no sequence are left as they were.
+ * NULL, take the rows beside, those that go to no page too; one past the RoPE
+ * table's last position comes out turned as at the last, one below zero (a length
+ * less than its sequence's rows) as at zero. Rows of no sequence are left as they
+ * were.
  * rope turns the first rope head_dim channels of a query or key head (NULL:
  * none), pairs (j, j + half), or (2j, 2j + 1) where interleaved, and must cover
  * max_pages pages. head_dim even, strides in whole elements; 16-byte aligned
@@ -553,7 +556,9 @@ int mi_kv_attention_batch(mi_kv_pages *const *kv, const int *seq_k, int count, i
  * counts[i] rows of cache i at positions [starts[i], starts[i] + counts[i]) of
  * `layer` (host memory, as mi_kv_store takes them, reserved before). Caches
  * that seal need k_out and v_out, which their pages are then filled and sealed
- * from in a launch for all of them. On the runtime's current stream; what is
+ * from: the pages of all caches together, a launch for each 24 of them, but for the
+ * whole pages of a cache whose rows touch more than 24, which take launches of
+ * their own. On the runtime's current stream; what is
  * refused is refused before the first launch. (mi_kv_attention_batch refuses a
  * sealing cache's token whose page these rows completed with others, as after
  * mi_kv_store: a prompt's attention reads k_out and v_out.) */

@@ -332,13 +332,13 @@ namespace mi
     // memory (steps of 64 ask L2 for each line twice: 8192^3 577 us, and 507),
     // pass through LDS, kStages of them, copied there directly: two stages where
     // two workgroups to a CU hide the copies, three where one is alone (1,777
-    // rows 8192 -> 2048 36.8, by two 43.3). Piece c (16 bytes) of row t lies at
+    // rows 8192 -> 2048 40.4, by two 46.6). Piece c (16 bytes) of row t lies at
     // place c ^ (t / 2 % 8) of its row: sixteen lanes that read a piece of
     // sixteen rows meet no bank twice. A wave reads the operands of the next 32
     // inputs while it multiplies these. 8192^3 takes 507 us, 2,170 TOP/s, where the
     // library's product reaches 2,069; 4,096 rows 1536 -> 8960 (1,504 tiles, 5.9 a
     // CU) 69 to 77 us with the clocks; 1,777 rows 8192 -> 2048, 224 tiles for 256
-    // CUs with a wave a SIMD, 40, waiting for copies two fifths of it.
+    // CUs with a wave a SIMD, 40.4, waiting for copies two fifths of it.
     // Where that leaves the device workgroups too few, kGroups such sets of four
     // waves share a tile's inputs, with stages of their own, and the first adds
     // the others' sums up.
@@ -372,7 +372,7 @@ namespace mi
       const int m0 = (band * kBand + tile % high) * kM;
       const int n0 = tile / high * kN;
 
-      // A lane's copies: places i * 256 + thread, rows of four.
+      // A lane's copies: places i * 256 + thread, rows of eight.
       const std::uint8_t *x0 = a.x + static_cast<std::size_t>(m0) * a.in;
       const std::uint8_t *w0 = a.w + static_cast<std::size_t>(n0) * a.in;
       unsigned row_at[kCopies];
@@ -383,7 +383,7 @@ namespace mi
         const int r = i * kCopyRows < kM ? min(t, a.rows - 1 - m0) : min(t - kM, a.features - 1 - n0);
         row_at[i] = static_cast<unsigned>(r) * a.in;
       }
-      // The piece a lane copies: place % 4 of its row, turned by the row.
+      // The piece a lane copies: place % 8 of its row, turned by the row.
       const int piece = (thread % kPieces) ^ (thread / kPieces / kSame % kPieces);
       // The group's steps.
       const int steps = ((a.in + kStep - 1) / kStep + kGroups - 1) / kGroups, begin = group * steps;

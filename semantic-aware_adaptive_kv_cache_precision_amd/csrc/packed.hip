@@ -21,11 +21,11 @@
 // second launch joins.
 //
 // Bound by the matrix cores and the vector unit in turn, two waves to a SIMD at
-// most: a prompt of 16K runs at 855 TFLOP/s at head_dim 128, some 800 at 64,
+// head_dim 128, four at 64: a prompt of 16K runs at 855 TFLOP/s at 128, some 800 at 64,
 // where the exponentials and their sums are half of the time; a large product
 // reaches 1,323. Ragged ones lose a quarter more to CUs that end early: eight
-// prompts of 12K rows (12 heads of 128) 152 us, 866 TFLOP/s; new turns behind
-// prefixes (32 heads of 64) 188 us, 646. Nine chats of 413 rows take 7.1 us, a
+// prompts of 12K rows (12 heads of 128) 151 us, 870 TFLOP/s; new turns behind
+// prefixes (32 heads of 64) 187 us, 650. Nine chats of 413 rows take 7.1 us, a
 // launch and a chain of trips.
 #include "attention_tiles.hpp"
 #include "packed_copies.hpp"

@@ -33,7 +33,7 @@
 // fp64, in one order. A weight below 2^-39 of its part's largest may count as none.
 //
 // One row of 128,256 takes 26 us, four launches that each are a chain of trips
-// and barriers (parts 5, plan 8, gather 5, choose 7); 48 rows of 151,936 44 us
+// and barriers (parts 5, plan 8, gather 5, choose 7); 48 rows of 151,936 45 us
 // (parts 14.5, where 29 MB are read and some 43 vector instructions a logit,
 // fp64 most, weigh as much as that; plan 9, gather 8, choose 14: borders in buckets of
 // thousands, of the rows with high temperatures).

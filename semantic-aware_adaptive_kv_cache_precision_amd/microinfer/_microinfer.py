@@ -1608,7 +1608,9 @@ def _device_append_batch(q, k, v, q_out, k_out, pages, tiers, lengths, offsets, 
     kernel runs. `rope` (a RopeTable that covers max_pages pages, of the
     channels that turn, or None) pairs channels (j, j + half), or (2j, 2j + 1)
     where `interleaved`. q_out, and k_out and v_out where not None, take the
-    rows (contiguous) for attention over them."""
+    rows (contiguous) for attention over them. A position past max_pages pages, or
+    below zero, goes to no page; one that `rope` does not cover comes out turned as
+    at the nearest it does."""
     _non_negative(batch, "batch")
     _non_negative(max_pages, "max_pages")
     rows_at = _append_rows(q, k, v, q_out, k_out, v_out, rows, heads, kv_heads, head_dim, q_stride,
