@@ -221,12 +221,13 @@ namespace mi
                                : exp_below((static_cast<double>(l) - static_cast<double>(top)) * inv_t);
     }
 
-    // The power of two that a logit's weight does not pass.
+    // The power of two that a logit's weight does not pass, 2^-128 at least (units of
+    // less would leave fp64, where a temperature next to 0 makes weights of nothing).
     __device__ inline int power_above(float l, float top, double inv_t)
     {
       return l >= top ? 0
                       : static_cast<int>(ceil(
-                            fmax((static_cast<double>(l) - static_cast<double>(top)) * inv_t * kLog2e, -1400.0)));
+                            fmax((static_cast<double>(l) - static_cast<double>(top)) * inv_t * kLog2e, -128.0)));
     }
     // The units of 2^-e that n weights of at most 2^high each, some `mass` in all,
     // are counted in: a weight is 2^51 of them at most, and all of them 2^62, by

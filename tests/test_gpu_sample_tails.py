@@ -11,6 +11,7 @@ import numpy as np
 import pytest
 
 from conftest import announce
+from oracle import ragged
 from test_gpu_sample import choose
 
 pytestmark = pytest.mark.gpu
@@ -98,3 +99,19 @@ def test_temperatures_that_put_a_row_into_one_bucket(ulps):
     for top_k in (0, vocab // 2):
         for j in borders(tail * (top_k or vocab) / vocab, vocab):
             run(row, t, steps, f"one bucket {ulps}", top_k, 1.0 - STEP * j)
+
+
+@pytest.mark.parametrize("t", [1.4e-45, 1e-40])
+def test_temperatures_next_to_zero(t):
+    """Buckets of a million nats each, whose logits weigh nothing, and of less."""
+    rng = np.random.default_rng(2)
+    row = rng.uniform(0, 1e-36, 50000).astype(np.float32)
+    u = np.array([0.0, 0.3, 0.999], np.float32)
+    t32 = float(np.float32(t))
+    for settings in (dict(), dict(top_k=25000), dict(top_k=40000, top_p=0.9), dict(top_p=0.5), dict(min_p=0.1)):
+        announce("next to zero", t, settings)
+        got = choose(np.repeat(row[None], len(u), 0), u, temperature=t, **settings)
+        exact = {name: v if name == "top_k" else float(np.float32(v)) for name, v in settings.items()}
+        want = [ragged.sample(row, float(mine), temperature=t32, **exact) for mine in u]
+        assert all(border > 2.0**-25 or mine == 0 for (_, border), mine in zip(want, u))
+        np.testing.assert_array_equal(got, [token for token, _ in want], err_msg=f"{t} {settings}")
